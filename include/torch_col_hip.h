@@ -375,6 +375,24 @@ int tch_softmax_ce_lm(tch_context* ctx, int dtype, const float* logits, int ld_l
 /* g += wd*p; buf = momentum*buf + g; p -= lr*buf; shadow_bf16 (may be NULL) = bf16(p) */
 int tch_sgd_momentum_step(tch_context* ctx, float* param, const float* grad, float* momentum_buf, void* shadow_bf16,
                           int64_t n, float lr, float momentum, float weight_decay);
+/* the same step on grad_scale[0] * grad (device memory: the coefficient of tch_grad_norm) */
+int tch_sgd_momentum_step_scaled(tch_context* ctx, float* param, const float* grad, float* momentum_buf,
+                                 void* shadow_bf16, int64_t n, float lr, float momentum, float weight_decay,
+                                 const float* grad_scale);
+/* Global norm of many gradient tensors: norm[0] = sqrt(sum of squares over all of them), added up in fp64 in a fixed
+ * order; coef[0] (may be NULL) = min(1, max_norm / (norm + 1e-6)), what the optimizer steps above take.  table: device
+ * memory, `pieces` rows of 32 bytes {source, destination, int32 elements, source is bf16, destination is bf16, aligned}
+ * with at most tch_grad_table_piece_elems() elements each; aligned: source and destination start on a boundary of four of
+ * their elements.  workspace: tch_grad_norm_workspace_bytes(pieces), in use until the launches are done.  bytes: what is
+ * read (written), for the profiler.
+ * clip: destination = coef * source instead (in place where they are the same).  A norm that is not a number makes
+ * every gradient one, an infinite norm makes finite gradients zero. */
+int64_t tch_grad_table_piece_elems(void);
+int64_t tch_grad_norm_workspace_bytes(int64_t pieces);
+int tch_grad_norm(tch_context* ctx, const void* table, int64_t pieces, int64_t bytes, double max_norm, float* norm,
+                  float* coef, void* workspace);
+int tch_clip_grad_norm(tch_context* ctx, const void* table, int64_t pieces, int64_t bytes_read, int64_t bytes_written,
+                       double max_norm, float* norm, void* workspace);
 /* global += grad; grad = 0   (pytorch/torch_col/accumulate.py:20-24) */
 int tch_grad_accumulate(tch_context* ctx, float* global, float* grad, int64_t n);
 int tch_fill_zero(tch_context* ctx, void* ptr, int64_t bytes);
@@ -428,6 +446,39 @@ int tch_layernorm_bwd_windowed(tch_context* ctx, int dtype, const void* dy, cons
 /* tanh_form 0: 0.5 x (1 + erf(x / sqrt 2)) (nn.GELU); 1: GPT-2's gelu_new.  n is a multiple of a 16-byte chunk. */
 int tch_gelu_fwd(tch_context* ctx, int dtype, const void* x, void* y, int64_t n, int tanh_form);
 int tch_gelu_bwd(tch_context* ctx, int dtype, const void* dy, const void* x, void* dx, int64_t n, int tanh_form);
+
+/* ---- linear layers with everything around them in one launch -------------------------
+ * The feed-forward halves of the blocks that train/gpt2.py:26 and train/swin_b.py:38 build: projection, activation,
+ * residual.  Matrices are row major, `ld*` elements from row to row (rows start on 16-byte boundaries, less than 4 MiB
+ * apart; columns beyond the layer's size are neither read nor written); weights [out][in] are dense and below 2 GiB.
+ * Sizes of a layer are multiples of a 16-byte chunk, M is any number of rows: 0 enqueues nothing.  Products, bias,
+ * activation and residual are fp32 and rounded once, when they are stored.
+ * act: 0 none, 1 ReLU, 2 GELU (erf), 3 GELU (tanh), 4 SiLU.
+ *   fwd:    y = act(x w^T + bias) + residual; pre (may be NULL) = x w^T + bias.  x [M][K], w [N][K], y [M][N].
+ *   dgrad:  dx = (dy w) . act'(pre) + residual, pre and act being those of the layer in FRONT of this one; wt [N][K] is
+ *           this layer's weight transposed (tch_filter_transpose_batched), dy [M][K], dx [M][N].
+ * A residual may be the output itself (in place); nothing else may overlap an output. */
+int tch_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* y, int64_t ldy,
+                   const float* bias, int act, const void* residual, int64_t ldr, void* pre, int64_t ldp, int64_t M,
+                   int64_t K, int64_t N);
+int tch_linear_dgrad(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, void* dx, int64_t lddx,
+                     int act, const void* pre, int64_t ldp, const void* residual, int64_t ldr, int64_t M, int64_t K,
+                     int64_t N);
+/* Gated layer: g = x wg^T + bg, u = x wu^T + bu, h = act(g) . u.  w [2F][K] and bias [2F] hold the gate's rows first,
+ * pre [M][2F] (may be NULL) = (g | u), h [M][F].
+ * dgrad_gated: dh = dy w (wt [F][K] the down projection's weight transposed, dy [M][K]) goes straight into
+ * dpre [M][2F] = (dh . u . act'(g) | dh . act(g)); h (may be NULL) [M][F] = act(g) . u again.  dpre may be pre itself. */
+int tch_gated_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* h, int64_t ldh,
+                         const float* bias, int act, void* pre, int64_t ldp, int64_t M, int64_t K, int64_t F);
+int tch_linear_dgrad_gated(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, const void* pre,
+                           int64_t ldp, void* dpre, int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t K,
+                           int64_t F);
+/* The same derivatives as a pass of their own: dz = dy . act'(pre) [M][N], and the gated form from dh [M][F].  The
+ * gradients may be written over dy (dz only) or pre. */
+int tch_act_bwd(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* pre, int64_t ldp, void* dz,
+                int64_t lddz, int act, int64_t M, int64_t N);
+int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp,
+                      void* dpre, int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t F);
 /* probs = softmax over the last dimension of scale * scores[batch, heads, Lq, Lk] + bias[heads, Lq, Lk]
  * + mask[windows, Lq, Lk] (window = batch index % windows); bias and mask may be NULL; causal != 0 keeps keys
  * j <= i only (Lq == Lk).  In place (probs == scores) is allowed. */
@@ -443,6 +494,10 @@ int tch_attn_softmax_bwd(tch_context* ctx, int dtype, const void* probs, const v
 int tch_adamw_step(tch_context* ctx, float* param, const float* grad, float* exp_avg, float* exp_avg_sq,
                    void* shadow_bf16, int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay,
                    int* step_dev, float* scalars_dev);
+/* the same step on grad_scale[0] * grad (device memory: the coefficient of tch_grad_norm) */
+int tch_adamw_step_scaled(tch_context* ctx, float* param, const float* grad, float* exp_avg, float* exp_avg_sq,
+                          void* shadow_bf16, int64_t n, double lr, double beta1, double beta2, double eps,
+                          double weight_decay, int* step_dev, float* scalars_dev, const float* grad_scale);
 /* out[b, t, :] = wte[ids[b, t], :] + wpe[t, :]; backward: dwte[id] += the dy rows of the positions that hold id,
  * dwpe (+)= sum over b.  chain: 2 * B * T int32 of scratch; with it the rows that share a token are added up in
  * position order by one thread (the same bits every run); NULL: fp32 atomics, order not fixed. */

@@ -24,6 +24,7 @@ inline ConvShape shape(int N, int H, int W, int Cc, int K, int R, int S, int str
   ConvShape s{N, H, W, Cc, K, R, S, stride, pad, c_logical};
   return s;
 }
+inline Rows rows(const void* p, int64_t ld) { return {const_cast<void*>(p), ld}; }
 }  // namespace
 
 extern "C" {
@@ -360,6 +361,52 @@ int tch_gelu_bwd(tch_context* ctx, int dtype, const void* dy, const void* x, voi
   return gelu_bwd(C(ctx), dtype, dy, x, dx, n, tanh_form);
 }
 
+int tch_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* y, int64_t ldy, const float* bias, int act,
+                   const void* residual, int64_t ldr, void* pre, int64_t ldp, int64_t M, int64_t K, int64_t N) {
+  return linear_fwd(C(ctx), dtype, rows(x, ldx), w, rows(y, ldy), bias, act, rows(residual, ldr), rows(pre, ldp), M, K, N);
+}
+
+int tch_linear_dgrad(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, void* dx, int64_t lddx, int act, const void* pre,
+                     int64_t ldp, const void* residual, int64_t ldr, int64_t M, int64_t K, int64_t N) {
+  return linear_dgrad(C(ctx), dtype, rows(dy, lddy), wt, rows(dx, lddx), act, rows(pre, ldp), rows(residual, ldr), M, K, N);
+}
+
+int tch_gated_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* h, int64_t ldh, const float* bias, int act,
+                         void* pre, int64_t ldp, int64_t M, int64_t K, int64_t F) {
+  return gated_linear_fwd(C(ctx), dtype, rows(x, ldx), w, rows(h, ldh), bias, act, rows(pre, ldp), M, K, F);
+}
+
+int tch_linear_dgrad_gated(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, const void* pre, int64_t ldp, void* dpre,
+                           int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t K, int64_t F) {
+  return linear_dgrad_gated(C(ctx), dtype, rows(dy, lddy), wt, rows(pre, ldp), rows(dpre, lddp), rows(h, ldh), act, M, K, F);
+}
+
+int tch_act_bwd(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* pre, int64_t ldp, void* dz, int64_t lddz, int act, int64_t M,
+                int64_t N) {
+  return act_bwd(C(ctx), dtype, rows(dy, lddy), rows(pre, ldp), rows(dz, lddz), rows(nullptr, 0), 0, act, M, N);
+}
+
+int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp, void* dpre, int64_t lddp, void* h,
+                      int64_t ldh, int act, int64_t M, int64_t F) {
+  return act_bwd(C(ctx), dtype, rows(dh, lddh), rows(pre, ldp), rows(dpre, lddp), rows(h, ldh), 1, act, M, F);
+}
+
+int64_t tch_grad_table_piece_elems(void) { return grad_table_piece_elems(); }
+int64_t tch_grad_norm_workspace_bytes(int64_t pieces) { return grad_norm_workspace_bytes(pieces); }
+
+int tch_grad_norm(tch_context* ctx, const void* table, int64_t pieces, int64_t bytes, double max_norm, float* norm, float* coef, void* workspace) {
+  if (coef && !(max_norm >= 0.0)) {
+    set_error("invalid argument: grad_norm: max_norm must not be negative");
+    return -22;
+  }
+  return grad_norm(C(ctx), table, pieces, bytes, 0, 0, coef ? max_norm : -1.0, norm, coef, workspace);
+}
+
+int tch_clip_grad_norm(tch_context* ctx, const void* table, int64_t pieces, int64_t bytes_read, int64_t bytes_written, double max_norm, float* norm,
+                       void* workspace) {
+  return grad_norm(C(ctx), table, pieces, bytes_read, bytes_written, 1, max_norm, norm, nullptr, workspace);
+}
+
 int tch_attn_softmax_fwd(tch_context* ctx, int dtype, const void* scores, void* probs, int64_t batch, int heads, int Lq,
                          int Lk, float scale, const float* bias, const float* mask, int windows, int causal) {
   return attn_softmax_fwd(C(ctx), dtype, scores, probs, batch, heads, Lq, Lk, scale, bias, mask, windows, causal);
@@ -375,6 +422,17 @@ int tch_adamw_step(tch_context* ctx, float* param, const float* grad, float* exp
                    int* step_dev, float* scalars_dev) {
   return adamw_step(C(ctx), param, grad, exp_avg, exp_avg_sq, shadow_bf16, n, lr, beta1, beta2, eps, weight_decay,
                     step_dev, scalars_dev);
+}
+
+int tch_adamw_step_scaled(tch_context* ctx, float* param, const float* grad, float* exp_avg, float* exp_avg_sq,
+                          void* shadow_bf16, int64_t n, double lr, double beta1, double beta2, double eps,
+                          double weight_decay, int* step_dev, float* scalars_dev, const float* grad_scale) {
+  if (!grad_scale) {
+    set_error("tch_adamw_step_scaled: null factor");
+    return -22;
+  }
+  return adamw_step(C(ctx), param, grad, exp_avg, exp_avg_sq, shadow_bf16, n, lr, beta1, beta2, eps, weight_decay,
+                    step_dev, scalars_dev, grad_scale);
 }
 
 int tch_embedding_fwd(tch_context* ctx, int dtype, const int64_t* ids, const void* wte, const void* wpe, void* out, int B,
@@ -656,6 +714,16 @@ int tch_bias_grad_ws(tch_context* ctx, int dtype, const void* dy, float* dbias, 
 int tch_sgd_momentum_step(tch_context* ctx, float* param, const float* grad, float* momentum_buf, void* shadow_bf16,
                           int64_t n, float lr, float momentum, float weight_decay) {
   return sgd_momentum_step(C(ctx), param, grad, momentum_buf, shadow_bf16, n, lr, momentum, weight_decay);
+}
+
+int tch_sgd_momentum_step_scaled(tch_context* ctx, float* param, const float* grad, float* momentum_buf,
+                                 void* shadow_bf16, int64_t n, float lr, float momentum, float weight_decay,
+                                 const float* grad_scale) {
+  if (!grad_scale) {
+    set_error("tch_sgd_momentum_step_scaled: null factor");
+    return -22;
+  }
+  return sgd_momentum_step(C(ctx), param, grad, momentum_buf, shadow_bf16, n, lr, momentum, weight_decay, grad_scale);
 }
 
 int tch_grad_accumulate(tch_context* ctx, float* global, float* grad, int64_t n) {

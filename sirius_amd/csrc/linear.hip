@@ -1,0 +1,182 @@
+// Linear layers with bias, activation and residual in one launch, gated feed-forward layers, and their data gradients: argument
+// checks, and the derivative of an activation as a pass of its own for a gradient that no product of this library ends in.
+// The products are in linear_kernels.h.
+//
+// Reference call sites: the feed-forward halves of the transformer blocks that train/gpt2.py:26 and train/swin_b.py:38 build
+// (a projection, an activation, a projection and the residual).
+#include "linear_kernels.h"
+
+#include <climits>
+
+#include "context.h"
+#include "ops.h"
+
+namespace tch {
+namespace {
+
+// ---------------------------------------------------------------------------
+// dz = dy * act'(z), and the gated form (dg, du, and h again on request) from dh and (g | u)
+// ---------------------------------------------------------------------------
+// Bound by memory: 6 (gated 10, with h 12) bytes per element in bf16.  A thread has kAtOnce chunks on their way at a time.
+struct ActBwdArgs {
+  const void* dy;
+  const void* z;
+  void* dz;
+  void* h;
+  int64_t lddy, ldz, lddz, ldh;
+  uint32_t chunks;    // rows * row_chunks
+  int row_chunks, N, act;
+  FastDiv div;        // by row_chunks
+};
+constexpr int kAtOnce = 4;
+
+template <typename T, int GATED>
+__global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
+  constexpr int E = Elem<T>::kPerChunk, MODE = GATED ? kGatedBwd : kLinBwd;
+  with_activation(p.act, [&](auto act_c) {
+    constexpr int ACT = decltype(act_c)::value;
+    const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * kAtOnce);
+    for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * kAtOnce) + threadIdx.x; base < p.chunks; base += stride) {
+      Chunk dy[kAtOnce], zg[kAtOnce], zu[kAtOnce];
+      uint32_t row[kAtOnce], col[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const uint64_t q = base + 256 * i;
+        if (q >= p.chunks) break;
+        p.div.divmod(static_cast<uint32_t>(q), row[i], col[i]);
+        dy[i].u = load_streaming_u4(static_cast<const T*>(p.dy) + row[i] * p.lddy, col[i]);
+        zg[i].u = load_streaming_u4(static_cast<const T*>(p.z) + row[i] * p.ldz, col[i]);
+        if (GATED) zu[i].u = load_streaming_u4(static_cast<const T*>(p.z) + row[i] * p.ldz + p.N, col[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (base + 256 * i >= p.chunks) break;
+        float v[E], fg[E], fu[E], u[E], o[E], h[E];
+        chunk_to_float<T>(dy[i], v);
+        chunk_to_float<T>(zg[i], fg);
+        if (GATED) chunk_to_float<T>(zu[i], fu);
+        combine<T, MODE, ACT, E>(v, u, fg, fu, o, h);
+        T* dz = static_cast<T*>(p.dz) + row[i] * p.lddz;
+        reinterpret_cast<uint4*>(dz)[col[i]] = float_to_chunk<T>(o).u;
+        if (GATED) {
+          reinterpret_cast<uint4*>(dz + p.N)[col[i]] = float_to_chunk<T>(u).u;
+          if (p.h) reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row[i] * p.ldh)[col[i]] = float_to_chunk<T>(h).u;
+        }
+      }
+    }
+  });
+}
+
+// a tensor [M][width] with rows ld elements apart: aligned for 16-byte accesses, and within reach of a tile's 32-bit offsets
+bool rows_fit(const void* t, int64_t ld, int64_t width, int eb) {
+  return !t || (ld >= width && ld % (16 / eb) == 0 && (reinterpret_cast<uintptr_t>(t) & 15) == 0 && ld * eb < (1ll << 31) / 512);
+}
+
+int check_common(const char* what, int dtype, int64_t M, int64_t K, int64_t N, int act) {
+  const std::string name(what);
+  TCH_CHECK_ARG(dtype == kBF16 || dtype == kF32, name + ": dtype must be f32(0) or bf16(1)");
+  const int E = dtype == kBF16 ? 8 : 4;
+  TCH_CHECK_ARG(M >= 0 && M <= INT_MAX - 1024 && K > 0 && N > 0, name + ": bad shape");
+  TCH_CHECK_ARG(K % E == 0 && N % E == 0, name + ": the layer's sizes must be multiples of a 16-byte chunk");
+  TCH_CHECK_ARG(act >= 0 && act < kActCount, name + ": unknown activation");
+  return 0;
+}
+
+int linear_launch(Context* ctx, const char* what, int dtype, int mode, LinearArgs& a, int64_t M, int64_t K, int64_t N) {
+  const std::string name(what);
+  if (int rc = check_common(what, dtype, M, K, N, a.act)) return rc;
+  if (M == 0) return 0;
+  const int eb = dtype == kBF16 ? 2 : 4;
+  const int64_t wide = is_gated(mode) ? 2 : 1;
+  const int64_t weight_rows = mode == kGatedFwd ? 2 * N : N;
+  TCH_CHECK_ARG(a.a && a.b && a.out, name + ": null tensor");
+  TCH_CHECK_ARG(weight_rows * K * eb < (1ll << 31) && K * eb < (1ll << 31) / 512, name + ": the weights exceed the 2 GiB reach of a buffer offset");
+  TCH_CHECK_ARG((reinterpret_cast<uintptr_t>(a.b) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0,
+                name + ": weights and bias must start on a 16-byte boundary");
+  TCH_CHECK_ARG(rows_fit(a.a, a.lda, K, eb) && rows_fit(a.out, a.ldo, mode == kGatedBwd ? 2 * N : N, eb) && rows_fit(a.add, a.ldadd, N, eb) &&
+                    rows_fit(a.z, a.ldz, wide * N, eb) && rows_fit(a.out2, a.ldo2, mode == kGatedFwd ? 2 * N : N, eb),
+                name + ": rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
+  a.M = static_cast<int>(M);
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  a.b_bytes = static_cast<uint32_t>(weight_rows * K * eb);
+  return dtype == kBF16 ? launch_linear_bf16(ctx, mode, a) : launch_linear_f32(ctx, mode, a);
+}
+
+}  // namespace
+
+int linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows& y, const float* bias, int act, const Rows& residual,
+               const Rows& pre, int64_t M, int64_t K, int64_t N) {
+  LinearArgs a{};
+  a.a = x.ptr, a.lda = x.ld;
+  a.b = w;
+  a.bias = bias;
+  a.add = residual.ptr, a.ldadd = residual.ld;
+  a.out = y.ptr, a.ldo = y.ld;
+  a.out2 = pre.ptr, a.ldo2 = pre.ld;
+  a.act = act;
+  return linear_launch(ctx, "linear_fwd", dtype, kLinFwd, a, M, K, N);
+}
+
+int linear_dgrad(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& dx, int act, const Rows& pre, const Rows& residual,
+                 int64_t M, int64_t K, int64_t N) {
+  TCH_CHECK_ARG(act == kActNone || pre.ptr || M == 0, "linear_dgrad: an activation's derivative needs its pre-activations");
+  LinearArgs a{};
+  a.a = dy.ptr, a.lda = dy.ld;
+  a.b = wt;
+  a.add = residual.ptr, a.ldadd = residual.ld;
+  a.z = act == kActNone ? nullptr : pre.ptr, a.ldz = pre.ld;
+  a.out = dx.ptr, a.ldo = dx.ld;
+  a.act = act;
+  return linear_launch(ctx, "linear_dgrad", dtype, kLinBwd, a, M, K, N);
+}
+
+int gated_linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows& h, const float* bias, int act, const Rows& pre, int64_t M,
+                     int64_t K, int64_t F) {
+  LinearArgs a{};
+  a.a = x.ptr, a.lda = x.ld;
+  a.b = w;
+  a.bias = bias;
+  a.out = h.ptr, a.ldo = h.ld;
+  a.out2 = pre.ptr, a.ldo2 = pre.ld;
+  a.act = act;
+  return linear_launch(ctx, "gated_linear_fwd", dtype, kGatedFwd, a, M, K, F);
+}
+
+int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& pre, const Rows& dpre, const Rows& h, int act,
+                       int64_t M, int64_t K, int64_t F) {
+  TCH_CHECK_ARG(pre.ptr || M == 0, "linear_dgrad_gated: null tensor");
+  LinearArgs a{};
+  a.a = dy.ptr, a.lda = dy.ld;
+  a.b = wt;
+  a.z = pre.ptr, a.ldz = pre.ld;
+  a.out = dpre.ptr, a.ldo = dpre.ld;
+  a.out2 = h.ptr, a.ldo2 = h.ld;
+  a.act = act;
+  return linear_launch(ctx, "linear_dgrad_gated", dtype, kGatedBwd, a, M, K, F);
+}
+
+int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, const Rows& h, int gated, int act, int64_t M, int64_t N) {
+  if (int rc = check_common("act_bwd", dtype, M, 16, N, act)) return rc;
+  if (M == 0) return 0;
+  const int eb = dtype == kBF16 ? 2 : 4;
+  const int64_t wide = gated ? 2 : 1;
+  TCH_CHECK_ARG(dy.ptr && pre.ptr && dz.ptr, "act_bwd: null tensor");
+  TCH_CHECK_ARG(rows_fit(dy.ptr, dy.ld, N, eb) && rows_fit(pre.ptr, pre.ld, wide * N, eb) && rows_fit(dz.ptr, dz.ld, wide * N, eb) &&
+                    rows_fit(h.ptr, h.ld, N, eb),
+                "act_bwd: rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
+  const int row_chunks = static_cast<int>(N * eb / 16);
+  TCH_CHECK_ARG(M * row_chunks < (1ll << 31), "act_bwd: tensor exceeds 2^31 chunks");
+  ActBwdArgs a{dy.ptr, pre.ptr, dz.ptr, h.ptr, dy.ld, pre.ld, dz.ld, h.ld, static_cast<uint32_t>(M * row_chunks), row_chunks, static_cast<int>(N), act,
+               FastDiv(static_cast<uint32_t>(row_chunks))};
+  const int64_t groups = (M * row_chunks + 256 * kAtOnce - 1) / (256 * kAtOnce);
+  const dim3 grid(static_cast<unsigned>(groups < (1 << 20) ? groups : (1 << 20)));
+  const double bytes = static_cast<double>(M) * N * eb * (gated ? (h.ptr ? 6.0 : 5.0) : 3.0);
+  if (gated)
+    return dtype == kBF16 ? launch(ctx, act_bwd_kernel<bf16, 1>, grid, dim3(256), a, "act_bwd_kernel<bf16,gated>", bytes, 1)
+                          : launch(ctx, act_bwd_kernel<float, 1>, grid, dim3(256), a, "act_bwd_kernel<f32,gated>", bytes, 1);
+  return dtype == kBF16 ? launch(ctx, act_bwd_kernel<bf16, 0>, grid, dim3(256), a, "act_bwd_kernel<bf16>", bytes, 1)
+                        : launch(ctx, act_bwd_kernel<float, 0>, grid, dim3(256), a, "act_bwd_kernel<f32>", bytes, 1);
+}
+
+}  // namespace tch

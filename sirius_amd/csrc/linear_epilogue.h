@@ -1,0 +1,135 @@
+// Activations of the linear layers and what their kernels do with a product before it is stored.
+//
+//   kLinFwd    v = x W^T + b (kept in pre on request);         y  = act(v) + residual
+//   kLinBwd    v = dy W;                                       dx = v * act'(z) + residual
+//   kGatedFwd  g = x Wg^T + bg, u = x Wu^T + bu (pre = g | u); h  = act(g) * u
+//   kGatedBwd  v = dy W (the gradient of h), z = g | u;        dg = v * u * act'(g), du = v * act(g), h again on request
+//
+// Everything here is fp32: products arrive in fp32 and are rounded once, when they are stored.  The activation is taken of the
+// unrounded product, not of the rounded copy that is kept in pre: one rounding less in y.
+#pragma once
+
+#include "kernels.h"
+
+namespace tch {
+
+enum LinearMode : int { kLinFwd = 0, kLinBwd = 1, kGatedFwd = 2, kGatedBwd = 3 };
+enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActCount = 5 };
+
+constexpr bool is_gated(int mode) { return mode == kGatedFwd || mode == kGatedBwd; }
+
+// T decides how exactly: bf16 results are rounded to 2^-9 of their size, so the hardware's exponential and reciprocal (a few
+// 2^-23) and an error function to 1.5e-7 do; fp32 results take the library's.
+template <typename T>
+__device__ inline float fast_exp(float x) {
+  if constexpr (sizeof(T) == 2)
+    return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
+  else
+    return expf(x);
+}
+template <typename T>
+__device__ inline float reciprocal(float x) {
+  if constexpr (sizeof(T) == 2)
+    return __builtin_amdgcn_rcpf(x);
+  else
+    return 1.f / x;
+}
+template <typename T>
+__device__ inline float sigmoid(float x) {
+  return reciprocal<T>(1.f + fast_exp<T>(-x));   // x -> -inf: 1 / inf = 0
+}
+
+// The normal distribution's integral and density at z.  bf16: formula 7.1.26 of Abramowitz and Stegun for erfc(|z| / sqrt 2), whose
+// exponential is the density's as well.
+template <typename T>
+__device__ inline void normal_cdf(float z, float& cdf, float& density) {
+  if constexpr (sizeof(T) == 2) {
+    const float x = fabsf(z) * 0.7071067811865476f;
+    const float e = fast_exp<T>(-x * x);
+    const float t = reciprocal<T>(1.f + 0.3275911f * x);
+    const float half_erfc =
+        0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    cdf = z < 0.f ? half_erfc : 1.f - half_erfc;
+    density = 0.3989422804014327f * e;
+  } else {
+    cdf = 0.5f * erfcf(z * -0.7071067811865476f);
+    density = 0.3989422804014327f * expf(-0.5f * z * z);
+  }
+}
+
+constexpr float kTanhA = 1.5957691216057308f;             // 2 sqrt(2 / pi): gelu_tanh(z) = z sigmoid(z (A + B z^2))
+constexpr float kTanhB = 1.5957691216057308f * 0.044715f;
+
+template <typename T, int ACT>
+__device__ inline float act_value(float z) {
+  if constexpr (ACT == kActRelu) return z > 0.f || z != z ? z : 0.f;   // a NaN stays one
+  if constexpr (ACT == kActGelu) {
+    float cdf, density;
+    normal_cdf<T>(z, cdf, density);
+    return z * cdf;
+  }
+  if constexpr (ACT == kActGeluTanh) return z * sigmoid<T>(z * (kTanhA + kTanhB * z * z));
+  if constexpr (ACT == kActSilu) return z * sigmoid<T>(z);
+  return z;
+}
+
+// The slope at z, and the value where it is asked for.  A slope is 0 or 1 to the last bit of fp32 from |z| = 16 (GELU) or 104 (SiLU)
+// on; z is held to that range for it, so that z^2 does not overflow and an infinite z gives the limit and not 0 * inf.
+template <typename T, int ACT>
+__device__ inline float act_slope(float z, float* value = nullptr) {
+  if constexpr (ACT == kActNone) {
+    if (value) *value = z;
+    return 1.f;
+  } else if constexpr (ACT == kActRelu) {
+    if (value) *value = act_value<T, ACT>(z);
+    return z != z ? z : z > 0.f ? 1.f : 0.f;
+  } else {
+    constexpr float kFlat = ACT == kActSilu ? 104.f : 16.f;
+    const float c = z > kFlat ? kFlat : z < -kFlat ? -kFlat : z;   // comparisons, not min / max: a NaN stays one
+    if constexpr (ACT == kActGelu) {
+      float cdf, density;
+      normal_cdf<T>(c, cdf, density);
+      if (value) *value = z * cdf;
+      return cdf + c * density;
+    } else {
+      const float x = ACT == kActSilu ? c : c * (kTanhA + kTanhB * c * c);
+      const float e = fast_exp<T>(-x), s = reciprocal<T>(1.f + e);
+      if (value) *value = z * s;
+      const float rest = x > 0.f ? e * s : 1.f - s;   // 1 - s without cancellation
+      return s + c * s * rest * (ACT == kActSilu ? 1.f : kTanhA + 3.f * kTanhB * c * c);
+    }
+  }
+}
+
+// E neighbouring columns of one row: v (and u, gated forward) hold the products with their bias; zg, zu the kept pre-activations
+// (backward).  out: what is stored first; u: the up half's gradient (gated backward); h: the layer's output again (gated backward).
+template <typename T, int MODE, int ACT, int E>
+__device__ inline void combine(const float* v, float* u, const float* zg, const float* zu, float* out, float* h) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if constexpr (MODE == kLinFwd) out[e] = act_value<T, ACT>(v[e]);
+    if constexpr (MODE == kLinBwd) out[e] = ACT == kActNone ? v[e] : v[e] * act_slope<T, ACT>(zg[e]);
+    if constexpr (MODE == kGatedFwd) out[e] = act_value<T, ACT>(v[e]) * u[e];
+    if constexpr (MODE == kGatedBwd) {
+      float value;
+      const float slope = act_slope<T, ACT>(zg[e], &value);
+      out[e] = v[e] * (zu[e] * slope);
+      u[e] = v[e] * value;
+      h[e] = value * zu[e];
+    }
+  }
+}
+
+// fn with the activation as a constant
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& fn) {
+  switch (act) {
+    case kActRelu: fn(std::integral_constant<int, kActRelu>{}); break;
+    case kActGelu: fn(std::integral_constant<int, kActGelu>{}); break;
+    case kActGeluTanh: fn(std::integral_constant<int, kActGeluTanh>{}); break;
+    case kActSilu: fn(std::integral_constant<int, kActSilu>{}); break;
+    default: fn(std::integral_constant<int, kActNone>{}); break;
+  }
+}
+
+}  // namespace tch

@@ -1,0 +1,843 @@
+// Device code of the linear layers: a product of two row-major operands, out(m, n) = sum_k A(m, k) B(n, k), with everything a
+// feed-forward layer does to it in the epilogue (linear_epilogue.h).  A has its own row stride, B (the weights) is dense.
+// Compiled once per element type (linear_bf16.hip, linear_f32.hip).
+//
+// Gated modes multiply both projections in one tile: 32 (or 16) rows of the gate's weights lie next to the same rows of the up
+// projection's, so that a lane ends up with both products of its columns and the epilogue needs nobody else's.
+#pragma once
+
+#include "direct_load.h"
+#include "fp32_split.h"
+#include "linear_epilogue.h"
+
+namespace tch {
+
+struct LinearArgs {
+  const void* a;      // [M][K], row stride lda (elements)
+  const void* b;      // [N][K] dense; gated forward: [2N][K], gate rows first
+  const float* bias;  // forward: [N] or [2N], may be null
+  const void* add;    // residual, laid out by ldadd; may be null
+  const void* z;      // backward: pre-activations [M][N] or [M][2N]
+  void* out;          // [M][N]; gated backward: [M][2N]
+  void* out2;         // forward: pre (may be null); gated backward: h (may be null)
+  int64_t lda, ldadd, ldz, ldo, ldo2;
+  int M, N, K, act;
+  uint32_t b_bytes;
+  int tiles_m, tiles_n, group_rows;
+  FastDiv div_tiles_n, div_group, div_rows;
+};
+
+namespace {
+
+// What a tile's epilogue reads and writes beside the accumulators: buffer resources that begin at the tile's first row and end
+// behind its last existing one, so that a row beyond M is dropped by its offset and 64-bit offsets stay out of the lanes.
+struct TileTensors {
+  __amdgpu_buffer_rsrc_t add, z, out, out2;
+};
+template <typename T>
+__device__ inline __amdgpu_buffer_rsrc_t rows_from(const void* base, int64_t ld, int row0, int rows, int width) {
+  const int64_t bytes = rows > 0 && base ? ((rows - 1) * ld + width) * static_cast<int64_t>(sizeof(T)) : 0;
+  return make_rsrc(base ? static_cast<const T*>(base) + row0 * ld : nullptr, static_cast<uint32_t>(bytes));
+}
+template <typename T, int MODE>
+__device__ inline TileTensors tile_tensors(const LinearArgs& p, int m0, int rows) {
+  constexpr int kWide = is_gated(MODE) ? 2 : 1;
+  TileTensors t;
+  t.add = rows_from<T>(p.add, p.ldadd, m0, rows, p.N);
+  t.z = rows_from<T>(p.z, p.ldz, m0, rows, kWide * p.N);
+  t.out = rows_from<T>(p.out, p.ldo, m0, rows, MODE == kGatedBwd ? 2 * p.N : p.N);
+  t.out2 = rows_from<T>(p.out2, p.ldo2, m0, rows, MODE == kGatedFwd ? 2 * p.N : p.N);
+  return t;
+}
+
+template <typename T>
+__device__ inline int at(int row, int64_t ld, int col, bool ok) {   // byte offset of a chunk in a tile's tensor
+  return ok ? (row * static_cast<int>(ld) + col) * static_cast<int>(sizeof(T)) : static_cast<int>(kOutOfRange);
+}
+__device__ inline Chunk read_chunk(__amdgpu_buffer_rsrc_t rsrc, int off) {
+  const uint4_t v = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0);
+  Chunk c;
+  c.w[0] = v[0];
+  c.w[1] = v[1];
+  c.w[2] = v[2];
+  c.w[3] = v[3];
+  return c;
+}
+template <typename T>
+__device__ inline void write_chunk(__amdgpu_buffer_rsrc_t rsrc, int off, const float* v) {
+  const Chunk c = float_to_chunk<T>(v);
+  const uint4_t w = {c.w[0], c.w[1], c.w[2], c.w[3]};
+  __builtin_amdgcn_raw_buffer_store_b128(w, rsrc, off, 0, 0);
+}
+
+// One 16-byte chunk of the output (E columns of a row) in two steps: what it reads, and the rest.
+template <typename T, int MODE>
+struct ChunkOperands {
+  Chunk zg, zu, add;
+  __device__ inline void request(const LinearArgs& p, const TileTensors& t, int row, int col) {
+    const bool ok = col < p.N;
+    if constexpr (MODE == kLinBwd || MODE == kGatedBwd) {
+      if (MODE == kGatedBwd || p.act != kActNone) zg = read_chunk(t.z, at<T>(row, p.ldz, col, ok));
+      if constexpr (MODE == kGatedBwd) zu = read_chunk(t.z, at<T>(row, p.ldz, p.N + col, ok));
+    }
+    if constexpr (!is_gated(MODE))
+      if (p.add) add = read_chunk(t.add, at<T>(row, p.ldadd, col, ok));
+  }
+  template <int ACT>
+  __device__ inline void finish(const LinearArgs& p, const TileTensors& t, int row, int col, const float* v, float* u) {
+    constexpr int E = Elem<T>::kPerChunk;
+    const bool ok = col < p.N;
+    float fg[E], fu[E], o[E], h[E];
+    if constexpr (MODE == kLinBwd || MODE == kGatedBwd) chunk_to_float<T>(zg, fg);
+    if constexpr (MODE == kGatedBwd) chunk_to_float<T>(zu, fu);
+    if constexpr (MODE == kLinFwd || MODE == kGatedFwd) {
+      if (p.out2) {
+        write_chunk<T>(t.out2, at<T>(row, p.ldo2, col, ok), v);
+        if constexpr (MODE == kGatedFwd) write_chunk<T>(t.out2, at<T>(row, p.ldo2, p.N + col, ok), u);
+      }
+    }
+    combine<T, MODE, ACT, E>(v, u, fg, fu, o, h);
+    if constexpr (!is_gated(MODE)) {
+      if (p.add) {
+        float r[E];
+        chunk_to_float<T>(add, r);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += r[e];
+      }
+    }
+    write_chunk<T>(t.out, at<T>(row, p.ldo, col, ok), o);
+    if constexpr (MODE == kGatedBwd) {
+      write_chunk<T>(t.out, at<T>(row, p.ldo, p.N + col, ok), u);
+      if (p.out2) write_chunk<T>(t.out2, at<T>(row, p.ldo2, col, ok), h);
+    }
+  }
+};
+
+template <typename T>
+__device__ inline void mma32(const uint4_t& first, const uint4_t& second, f32x16_t& acc) {
+  if constexpr (sizeof(T) == 2) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, first), __builtin_bit_cast(bf16x8_t, second), acc, 0, 0, 0);
+  } else {
+    // a lane holds four neighbouring reduction elements: instruction e multiplies element e of both halves of the lanes
+    const f32x4_t x = __builtin_bit_cast(f32x4_t, first), y = __builtin_bit_cast(f32x4_t, second);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], acc, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// large products: a persistent grid whose workgroups walk output tiles as one sequence of reduction steps
+// ---------------------------------------------------------------------------
+// WM x WN wavefronts of TM x TN MFMA tiles (32 x 32).  Operand tiles go from global memory straight into LDS (16 bytes a lane,
+// rows of RB bytes, the 16-byte slot XOR-ed by the row so that an operand read touches every bank once), NBUF of them; the
+// slice of 32 bytes that is multiplied next is read while this one is multiplied, and the direct loads of the tile NBUF - 1
+// steps ahead go out between the multiplies.  The tiles of a workgroup are one sequence: the next tile's first loads are on
+// their way during this tile's last steps and its epilogue.  A row of the operands that does not exist is outside its buffer
+// resource and lands as zeros; a chunk behind K is turned away by its lane's offset in the last step of a tile.
+template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int RB, int PER_CU>
+__global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_kernel(LinearArgs p) {
+  constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T);
+  constexpr int KS = RB / EB, SL = RB / 32, SLOTS = RB / 16, LD_ROWS = 1024 / RB;
+  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, NW = WM * WN;
+  constexpr bool GATED_FWD = MODE == kGatedFwd;
+  constexpr int BN_OUT = GATED_FWD ? BN / 2 : BN;
+  static_assert(!GATED_FWD || TN % 2 == 0, "gate and up tiles come in pairs");
+  static_assert((RB == 128 || RB == 64) && BM % (LD_ROWS * NW) == 0 && BN % (LD_ROWS * NW) == 0, "tile/loader mismatch");
+  constexpr int A_LD = BM / LD_ROWS / NW, B_LD = BN / LD_ROWS / NW, LOADS = A_LD + B_LD;
+  constexpr int A_BYTES = BM * RB, BUF_BYTES = A_BYTES + BN * RB;
+  // with two buffers the requested tile is waited for at the end of the step: all requests go out in its first half
+  constexpr int LOAD_SL = NBUF == 2 ? (SL + 1) / 2 : SL;
+  constexpr int AHEAD = (NBUF - 2) * LOADS;
+  static_assert(AHEAD < 48, "vmcnt range");
+  constexpr bool BIAS = MODE == kLinFwd || MODE == kGatedFwd;
+  // the bias of a wavefront's columns travels with the operands, requested with the first step of a tile
+  constexpr int BIAS_BYTES = TN * 32 * 4, BIAS_OFF = NBUF * BUF_BYTES;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[BIAS_OFF + (BIAS ? NW * (NBUF + 1) * BIAS_BYTES : 0)];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int frag_row = lane & 31, frag_half = lane >> 5;
+  const int nk = (p.K + KS - 1) / KS;
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int first = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x));
+  auto swizzle = [](int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
+
+  // consecutive tiles walk down group_rows row tiles before they move one column tile on: the tiles an XCD works on at one time
+  // form a block, with fewer distinct operand rows through its L2
+  auto locate = [&](int id, int& m0, int& n0) {
+    uint32_t q, rem;
+    if (p.group_rows <= 1) {
+      p.div_tiles_n.divmod(static_cast<uint32_t>(id), q, rem);
+      m0 = static_cast<int>(q) * BM;
+      n0 = static_cast<int>(rem) * BN_OUT;
+      return;
+    }
+    p.div_group.divmod(static_cast<uint32_t>(id), q, rem);
+    const uint32_t row0 = q * p.group_rows, rows = min(static_cast<uint32_t>(p.group_rows), static_cast<uint32_t>(p.tiles_m) - row0);
+    const uint32_t col = rows == static_cast<uint32_t>(p.group_rows) ? p.div_rows.div(rem) : rem / rows;
+    m0 = static_cast<int>(row0 + (rem - col * rows)) * BM;
+    n0 = static_cast<int>(col) * BN_OUT;
+  };
+
+  // ---- the walk of the loads: offsets are the same for every tile, the resources move ----
+  const int sub_row = lane / SLOTS, slot = lane % SLOTS;
+  uint32_t a_off[A_LD], b_off[B_LD];
+  uint32_t behind_k[2] = {0u, 0u};   // the lane's chunk of an even / odd direct load lies behind K in the last step
+#pragma unroll
+  for (int j = 0; j < A_LD; ++j) {
+    const int trow = (wave * A_LD + j) * LD_ROWS + sub_row;
+    a_off[j] = (static_cast<uint32_t>(trow) * static_cast<uint32_t>(p.lda) + (slot ^ swizzle(trow)) * E) * EB;
+  }
+#pragma unroll
+  for (int j = 0; j < B_LD; ++j) {
+    const int trow = (wave * B_LD + j) * LD_ROWS + sub_row;
+    const int block = trow >> 5;
+    const uint32_t row = GATED_FWD ? static_cast<uint32_t>((block & 1) * p.N + (block >> 1) * 32 + (trow & 31)) : static_cast<uint32_t>(trow);
+    b_off[j] = (row * static_cast<uint32_t>(p.K) + (slot ^ swizzle(trow)) * E) * EB;
+  }
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd)
+    behind_k[odd] = (nk - 1) * KS + (slot ^ swizzle(odd * LD_ROWS + sub_row)) * E >= p.K ? kOutOfRange : 0u;
+  const bool ragged_k = p.K % KS != 0;
+
+  __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
+  const __amdgpu_buffer_rsrc_t rsrc_bias = make_rsrc(p.bias, BIAS && p.bias ? static_cast<uint32_t>(p.N) * (GATED_FWD ? 8u : 4u) : 0u);
+  int ld_id = first, ld_kt = 0, ld_bias = 0;
+  auto mark_tail = [&] {
+#pragma unroll
+    for (int j = 0; j < A_LD; ++j) a_off[j] |= behind_k[(wave * A_LD + j) & 1];
+#pragma unroll
+    for (int j = 0; j < B_LD; ++j) b_off[j] |= behind_k[(wave * B_LD + j) & 1];
+  };
+  auto enter_tile = [&] {
+    int m0 = 0, n0 = 0;
+    const bool any = ld_id < tiles;
+    if (any) locate(ld_id, m0, n0);
+    const int rows = min(BM, p.M - m0);
+    rsrc_a = make_rsrc(static_cast<const T*>(p.a) + m0 * p.lda, static_cast<uint32_t>(((rows - 1) * p.lda + p.K) * EB));
+    const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
+    rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
+    if constexpr (BIAS) {
+      if (p.bias) {
+        unsigned char* dst = lds + BIAS_OFF + (wave * (NBUF + 1) + ld_bias) * BIAS_BYTES;
+        const int block = wn * TN + (lane >> 3);
+        const int col = n0 + (GATED_FWD ? (block >> 1) * 32 : block * 32) + (lane & 7) * 4;
+        const int at_col = GATED_FWD && (block & 1) ? p.N + col : col;
+        if (lane < TN * 8) load_to_lds(rsrc_bias, dst, any && col < p.N ? at_col * 4 : static_cast<int>(kOutOfRange), 0);
+        ld_bias = ld_bias == NBUF ? 0 : ld_bias + 1;
+      }
+    }
+    if (ragged_k || !any) {   // behind the last tile every offset is out of range: zeros land
+      const uint32_t set = any ? 0u : kOutOfRange;
+#pragma unroll
+      for (int j = 0; j < A_LD; ++j) a_off[j] = (a_off[j] & ~kOutOfRange) | set;
+#pragma unroll
+      for (int j = 0; j < B_LD; ++j) b_off[j] = (b_off[j] & ~kOutOfRange) | set;
+      if (ragged_k && nk == 1) mark_tail();
+    }
+  };
+  auto issue_load = [&](uint32_t buf, int j) {   // direct load j of the step the walk stands at
+    if (j < A_LD)
+      load_to_lds(rsrc_a, lds + buf + (wave * A_LD + j) * 1024, static_cast<int>(a_off[j]), ld_kt * RB);
+    else
+      load_to_lds(rsrc_b, lds + buf + A_BYTES + (wave * B_LD + j - A_LD) * 1024, static_cast<int>(b_off[j - A_LD]), ld_kt * RB);
+  };
+  auto next_step = [&] {
+    if (++ld_kt == nk) {
+      ld_kt = 0;
+      ld_id += gridDim.x;
+      enter_tile();
+    } else if (ragged_k && ld_kt == nk - 1) {
+      mark_tail();
+    }
+  };
+
+  f32x16_t acc[TM][TN];
+  clear(acc);
+  const int swz = swizzle(frag_row);
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  const uint32_t a_rd = lds_base + (wm * TM * 32 + frag_row) * RB + swz * 16;
+  const uint32_t b_rd = lds_base + A_BYTES + (wn * TN * 32 + frag_row) * RB + swz * 16;
+  uint4_t fa[2][TM], fb[2][TN];
+  // The operand reads are asm: the compiler would put a wait for every direct load in flight in front of an LDS read it can see.
+  auto read_one = [&](uint32_t pa, uint32_t pb, int set, int i) {
+    if (i < TM)
+      asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(fa[set][i]) : "v"(pa), "n"(i * 32 * RB));
+    else
+      asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(fb[set][i - TM]) : "v"(pb), "n"((i - TM) * 32 * RB));
+  };
+  auto hold_set = [&](int set) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) asm volatile("" : "+v"(fa[set][i]));
+#pragma unroll
+    for (int i = 0; i < TN; ++i) asm volatile("" : "+v"(fb[set][i]));
+  };
+  // multiplies the slice in `set`; meanwhile slice kk of the step in `buf` is read into the other set and part `q` of the loads
+  // goes to `ld_buf`
+  auto slice = [&](auto set_c, uint32_t buf, auto kk_c, auto q_c, uint32_t ld_buf) {
+    constexpr int set = decltype(set_c)::value, kk = decltype(kk_c)::value, q = decltype(q_c)::value;
+    constexpr int READS = TM + TN, MF = TM * TN, FIRST = (q < LOAD_SL ? q : LOAD_SL) * LOADS / LOAD_SL;
+    constexpr int AUX = READS + (q < LOAD_SL ? (q + 1) * LOADS / LOAD_SL - FIRST : 0);
+    constexpr int PER = (AUX + MF - 1) / MF > 2 ? (AUX + MF - 1) / MF : 2;
+    const uint32_t pa = (a_rd ^ static_cast<uint32_t>((2 * kk + frag_half) * 16)) + buf;
+    const uint32_t pb = (b_rd ^ static_cast<uint32_t>((2 * kk + frag_half) * 16)) + buf;
+    unrolled<MF>([&](auto m_c) {
+      constexpr int m = decltype(m_c)::value, tm = m / TN, tn = m % TN;
+      mma32<T>(fb[set][tn], fa[set][tm], acc[tm][tn]);
+      unrolled<PER>([&](auto a_c) {
+        constexpr int a = m * PER + decltype(a_c)::value;
+        if constexpr (a < READS) read_one(pa, pb, set ^ 1, a);
+        else if constexpr (a < AUX) issue_load(ld_buf, FIRST + a - READS);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    hold_set(set ^ 1);
+  };
+
+  // ---- the output: a lane's accumulators are four neighbouring columns of one row at a time; lanes 32 apart exchange every second
+  // group, so that each has eight neighbouring columns (16 bytes of bf16) to read, combine and store ----
+  int bias_at = 0;
+  auto epilogue = [&](int id) {
+    int m0, n0;
+    locate(id, m0, n0);
+    const TileTensors t = tile_tensors<T, MODE>(p, m0, min(BM, p.M - m0));
+    constexpr int PARTS = 8 / E;                          // chunks of eight columns: 1 in bf16, 2 in fp32
+    constexpr int PAIRS = GATED_FWD ? TN / 2 : TN;        // groups of 32 output columns of a wavefront
+    ChunkOperands<T, MODE> operands[2][TM * PARTS];       // of sixteen columns, requested that much ahead
+    auto col_of = [&](int pair, int jp) { return n0 + (wn * PAIRS + pair) * 32 + 16 * jp + 8 * frag_half; };
+    auto row_of = [&](int tm) { return (wm * TM + tm) * 32 + frag_row; };
+    auto request = [&](int step) {
+      if constexpr (MODE != kGatedFwd) {
+        int col = col_of(step >> 1, step & 1);
+        asm volatile("" : "+v"(col));   // offsets are made where they are used, not all of them ahead of the first
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+          for (int h = 0; h < PARTS; ++h) operands[step & 1][tm * PARTS + h].request(p, t, row_of(tm), col + h * E);
+      }
+    };
+    // eight neighbouring columns (16 jp + 8 half ..) out of an accumulator, which is left empty
+    auto eight = [&](f32x16_t& c, int jp, float* v) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[8 * jp + i]), __float_as_uint(c[8 * jp + 4 + i]), false, false);
+        v[i] = __uint_as_float(x[0]);
+        v[4 + i] = __uint_as_float(x[1]);
+        c[8 * jp + i] = 0.f;
+        c[8 * jp + 4 + i] = 0.f;
+      }
+    };
+    auto add_bias = [&](int tn, int jp, float* v) {
+      if constexpr (BIAS) {
+        uint4_t b0, b1;
+        const uint32_t from = lds_base + BIAS_OFF + (wave * (NBUF + 1) + bias_at) * BIAS_BYTES + tn * 128 + jp * 64 + frag_half * 32;
+        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:16\n\ts_waitcnt lgkmcnt(0)" : "=&v"(b0), "=&v"(b1) : "v"(from) : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = __uint_as_float(b0[i]);
+          v[4 + i] = __uint_as_float(b1[i]);
+        }
+      }
+    };
+    with_activation(p.act, [&](auto act_c) {
+      constexpr int ACT = decltype(act_c)::value;
+      request(0);
+#pragma unroll
+      for (int pair = 0; pair < PAIRS; ++pair) {
+#pragma unroll
+        for (int jp = 0; jp < 2; ++jp) {
+          if (2 * pair + jp + 1 < 2 * PAIRS) request(2 * pair + jp + 1);
+          const int tn = GATED_FWD ? 2 * pair : pair;
+          int col = col_of(pair, jp);
+          asm volatile("" : "+v"(col));
+          float bv[8], bu[8];
+          if (BIAS && p.bias) {
+            add_bias(tn, jp, bv);
+            if constexpr (GATED_FWD) add_bias(tn + 1, jp, bu);
+          }
+#pragma unroll
+          for (int tm = 0; tm < TM; ++tm) {
+            float v[8], u[8];
+            eight(acc[tm][tn], jp, v);
+            if constexpr (GATED_FWD) eight(acc[tm][tn + 1], jp, u);
+            if (BIAS && p.bias) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                v[i] += bv[i];
+                if constexpr (GATED_FWD) u[i] += bu[i];
+              }
+            }
+#pragma unroll
+            for (int h = 0; h < PARTS; ++h)
+              operands[jp][tm * PARTS + h].template finish<ACT>(p, t, row_of(tm), col + h * E, v + h * E, u + h * E);
+            __builtin_amdgcn_sched_barrier(0);   // one chunk at a time: the registers are the accumulators'
+          }
+        }
+      }
+    });
+    bias_at = bias_at == NBUF ? 0 : bias_at + 1;
+  };
+
+  // Behind an epilogue its stores (this many at least; one that is turned away counts too) are newer requests than the tile that
+  // has to land, with three buffers or more: with two, that tile is requested behind them.
+  constexpr int STORES = TM * (GATED_FWD ? TN / 2 : TN) * 2 * (8 / E) * (MODE == kGatedBwd ? 2 : 1);
+  constexpr int AFTER_STORES = NBUF == 2 ? 0 : AHEAD + STORES < 63 ? AHEAD + STORES : 63;
+  enter_tile();
+#pragma unroll
+  for (int s = 0; s < NBUF - 1; ++s) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) issue_load(s * BUF_BYTES, j);
+    next_step();
+  }
+#pragma unroll
+  for (int j = 0; j < LOADS / LOAD_SL; ++j) issue_load((NBUF - 1) * BUF_BYTES, j);
+  wait_and_meet<AHEAD + LOADS / LOAD_SL>();
+#pragma unroll
+  for (int i = 0; i < TM + TN; ++i) read_one(a_rd ^ static_cast<uint32_t>(frag_half * 16), b_rd ^ static_cast<uint32_t>(frag_half * 16), 0, i);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  hold_set(0);
+  uint32_t buf = 0, before = (NBUF - 1) * BUF_BYTES;
+  bool stored = false;
+  for (int id = first; id < tiles; id += gridDim.x) {
+    for (int kt = 0; kt < nk; ++kt) {
+      unrolled<SL - 1>([&](auto s_c) {
+        constexpr int s = decltype(s_c)::value;
+        slice(std::integral_constant<int, (s & 1)>{}, buf, std::integral_constant<int, s + 1>{}, std::integral_constant<int, s + 1>{}, before);
+      });
+      next_step();
+      if (stored && kt == 0)
+        wait_and_meet<AFTER_STORES>();
+      else
+        wait_and_meet<AHEAD>();
+      before = buf;
+      buf = buf == (NBUF - 1) * BUF_BYTES ? 0 : buf + BUF_BYTES;
+      slice(std::integral_constant<int, ((SL - 1) & 1)>{}, buf, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, before);
+    }
+    epilogue(id);
+    stored = true;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the zeros behind the last tile land before the LDS goes
+}
+
+// ---------------------------------------------------------------------------
+// few tiles: every wavefront of a workgroup has the whole tile for every KG-th reduction step
+// ---------------------------------------------------------------------------
+// Each wavefront has a ring of NBUF operand tiles (64-byte rows) of its own, filled with direct loads, and waits for its own loads
+// only: no barrier before the partial tiles meet in LDS, where they are added in the order of the wavefronts.  What that buys
+// where workgroups are few: KG * (NBUF - 1) operand tiles in flight per compute unit and a chain of nk / KG steps instead of nk.
+template <typename T, int MODE, int TM, int TN, int KG, int NBUF>
+__global__ __launch_bounds__(KG * 64, KG / 4) void linear_split_kernel(LinearArgs p) {
+  constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), RB = 64, KS = RB / EB;
+  constexpr bool GATED_FWD = MODE == kGatedFwd;
+  constexpr int BM = TM * 32, BN = TN * 32, BN_OUT = GATED_FWD ? BN / 2 : BN;
+  static_assert(!GATED_FWD || TN % 2 == 0, "gate and up tiles come in pairs");
+  constexpr int A_LD = BM / 16, B_LD = BN / 16, A_BYTES = BM * RB, BUF_BYTES = (BM + BN) * RB;
+  constexpr int NT = KG * 64, LD = BN + 4;
+  constexpr int RED_BYTES = KG * BM * LD * 4, RING_BYTES = KG * NBUF * BUF_BYTES;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[RED_BYTES > RING_BYTES ? RED_BYTES : RING_BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // consecutive tiles (one XCD) share the rows of the larger operand: group_rows != 0: walk down the row tiles of a column tile
+  uint32_t slow, fast;
+  p.div_tiles_n.divmod(xcd_remap(blockIdx.x, gridDim.x), slow, fast);
+  const int m0 = static_cast<int>(p.group_rows ? fast : slow) * BM, n0 = static_cast<int>(p.group_rows ? slow : fast) * BN_OUT;
+  const int rows = min(BM, p.M - m0);
+  const int nk = (p.K + KS - 1) / KS;
+  const int my_steps = nk > wave ? (nk - wave + KG - 1) / KG : 0;
+
+  const int sub_row = lane >> 2, slot = lane & 3;
+  const int chunk = slot ^ ((sub_row >> 2) & 3);
+  uint32_t a_off[A_LD], b_off[B_LD];
+#pragma unroll
+  for (int j = 0; j < A_LD; ++j) a_off[j] = (static_cast<uint32_t>(j * 16 + sub_row) * static_cast<uint32_t>(p.lda) + chunk * E) * EB;
+#pragma unroll
+  for (int j = 0; j < B_LD; ++j) {
+    const int trow = j * 16 + sub_row, block = trow >> 5;
+    const uint32_t row = GATED_FWD ? static_cast<uint32_t>((block & 1) * p.N + (block >> 1) * 32 + (trow & 31)) : static_cast<uint32_t>(trow);
+    b_off[j] = (row * static_cast<uint32_t>(p.K) + chunk * E) * EB;
+  }
+  const __amdgpu_buffer_rsrc_t rsrc_a =
+      make_rsrc(static_cast<const T*>(p.a) + m0 * p.lda, static_cast<uint32_t>(((rows - 1) * p.lda + p.K) * EB));
+  const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
+  const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
+
+  unsigned char* ring = lds + wave * (NBUF * BUF_BYTES);
+  int ld_kt = wave;
+  auto issue_loads = [&](int buf) {
+    const uint32_t behind = ld_kt * KS + chunk * E >= p.K ? kOutOfRange : 0u;   // the chunk lies behind K
+    unsigned char* dst = ring + buf * BUF_BYTES;
+#pragma unroll
+    for (int j = 0; j < A_LD; ++j) load_to_lds(rsrc_a, dst + j * 1024, static_cast<int>(a_off[j] | behind), ld_kt * RB);
+#pragma unroll
+    for (int j = 0; j < B_LD; ++j) load_to_lds(rsrc_b, dst + A_BYTES + j * 1024, static_cast<int>(b_off[j] | behind), ld_kt * RB);
+    ld_kt += KG;
+  };
+
+  f32x16_t acc[TM][TN];
+  clear(acc);
+  const int frag_row = lane & 31, frag_half = lane >> 5;
+  const uint32_t rd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring)) + frag_row * RB + ((frag_row >> 2) & 3) * 16;
+  auto read_frags = [&](int buf, int kk, uint4_t* fa, uint4_t* fb) {
+    const uint32_t pa = (rd ^ static_cast<uint32_t>((2 * kk + frag_half) * 16)) + buf * BUF_BYTES;
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(fa[tm]) : "v"(pa), "n"(tm * 32 * RB));
+#pragma unroll
+    for (int tn = 0; tn < TN; ++tn) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(fb[tn]) : "v"(pa), "n"(A_BYTES + tn * 32 * RB));
+  };
+  auto multiply = [&](uint4_t* fa, uint4_t* fb) {
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) asm volatile("" : "+v"(fa[tm]));
+#pragma unroll
+    for (int tn = 0; tn < TN; ++tn) asm volatile("" : "+v"(fb[tn]));
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn) mma32<T>(fb[tn], fa[tm], acc[tm][tn]);
+  };
+  // The tile of step i has landed when at most the NBUF - 2 requested behind it are outstanding (near the end fewer follow: wait
+  // for everything).  The reads of step i - 1 were waited for before its multiplies, so its buffer is free.
+  constexpr int AHEAD = (NBUF - 2) * (A_LD + B_LD);
+  static_assert(AHEAD < 64, "vmcnt range");
+  auto step = [&](int i, int buf) {
+    if (i + NBUF - 1 <= my_steps)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (i + NBUF - 1 < my_steps) issue_loads((buf + NBUF - 1) % NBUF);
+    uint4_t fa0[TM], fb0[TN], fa1[TM], fb1[TN];
+    read_frags(buf, 0, fa0, fb0);
+    read_frags(buf, 1, fa1, fb1);
+    asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(TM + TN) : "memory");
+    multiply(fa0, fb0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    multiply(fa1, fb1);
+  };
+#pragma unroll
+  for (int i = 0; i < NBUF - 1; ++i)
+    if (i < my_steps) issue_loads(i);
+  int i0 = 0;
+  for (; i0 + NBUF <= my_steps; i0 += NBUF) {
+#pragma unroll
+    for (int u = 0; u < NBUF; ++u) step(i0 + u, u);
+  }
+#pragma unroll
+  for (int u = 0; u < NBUF - 1; ++u)
+    if (i0 + u < my_steps) step(i0 + u, u);
+
+  // ---- the partial tiles meet: [wave][BM][LD] fp32, over the rings ----
+  float* red = reinterpret_cast<float*>(lds);
+  const TileTensors t = tile_tensors<T, MODE>(p, m0, rows);
+  constexpr int CH = BN_OUT / E, ITEMS = BM * CH, VISITS = (ITEMS + NT - 1) / NT;
+  ChunkOperands<T, MODE> operands[VISITS];
+#pragma unroll
+  for (int visit = 0; visit < VISITS; ++visit) {
+    const int q = tid + visit * NT;
+    operands[visit].request(p, t, q / CH, q < ITEMS ? n0 + q % CH * E : p.N);
+  }
+  __syncthreads();   // every wavefront is done with its ring
+#pragma unroll
+  for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+    for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(red + wave * (BM * LD) + (tm * 32 + frag_row) * LD + tn * 32 + 8 * j + 4 * frag_half) =
+            make_float4(acc[tm][tn][4 * j], acc[tm][tn][4 * j + 1], acc[tm][tn][4 * j + 2], acc[tm][tn][4 * j + 3]);
+  __syncthreads();
+  auto total = [&](int row, int col, float* v) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll
+    for (int g = 0; g < KG; ++g)
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(red + (g * BM + row) * LD + col + e);
+        v[e] += s.x;
+        v[e + 1] += s.y;
+        v[e + 2] += s.z;
+        v[e + 3] += s.w;
+      }
+  };
+  auto add_bias = [&](int col, float* v) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 b = *reinterpret_cast<const float4*>(p.bias + col + e);
+      v[e] += b.x;
+      v[e + 1] += b.y;
+      v[e + 2] += b.z;
+      v[e + 3] += b.w;
+    }
+  };
+  with_activation(p.act, [&](auto act_c) {
+    constexpr int ACT = decltype(act_c)::value;
+#pragma unroll
+    for (int visit = 0; visit < VISITS; ++visit) {
+      const int q = tid + visit * NT;
+      const int row = q / CH, c = q % CH * E;
+      if (q >= ITEMS || n0 + c >= p.N) continue;
+      float v[E], u[E];
+      if constexpr (GATED_FWD) {
+        total(row, (c >> 5) * 64 + (c & 31), v);
+        total(row, (c >> 5) * 64 + 32 + (c & 31), u);
+      } else {
+        total(row, c, v);
+      }
+      if constexpr (MODE == kLinFwd || MODE == kGatedFwd) {
+        if (p.bias) {
+          add_bias(n0 + c, v);
+          if constexpr (GATED_FWD) add_bias(p.N + n0 + c, u);
+        }
+      }
+      operands[visit].template finish<ACT>(p, t, row, n0 + c, v, u);
+    }
+  });
+}
+
+// ---------------------------------------------------------------------------
+// up to 16 rows (tokens that decode together): the weights are read once, straight into registers
+// ---------------------------------------------------------------------------
+// A workgroup has 16 TN output columns; its KG wavefronts take 256-byte pieces of the reduction in turn.  Weight rows are the rows
+// and the tokens the columns of 16 x 16 MFMA tiles; lane l holds the 16-byte chunk l / 16 (of four) of row l % 16, so that a
+// load covers 64 neighbouring bytes of sixteen rows.  The next piece is requested before this one is multiplied.  Bound by the
+// bytes of the weights.
+template <typename T>
+__device__ inline void mma16(const uint4_t& first, const uint4_t& second, f32x4_t& acc) {
+  if constexpr (sizeof(T) == 2) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, first), __builtin_bit_cast(bf16x8_t, second), acc, 0, 0, 0);
+  } else {
+    const f32x4_t x = __builtin_bit_cast(f32x4_t, first), y = __builtin_bit_cast(f32x4_t, second);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
+  }
+}
+
+template <typename T>
+__device__ inline void load_four(const T* p, float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = Elem<T>::load(p + e);
+}
+template <typename T>
+__device__ inline void store_four(T* p, const float* v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) Elem<T>::store(p + e, v[e]);
+}
+
+template <typename T, int MODE, int TN, int KG>
+__global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
+  constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T);
+  constexpr bool GATED_FWD = MODE == kGatedFwd;
+  constexpr int W = GATED_FWD ? 2 * TN : TN;   // weight tiles of 16 rows: gate and up next to each other
+  constexpr int U = 4, PIECE = U * 4 * E;      // loads per piece and tile; elements of a piece
+  __shared__ float red[KG][W][16 * 20];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x)) * (16 * TN);
+  const int pieces = (p.K + PIECE - 1) / PIECE;
+  const int row16 = lane & 15, quarter = lane >> 4;
+
+  const __amdgpu_buffer_rsrc_t rsrc_a = rows_from<T>(p.a, p.lda, 0, p.M, p.K);
+  const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
+  const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
+  const uint32_t a_off = (static_cast<uint32_t>(row16) * static_cast<uint32_t>(p.lda) + quarter * E) * EB;
+  uint32_t b_off[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const uint32_t row = GATED_FWD ? static_cast<uint32_t>((w & 1) * p.N + (w >> 1) * 16 + row16) : static_cast<uint32_t>(w * 16 + row16);
+    b_off[w] = (row * static_cast<uint32_t>(p.K) + quarter * E) * EB;
+  }
+  f32x4_t acc[W];
+#pragma unroll
+  for (int w = 0; w < W; ++w) acc[w] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  uint4_t fa[2][U], fb[2][U][W];
+  auto request = [&](int piece, int set) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = piece * PIECE + u * (4 * E);
+      const uint32_t behind = k + quarter * E >= p.K ? kOutOfRange : 0u, from = static_cast<uint32_t>(k) * EB;
+#pragma unroll
+      for (int w = 0; w < W; ++w) fb[set][u][w] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_b, static_cast<int>((b_off[w] + from) | behind), 0, 0);
+      fa[set][u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_a, static_cast<int>((a_off + from) | behind), 0, 0);
+    }
+  };
+  auto multiply = [&](int set) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int w = 0; w < W; ++w) mma16<T>(fb[set][u][w], fa[set][u], acc[w]);
+  };
+  // pieces behind the last one are requested out of range and add zeros: no branch around the loads in flight
+  request(wave, 0);
+  for (int piece = wave; piece < pieces; piece += 2 * KG) {
+    request(piece + KG, 1);
+    multiply(0);
+    request(piece + 2 * KG, 0);
+    multiply(1);
+  }
+
+  // acc[w][i] is column 4 * quarter + i of the tile, token row16; the wavefronts' sums meet in LDS, added in their order
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+    *reinterpret_cast<float4*>(&red[wave][w][row16 * 20 + quarter * 4]) = make_float4(acc[w][0], acc[w][1], acc[w][2], acc[w][3]);
+  __syncthreads();
+  for (int q = tid; q < 64 * TN; q += KG * 64) {   // four columns of one token a thread
+    const int tile = q >> 6, row = (q >> 2) & 15, c = (q & 3) * 4, col = n0 + tile * 16 + c;
+    if (row >= p.M || col >= p.N) continue;
+    auto total = [&](int w, float* v) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = 0.f;
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+        const float4 s = *reinterpret_cast<const float4*>(&red[g][w][row * 20 + c]);
+        v[0] += s.x;
+        v[1] += s.y;
+        v[2] += s.z;
+        v[3] += s.w;
+      }
+    };
+    float v[4], u[4], zg[4], zu[4], o[4], h[4];
+    if constexpr (GATED_FWD) {
+      total(2 * tile, v);
+      total(2 * tile + 1, u);
+    } else {
+      total(tile, v);
+    }
+    T* out = static_cast<T*>(p.out) + row * p.ldo + col;
+    T* out2 = static_cast<T*>(p.out2) + row * p.ldo2 + col;
+    if constexpr (MODE == kLinFwd || MODE == kGatedFwd) {
+      if (p.bias) {
+        float b[4];
+        load_four(p.bias + col, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += b[e];
+        if constexpr (GATED_FWD) {
+          load_four(p.bias + p.N + col, b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] += b[e];
+        }
+      }
+      if (p.out2) {
+        store_four(out2, v);
+        if constexpr (GATED_FWD) store_four(out2 + p.N, u);
+      }
+    } else {
+      const T* z = static_cast<const T*>(p.z) + row * p.ldz + col;
+      if (MODE == kGatedBwd || p.act != kActNone) load_four(z, zg);
+      if constexpr (MODE == kGatedBwd) load_four(z + p.N, zu);
+    }
+    with_activation(p.act, [&](auto act_c) { combine<T, MODE, decltype(act_c)::value, 4>(v, u, zg, zu, o, h); });
+    if constexpr (!is_gated(MODE)) {
+      if (p.add) {
+        float r[4];
+        load_four(static_cast<const T*>(p.add) + row * p.ldadd + col, r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += r[e];
+      }
+    }
+    store_four(out, o);
+    if constexpr (MODE == kGatedBwd) {
+      store_four(out + p.N, u);
+      if (p.out2) store_four(out2, h);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+template <typename T>
+constexpr const char* type_name() { return sizeof(T) == 2 ? "bf16," : "f32,"; }
+inline std::string mode_name(int mode) {
+  static const char* const names[] = {"fwd,", "dgrad,", "gated_fwd,", "gated_dgrad,"};
+  return names[mode];
+}
+inline double linear_flops(const LinearArgs& a, int mode) { return (mode == kGatedFwd ? 4.0 : 2.0) * a.M * a.N * a.K; }
+inline double linear_bytes(const LinearArgs& a, int mode, int eb) {
+  const double mn = static_cast<double>(a.M) * a.N, wide = is_gated(mode) ? 2.0 : 1.0;
+  double elems = static_cast<double>(a.M) * a.K + mn;
+  if (a.add) elems += mn;
+  if (mode == kLinBwd || mode == kGatedBwd) elems += a.z ? wide * mn : 0.0;
+  if (mode == kGatedBwd) elems += mn;
+  if (a.out2) elems += mode == kGatedFwd ? 2.0 * mn : mn;
+  return elems * eb + a.b_bytes;
+}
+inline int tiles_over(int n, int tile) { return (n + tile - 1) / tile; }
+
+template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int RB, int PER_CU>
+int launch_linear_tile(Context* ctx, LinearArgs& a) {
+  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, BN_OUT = MODE == kGatedFwd ? BN / 2 : BN;
+  static const std::string name = std::string("linear_tile_kernel<") + type_name<T>() + mode_name(MODE) + std::to_string(BM) + "x" +
+                                  std::to_string(BN) + "," + std::to_string(NBUF) + "buf>";
+  a.tiles_m = tiles_over(a.M, BM);
+  a.tiles_n = tiles_over(a.N, BN_OUT);
+  const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+  TCH_CHECK_ARG(tiles <= 0x3fffffff, "linear: grid out of range");
+  a.group_rows = a.tiles_n > 8 ? 4 : 0;
+  a.div_tiles_n = FastDiv(a.tiles_n);
+  a.div_group = FastDiv(static_cast<uint32_t>(a.group_rows > 1 ? a.group_rows * a.tiles_n : 1));
+  a.div_rows = FastDiv(a.group_rows > 1 ? a.group_rows : 1);
+  const unsigned grid = static_cast<unsigned>(tiles < 256 * PER_CU ? tiles : 256 * PER_CU);
+  return launch(ctx, linear_tile_kernel<T, MODE, WM, WN, TM, TN, NBUF, RB, PER_CU>, dim3(grid), dim3(WM * WN * 64), a, name.c_str(),
+                linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
+}
+
+template <typename T, int MODE, int TM, int TN, int KG, int NBUF>
+int launch_linear_split(Context* ctx, LinearArgs& a) {
+  constexpr int BM = TM * 32, BN = TN * 32, BN_OUT = MODE == kGatedFwd ? BN / 2 : BN;
+  static const std::string name = std::string("linear_split_kernel<") + type_name<T>() + mode_name(MODE) + std::to_string(BM) + "x" +
+                                  std::to_string(BN) + "," + std::to_string(KG) + "way>";
+  a.tiles_m = tiles_over(a.M, BM);
+  a.tiles_n = tiles_over(a.N, BN_OUT);
+  const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+  TCH_CHECK_ARG(tiles <= 0x3fffffff, "linear: grid out of range");
+  // the larger operand is the one an XCD should fetch once
+  a.group_rows = (MODE == kGatedFwd ? 2.0 : 1.0) * a.N > a.M ? 1 : 0;
+  a.div_tiles_n = FastDiv(a.group_rows ? a.tiles_m : a.tiles_n);
+  return launch(ctx, linear_split_kernel<T, MODE, TM, TN, KG, NBUF>, dim3(static_cast<unsigned>(tiles)), dim3(KG * 64), a, name.c_str(),
+                linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
+}
+
+template <typename T, int MODE, int TN, int KG>
+int launch_linear_rows(Context* ctx, LinearArgs& a) {
+  static const std::string name = std::string("linear_rows_kernel<") + type_name<T>() + mode_name(MODE) + std::to_string(16 * TN) + "," +
+                                  std::to_string(KG) + "way>";
+  return launch(ctx, linear_rows_kernel<T, MODE, TN, KG>, dim3(static_cast<unsigned>(tiles_over(a.N, 16 * TN))), dim3(KG * 64), a, name.c_str(),
+                linear_bytes(a, MODE, sizeof(T)), 1);
+}
+
+template <typename T, int MODE>
+int launch_linear_mode(Context* ctx, LinearArgs& a) {
+  constexpr bool kWide = MODE == kGatedFwd;
+  if (a.M <= 16) return launch_linear_rows<T, MODE, 1, 8>(ctx, a);
+  const int64_t tiles = static_cast<int64_t>(tiles_over(a.M, 128)) * tiles_over(a.N, kWide ? 64 : 128);
+  if (tiles >= 192) {
+    if constexpr (sizeof(T) == 2) {
+      if (tiles >= 512) return launch_linear_tile<T, MODE, 2, 2, 2, 4, 3, 64, 2>(ctx, a);
+      return launch_linear_tile<T, MODE, 2, 2, 2, 2, 4, 64, 2>(ctx, a);
+    } else {
+      return launch_linear_tile<T, MODE, 2, 2, 2, 2, 2, 128, 2>(ctx, a);
+    }
+  }
+  if (static_cast<int64_t>(tiles_over(a.M, 64)) * tiles_over(a.N, kWide ? 32 : 64) >= 256) return launch_linear_split<T, MODE, 2, 2, 4, 4>(ctx, a);
+  return launch_linear_split<T, MODE, 1, kWide ? 2 : 1, 8, kWide ? 3 : 4>(ctx, a);
+}
+
+template <typename T>
+int launch_linear_typed(Context* ctx, int mode, LinearArgs& a) {
+  switch (mode) {
+    case kLinFwd: return launch_linear_mode<T, kLinFwd>(ctx, a);
+    case kLinBwd: return launch_linear_mode<T, kLinBwd>(ctx, a);
+    case kGatedFwd: return launch_linear_mode<T, kGatedFwd>(ctx, a);
+    default: return launch_linear_mode<T, kGatedBwd>(ctx, a);
+  }
+}
+
+}  // namespace
+
+int launch_linear_bf16(Context* ctx, int mode, LinearArgs& a);   // linear_bf16.hip
+int launch_linear_f32(Context* ctx, int mode, LinearArgs& a);    // linear_f32.hip
+
+}  // namespace tch

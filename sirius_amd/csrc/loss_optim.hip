@@ -216,14 +216,18 @@ struct SgdArgs {
   int64_t n;
   float lr, momentum, wd;
   int aligned;   // every buffer starts on a 16-byte boundary (the shadow on 8): 16-byte accesses are in order
+  const float* grad_scale;   // SCALED: a factor on every gradient, in device memory
 };
 
+template <bool SCALED>
 __global__ __launch_bounds__(256) void sgd_kernel(SgdArgs p) {
+  const float scale = SCALED ? *p.grad_scale : 1.f;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256 * 4;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4; i < p.n; i += stride) {
     if (p.aligned && i + 4 <= p.n) {
       float4 w = load_streaming_f4(p.param + i);
       float4 g = load_streaming_f4(p.grad + i);
+      if (SCALED) g = make_float4(g.x * scale, g.y * scale, g.z * scale, g.w * scale);
       float4 b = load_streaming_f4(p.buf + i);
       b.x = p.momentum * b.x + (g.x + p.wd * w.x);
       b.y = p.momentum * b.y + (g.y + p.wd * w.y);
@@ -244,7 +248,7 @@ __global__ __launch_bounds__(256) void sgd_kernel(SgdArgs p) {
     } else {
       for (int64_t j = i; j < p.n && j < i + 4; ++j) {
         float w = p.param[j];
-        float b = p.momentum * p.buf[j] + (p.grad[j] + p.wd * w);
+        float b = p.momentum * p.buf[j] + ((SCALED ? p.grad[j] * scale : p.grad[j]) + p.wd * w);
         w -= p.lr * b;
         p.param[j] = w;
         p.buf[j] = b;
@@ -420,13 +424,14 @@ int softmax_ce_lm(Context* ctx, int dtype, const float* logits, int ld_logits, c
 }
 
 int sgd_momentum_step(Context* ctx, float* param, const float* grad, float* momentum_buf, void* shadow_bf16,
-                      int64_t n, float lr, float momentum, float weight_decay) {
+                      int64_t n, float lr, float momentum, float weight_decay, const float* grad_scale) {
   TCH_CHECK_ARG(param && grad && momentum_buf && n > 0, "sgd_momentum_step: null tensor or empty");
-  SgdArgs a{param, grad, momentum_buf, static_cast<uint16_t*>(shadow_bf16), n, lr, momentum, weight_decay, 0};
+  SgdArgs a{param, grad, momentum_buf, static_cast<uint16_t*>(shadow_bf16), n, lr, momentum, weight_decay, 0, grad_scale};
   a.aligned = ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(momentum_buf)) & 15) == 0 &&
               (reinterpret_cast<uintptr_t>(shadow_bf16) & 7) == 0;
-  return launch(ctx, sgd_kernel, dim3(flat_blocks((n + 3) / 4)), dim3(256), a, "sgd_kernel",
-                static_cast<double>(n) * (shadow_bf16 ? 22.0 : 20.0), 1);
+  const double bytes = static_cast<double>(n) * (shadow_bf16 ? 22.0 : 20.0);
+  return grad_scale ? launch(ctx, sgd_kernel<true>, dim3(flat_blocks((n + 3) / 4)), dim3(256), a, "sgd_kernel<scaled>", bytes, 1)
+                    : launch(ctx, sgd_kernel<false>, dim3(flat_blocks((n + 3) / 4)), dim3(256), a, "sgd_kernel", bytes, 1);
 }
 
 int grad_accumulate(Context* ctx, float* global, float* grad, int64_t n) {

@@ -157,7 +157,7 @@ int attn_softmax_bwd(Context* ctx, int dtype, const void* probs, const void* dpr
                      int Lk, float scale, int causal);
 int adamw_step(Context* ctx, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, void* shadow_bf16,
                int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay, int* step_dev,
-               float* scalars_dev);
+               float* scalars_dev, const float* grad_scale = nullptr);
 int embedding_fwd(Context* ctx, int dtype, const int64_t* ids, const void* wte, const void* wpe, void* out, int B, int T,
                   int C, int vocab);
 int embedding_bwd(Context* ctx, int dtype, const int64_t* ids, const void* dy, float* dwte, float* dwpe, int B, int T,
@@ -187,6 +187,27 @@ int relpos_bias_scatter_csr(Context* ctx, const float* dbias, const int32_t* ptr
                             int heads, int pairs, int entries, int accumulate);
 int64_t column_sum_workspace_floats(int rows, int cols);
 int column_sum(Context* ctx, int dtype, const void* x, float* out, int rows, int cols, int accumulate, float* workspace);
+
+// linear.hip -- linear layers with bias, activation and residual in one launch, gated layers, data gradients
+struct Rows {   // a matrix whose rows lie ld elements apart; ptr may be null where the operator allows it
+  void* ptr;
+  int64_t ld;
+};
+int linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows& y, const float* bias, int act, const Rows& residual,
+               const Rows& pre, int64_t M, int64_t K, int64_t N);
+int linear_dgrad(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& dx, int act, const Rows& pre, const Rows& residual,
+                 int64_t M, int64_t K, int64_t N);
+int gated_linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows& h, const float* bias, int act, const Rows& pre, int64_t M,
+                     int64_t K, int64_t F);
+int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& pre, const Rows& dpre, const Rows& h, int act,
+                       int64_t M, int64_t K, int64_t F);
+int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, const Rows& h, int gated, int act, int64_t M, int64_t N);
+
+// grad_norm.hip -- the global norm of many tensors, listed in pieces in device memory, and clipping by it
+int64_t grad_table_piece_elems();
+int64_t grad_norm_workspace_bytes(int64_t pieces);
+int grad_norm(Context* ctx, const void* table, int64_t pieces, int64_t bytes_read, int64_t bytes_written, int clip, double max_norm, float* norm,
+              float* coef, void* workspace);
 
 // bgemm.hip
 int batched_gemm(Context* ctx, int dtype, const void* a, const void* b, void* c, int M, int N, int K, int64_t a_rs,
@@ -226,7 +247,7 @@ int softmax_ce_lm(Context* ctx, int dtype, const float* logits, int ld_logits, c
                   float* loss_mean, void* dlogits, int ld_dlogits, int rows, int classes, int valid_rows,
                   float loss_scale);
 int sgd_momentum_step(Context* ctx, float* param, const float* grad, float* momentum_buf, void* shadow_bf16,
-                      int64_t n, float lr, float momentum, float weight_decay);
+                      int64_t n, float lr, float momentum, float weight_decay, const float* grad_scale = nullptr);
 int grad_accumulate(Context* ctx, float* global, float* grad, int64_t n);
 int fill_zero(Context* ctx, void* ptr, int64_t bytes);
 int bias_grad(Context* ctx, int dtype, const void* dy, float* dbias, int rows, int cols, int ld, int accumulate,

@@ -427,6 +427,7 @@ struct AdamArgs {
   // 1 - 0.999f is off by 1e-5 relative)
   float lr, beta2, one_minus_beta1, one_minus_beta2, eps, decay;
   int aligned;   // every buffer starts on a 16-byte boundary (the shadow on 8): 16-byte accesses are in order
+  const float* grad_scale;   // SCALED: a factor on every gradient, in device memory
 };
 
 __device__ inline void adamw_element(const AdamArgs& p, float step_size, float bc2_sqrt, float g, float& w, float& m,
@@ -439,13 +440,16 @@ __device__ inline void adamw_element(const AdamArgs& p, float step_size, float b
 }
 
 // four elements per thread and trip, 16-byte streaming accesses; the last n % 4 elements one by one
+template <bool SCALED>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamArgs p) {
   const float bc1 = p.scalars[0], bc2_sqrt = p.scalars[1];
+  const float scale = SCALED ? *p.grad_scale : 1.f;
   const float step_size = p.lr / bc1;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256 * 4;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4; i < p.n; i += stride) {
     if (p.aligned && i + 4 <= p.n) {
-      const float4 g = load_streaming_f4(p.grad + i);
+      float4 g = load_streaming_f4(p.grad + i);
+      if (SCALED) g = make_float4(g.x * scale, g.y * scale, g.z * scale, g.w * scale);
       float4 w = load_streaming_f4(p.param + i);
       float4 m = load_streaming_f4(p.m + i);
       float4 v = load_streaming_f4(p.v + i);
@@ -465,7 +469,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamArgs p) {
     } else {
       for (int64_t j = i; j < p.n && j < i + 4; ++j) {
         float w = p.param[j], m = p.m[j], v = p.v[j];
-        adamw_element(p, step_size, bc2_sqrt, p.grad[j], w, m, v);
+        adamw_element(p, step_size, bc2_sqrt, SCALED ? p.grad[j] * scale : p.grad[j], w, m, v);
         p.param[j] = w;
         p.m[j] = m;
         p.v[j] = v;
@@ -812,7 +816,7 @@ int attn_softmax_bwd(Context* ctx, int dtype, const void* probs, const void* dpr
 
 int adamw_step(Context* ctx, float* param, const float* grad, float* exp_avg, float* exp_avg_sq, void* shadow_bf16,
                int64_t n, double lr, double beta1, double beta2, double eps, double weight_decay, int* step_dev,
-               float* scalars_dev) {
+               float* scalars_dev, const float* grad_scale) {
   TCH_CHECK_ARG(param && grad && exp_avg && exp_avg_sq && step_dev && scalars_dev && n > 0, "adamw_step: null tensor or empty");
   AdamTickArgs t{step_dev, scalars_dev, beta1, beta2};
   if (int rc = launch(ctx, adamw_tick_kernel, dim3(1), dim3(64), t, "adamw_tick_kernel", 12.0, 1)) return rc;
@@ -829,12 +833,14 @@ int adamw_step(Context* ctx, float* param, const float* grad, float* exp_avg, fl
              static_cast<float>(1.0 - beta2),
              static_cast<float>(eps),
              static_cast<float>(1.0 - lr * weight_decay),
-             0};
+             0,
+             grad_scale};
   a.aligned = ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(exp_avg) |
                 reinterpret_cast<uintptr_t>(exp_avg_sq)) & 15) == 0 &&
               (reinterpret_cast<uintptr_t>(shadow_bf16) & 7) == 0;
-  return launch(ctx, adamw_kernel, dim3(flat_blocks((n + 3) / 4)), dim3(256), a, "adamw_kernel",
-                static_cast<double>(n) * (shadow_bf16 ? 30.0 : 28.0), 1);
+  const double bytes = static_cast<double>(n) * (shadow_bf16 ? 30.0 : 28.0);
+  return grad_scale ? launch(ctx, adamw_kernel<true>, dim3(flat_blocks((n + 3) / 4)), dim3(256), a, "adamw_kernel<scaled>", bytes, 1)
+                    : launch(ctx, adamw_kernel<false>, dim3(flat_blocks((n + 3) / 4)), dim3(256), a, "adamw_kernel", bytes, 1);
 }
 
 int embedding_fwd(Context* ctx, int dtype, const int64_t* ids, const void* wte, const void* wpe, void* out, int B, int T,

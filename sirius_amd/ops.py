@@ -5,6 +5,7 @@ that already live on the GPU, passes their raw pointers to the shared library,
 and the library enqueues hand-written HIP kernels.  Layout is NHWC throughout;
 filters are [K, R, S, C].
 """
+import bisect
 import contextlib
 import ctypes
 import time
@@ -675,12 +676,98 @@ def softmax_ce_lm(ctx, logits, labels, loss_rows, loss_mean, dlogits, classes, v
                                   float(loss_scale)), "tch_softmax_ce_lm")
 
 
-def sgd_momentum_step(ctx, param, grad, buf, lr, momentum, weight_decay, shadow=None):
+def _check_grad_scale(grad_scale):
+    assert grad_scale.dtype == torch.float32 and grad_scale.numel() == 1, "grad_scale: one fp32 number on the GPU"
+
+
+def sgd_momentum_step(ctx, param, grad, buf, lr, momentum, weight_decay, shadow=None, grad_scale=None):
+    """grad_scale (one fp32 number on the GPU, e.g. the coefficient of grad_norm): a factor on every gradient."""
     n = param.numel()
     assert param.dtype == grad.dtype == buf.dtype == torch.float32 and grad.numel() == n and buf.numel() == n
     assert shadow is None or (shadow.dtype == torch.bfloat16 and shadow.numel() == n)
+    if grad_scale is not None:
+        _check_grad_scale(grad_scale)
+        check(lib().tch_sgd_momentum_step_scaled(ctx.handle, _p(param), _p(grad), _p(buf), _p(shadow), n, lr, momentum,
+                                                 weight_decay, _p(grad_scale)), "tch_sgd_momentum_step_scaled")
+        return
     check(lib().tch_sgd_momentum_step(ctx.handle, _p(param), _p(grad), _p(buf), _p(shadow), n, lr, momentum,
                                       weight_decay), "tch_sgd_momentum_step")
+
+
+class GradTable:
+    """Device table of gradient tensors (fp32 or bf16, contiguous, any number and sizes, empty ones too) for grad_norm and
+    clip_grad_norm; `out`: tensors of the same sizes that clip_grad_norm writes instead of the gradients themselves.  It holds
+    the tensors' addresses, and the tensors."""
+
+    def __init__(self, tensors, out=None):
+        tensors = list(tensors)
+        out = tensors if out is None else list(out)
+        assert len(out) == len(tensors), "as many outputs as gradients"
+        assert tensors, "no tensors"
+        self.device = tensors[0].device
+        piece = int(lib().tch_grad_table_piece_elems())
+        rows, writes, reads = [], [], []
+        self.bytes_read = self.bytes_written = 0
+        for t, o in zip(tensors, out):
+            for x in (t, o):
+                dtype_code(x)
+                _p(x)
+                assert x.device == self.device, "gradients on different devices"
+            assert t.numel() == o.numel(), "an output of another size than its gradient"
+            n, eb, ob = t.numel(), t.element_size(), o.element_size()
+            if n == 0:
+                continue
+            self.bytes_read += n * eb
+            self.bytes_written += n * ob
+            src, dst = t.data_ptr(), o.data_ptr()
+            writes.append((dst, dst + n * ob, src if eb == ob else None))
+            reads.append((src, src + n * eb))
+            aligned = int(src % (4 * eb) == 0 and dst % (4 * ob) == 0)
+            codes = dtype_code(t) << 32
+            for at in range(0, n, piece):
+                rows.append((src + at * eb, dst + at * ob, min(piece, n - at) | codes, dtype_code(o) | aligned << 32))
+        # an element may be written once, and read only where it is written from
+        writes.sort()
+        for (_, end, _), (start, _, _) in zip(writes, writes[1:]):
+            assert end <= start, "clip_grad_norm would write an element twice: a tensor given twice, or overlapping views"
+        starts = [w[0] for w in writes]
+        for lo, hi in reads:
+            i = max(bisect.bisect_right(starts, lo) - 1, 0)
+            while i < len(writes) and writes[i][0] < hi:
+                assert writes[i][1] <= lo or (writes[i][0] == lo and writes[i][2] == lo), "an output overlaps another gradient"
+                i += 1
+        self.pieces = len(rows)
+        self.table = torch.tensor(rows if rows else [(0, 0, 0, 0)], dtype=torch.int64).to(self.device)
+        self.tensors, self.out = tensors, out
+
+
+def grad_norm_workspace_bytes(table):
+    return int(lib().tch_grad_norm_workspace_bytes(table.pieces))
+
+
+def _check_norm(ctx, table, norm, workspace):
+    assert norm.dtype == torch.float32 and norm.numel() == 1, "norm: one fp32 number on the GPU"
+    assert norm.device == workspace.device == table.device == ctx.stream.device, "tensors on different devices"
+    assert workspace.numel() * workspace.element_size() >= grad_norm_workspace_bytes(table), "grad_norm workspace too small"
+
+
+def grad_norm(ctx, table, norm, workspace, max_norm=None, coef=None):
+    """norm[0] = the square root of the sum of squares over all tensors of `table` (GradTable), added up in fp64 in a fixed
+    order.  With coef also coef[0] = min(1, max_norm / (norm + 1e-6)): what the optimizer steps take as grad_scale, which
+    clips without a pass of its own."""
+    _check_norm(ctx, table, norm, workspace)
+    assert (max_norm is None) == (coef is None), "max_norm and coef come together"
+    assert coef is None or (coef.dtype == torch.float32 and coef.numel() == 1 and coef.device == table.device)
+    check(lib().tch_grad_norm(ctx.handle, _p(table.table), table.pieces, table.bytes_read,
+                              -1.0 if max_norm is None else float(max_norm), _p(norm), _p(coef), _p(workspace)), "tch_grad_norm")
+
+
+def clip_grad_norm(ctx, table, max_norm, norm, workspace):
+    """grad_norm, and every gradient times min(1, max_norm / (norm + 1e-6)), in place or into the table's `out`.  As in
+    torch.nn.utils.clip_grad_norm_ a norm that is not a number makes every gradient one; norm[0] tells."""
+    _check_norm(ctx, table, norm, workspace)
+    check(lib().tch_clip_grad_norm(ctx.handle, _p(table.table), table.pieces, table.bytes_read, table.bytes_written, float(max_norm),
+                                   _p(norm), _p(workspace)), "tch_clip_grad_norm")
 
 
 def grad_accumulate(ctx, global_grad, grad):
@@ -835,6 +922,184 @@ def gelu_bwd(ctx, dy, x, dx, tanh_form=False):
     check(lib().tch_gelu_bwd(ctx.handle, dtype_code(x), _p(dy), _p(x), _p(dx), x.numel(), int(tanh_form)), "tch_gelu_bwd")
 
 
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _act_code(act):
+    if act not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+    return ACTIVATIONS[act]
+
+
+def _matrix(ctx, name, t, width, rows=None, dtype=None):
+    """(address, elements from row to row, rows) of a tensor [..., width] whose rows are evenly spaced: a contiguous one, or columns
+    of a wider one."""
+    if t is None:
+        return None, 0, rows
+    if not t.is_cuda:
+        raise ValueError("device operators need GPU tensors")
+    assert t.device == ctx.stream.device, f"{name} is not on the context's device"
+    assert t.dim() >= 1 and t.shape[-1] == width, f"{name}: rows of {t.shape[-1] if t.dim() else 0} elements instead of {width}"
+    assert dtype is None or t.dtype == dtype, f"{name}: {t.dtype} instead of {dtype}"
+    if t.is_contiguous():
+        n, ld = t.numel() // width, width
+    else:
+        try:
+            v = t.view(-1, width)
+        except RuntimeError:
+            raise ValueError(f"{name}: rows must be evenly spaced") from None
+        if v.stride(1) != 1 or (v.shape[0] > 1 and v.stride(0) < width):
+            raise ValueError(f"{name}: the elements of a row must be neighbours, and rows must not overlap")
+        n, ld = v.shape[0], v.stride(0) if v.shape[0] > 1 else width
+    assert rows is None or n == rows, f"{name}: {n} rows instead of {rows}"
+    return ctypes.c_void_p(t.data_ptr()), ld, n
+
+
+def _vector(ctx, name, t, numel):
+    assert t is None or (t.dtype == torch.float32 and t.numel() == numel and t.device == ctx.stream.device), f"{name}: {numel} fp32 numbers"
+    return _p(t)
+
+
+def _weights(ctx, name, w, dtype):
+    assert w.dim() == 2 and w.dtype == dtype and w.device == ctx.stream.device, f"{name}: a matrix of {dtype} on the context's device"
+    return _p(w)
+
+
+def linear_fwd(ctx, x, w, y, bias=None, act="none", residual=None, pre=None):
+    """y = act(x w^T + bias) + residual in one launch: x [..., K], w [N, K], y [..., N], bias [N] fp32; pre (like y) keeps
+    x w^T + bias for the backward pass.  Any number of rows; K and N multiples of a 16-byte chunk.  x, y, residual and pre may be
+    columns of wider tensors (rows on 16-byte boundaries); residual may be y itself.  act: one of ACTIVATIONS."""
+    N, K = w.shape
+    xp, ldx, M = _matrix(ctx, "x", x, K)
+    yp, ldy, _ = _matrix(ctx, "y", y, N, M, x.dtype)
+    rp, ldr, _ = _matrix(ctx, "residual", residual, N, M, x.dtype)
+    pp, ldp, _ = _matrix(ctx, "pre", pre, N, M, x.dtype)
+    check(lib().tch_linear_fwd(ctx.handle, dtype_code(x), xp, ldx, _weights(ctx, "w", w, x.dtype), yp, ldy,
+                               _vector(ctx, "bias", bias, N), _act_code(act), rp, ldr, pp, ldp, M, K, N), "tch_linear_fwd")
+
+
+def linear_dgrad(ctx, dy, wt, dx, act="none", pre=None, residual=None):
+    """dx = (dy w) . act'(pre) + residual in one launch: wt [K, N] is the weight [N, K] transposed (as for conv2d_dgrad), dy [..., N],
+    dx, pre and residual [..., K].  pre and act are those of the layer in FRONT of this one, whose output this layer read: dx is
+    then the gradient of that layer's pre-activation."""
+    K, N = wt.shape
+    dyp, lddy, M = _matrix(ctx, "dy", dy, N)
+    dxp, lddx, _ = _matrix(ctx, "dx", dx, K, M, dy.dtype)
+    pp, ldp, _ = _matrix(ctx, "pre", pre, K, M, dy.dtype)
+    rp, ldr, _ = _matrix(ctx, "residual", residual, K, M, dy.dtype)
+    check(lib().tch_linear_dgrad(ctx.handle, dtype_code(dy), dyp, lddy, _weights(ctx, "wt", wt, dy.dtype), dxp, lddx, _act_code(act),
+                                 pp, ldp, rp, ldr, M, N, K), "tch_linear_dgrad")
+
+
+def act_bwd(ctx, dy, pre, dz, act):
+    """dz = dy . act'(pre), element by element; dz may be dy or pre."""
+    N = dy.shape[-1]
+    dyp, lddy, M = _matrix(ctx, "dy", dy, N)
+    pp, ldp, _ = _matrix(ctx, "pre", pre, N, M, dy.dtype)
+    dzp, lddz, _ = _matrix(ctx, "dz", dz, N, M, dy.dtype)
+    check(lib().tch_act_bwd(ctx.handle, dtype_code(dy), dyp, lddy, pp, ldp, dzp, lddz, _act_code(act), M, N), "tch_act_bwd")
+
+
+def _wgrad_blocks(rows, K, N, element):
+    """(first row, rows) of the pieces in which a weight gradient takes its rows: tensors of a piece stay below the 2 GiB that a
+    buffer offset reaches."""
+    most = (2 ** 31 - 1) // (max(K, N) * element)
+    most = max(most // 1024 * 1024, 1) if most >= 1024 else max(most, 1)
+    return [(at, min(most, rows - at)) for at in range(0, rows, most)]
+
+
+def _wgrad_splits(x, K, N, rows):
+    return int(lib().tch_conv2d_wgrad_pick_splits(dtype_code(x), rows, 1, 1, K, N, 1, 1, 1, 0))
+
+
+def linear_bwd_workspace_bytes(x, N):
+    """Bytes of workspace that linear_bwd (gated_linear_bwd: N = 2 F) wants for a layer with the input x [..., K] and N outputs."""
+    K = x.shape[-1]
+    blocks = {rows for _, rows in _wgrad_blocks(x.numel() // K, K, N, x.element_size())}
+    return max([conv2d_wgrad_workspace_bytes(dtype_code(x), N, 1, 1, K, _wgrad_splits(x, K, N, rows)) for rows in blocks] + [4])
+
+
+def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=None, residual=None, accumulate=False, workspace=None):
+    """The gradients of linear_fwd: dpre = dy . act'(pre) (act "none": dy itself, and dpre stays untouched), dx = dpre w + residual,
+    dw (+)= dpre^T x and dbias (+)= column sums of dpre, both fp32.  The residual's own gradient is dy.  dx (with wt) or dw may be
+    None.  x and the gradient it meets are contiguous; workspace: linear_bwd_workspace_bytes (without it the weight gradient
+    is not split over its rows)."""
+    K = x.shape[-1]
+    N = dy.shape[-1]
+    M = _matrix(ctx, "x", x, K, None, dy.dtype)[2]
+    assert dy.numel() == M * N, "dy and x have different rows"
+    g = dy
+    if act != "none":
+        assert pre is not None and dpre is not None, "an activation's derivative needs pre, and dpre to keep its result"
+        act_bwd(ctx, dy, pre, dpre, act)
+        g = dpre
+    if dx is not None:
+        linear_dgrad(ctx, g, wt, dx, residual=residual)
+    else:
+        assert residual is None, "a residual without dx"
+    if dw is None:
+        assert dbias is None, "dbias comes with dw"
+        return
+    assert tuple(dw.shape) == (N, K) and dw.dtype == torch.float32 and dw.device == ctx.stream.device, f"dw: [{N}, {K}] fp32"
+    assert x.is_contiguous() and g.is_contiguous(), "a weight gradient needs contiguous tensors"
+    _vector(ctx, "dbias", dbias, N)
+    if M == 0:
+        for t in (dw, dbias):
+            if t is not None and not accumulate:
+                fill_zero(ctx, t)
+        return
+    x2, g2, dw4 = x.view(M, 1, 1, K), g.view(M, 1, 1, N), dw.view(N, 1, 1, K)
+    for at, rows in _wgrad_blocks(M, K, N, x.element_size()):
+        splits = 1 if workspace is None else _wgrad_splits(x, K, N, rows)
+        conv2d_wgrad(ctx, x2[at:at + rows], g2[at:at + rows], dw4, 1, 0, workspace=workspace, splits=splits, accumulate=accumulate or at > 0,
+                     dbias=dbias)
+
+
+def gated_linear_fwd(ctx, x, w, h, bias=None, act="silu", pre=None):
+    """A gated feed-forward layer in one launch: g = x wg^T + bg, u = x wu^T + bu, h = act(g) . u.  w [2F, K] and bias [2F] fp32 hold
+    the gate's rows first; x [..., K], h [..., F]; pre [..., 2F] keeps (g | u) for the backward pass.  Sizes, strides and
+    activations as for linear_fwd."""
+    F2, K = w.shape
+    F = F2 // 2
+    assert F2 == 2 * F, "w holds the gate's and the up projection's rows"
+    xp, ldx, M = _matrix(ctx, "x", x, K)
+    hp, ldh, _ = _matrix(ctx, "h", h, F, M, x.dtype)
+    pp, ldp, _ = _matrix(ctx, "pre", pre, F2, M, x.dtype)
+    check(lib().tch_gated_linear_fwd(ctx.handle, dtype_code(x), xp, ldx, _weights(ctx, "w", w, x.dtype), hp, ldh,
+                                     _vector(ctx, "bias", bias, F2), _act_code(act), pp, ldp, M, K, F), "tch_gated_linear_fwd")
+
+
+def gated_act_bwd(ctx, dh, pre, dpre, act="silu", h=None):
+    """dpre = (dh . u . act'(g) | dh . act(g)) from pre = (g | u), element by element; h = act(g) . u again.  dpre may be pre."""
+    F = dh.shape[-1]
+    dhp, lddh, M = _matrix(ctx, "dh", dh, F)
+    pp, ldp, _ = _matrix(ctx, "pre", pre, 2 * F, M, dh.dtype)
+    dpp, lddp, _ = _matrix(ctx, "dpre", dpre, 2 * F, M, dh.dtype)
+    hp, ldh, _ = _matrix(ctx, "h", h, F, M, dh.dtype)
+    check(lib().tch_gated_act_bwd(ctx.handle, dtype_code(dh), dhp, lddh, pp, ldp, dpp, lddp, hp, ldh, _act_code(act), M, F),
+          "tch_gated_act_bwd")
+
+
+def linear_dgrad_gated(ctx, dy, wt, pre, dpre, act="silu", h=None):
+    """The data gradient of a projection behind a gated layer, through that layer's product and activation, in one launch:
+    dh = dy w stays on the chip, dpre = (dh . u . act'(g) | dh . act(g)) [..., 2F] is stored, and h = act(g) . u again where it is
+    asked for (the forward pass need not keep it).  wt [F, N] is the projection's weight [N, F] transposed, dy [..., N]."""
+    F, N = wt.shape
+    dyp, lddy, M = _matrix(ctx, "dy", dy, N)
+    pp, ldp, _ = _matrix(ctx, "pre", pre, 2 * F, M, dy.dtype)
+    dpp, lddp, _ = _matrix(ctx, "dpre", dpre, 2 * F, M, dy.dtype)
+    hp, ldh, _ = _matrix(ctx, "h", h, F, M, dy.dtype)
+    check(lib().tch_linear_dgrad_gated(ctx.handle, dtype_code(dy), dyp, lddy, _weights(ctx, "wt", wt, dy.dtype), pp, ldp, dpp, lddp, hp, ldh,
+                                       _act_code(act), M, N, F), "tch_linear_dgrad_gated")
+
+
+def gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=None, act="silu", residual=None, accumulate=False, workspace=None):
+    """The gradients of gated_linear_fwd from dh [..., F]: dpre [..., 2F] as in gated_act_bwd, dx = dpre w + residual,
+    dw (+)= dpre^T x, dbias (+)= column sums of dpre.  wt [K, 2F] is w transposed; the rest as for linear_bwd."""
+    gated_act_bwd(ctx, dh, pre, dpre, act)
+    linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=dbias, residual=residual, accumulate=accumulate, workspace=workspace)
+
+
 def attn_softmax_fwd(ctx, scores, probs, scale=1.0, bias=None, mask=None, causal=False):
     """scores / probs [batch, heads, Lq, Lk]; bias [heads, Lq, Lk] fp32; mask [windows, Lq, Lk] fp32."""
     Bn, Hn, Lq, Lk = scores.shape
@@ -857,13 +1122,20 @@ def attn_softmax_bwd(ctx, probs, dprobs, dscores, scale=1.0, causal=False):
 
 
 def adamw_step(ctx, param, grad, exp_avg, exp_avg_sq, step_dev, scalars_dev, lr, beta1=0.9, beta2=0.999, eps=1e-8,
-               weight_decay=0.01, shadow=None):
+               weight_decay=0.01, shadow=None, grad_scale=None):
+    """grad_scale (one fp32 number on the GPU, e.g. the coefficient of grad_norm): a factor on every gradient."""
     n = param.numel()
     for t in (grad, exp_avg, exp_avg_sq):
         assert t.dtype == torch.float32 and t.numel() == n
     assert param.dtype == torch.float32 and step_dev.dtype == torch.int32 and scalars_dev.dtype == torch.float32
     assert step_dev.numel() >= 1 and scalars_dev.numel() >= 2
     assert shadow is None or (shadow.dtype == torch.bfloat16 and shadow.numel() == n)
+    if grad_scale is not None:
+        _check_grad_scale(grad_scale)
+        check(lib().tch_adamw_step_scaled(ctx.handle, _p(param), _p(grad), _p(exp_avg), _p(exp_avg_sq), _p(shadow), n, lr,
+                                          beta1, beta2, eps, weight_decay, _p(step_dev), _p(scalars_dev), _p(grad_scale)),
+              "tch_adamw_step_scaled")
+        return
     check(lib().tch_adamw_step(ctx.handle, _p(param), _p(grad), _p(exp_avg), _p(exp_avg_sq), _p(shadow), n, lr, beta1,
                                beta2, eps, weight_decay, _p(step_dev), _p(scalars_dev)), "tch_adamw_step")
 
