@@ -169,6 +169,16 @@ __device__ inline void store_streaming_f4(float* p, const float4& v) {
   __builtin_nontemporal_store(s, reinterpret_cast<stream_f4*>(p));
 }
 
+// a gradient times a factor, rounded by itself (not the product half of a fused multiply-add): an optimizer step with a factor is
+// the step on gradients that were scaled ahead, bit for bit
+__device__ inline float scaled_gradient(float g, float scale) {
+#pragma clang fp contract(off)
+  return g * scale;
+}
+__device__ inline float4 scaled_gradient(const float4& g, float scale) {
+  return make_float4(scaled_gradient(g.x, scale), scaled_gradient(g.y, scale), scaled_gradient(g.z, scale), scaled_gradient(g.w, scale));
+}
+
 // ---------------------------------------------------------------------------
 // wavefront reductions (64 lanes)
 // ---------------------------------------------------------------------------

@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256) void sgd_kernel(SgdArgs p) {
     if (p.aligned && i + 4 <= p.n) {
       float4 w = load_streaming_f4(p.param + i);
       float4 g = load_streaming_f4(p.grad + i);
-      if (SCALED) g = make_float4(g.x * scale, g.y * scale, g.z * scale, g.w * scale);
+      if (SCALED) g = scaled_gradient(g, scale);
       float4 b = load_streaming_f4(p.buf + i);
       b.x = p.momentum * b.x + (g.x + p.wd * w.x);
       b.y = p.momentum * b.y + (g.y + p.wd * w.y);
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256) void sgd_kernel(SgdArgs p) {
     } else {
       for (int64_t j = i; j < p.n && j < i + 4; ++j) {
         float w = p.param[j];
-        float b = p.momentum * p.buf[j] + ((SCALED ? p.grad[j] * scale : p.grad[j]) + p.wd * w);
+        float b = p.momentum * p.buf[j] + ((SCALED ? scaled_gradient(p.grad[j], scale) : p.grad[j]) + p.wd * w);
         w -= p.lr * b;
         p.param[j] = w;
         p.buf[j] = b;

@@ -449,7 +449,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamArgs p) {
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4; i < p.n; i += stride) {
     if (p.aligned && i + 4 <= p.n) {
       float4 g = load_streaming_f4(p.grad + i);
-      if (SCALED) g = make_float4(g.x * scale, g.y * scale, g.z * scale, g.w * scale);
+      if (SCALED) g = scaled_gradient(g, scale);
       float4 w = load_streaming_f4(p.param + i);
       float4 m = load_streaming_f4(p.m + i);
       float4 v = load_streaming_f4(p.v + i);
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamArgs p) {
     } else {
       for (int64_t j = i; j < p.n && j < i + 4; ++j) {
         float w = p.param[j], m = p.m[j], v = p.v[j];
-        adamw_element(p, step_size, bc2_sqrt, SCALED ? p.grad[j] * scale : p.grad[j], w, m, v);
+        adamw_element(p, step_size, bc2_sqrt, SCALED ? scaled_gradient(p.grad[j], scale) : p.grad[j], w, m, v);
         p.param[j] = w;
         p.m[j] = m;
         p.v[j] = v;
