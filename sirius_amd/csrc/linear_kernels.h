@@ -141,18 +141,18 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   constexpr int BM = WM * TM * 32, BN = WN * TN * 32, NW = WM * WN;
   constexpr bool GATED_FWD = MODE == kGatedFwd;
   constexpr int BN_OUT = GATED_FWD ? BN / 2 : BN;
-  static_assert(!GATED_FWD || TN % 2 == 0, "gate and up tiles come in pairs");
+  static_assert(TN == 2, "a wavefront has 64 columns: gate and up tiles, or the whole lines of the epilogue");
   static_assert((RB == 128 || RB == 64) && BM % (LD_ROWS * NW) == 0 && BN % (LD_ROWS * NW) == 0, "tile/loader mismatch");
   constexpr int A_LD = BM / LD_ROWS / NW, B_LD = BN / LD_ROWS / NW, LOADS = A_LD + B_LD;
+  constexpr bool OWN_STAGE = NBUF == 2;   // the epilogue's staging has a place of its own
+  static_assert(OWN_STAGE || A_LD >= 4, "4 KB of a wavefront's own loads stage its epilogue");
   constexpr int A_BYTES = BM * RB, BUF_BYTES = A_BYTES + BN * RB;
   // with two buffers the requested tile is waited for at the end of the step: all requests go out in its first half
   constexpr int LOAD_SL = NBUF == 2 ? (SL + 1) / 2 : SL;
   constexpr int AHEAD = (NBUF - 2) * LOADS;
   static_assert(AHEAD < 48, "vmcnt range");
   constexpr bool BIAS = MODE == kLinFwd || MODE == kGatedFwd;
-  // the bias of a wavefront's columns travels with the operands, requested with the first step of a tile
-  constexpr int BIAS_BYTES = TN * 32 * 4, BIAS_OFF = NBUF * BUF_BYTES;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[BIAS_OFF + (BIAS ? NW * (NBUF + 1) * BIAS_BYTES : 0)];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[NBUF * BUF_BYTES + (OWN_STAGE ? NW * 4096 : 0)];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
 
   __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
   const __amdgpu_buffer_rsrc_t rsrc_bias = make_rsrc(p.bias, BIAS && p.bias ? static_cast<uint32_t>(p.N) * (GATED_FWD ? 8u : 4u) : 0u);
-  int ld_id = first, ld_kt = 0, ld_bias = 0;
+  int ld_id = first, ld_kt = 0;
   auto mark_tail = [&] {
 #pragma unroll
     for (int j = 0; j < A_LD; ++j) a_off[j] |= behind_k[(wave * A_LD + j) & 1];
@@ -218,16 +218,6 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
     rsrc_a = make_rsrc(static_cast<const T*>(p.a) + m0 * p.lda, static_cast<uint32_t>(((rows - 1) * p.lda + p.K) * EB));
     const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
     rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
-    if constexpr (BIAS) {
-      if (p.bias) {
-        unsigned char* dst = lds + BIAS_OFF + (wave * (NBUF + 1) + ld_bias) * BIAS_BYTES;
-        const int block = wn * TN + (lane >> 3);
-        const int col = n0 + (GATED_FWD ? (block >> 1) * 32 : block * 32) + (lane & 7) * 4;
-        const int at_col = GATED_FWD && (block & 1) ? p.N + col : col;
-        if (lane < TN * 8) load_to_lds(rsrc_bias, dst, any && col < p.N ? at_col * 4 : static_cast<int>(kOutOfRange), 0);
-        ld_bias = ld_bias == NBUF ? 0 : ld_bias + 1;
-      }
-    }
     if (ragged_k || !any) {   // behind the last tile every offset is out of range: zeros land
       const uint32_t set = any ? 0u : kOutOfRange;
 #pragma unroll
@@ -274,11 +264,11 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
     for (int i = 0; i < TN; ++i) asm volatile("" : "+v"(fb[set][i]));
   };
   // multiplies the slice in `set`; meanwhile slice kk of the step in `buf` is read into the other set and part `q` of the loads
-  // goes to `ld_buf`
+  // (-1: all of them) goes to `ld_buf`
   auto slice = [&](auto set_c, uint32_t buf, auto kk_c, auto q_c, uint32_t ld_buf) {
     constexpr int set = decltype(set_c)::value, kk = decltype(kk_c)::value, q = decltype(q_c)::value;
-    constexpr int READS = TM + TN, MF = TM * TN, FIRST = (q < LOAD_SL ? q : LOAD_SL) * LOADS / LOAD_SL;
-    constexpr int AUX = READS + (q < LOAD_SL ? (q + 1) * LOADS / LOAD_SL - FIRST : 0);
+    constexpr int READS = TM + TN, MF = TM * TN, FIRST = q < 0 ? 0 : (q < LOAD_SL ? q : LOAD_SL) * LOADS / LOAD_SL;
+    constexpr int AUX = READS + (q < 0 ? LOADS : q < LOAD_SL ? (q + 1) * LOADS / LOAD_SL - FIRST : 0);
     constexpr int PER = (AUX + MF - 1) / MF > 2 ? (AUX + MF - 1) / MF : 2;
     const uint32_t pa = (a_rd ^ static_cast<uint32_t>((2 * kk + frag_half) * 16)) + buf;
     const uint32_t pb = (b_rd ^ static_cast<uint32_t>((2 * kk + frag_half) * 16)) + buf;
@@ -296,94 +286,117 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
     hold_set(set ^ 1);
   };
 
-  // ---- the output: a lane's accumulators are four neighbouring columns of one row at a time; lanes 32 apart exchange every second
-  // group, so that each has eight neighbouring columns (16 bytes of bf16) to read, combine and store ----
-  int bias_at = 0;
-  auto epilogue = [&](int id) {
+  // ---- the output: sixteen rows of a wavefront's accumulators at a time go through LDS (fp32, 16-byte slots XOR-ed by the row) and
+  // come back row by row, so that every load and store of the epilogue moves whole cache lines ----
+  // A lane's accumulators are four columns of one row at a time, 32 rows apart in memory: stored from there, a line is written in
+  // four pieces over the whole epilogue, and the output of the tiles at work is more than L2 holds.
+  // The 4 KB lie behind the buffers where there are two.  Where there are three, they are this wavefront's own part of the buffer
+  // that the tile's last step was read from: nobody else touches it before this wavefront requests the step that goes there,
+  // behind the epilogue.
+  auto epilogue = [&](int id, uint32_t stage) {
     int m0, n0;
     locate(id, m0, n0);
     const TileTensors t = tile_tensors<T, MODE>(p, m0, min(BM, p.M - m0));
-    constexpr int PARTS = 8 / E;                          // chunks of eight columns: 1 in bf16, 2 in fp32
-    constexpr int PAIRS = GATED_FWD ? TN / 2 : TN;        // groups of 32 output columns of a wavefront
-    ChunkOperands<T, MODE> operands[2][TM * PARTS];       // of sixteen columns, requested that much ahead
-    auto col_of = [&](int pair, int jp) { return n0 + (wn * PAIRS + pair) * 32 + 16 * jp + 8 * frag_half; };
-    auto row_of = [&](int tm) { return (wm * TM + tm) * 32 + frag_row; };
-    auto request = [&](int step) {
-      if constexpr (MODE != kGatedFwd) {
-        int col = col_of(step >> 1, step & 1);
-        asm volatile("" : "+v"(col));   // offsets are made where they are used, not all of them ahead of the first
-#pragma unroll
-        for (int tm = 0; tm < TM; ++tm)
-#pragma unroll
-          for (int h = 0; h < PARTS; ++h) operands[step & 1][tm * PARTS + h].request(p, t, row_of(tm), col + h * E);
-      }
+    constexpr int COLS = GATED_FWD ? 32 : 64;             // output columns of a wavefront
+    constexpr int LANES = COLS / E, ROWS = 64 / LANES;    // lanes per row, rows per pass
+    constexpr int PASSES = 16 / ROWS, BLOCKS = TM * 2, TOTAL = BLOCKS * PASSES;
+    constexpr int DEPTH = TM > 2 ? 2 : 4;                 // passes whose operands are on their way, as the registers allow
+    const int lane_row = lane / LANES, lane_col = lane % LANES * E;
+    const int col = n0 + wn * COLS + lane_col;
+    ChunkOperands<T, MODE> operands[DEPTH];
+    auto row_of = [&](int pass) {
+      int row = (wm * BLOCKS + pass / PASSES) * 16 + pass % PASSES * ROWS + lane_row;
+      asm volatile("" : "+v"(row));   // offsets are made where they are used, not all of them ahead of the first
+      return row;
     };
-    // eight neighbouring columns (16 jp + 8 half ..) out of an accumulator, which is left empty
-    auto eight = [&](f32x16_t& c, int jp, float* v) {
+    auto request = [&](int pass) { operands[pass % DEPTH].request(p, t, row_of(pass), col); };
+    float bv[E], bu[E];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[8 * jp + i]), __float_as_uint(c[8 * jp + 4 + i]), false, false);
-        v[i] = __uint_as_float(x[0]);
-        v[4 + i] = __uint_as_float(x[1]);
-        c[8 * jp + i] = 0.f;
-        c[8 * jp + 4 + i] = 0.f;
-      }
-    };
-    auto add_bias = [&](int tn, int jp, float* v) {
-      if constexpr (BIAS) {
-        uint4_t b0, b1;
-        const uint32_t from = lds_base + BIAS_OFF + (wave * (NBUF + 1) + bias_at) * BIAS_BYTES + tn * 128 + jp * 64 + frag_half * 32;
-        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:16\n\ts_waitcnt lgkmcnt(0)" : "=&v"(b0), "=&v"(b1) : "v"(from) : "memory");
+    for (int e = 0; e < E; ++e) bv[e] = bu[e] = 0.f;
+    if (BIAS && p.bias) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const int off = col < p.N ? (col + e) * 4 : static_cast<int>(kOutOfRange);
+        const uint4_t b = __builtin_amdgcn_raw_buffer_load_b128(rsrc_bias, off, 0, 0);
+        const uint4_t c = GATED_FWD ? __builtin_amdgcn_raw_buffer_load_b128(rsrc_bias, col < p.N ? off + p.N * 4 : off, 0, 0) : b;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[i] = __uint_as_float(b0[i]);
-          v[4 + i] = __uint_as_float(b1[i]);
+          bv[e + i] = __uint_as_float(b[i]);
+          bu[e + i] = __uint_as_float(c[i]);
         }
+      }
+    }
+    // slot of four columns: (column / 4) ^ row; columns of the up projection lie behind the gate's 32
+    const uint32_t mine = lds_base + (OWN_STAGE ? NBUF * BUF_BYTES + wave * 4096 : stage + wave * A_LD * 1024);
+    const uint32_t wr = mine + (frag_row & 15) * 256;
+    auto stage_block = [&](auto block_c) {   // 16 rows: half the lanes
+      constexpr int block = decltype(block_c)::value, tm = block >> 1;
+      if ((frag_row >> 4) == (block & 1)) {
+#pragma unroll
+        for (int tn = 0; tn < 2; ++tn)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4_t v = {__float_as_uint(acc[tm][tn][4 * j]), __float_as_uint(acc[tm][tn][4 * j + 1]), __float_as_uint(acc[tm][tn][4 * j + 2]),
+                               __float_as_uint(acc[tm][tn][4 * j + 3])};
+            const uint32_t to = wr + (static_cast<uint32_t>((tn * 8 + j * 2 + frag_half) ^ (frag_row & 15)) << 4);
+            asm volatile("ds_write_b128 %0, %1" ::"v"(to), "v"(v) : "memory");
+          }
       }
     };
+    auto from_stage = [&](int row16, int first_col, float* v) {   // E columns of a row; LDS accesses of a wavefront keep their order
+      if constexpr (E == 8) {
+        uint4_t x, y;
+        const uint32_t s0 = mine + row16 * 256 + (((first_col >> 2) ^ row16) << 4), s1 = mine + row16 * 256 + (((first_col >> 2) + 1 ^ row16) << 4);
+        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x), "=&v"(y) : "v"(s0), "v"(s1) : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = __uint_as_float(x[i]);
+          v[4 + i] = __uint_as_float(y[i]);
+        }
+      } else {
+        uint4_t x;
+        asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x) : "v"(mine + row16 * 256 + (((first_col >> 2) ^ row16) << 4)) : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(x[i]);
+      }
+    };
+    // the multiplies are done before their results are read by hand-written instructions
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
     with_activation(p.act, [&](auto act_c) {
       constexpr int ACT = decltype(act_c)::value;
-      request(0);
 #pragma unroll
-      for (int pair = 0; pair < PAIRS; ++pair) {
+      for (int pass = 0; pass < DEPTH; ++pass) request(pass);
+      unrolled<BLOCKS>([&](auto block_c) {
+        stage_block(block_c);
 #pragma unroll
-        for (int jp = 0; jp < 2; ++jp) {
-          if (2 * pair + jp + 1 < 2 * PAIRS) request(2 * pair + jp + 1);
-          const int tn = GATED_FWD ? 2 * pair : pair;
-          int col = col_of(pair, jp);
-          asm volatile("" : "+v"(col));
-          float bv[8], bu[8];
-          if (BIAS && p.bias) {
-            add_bias(tn, jp, bv);
-            if constexpr (GATED_FWD) add_bias(tn + 1, jp, bu);
-          }
+        for (int i = 0; i < PASSES; ++i) {
+          const int pass = decltype(block_c)::value * PASSES + i;
+          float v[E], u[E];
+          from_stage(i * ROWS + lane_row, lane_col, v);
+          if constexpr (GATED_FWD) from_stage(i * ROWS + lane_row, 32 + lane_col, u);
+          if constexpr (BIAS) {
 #pragma unroll
-          for (int tm = 0; tm < TM; ++tm) {
-            float v[8], u[8];
-            eight(acc[tm][tn], jp, v);
-            if constexpr (GATED_FWD) eight(acc[tm][tn + 1], jp, u);
-            if (BIAS && p.bias) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                v[i] += bv[i];
-                if constexpr (GATED_FWD) u[i] += bu[i];
-              }
+            for (int e = 0; e < E; ++e) {
+              v[e] += bv[e];
+              if constexpr (GATED_FWD) u[e] += bu[e];
             }
-#pragma unroll
-            for (int h = 0; h < PARTS; ++h)
-              operands[jp][tm * PARTS + h].template finish<ACT>(p, t, row_of(tm), col + h * E, v + h * E, u + h * E);
-            __builtin_amdgcn_sched_barrier(0);   // one chunk at a time: the registers are the accumulators'
           }
+          operands[pass % DEPTH].template finish<ACT>(p, t, row_of(pass), col, v, u);
+          if (pass + DEPTH < TOTAL) request(pass + DEPTH);
+          __builtin_amdgcn_sched_barrier(0);   // one pass at a time: the registers are the accumulators'
         }
-      }
+      });
     });
-    bias_at = bias_at == NBUF ? 0 : bias_at + 1;
+    clear(acc);
   };
 
-  // Behind an epilogue its stores (this many at least; one that is turned away counts too) are newer requests than the tile that
-  // has to land, with three buffers or more: with two, that tile is requested behind them.
-  constexpr int STORES = TM * (GATED_FWD ? TN / 2 : TN) * 2 * (8 / E) * (MODE == kGatedBwd ? 2 : 1);
-  constexpr int AFTER_STORES = NBUF == 2 ? 0 : AHEAD + STORES < 63 ? AHEAD + STORES : 63;
+  // Behind an epilogue its stores (this many of an output; one that is turned away counts too) are newer requests than the step that
+  // has to land: they are not waited for.  With two buffers all of that step is requested ahead of the epilogue for this.
+  constexpr int STORES = TM * 32 * (GATED_FWD ? 32 : 64) / (64 * E);
+  constexpr int NEWER = NBUF == 2 ? 0 : AHEAD;
+  constexpr int OUTPUTS = MODE == kGatedBwd ? 2 : 1, MORE = MODE == kGatedFwd ? 2 : MODE == kLinBwd ? 0 : 1;   // `out`, `out2`
+  constexpr int AFTER_ONE = NEWER + STORES * OUTPUTS < 63 ? NEWER + STORES * OUTPUTS : 63;
+  constexpr int AFTER_BOTH = NEWER + STORES * (OUTPUTS + MORE) < 63 ? NEWER + STORES * (OUTPUTS + MORE) : 63;
   enter_tile();
 #pragma unroll
   for (int s = 0; s < NBUF - 1; ++s) {
@@ -391,32 +404,57 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
     for (int j = 0; j < LOADS; ++j) issue_load(s * BUF_BYTES, j);
     next_step();
   }
+  constexpr int STARTED = NBUF == 2 ? LOADS : LOADS / LOAD_SL;
 #pragma unroll
-  for (int j = 0; j < LOADS / LOAD_SL; ++j) issue_load((NBUF - 1) * BUF_BYTES, j);
-  wait_and_meet<AHEAD + LOADS / LOAD_SL>();
+  for (int j = 0; j < STARTED; ++j) issue_load((NBUF - 1) * BUF_BYTES, j);
+  if (NBUF == 2) next_step();
+  wait_and_meet<AHEAD + STARTED>();
 #pragma unroll
   for (int i = 0; i < TM + TN; ++i) read_one(a_rd ^ static_cast<uint32_t>(frag_half * 16), b_rd ^ static_cast<uint32_t>(frag_half * 16), 0, i);
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   hold_set(0);
   uint32_t buf = 0, before = (NBUF - 1) * BUF_BYTES;
-  bool stored = false;
+  // One step: its last slice is multiplied behind the barrier that hands over the next one, with the first part of the requests
+  // for the step that takes its buffer.  Behind a tile's last step: all of them where there are two buffers (the first step of
+  // the next tile then requests nothing), none where there are three (the buffer stages the epilogue).
+  constexpr int NONE = LOAD_SL, ALL = -1;
+  auto step = [&](int after_stores, auto first_c, auto last_part) {
+    unrolled<SL - 1>([&](auto s_c) {
+      constexpr int s = decltype(s_c)::value, part = decltype(first_c)::value && NBUF == 2 ? NONE : s + 1;
+      slice(std::integral_constant<int, (s & 1)>{}, buf, std::integral_constant<int, s + 1>{}, std::integral_constant<int, part>{}, before);
+    });
+    if (!(decltype(first_c)::value && NBUF == 2)) next_step();
+    if (after_stores == 0)
+      wait_and_meet<AHEAD>();
+    else if (after_stores == 1)
+      wait_and_meet<AFTER_ONE>();
+    else
+      wait_and_meet<AFTER_BOTH>();
+    before = buf;
+    buf = buf == (NBUF - 1) * BUF_BYTES ? 0 : buf + BUF_BYTES;
+    slice(std::integral_constant<int, ((SL - 1) & 1)>{}, buf, std::integral_constant<int, 0>{}, last_part, before);
+  };
+  std::integral_constant<int, 0> middle;
+  std::integral_constant<int, 1> start;
+  std::integral_constant<int, NBUF == 2 ? ALL : NONE> finish;
+  constexpr bool ONE_STEP = TM <= 2;   // reductions of one step; with 128 accumulators the second way there costs registers (spilled)
+  const int outputs = p.out2 ? 2 : 1;
+  int stored = 0;
   for (int id = first; id < tiles; id += gridDim.x) {
-    for (int kt = 0; kt < nk; ++kt) {
-      unrolled<SL - 1>([&](auto s_c) {
-        constexpr int s = decltype(s_c)::value;
-        slice(std::integral_constant<int, (s & 1)>{}, buf, std::integral_constant<int, s + 1>{}, std::integral_constant<int, s + 1>{}, before);
-      });
-      next_step();
-      if (stored && kt == 0)
-        wait_and_meet<AFTER_STORES>();
-      else
-        wait_and_meet<AHEAD>();
-      before = buf;
-      buf = buf == (NBUF - 1) * BUF_BYTES ? 0 : buf + BUF_BYTES;
-      slice(std::integral_constant<int, ((SL - 1) & 1)>{}, buf, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, before);
+    if (ONE_STEP && nk == 1) {
+      step(stored, start, finish);
+    } else {
+      step(stored, start, middle);
+      for (int kt = 1; kt < nk - 1; ++kt) step(0, middle, middle);
+      step(0, middle, finish);
     }
-    epilogue(id);
-    stored = true;
+    if (NBUF == 2) next_step();
+    epilogue(id, before);
+    if (NBUF > 2) {
+#pragma unroll
+      for (int j = 0; j < LOADS / LOAD_SL; ++j) issue_load(before, j);
+    }
+    stored = outputs;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the zeros behind the last tile land before the LDS goes
 }
@@ -815,8 +853,9 @@ int launch_linear_mode(Context* ctx, LinearArgs& a) {
   const int64_t tiles = static_cast<int64_t>(tiles_over(a.M, 128)) * tiles_over(a.N, kWide ? 64 : 128);
   if (tiles >= 192) {
     if constexpr (sizeof(T) == 2) {
-      if (tiles >= 512) return launch_linear_tile<T, MODE, 2, 2, 2, 4, 3, 64, 2>(ctx, a);
-      return launch_linear_tile<T, MODE, 2, 2, 2, 2, 4, 64, 2>(ctx, a);
+      if (tiles >= 1024 && a.K > 64) return launch_linear_tile<T, MODE, 2, 4, 4, 2, 2, 128, 1>(ctx, a);
+      if (tiles >= 512) return launch_linear_tile<T, MODE, 4, 2, 2, 2, 3, 128, 1>(ctx, a);
+      return launch_linear_tile<T, MODE, 2, 2, 2, 2, 2, 128, 2>(ctx, a);
     } else {
       return launch_linear_tile<T, MODE, 2, 2, 2, 2, 2, 128, 2>(ctx, a);
     }
