@@ -467,18 +467,20 @@ int tch_linear_dgrad(tch_context* ctx, int dtype, const void* dy, int64_t lddy, 
 /* Gated layer: g = x wg^T + bg, u = x wu^T + bu, h = act(g) . u.  w [2F][K] and bias [2F] hold the gate's rows first,
  * pre [M][2F] (may be NULL) = (g | u), h [M][F].
  * dgrad_gated: dh = dy w (wt [F][K] the down projection's weight transposed, dy [M][K]) goes straight into
- * dpre [M][2F] = (dh . u . act'(g) | dh . act(g)); h (may be NULL) [M][F] = act(g) . u again.  dpre may be pre itself. */
+ * dpre [M][2F] = (dh . u . act'(g) | dh . act(g)); h (may be NULL) [M][F] = act(g) . u again.  dpre may be pre itself.
+ * dpre_low, h_low (bf16, may be NULL; laid out like dpre and h): what rounding took off.  A weight gradient of a bf16
+ * gradient and its low part is that of the unrounded gradient, as exact as its fp32 sums. */
 int tch_gated_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* h, int64_t ldh,
                          const float* bias, int act, void* pre, int64_t ldp, int64_t M, int64_t K, int64_t F);
 int tch_linear_dgrad_gated(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, const void* pre,
-                           int64_t ldp, void* dpre, int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t K,
-                           int64_t F);
+                           int64_t ldp, void* dpre, void* dpre_low, int64_t lddp, void* h, void* h_low, int64_t ldh,
+                           int act, int64_t M, int64_t K, int64_t F);
 /* The same derivatives as a pass of their own: dz = dy . act'(pre) [M][N], and the gated form from dh [M][F].  The
- * gradients may be written over dy (dz only) or pre. */
+ * gradients may be written over dy (dz only) or pre; low parts as above. */
 int tch_act_bwd(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* pre, int64_t ldp, void* dz,
-                int64_t lddz, int act, int64_t M, int64_t N);
+                void* dz_low, int64_t lddz, int act, int64_t M, int64_t N);
 int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp,
-                      void* dpre, int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t F);
+                      void* dpre, void* dpre_low, int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t F);
 /* probs = softmax over the last dimension of scale * scores[batch, heads, Lq, Lk] + bias[heads, Lq, Lk]
  * + mask[windows, Lq, Lk] (window = batch index % windows); bias and mask may be NULL; causal != 0 keeps keys
  * j <= i only (Lq == Lk).  In place (probs == scores) is allowed. */

@@ -377,18 +377,18 @@ int tch_gated_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx
 }
 
 int tch_linear_dgrad_gated(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, const void* pre, int64_t ldp, void* dpre,
-                           int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t K, int64_t F) {
-  return linear_dgrad_gated(C(ctx), dtype, rows(dy, lddy), wt, rows(pre, ldp), rows(dpre, lddp), rows(h, ldh), act, M, K, F);
+                           void* dpre_low, int64_t lddp, void* h, void* h_low, int64_t ldh, int act, int64_t M, int64_t K, int64_t F) {
+  return linear_dgrad_gated(C(ctx), dtype, rows(dy, lddy), wt, rows(pre, ldp), rows(dpre, lddp), dpre_low, rows(h, ldh), h_low, act, M, K, F);
 }
 
-int tch_act_bwd(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* pre, int64_t ldp, void* dz, int64_t lddz, int act, int64_t M,
-                int64_t N) {
-  return act_bwd(C(ctx), dtype, rows(dy, lddy), rows(pre, ldp), rows(dz, lddz), rows(nullptr, 0), 0, act, M, N);
+int tch_act_bwd(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* pre, int64_t ldp, void* dz, void* dz_low, int64_t lddz,
+                int act, int64_t M, int64_t N) {
+  return act_bwd(C(ctx), dtype, rows(dy, lddy), rows(pre, ldp), rows(dz, lddz), dz_low, rows(nullptr, 0), 0, act, M, N);
 }
 
-int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp, void* dpre, int64_t lddp, void* h,
-                      int64_t ldh, int act, int64_t M, int64_t F) {
-  return act_bwd(C(ctx), dtype, rows(dh, lddh), rows(pre, ldp), rows(dpre, lddp), rows(h, ldh), 1, act, M, F);
+int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp, void* dpre, void* dpre_low,
+                      int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t F) {
+  return act_bwd(C(ctx), dtype, rows(dh, lddh), rows(pre, ldp), rows(dpre, lddp), dpre_low, rows(h, ldh), 1, act, M, F);
 }
 
 int64_t tch_grad_table_piece_elems(void) { return grad_table_piece_elems(); }

@@ -23,6 +23,7 @@ struct ActBwdArgs {
   const void* z;
   void* dz;
   void* h;
+  void* low;   // bf16: what rounding took off dz, laid out like it; may be null
   int64_t lddy, ldz, lddz, ldh;
   uint32_t chunks;    // rows * row_chunks
   int row_chunks, N, act;
@@ -62,6 +63,18 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
           reinterpret_cast<uint4*>(dz + p.N)[col[i]] = float_to_chunk<T>(u).u;
           if (p.h) reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row[i] * p.ldh)[col[i]] = float_to_chunk<T>(h).u;
         }
+        if constexpr (sizeof(T) == 2) {
+          if (p.low) {
+            T* low = static_cast<T*>(p.low) + row[i] * p.lddz;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              o[e] = rounded_off(o[e]);
+              if (GATED) u[e] = rounded_off(u[e]);
+            }
+            reinterpret_cast<uint4*>(low)[col[i]] = float_to_chunk<T>(o).u;
+            if (GATED) reinterpret_cast<uint4*>(low + p.N)[col[i]] = float_to_chunk<T>(u).u;
+          }
+        }
       }
     }
   });
@@ -94,7 +107,8 @@ int linear_launch(Context* ctx, const char* what, int dtype, int mode, LinearArg
   TCH_CHECK_ARG((reinterpret_cast<uintptr_t>(a.b) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0,
                 name + ": weights and bias must start on a 16-byte boundary");
   TCH_CHECK_ARG(rows_fit(a.a, a.lda, K, eb) && rows_fit(a.out, a.ldo, mode == kGatedBwd ? 2 * N : N, eb) && rows_fit(a.add, a.ldadd, N, eb) &&
-                    rows_fit(a.z, a.ldz, wide * N, eb) && rows_fit(a.out2, a.ldo2, mode == kGatedFwd ? 2 * N : N, eb),
+                    rows_fit(a.z, a.ldz, wide * N, eb) && rows_fit(a.out2, a.ldo2, mode == kGatedFwd ? 2 * N : N, eb) &&
+                    rows_fit(a.low, a.ldo, 2 * N, eb) && rows_fit(a.low2, a.ldo2, N, eb),
                 name + ": rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
   a.M = static_cast<int>(M);
   a.N = static_cast<int>(N);
@@ -143,35 +157,41 @@ int gated_linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, cons
   return linear_launch(ctx, "gated_linear_fwd", dtype, kGatedFwd, a, M, K, F);
 }
 
-int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& pre, const Rows& dpre, const Rows& h, int act,
-                       int64_t M, int64_t K, int64_t F) {
+int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& pre, const Rows& dpre, void* dpre_low, const Rows& h,
+                       void* h_low, int act, int64_t M, int64_t K, int64_t F) {
   TCH_CHECK_ARG(pre.ptr || M == 0, "linear_dgrad_gated: null tensor");
+  TCH_CHECK_ARG(dtype == kBF16 || (!dpre_low && !h_low), "linear_dgrad_gated: fp32 gradients are not rounded: there is no low part");
+  TCH_CHECK_ARG(h.ptr || !h_low, "linear_dgrad_gated: the low part of h comes with h");
   LinearArgs a{};
   a.a = dy.ptr, a.lda = dy.ld;
   a.b = wt;
   a.z = pre.ptr, a.ldz = pre.ld;
   a.out = dpre.ptr, a.ldo = dpre.ld;
   a.out2 = h.ptr, a.ldo2 = h.ld;
+  a.low = dpre_low;
+  a.low2 = h_low;
   a.act = act;
   return linear_launch(ctx, "linear_dgrad_gated", dtype, kGatedBwd, a, M, K, F);
 }
 
-int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, const Rows& h, int gated, int act, int64_t M, int64_t N) {
+int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, void* dz_low, const Rows& h, int gated, int act, int64_t M,
+            int64_t N) {
   if (int rc = check_common("act_bwd", dtype, M, 16, N, act)) return rc;
+  TCH_CHECK_ARG(dtype == kBF16 || !dz_low, "act_bwd: fp32 gradients are not rounded: there is no low part");
   if (M == 0) return 0;
   const int eb = dtype == kBF16 ? 2 : 4;
   const int64_t wide = gated ? 2 : 1;
   TCH_CHECK_ARG(dy.ptr && pre.ptr && dz.ptr, "act_bwd: null tensor");
   TCH_CHECK_ARG(rows_fit(dy.ptr, dy.ld, N, eb) && rows_fit(pre.ptr, pre.ld, wide * N, eb) && rows_fit(dz.ptr, dz.ld, wide * N, eb) &&
-                    rows_fit(h.ptr, h.ld, N, eb),
+                    rows_fit(h.ptr, h.ld, N, eb) && rows_fit(dz_low, dz.ld, wide * N, eb),
                 "act_bwd: rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
   const int row_chunks = static_cast<int>(N * eb / 16);
   TCH_CHECK_ARG(M * row_chunks < (1ll << 31), "act_bwd: tensor exceeds 2^31 chunks");
-  ActBwdArgs a{dy.ptr, pre.ptr, dz.ptr, h.ptr, dy.ld, pre.ld, dz.ld, h.ld, static_cast<uint32_t>(M * row_chunks), row_chunks, static_cast<int>(N), act,
+  ActBwdArgs a{dy.ptr, pre.ptr, dz.ptr, h.ptr, dz_low, dy.ld, pre.ld, dz.ld, h.ld, static_cast<uint32_t>(M * row_chunks), row_chunks, static_cast<int>(N), act,
                FastDiv(static_cast<uint32_t>(row_chunks))};
   const int64_t groups = (M * row_chunks + 256 * kAtOnce - 1) / (256 * kAtOnce);
   const dim3 grid(static_cast<unsigned>(groups < (1 << 20) ? groups : (1 << 20)));
-  const double bytes = static_cast<double>(M) * N * eb * (gated ? (h.ptr ? 6.0 : 5.0) : 3.0);
+  const double bytes = static_cast<double>(M) * N * eb * ((gated ? (h.ptr ? 6.0 : 5.0) : 3.0) + (dz_low ? wide : 0));
   if (gated)
     return dtype == kBF16 ? launch(ctx, act_bwd_kernel<bf16, 1>, grid, dim3(256), a, "act_bwd_kernel<bf16,gated>", bytes, 1)
                           : launch(ctx, act_bwd_kernel<float, 1>, grid, dim3(256), a, "act_bwd_kernel<f32,gated>", bytes, 1);

@@ -120,6 +120,12 @@ __device__ inline void combine(const float* v, float* u, const float* zg, const 
   }
 }
 
+// what rounding v to bf16 takes off (nothing of a value that becomes infinite): with it, a weight gradient is that of the unrounded v
+__device__ inline float rounded_off(float v) {
+  const float r = bf16_bits_to_float(float_to_bf16_bits(v));
+  return fabsf(r) < INFINITY ? v - r : 0.f;
+}
+
 // fn with the activation as a constant
 template <typename F>
 __device__ __forceinline__ void with_activation(int act, F&& fn) {

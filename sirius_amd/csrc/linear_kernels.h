@@ -20,6 +20,8 @@ struct LinearArgs {
   const void* z;      // backward: pre-activations [M][N] or [M][2N]
   void* out;          // [M][N]; gated backward: [M][2N]
   void* out2;         // forward: pre (may be null); gated backward: h (may be null)
+  void* low;          // gated backward, bf16: what rounding took off out and out2 (may be null), laid out like them
+  void* low2;
   int64_t lda, ldadd, ldz, ldo, ldo2;
   int M, N, K, act;
   uint32_t b_bytes;
@@ -32,7 +34,7 @@ namespace {
 // What a tile's epilogue reads and writes beside the accumulators: buffer resources that begin at the tile's first row and end
 // behind its last existing one, so that a row beyond M is dropped by its offset and 64-bit offsets stay out of the lanes.
 struct TileTensors {
-  __amdgpu_buffer_rsrc_t add, z, out, out2;
+  __amdgpu_buffer_rsrc_t add, z, out, out2, low, low2;
 };
 template <typename T>
 __device__ inline __amdgpu_buffer_rsrc_t rows_from(const void* base, int64_t ld, int row0, int rows, int width) {
@@ -47,6 +49,10 @@ __device__ inline TileTensors tile_tensors(const LinearArgs& p, int m0, int rows
   t.z = rows_from<T>(p.z, p.ldz, m0, rows, kWide * p.N);
   t.out = rows_from<T>(p.out, p.ldo, m0, rows, MODE == kGatedBwd ? 2 * p.N : p.N);
   t.out2 = rows_from<T>(p.out2, p.ldo2, m0, rows, MODE == kGatedFwd ? 2 * p.N : p.N);
+  if constexpr (MODE == kGatedBwd) {
+    t.low = rows_from<T>(p.low, p.ldo, m0, rows, 2 * p.N);
+    t.low2 = rows_from<T>(p.low2, p.ldo2, m0, rows, p.N);
+  }
   return t;
 }
 
@@ -109,6 +115,19 @@ struct ChunkOperands {
     if constexpr (MODE == kGatedBwd) {
       write_chunk<T>(t.out, at<T>(row, p.ldo, p.N + col, ok), u);
       if (p.out2) write_chunk<T>(t.out2, at<T>(row, p.ldo2, col, ok), h);
+      if constexpr (sizeof(T) == 2) {
+        if (p.low) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = rounded_off(o[e]), u[e] = rounded_off(u[e]);
+          write_chunk<T>(t.low, at<T>(row, p.ldo, col, ok), o);
+          write_chunk<T>(t.low, at<T>(row, p.ldo, p.N + col, ok), u);
+        }
+        if (p.low2) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) h[e] = rounded_off(h[e]);
+          write_chunk<T>(t.low2, at<T>(row, p.ldo2, col, ok), h);
+        }
+      }
     }
   }
 };
@@ -779,6 +798,20 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
     if constexpr (MODE == kGatedBwd) {
       store_four(out + p.N, u);
       if (p.out2) store_four(out2, h);
+      if constexpr (sizeof(T) == 2) {
+        if (p.low) {
+          T* low = static_cast<T*>(p.low) + row * p.ldo + col;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = rounded_off(o[e]), u[e] = rounded_off(u[e]);
+          store_four(low, o);
+          store_four(low + p.N, u);
+        }
+        if (p.low2) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) h[e] = rounded_off(h[e]);
+          store_four(static_cast<T*>(p.low2) + row * p.ldo2 + col, h);
+        }
+      }
     }
   }
 }
@@ -800,6 +833,7 @@ inline double linear_bytes(const LinearArgs& a, int mode, int eb) {
   if (mode == kLinBwd || mode == kGatedBwd) elems += a.z ? wide * mn : 0.0;
   if (mode == kGatedBwd) elems += mn;
   if (a.out2) elems += mode == kGatedFwd ? 2.0 * mn : mn;
+  elems += (a.low ? 2.0 * mn : 0.0) + (a.low2 ? mn : 0.0);
   return elems * eb + a.b_bytes;
 }
 inline int tiles_over(int n, int tile) { return (n + tile - 1) / tile; }

@@ -199,9 +199,10 @@ int linear_dgrad(Context* ctx, int dtype, const Rows& dy, const void* wt, const 
                  int64_t M, int64_t K, int64_t N);
 int gated_linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows& h, const float* bias, int act, const Rows& pre, int64_t M,
                      int64_t K, int64_t F);
-int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& pre, const Rows& dpre, const Rows& h, int act,
-                       int64_t M, int64_t K, int64_t F);
-int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, const Rows& h, int gated, int act, int64_t M, int64_t N);
+int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& pre, const Rows& dpre, void* dpre_low, const Rows& h,
+                       void* h_low, int act, int64_t M, int64_t K, int64_t F);
+int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, void* dz_low, const Rows& h, int gated, int act, int64_t M,
+            int64_t N);
 
 // grad_norm.hip -- the global norm of many tensors, listed in pieces in device memory, and clipping by it
 int64_t grad_table_piece_elems();

@@ -991,13 +991,23 @@ def linear_dgrad(ctx, dy, wt, dx, act="none", pre=None, residual=None):
                                  pp, ldp, rp, ldr, M, N, K), "tch_linear_dgrad")
 
 
-def act_bwd(ctx, dy, pre, dz, act):
-    """dz = dy . act'(pre), element by element; dz may be dy or pre."""
+def _low(ctx, name, low, high):
+    """The address of a low part: laid out like the tensor it belongs to."""
+    if low is None:
+        return None
+    assert high is not None and low.dtype == high.dtype == torch.bfloat16, f"{name}: the low part of a bf16 tensor"
+    assert low.shape == high.shape and low.stride() == high.stride() and low.device == high.device, f"{name}: laid out like its high part"
+    return ctypes.c_void_p(low.data_ptr())
+
+
+def act_bwd(ctx, dy, pre, dz, act, dz_low=None):
+    """dz = dy . act'(pre), element by element; dz may be dy or pre.  dz_low (bf16): what rounding took off dz, for linear_wgrad."""
     N = dy.shape[-1]
     dyp, lddy, M = _matrix(ctx, "dy", dy, N)
     pp, ldp, _ = _matrix(ctx, "pre", pre, N, M, dy.dtype)
     dzp, lddz, _ = _matrix(ctx, "dz", dz, N, M, dy.dtype)
-    check(lib().tch_act_bwd(ctx.handle, dtype_code(dy), dyp, lddy, pp, ldp, dzp, lddz, _act_code(act), M, N), "tch_act_bwd")
+    check(lib().tch_act_bwd(ctx.handle, dtype_code(dy), dyp, lddy, pp, ldp, dzp, _low(ctx, "dz_low", dz_low, dz), lddz, _act_code(act), M, N),
+          "tch_act_bwd")
 
 
 def _wgrad_blocks(rows, K, N, element):
@@ -1019,40 +1029,60 @@ def linear_bwd_workspace_bytes(x, N):
     return max([conv2d_wgrad_workspace_bytes(dtype_code(x), N, 1, 1, K, _wgrad_splits(x, K, N, rows)) for rows in blocks] + [4])
 
 
-def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=None, residual=None, accumulate=False, workspace=None):
-    """The gradients of linear_fwd: dpre = dy . act'(pre) (act "none": dy itself, and dpre stays untouched), dx = dpre w + residual,
-    dw (+)= dpre^T x and dbias (+)= column sums of dpre, both fp32.  The residual's own gradient is dy.  dx (with wt) or dw may be
-    None.  x and the gradient it meets are contiguous; workspace: linear_bwd_workspace_bytes (without it the weight gradient
-    is not split over its rows)."""
-    K = x.shape[-1]
-    N = dy.shape[-1]
+def linear_wgrad(ctx, x, dy, dw, dbias=None, accumulate=False, workspace=None, dy_low=None, x_low=None):
+    """dw (+)= dy^T x and dbias (+)= column sums of dy, both fp32: x [..., K] and dy [..., N] contiguous, dw [N, K].  dy_low or x_low
+    (bf16): the low part of dy or x (act_bwd, linear_dgrad_gated): the result is then that of the unrounded tensor, in twice the
+    products.  workspace: linear_bwd_workspace_bytes (without it the rows are not split)."""
+    K, N = x.shape[-1], dy.shape[-1]
     M = _matrix(ctx, "x", x, K, None, dy.dtype)[2]
-    assert dy.numel() == M * N, "dy and x have different rows"
-    g = dy
-    if act != "none":
-        assert pre is not None and dpre is not None, "an activation's derivative needs pre, and dpre to keep its result"
-        act_bwd(ctx, dy, pre, dpre, act)
-        g = dpre
-    if dx is not None:
-        linear_dgrad(ctx, g, wt, dx, residual=residual)
-    else:
-        assert residual is None, "a residual without dx"
-    if dw is None:
-        assert dbias is None, "dbias comes with dw"
-        return
+    _matrix(ctx, "dy", dy, N, M)
     assert tuple(dw.shape) == (N, K) and dw.dtype == torch.float32 and dw.device == ctx.stream.device, f"dw: [{N}, {K}] fp32"
-    assert x.is_contiguous() and g.is_contiguous(), "a weight gradient needs contiguous tensors"
+    assert x.is_contiguous() and dy.is_contiguous(), "a weight gradient needs contiguous tensors"
+    assert dy_low is None or x_low is None, "one low part at a time"
+    _low(ctx, "dy_low", dy_low, dy)
+    _low(ctx, "x_low", x_low, x)
     _vector(ctx, "dbias", dbias, N)
     if M == 0:
         for t in (dw, dbias):
             if t is not None and not accumulate:
                 fill_zero(ctx, t)
         return
-    x2, g2, dw4 = x.view(M, 1, 1, K), g.view(M, 1, 1, N), dw.view(N, 1, 1, K)
-    for at, rows in _wgrad_blocks(M, K, N, x.element_size()):
-        splits = 1 if workspace is None else _wgrad_splits(x, K, N, rows)
-        conv2d_wgrad(ctx, x2[at:at + rows], g2[at:at + rows], dw4, 1, 0, workspace=workspace, splits=splits, accumulate=accumulate or at > 0,
-                     dbias=dbias)
+    pairs = [(x, dy, dbias)]
+    if dy_low is not None:
+        pairs.append((x, dy_low, dbias))
+    if x_low is not None:
+        pairs.append((x_low, dy, None))
+    dw4 = dw.view(N, 1, 1, K)
+    for i, (a, g, db) in enumerate(pairs):
+        a, g = a.view(M, 1, 1, K), g.view(M, 1, 1, N)
+        for at, rows in _wgrad_blocks(M, K, N, a.element_size()):
+            splits = 1 if workspace is None else _wgrad_splits(a, K, N, rows)
+            conv2d_wgrad(ctx, a[at:at + rows], g[at:at + rows], dw4, 1, 0, workspace=workspace, splits=splits,
+                         accumulate=accumulate or at > 0 or i > 0, dbias=db)
+
+
+def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=None, residual=None, accumulate=False, workspace=None,
+               dpre_low=None, dy_low=None, x_low=None):
+    """The gradients of linear_fwd: dpre = dy . act'(pre) (act "none": dy itself, and dpre stays untouched), dx = dpre w + residual,
+    dw (+)= dpre^T x and dbias (+)= column sums of dpre, both fp32.  The residual's own gradient is dy.  dx (with wt) or dw may be
+    None.  x and the gradient it meets are contiguous; workspace: linear_bwd_workspace_bytes (without it the weight gradient
+    is not split over its rows).  bf16: dpre is rounded, and so are its products, except where dpre_low (like dpre) keeps what
+    rounding takes off it: dw and dbias are then those of the unrounded dpre.  dy_low, x_low: as for linear_wgrad."""
+    N = dy.shape[-1]
+    g, low = dy, dy_low
+    if act != "none":
+        assert pre is not None and dpre is not None, "an activation's derivative needs pre, and dpre to keep its result"
+        assert dy_low is None, "dy_low goes with a gradient that is multiplied as it is"
+        act_bwd(ctx, dy, pre, dpre, act, dz_low=dpre_low)
+        g, low = dpre, dpre_low
+    if dx is not None:
+        linear_dgrad(ctx, g, wt, dx, residual=residual)
+    else:
+        assert residual is None, "a residual without dx"
+    if dw is not None:
+        linear_wgrad(ctx, x, g, dw, dbias=dbias, accumulate=accumulate, workspace=workspace, dy_low=low, x_low=x_low)
+    else:
+        assert dbias is None, "dbias comes with dw"
 
 
 def gated_linear_fwd(ctx, x, w, h, bias=None, act="silu", pre=None):
@@ -1069,35 +1099,38 @@ def gated_linear_fwd(ctx, x, w, h, bias=None, act="silu", pre=None):
                                      _vector(ctx, "bias", bias, F2), _act_code(act), pp, ldp, M, K, F), "tch_gated_linear_fwd")
 
 
-def gated_act_bwd(ctx, dh, pre, dpre, act="silu", h=None):
-    """dpre = (dh . u . act'(g) | dh . act(g)) from pre = (g | u), element by element; h = act(g) . u again.  dpre may be pre."""
+def gated_act_bwd(ctx, dh, pre, dpre, act="silu", h=None, dpre_low=None):
+    """dpre = (dh . u . act'(g) | dh . act(g)) from pre = (g | u), element by element; h = act(g) . u again.  dpre may be pre.
+    dpre_low (bf16): what rounding took off dpre, for linear_wgrad."""
     F = dh.shape[-1]
     dhp, lddh, M = _matrix(ctx, "dh", dh, F)
     pp, ldp, _ = _matrix(ctx, "pre", pre, 2 * F, M, dh.dtype)
     dpp, lddp, _ = _matrix(ctx, "dpre", dpre, 2 * F, M, dh.dtype)
     hp, ldh, _ = _matrix(ctx, "h", h, F, M, dh.dtype)
-    check(lib().tch_gated_act_bwd(ctx.handle, dtype_code(dh), dhp, lddh, pp, ldp, dpp, lddp, hp, ldh, _act_code(act), M, F),
-          "tch_gated_act_bwd")
+    check(lib().tch_gated_act_bwd(ctx.handle, dtype_code(dh), dhp, lddh, pp, ldp, dpp, _low(ctx, "dpre_low", dpre_low, dpre), lddp, hp, ldh,
+                                  _act_code(act), M, F), "tch_gated_act_bwd")
 
 
-def linear_dgrad_gated(ctx, dy, wt, pre, dpre, act="silu", h=None):
+def linear_dgrad_gated(ctx, dy, wt, pre, dpre, act="silu", h=None, dpre_low=None, h_low=None):
     """The data gradient of a projection behind a gated layer, through that layer's product and activation, in one launch:
     dh = dy w stays on the chip, dpre = (dh . u . act'(g) | dh . act(g)) [..., 2F] is stored, and h = act(g) . u again where it is
-    asked for (the forward pass need not keep it).  wt [F, N] is the projection's weight [N, F] transposed, dy [..., N]."""
+    asked for (the forward pass need not keep it).  wt [F, N] is the projection's weight [N, F] transposed, dy [..., N].
+    dpre_low, h_low (bf16): what rounding took off dpre and h, for linear_wgrad."""
     F, N = wt.shape
     dyp, lddy, M = _matrix(ctx, "dy", dy, N)
     pp, ldp, _ = _matrix(ctx, "pre", pre, 2 * F, M, dy.dtype)
     dpp, lddp, _ = _matrix(ctx, "dpre", dpre, 2 * F, M, dy.dtype)
     hp, ldh, _ = _matrix(ctx, "h", h, F, M, dy.dtype)
-    check(lib().tch_linear_dgrad_gated(ctx.handle, dtype_code(dy), dyp, lddy, _weights(ctx, "wt", wt, dy.dtype), pp, ldp, dpp, lddp, hp, ldh,
+    check(lib().tch_linear_dgrad_gated(ctx.handle, dtype_code(dy), dyp, lddy, _weights(ctx, "wt", wt, dy.dtype), pp, ldp, dpp,
+                                       _low(ctx, "dpre_low", dpre_low, dpre), lddp, hp, _low(ctx, "h_low", h_low, h), ldh,
                                        _act_code(act), M, N, F), "tch_linear_dgrad_gated")
 
 
-def gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=None, act="silu", residual=None, accumulate=False, workspace=None):
+def gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=None, act="silu", residual=None, accumulate=False, workspace=None, dpre_low=None):
     """The gradients of gated_linear_fwd from dh [..., F]: dpre [..., 2F] as in gated_act_bwd, dx = dpre w + residual,
     dw (+)= dpre^T x, dbias (+)= column sums of dpre.  wt [K, 2F] is w transposed; the rest as for linear_bwd."""
-    gated_act_bwd(ctx, dh, pre, dpre, act)
-    linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=dbias, residual=residual, accumulate=accumulate, workspace=workspace)
+    gated_act_bwd(ctx, dh, pre, dpre, act, dpre_low=dpre_low)
+    linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=dbias, residual=residual, accumulate=accumulate, workspace=workspace, dy_low=dpre_low)
 
 
 def attn_softmax_fwd(ctx, scores, probs, scale=1.0, bias=None, mask=None, causal=False):

@@ -187,11 +187,13 @@ def test_data_gradients(ctx, M, K, N, dtype):
             near(h.view, ref, tol + u * (ref.abs() + tol), f"{act} h")
 
 
-def check_backward(got, dpre, x, w, u, extra, residual=None, dw0=None, db0=None):
-    """dx, dw, db against fp64; dpre [M, N] in fp64 with `extra`, what it may be off before it is rounded to the type."""
+def check_backward(got, dpre, x, w, u, extra, residual=None, dw0=None, db0=None, low=False):
+    """dx, dw, db against fp64; dpre [M, N] in fp64 with `extra`, what it may be off before it is rounded to the type.  low: the
+    weight gradient had its low part, which leaves 2^-8 of what rounding took off (2^-8): 2^-16."""
     dx, dw, db = got
     M, N = dpre.shape
     edp = extra + u * (dpre.abs() + extra)
+    edw = extra + 2.0 ** -16 * (dpre.abs() + extra) if low else edp
     wd, xd = w.double(), x.double()
     ref = dpre @ wd
     tol = edp @ wd.abs() + (N + 8) * 2.0 ** -23 * (dpre.abs() @ wd.abs())
@@ -199,13 +201,13 @@ def check_backward(got, dpre, x, w, u, extra, residual=None, dw0=None, db0=None)
         ref = ref + residual.double()
         tol = tol + 2.0 ** -23 * ref.abs()
     near(dx, ref, tol + u * (ref.abs() + tol), "dx")
-    sums = (M + 64) * 2.0 ** -23      # the split reduction adds partial sums on top
-    ref, tol = dpre.t() @ xd, edp.t() @ xd.abs() + sums * (dpre.abs().t() @ xd.abs())
+    sums = ((2 if low else 1) * M + 64) * 2.0 ** -23      # the split reduction adds partial sums on top
+    ref, tol = dpre.t() @ xd, edw.t() @ xd.abs() + sums * (dpre.abs().t() @ xd.abs())
     if dw0 is not None:
         ref = ref + dw0.double()
         tol = tol + 2.0 ** -23 * ref.abs()
     near(dw, ref, tol + 2.0 ** -23 * ref.abs() + 1e-30, "dw")
-    ref, tol = dpre.sum(0), edp.sum(0) + sums * dpre.abs().sum(0)
+    ref, tol = dpre.sum(0), edw.sum(0) + sums * dpre.abs().sum(0)
     if db0 is not None:
         ref = ref + db0.double()
         tol = tol + 2.0 ** -23 * ref.abs()
@@ -225,16 +227,17 @@ def test_linear_bwd(ctx, M, K, N, dtype):
     wt = w.t().contiguous()
     for i, act in enumerate(ACTS):
         accumulate, with_res, split = i in (1, 3), i in (1, 2), i != 2
+        low = torch.empty_like(dy) if dtype == BF16 and i in (1, 2, 4) else None
         dx, dpre = torch.empty_like(x), torch.empty_like(dy)
         dw, db = rnd(N, K, dtype=F32, seed=6), rnd(N, dtype=F32, seed=7)
         dw0, db0 = (dw.clone(), db.clone()) if accumulate else (None, None)
         ws = torch.empty(ops.linear_bwd_workspace_bytes(x, N), dtype=torch.uint8, device="cuda") if split else None
         ops.linear_bwd(ctx, dy, x, wt, dx, dw, dbias=db, act=act, pre=pre, dpre=dpre, residual=res if with_res else None,
-                       accumulate=accumulate, workspace=ws)
+                       accumulate=accumulate, workspace=ws, dpre_low=low)
         s = slope(pre.double(), act)
         ref = dy.double() * s
         extra = torch.zeros_like(ref) if act == "none" else 2.0 ** -19 * dy.double().abs()
-        check_backward((dx, dw, db), ref, x, w, u, extra, res if with_res else None, dw0, db0)
+        check_backward((dx, dw, db), ref, x, w, u, extra, res if with_res else None, dw0, db0, low is not None)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
@@ -245,12 +248,62 @@ def test_gated_linear_bwd(ctx, M, K, F, dtype):
     x, w = rnd(M, K, dtype=dtype, seed=1), rnd(2 * F, K, dtype=dtype, seed=2, std=1 / math.sqrt(K))
     dh, pre = rnd(M, F, dtype=dtype, seed=3), rnd(M, 2 * F, dtype=dtype, seed=4, std=2.0)
     wt = w.t().contiguous()
-    for act in ACTS:
+    for i, act in enumerate(ACTS):
+        low = torch.empty_like(pre) if dtype == BF16 and i in (0, 2, 4) else None
         dx, dpre = torch.empty_like(x), torch.empty_like(pre)
         dw, db = torch.empty(2 * F, K, device="cuda"), torch.empty(2 * F, device="cuda")
         ws = torch.empty(ops.linear_bwd_workspace_bytes(x, 2 * F), dtype=torch.uint8, device="cuda")
-        ops.gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=db, act=act, workspace=ws)
+        ops.gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=db, act=act, workspace=ws, dpre_low=low)
         d, g, up = dh.double(), pre[:, :F].double(), pre[:, F:].double()
         ref = torch.cat([d * up * slope(g, act), d * value(g, act)], 1)
         extra = torch.cat([2.0 ** -19 * (d * up).abs(), 2.0 ** -20 * (d * g).abs()], 1) + 2.0 ** -22 * ref.abs()
-        check_backward((dx, dw, db), ref, x, w, u, extra)
+        check_backward((dx, dw, db), ref, x, w, u, extra, low=low is not None)
+
+
+@pytest.mark.parametrize("M,C,F", [(5, 72, 40), (130, 264, 520), (1100, 512, 1544), (2100, 520, 2056)])
+def test_feed_forward_block(ctx, M, C, F):
+    """A whole gated block as a training step runs it: gated layer, down projection with the block's residual, and back through
+    linear_dgrad_gated with low parts; the inner results are the program's own rounded ones, everything against fp64."""
+    from sirius_amd import ops
+    u = half_step(BF16)
+    x, res = rnd(M, C, dtype=BF16, seed=1), rnd(M, C, dtype=BF16, seed=2)
+    w, wd = rnd(2 * F, C, dtype=BF16, seed=3, std=1 / math.sqrt(C)), rnd(C, F, dtype=BF16, seed=4, std=1 / math.sqrt(F))
+    bias, dy = rnd(2 * F, dtype=F32, seed=5), rnd(M, C, dtype=BF16, seed=6)
+    wt, wdt = w.t().contiguous(), wd.t().contiguous()
+
+    def new(*shape, dtype=BF16):
+        return torch.empty(shape, dtype=dtype, device="cuda")
+    h, pre, y = new(M, F), new(M, 2 * F), new(M, C)
+    dpre, dpre_low, h2, h2_low, dx = new(M, 2 * F), new(M, 2 * F), new(M, F), new(M, F), new(M, C)
+    dw, db, dwd = new(2 * F, C, dtype=F32), new(2 * F, dtype=F32), new(C, F, dtype=F32)
+    ws, wsd = (new(ops.linear_bwd_workspace_bytes(*a), dtype=torch.uint8) for a in ((x, 2 * F), (h, C)))
+    ops.gated_linear_fwd(ctx, x, w, h, bias=bias, act="silu", pre=pre)
+    ops.linear_fwd(ctx, h, wd, y, residual=res)
+    ops.linear_dgrad_gated(ctx, dy, wdt, pre, dpre, act="silu", h=h2, dpre_low=dpre_low, h_low=h2_low)
+    ops.linear_wgrad(ctx, h2, dy, dwd, workspace=wsd, x_low=h2_low)
+    ops.linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=db, residual=dy, workspace=ws, dy_low=dpre_low)
+
+    z, e = product(x, w)
+    z, e = z + bias.double(), e + 2.0 ** -23 * (z.abs() + bias.abs().double())
+    near(pre, z, e + u * (z.abs() + e), "pre")
+    g, up = z[:, :F], z[:, F:]
+    a, ea = value(g, "silu"), 1.2 * e[:, :F] + 2.0 ** -20 * g.abs()
+    ref, tol = a * up, ea * (up.abs() + e[:, F:]) + a.abs() * e[:, F:] + 2.0 ** -23 * (a * up).abs()
+    near(h, ref, tol + u * (ref.abs() + tol), "h")
+    v, ev = product(h, wd)
+    ref = v + res.double()
+    near(y, ref, ev + u * (ref.abs() + ev) + 2.0 ** -23 * ref.abs(), "y")
+
+    dh, edh = product(dy, wdt)
+    g, up = pre[:, :F].double(), pre[:, F:].double()
+    a, s = value(g, "silu"), slope(g, "silu")
+    exact = torch.cat([dh * up * s, dh * a], 1)
+    edp = torch.cat([(edh * s.abs() + 2.0 ** -19 * (dh.abs() + edh)) * up.abs(), edh * a.abs() + 2.0 ** -20 * g.abs() * (dh.abs() + edh)], 1)
+    edp = edp + 2.0 ** -22 * exact.abs()
+    both = dpre.double() + dpre_low.double()
+    near(both, exact, edp + 2.0 ** -16 * (exact.abs() + edp), "dpre and its low part")
+    eh = 2.0 ** -20 * (g * up).abs() + 2.0 ** -16 * (a * up).abs()
+    near(h2.double() + h2_low.double(), a * up, eh, "h and its low part")
+    ref = dy.double().t() @ (a * up)
+    near(dwd, ref, dy.abs().double().t() @ eh + (2 * M + 64) * 2.0 ** -23 * (dy.abs().double().t() @ (a * up).abs()) + 2.0 ** -23 * ref.abs(), "dw_down")
+    check_backward((dx, dw, db), exact, x, w, u, edp, residual=dy, low=True)
