@@ -191,22 +191,26 @@ def _record(s, case):
             wt = s["w"].t().contiguous()
             dx, dpre = new(M, K), new(M, wide)
             dw, db = new(wide, K, dtype=torch.float32), new(wide, dtype=torch.float32)
+            # weight gradients are fp32: those of bf16 gradients take the gradients' low parts as well
+            dpre_low = new(M, wide) if case["dtype"] == "bf16" else None
             scratch = new(ops.linear_bwd_workspace_bytes(s["x"], wide), dtype=torch.uint8)
-            s["keep"], s["out"] = (wt, dpre, scratch), [dx, dw, db]
+            s["keep"], s["out"] = (wt, dpre, dpre_low, scratch), [dx, dw, db]
             if op == "linear_bwd":
                 calls = [lambda: ops.linear_bwd(ctx, s["dy"], s["x"], wt, dx, dw, dbias=db, act=act, pre=s["pre"], dpre=dpre,
-                                                workspace=scratch)]
+                                                workspace=scratch, dpre_low=dpre_low)]
             elif op == "gated_bwd":
                 calls = [lambda: ops.gated_linear_bwd(ctx, s["dy"], s["x"], wt, dx, dw, s["pre"], dpre, dbias=db, act=act,
-                                                      workspace=scratch)]
+                                                      workspace=scratch, dpre_low=dpre_low)]
             else:
                 wt_down = s["w_down"].t().contiguous()
                 h, dw_down = new(M, N), new(K, N, dtype=torch.float32)
+                h_low = new(M, N) if case["dtype"] == "bf16" else None
                 scratch_down = new(ops.linear_bwd_workspace_bytes(h, K), dtype=torch.uint8)
-                s["keep"], s["out"] = (wt, wt_down, dpre, h, scratch, scratch_down), [dx, dw, dw_down]
-                calls = [lambda: ops.linear_dgrad_gated(ctx, s["dy"], wt_down, s["pre"], dpre, act=act, h=h),
-                         lambda: ops.linear_bwd(ctx, s["dy"], h, None, None, dw_down, workspace=scratch_down),
-                         lambda: ops.linear_bwd(ctx, dpre, s["x"], wt, dx, dw, workspace=scratch)]
+                s["keep"], s["out"] = (wt, wt_down, dpre, dpre_low, h, h_low, scratch, scratch_down), [dx, dw, dw_down]
+                calls = [lambda: ops.linear_dgrad_gated(ctx, s["dy"], wt_down, s["pre"], dpre, act=act, h=h, dpre_low=dpre_low,
+                                                        h_low=h_low),
+                         lambda: ops.linear_bwd(ctx, s["dy"], h, None, None, dw_down, workspace=scratch_down, x_low=h_low),
+                         lambda: ops.linear_bwd(ctx, dpre, s["x"], wt, dx, dw, workspace=scratch, dy_low=dpre_low)]
     prog = ops.Program()
     ctx.begin_record(prog)
     try:
