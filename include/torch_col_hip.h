@@ -481,6 +481,14 @@ int tch_act_bwd(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const
                 void* dz_low, int64_t lddz, int act, int64_t M, int64_t N);
 int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp,
                       void* dpre, void* dpre_low, int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t F);
+/* Weight and bias gradients of a bf16 layer: dw [N][K] (+)= dy^T x, dbias [N] (may be NULL) (+)= column sums of dy, both
+ * fp32; x [M][K] and dy [M][N] dense.  x_low or dy_low (one of them, or none): the low part of that operand; both parts
+ * are multiplied.  workspace: partial sums where the rows are split, at least tch_linear_wgrad_workspace_bytes; NULL: the
+ * rows are not split.  (fp32 layers: tch_conv2d_wgrad with 1x1 filters.) */
+int64_t tch_linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int tch_linear_wgrad(tch_context* ctx, const void* x, const void* x_low, const void* dy, const void* dy_low, float* dw,
+                     float* dbias, int accumulate, int64_t M, int64_t K, int64_t N, void* workspace,
+                     int64_t workspace_bytes);
 /* probs = softmax over the last dimension of scale * scores[batch, heads, Lq, Lk] + bias[heads, Lq, Lk]
  * + mask[windows, Lq, Lk] (window = batch index % windows); bias and mask may be NULL; causal != 0 keeps keys
  * j <= i only (Lq == Lk).  In place (probs == scores) is allowed. */

@@ -391,6 +391,13 @@ int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh,
   return act_bwd(C(ctx), dtype, rows(dh, lddh), rows(pre, ldp), rows(dpre, lddp), dpre_low, rows(h, ldh), 1, act, M, F);
 }
 
+int64_t tch_linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N) { return linear_wgrad_workspace_bytes(M, K, N); }
+
+int tch_linear_wgrad(tch_context* ctx, const void* x, const void* x_low, const void* dy, const void* dy_low, float* dw, float* dbias, int accumulate,
+                     int64_t M, int64_t K, int64_t N, void* workspace, int64_t workspace_bytes) {
+  return linear_wgrad(C(ctx), x, x_low, dy, dy_low, dw, dbias, accumulate, M, K, N, workspace, workspace_bytes);
+}
+
 int64_t tch_grad_table_piece_elems(void) { return grad_table_piece_elems(); }
 int64_t tch_grad_norm_workspace_bytes(int64_t pieces) { return grad_norm_workspace_bytes(pieces); }
 

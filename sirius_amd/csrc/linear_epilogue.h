@@ -13,6 +13,9 @@
 
 namespace tch {
 
+// Left to itself the compiler stops inlining where a kernel gets long, and whatever a lambda refers to, accumulators too, is in memory then.
+#define LINEAR_INLINE __attribute__((always_inline))
+
 enum LinearMode : int { kLinFwd = 0, kLinBwd = 1, kGatedFwd = 2, kGatedBwd = 3 };
 enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActCount = 5 };
 

@@ -80,7 +80,7 @@ __device__ inline void write_chunk(__amdgpu_buffer_rsrc_t rsrc, int off, const f
 template <typename T, int MODE>
 struct ChunkOperands {
   Chunk zg, zu, add;
-  __device__ inline void request(const LinearArgs& p, const TileTensors& t, int row, int col) {
+  __device__ __forceinline__ void request(const LinearArgs& p, const TileTensors& t, int row, int col) {
     const bool ok = col < p.N;
     if constexpr (MODE == kLinBwd || MODE == kGatedBwd) {
       if (MODE == kGatedBwd || p.act != kActNone) zg = read_chunk(t.z, at<T>(row, p.ldz, col, ok));
@@ -90,7 +90,7 @@ struct ChunkOperands {
       if (p.add) add = read_chunk(t.add, at<T>(row, p.ldadd, col, ok));
   }
   template <int ACT>
-  __device__ inline void finish(const LinearArgs& p, const TileTensors& t, int row, int col, const float* v, float* u) {
+  __device__ __forceinline__ void finish(const LinearArgs& p, const TileTensors& t, int row, int col, const float* v, float* u) {
     constexpr int E = Elem<T>::kPerChunk;
     const bool ok = col < p.N;
     float fg[E], fu[E], o[E], h[E];
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
 
   // consecutive tiles walk down group_rows row tiles before they move one column tile on: the tiles an XCD works on at one time
   // form a block, with fewer distinct operand rows through its L2
-  auto locate = [&](int id, int& m0, int& n0) {
+  auto locate = [&](int id, int& m0, int& n0) LINEAR_INLINE {
     uint32_t q, rem;
     if (p.group_rows <= 1) {
       p.div_tiles_n.divmod(static_cast<uint32_t>(id), q, rem);
@@ -223,13 +223,13 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
   const __amdgpu_buffer_rsrc_t rsrc_bias = make_rsrc(p.bias, BIAS && p.bias ? static_cast<uint32_t>(p.N) * (GATED_FWD ? 8u : 4u) : 0u);
   int ld_id = first, ld_kt = 0;
-  auto mark_tail = [&] {
+  auto mark_tail = [&]() LINEAR_INLINE {
 #pragma unroll
     for (int j = 0; j < A_LD; ++j) a_off[j] |= behind_k[(wave * A_LD + j) & 1];
 #pragma unroll
     for (int j = 0; j < B_LD; ++j) b_off[j] |= behind_k[(wave * B_LD + j) & 1];
   };
-  auto enter_tile = [&] {
+  auto enter_tile = [&]() LINEAR_INLINE {
     int m0 = 0, n0 = 0;
     const bool any = ld_id < tiles;
     if (any) locate(ld_id, m0, n0);
@@ -246,13 +246,13 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
       if (ragged_k && nk == 1) mark_tail();
     }
   };
-  auto issue_load = [&](uint32_t buf, int j) {   // direct load j of the step the walk stands at
+  auto issue_load = [&](uint32_t buf, int j) LINEAR_INLINE {   // direct load j of the step the walk stands at
     if (j < A_LD)
       load_to_lds(rsrc_a, lds + buf + (wave * A_LD + j) * 1024, static_cast<int>(a_off[j]), ld_kt * RB);
     else
       load_to_lds(rsrc_b, lds + buf + A_BYTES + (wave * B_LD + j - A_LD) * 1024, static_cast<int>(b_off[j - A_LD]), ld_kt * RB);
   };
-  auto next_step = [&] {
+  auto next_step = [&]() LINEAR_INLINE {
     if (++ld_kt == nk) {
       ld_kt = 0;
       ld_id += gridDim.x;
@@ -284,17 +284,17 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   };
   // multiplies the slice in `set`; meanwhile slice kk of the step in `buf` is read into the other set and part `q` of the loads
   // (-1: all of them) goes to `ld_buf`
-  auto slice = [&](auto set_c, uint32_t buf, auto kk_c, auto q_c, uint32_t ld_buf) {
+  auto slice = [&](auto set_c, uint32_t buf, auto kk_c, auto q_c, uint32_t ld_buf) LINEAR_INLINE {
     constexpr int set = decltype(set_c)::value, kk = decltype(kk_c)::value, q = decltype(q_c)::value;
     constexpr int READS = TM + TN, MF = TM * TN, FIRST = q < 0 ? 0 : (q < LOAD_SL ? q : LOAD_SL) * LOADS / LOAD_SL;
     constexpr int AUX = READS + (q < 0 ? LOADS : q < LOAD_SL ? (q + 1) * LOADS / LOAD_SL - FIRST : 0);
     constexpr int PER = (AUX + MF - 1) / MF > 2 ? (AUX + MF - 1) / MF : 2;
     const uint32_t pa = (a_rd ^ static_cast<uint32_t>((2 * kk + frag_half) * 16)) + buf;
     const uint32_t pb = (b_rd ^ static_cast<uint32_t>((2 * kk + frag_half) * 16)) + buf;
-    unrolled<MF>([&](auto m_c) {
+    unrolled<MF>([&](auto m_c) LINEAR_INLINE {
       constexpr int m = decltype(m_c)::value, tm = m / TN, tn = m % TN;
       mma32<T>(fb[set][tn], fa[set][tm], acc[tm][tn]);
-      unrolled<PER>([&](auto a_c) {
+      unrolled<PER>([&](auto a_c) LINEAR_INLINE {
         constexpr int a = m * PER + decltype(a_c)::value;
         if constexpr (a < READS) read_one(pa, pb, set ^ 1, a);
         else if constexpr (a < AUX) issue_load(ld_buf, FIRST + a - READS);
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   // The 4 KB lie behind the buffers where there are two.  Where there are three, they are this wavefront's own part of the buffer
   // that the tile's last step was read from: nobody else touches it before this wavefront requests the step that goes there,
   // behind the epilogue.
-  auto epilogue = [&](int id, uint32_t stage) {
+  auto epilogue = [&](int id, uint32_t stage) LINEAR_INLINE {
     int m0, n0;
     locate(id, m0, n0);
     const TileTensors t = tile_tensors<T, MODE>(p, m0, min(BM, p.M - m0));
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
       asm volatile("" : "+v"(row));   // offsets are made where they are used, not all of them ahead of the first
       return row;
     };
-    auto request = [&](int pass) { operands[pass % DEPTH].request(p, t, row_of(pass), col); };
+    auto request = [&](int pass) LINEAR_INLINE { operands[pass % DEPTH].request(p, t, row_of(pass), col); };
     float bv[E], bu[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) bv[e] = bu[e] = 0.f;
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
     // slot of four columns: (column / 4) ^ row; columns of the up projection lie behind the gate's 32
     const uint32_t mine = lds_base + (OWN_STAGE ? NBUF * BUF_BYTES + wave * 4096 : stage + wave * A_LD * 1024);
     const uint32_t wr = mine + (frag_row & 15) * 256;
-    auto stage_block = [&](auto block_c) {   // 16 rows: half the lanes
+    auto stage_block = [&](auto block_c) LINEAR_INLINE {   // 16 rows: half the lanes
       constexpr int block = decltype(block_c)::value, tm = block >> 1;
       if ((frag_row >> 4) == (block & 1)) {
 #pragma unroll
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
           }
       }
     };
-    auto from_stage = [&](int row16, int first_col, float* v) {   // E columns of a row; LDS accesses of a wavefront keep their order
+    auto from_stage = [&](int row16, int first_col, float* v) LINEAR_INLINE {   // E columns of a row; LDS accesses of a wavefront keep their order
       if constexpr (E == 8) {
         uint4_t x, y;
         const uint32_t s0 = mine + row16 * 256 + (((first_col >> 2) ^ row16) << 4), s1 = mine + row16 * 256 + (((first_col >> 2) + 1 ^ row16) << 4);
@@ -381,11 +381,11 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
     };
     // the multiplies are done before their results are read by hand-written instructions
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-    with_activation(p.act, [&](auto act_c) {
+    with_activation(p.act, [&](auto act_c) LINEAR_INLINE {
       constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
       for (int pass = 0; pass < DEPTH; ++pass) request(pass);
-      unrolled<BLOCKS>([&](auto block_c) {
+      unrolled<BLOCKS>([&](auto block_c) LINEAR_INLINE {
         stage_block(block_c);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
@@ -437,8 +437,8 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   // for the step that takes its buffer.  Behind a tile's last step: all of them where there are two buffers (the first step of
   // the next tile then requests nothing), none where there are three (the buffer stages the epilogue).
   constexpr int NONE = LOAD_SL, ALL = -1;
-  auto step = [&](int after_stores, auto first_c, auto last_part) {
-    unrolled<SL - 1>([&](auto s_c) {
+  auto step = [&](int after_stores, auto first_c, auto last_part) LINEAR_INLINE {
+    unrolled<SL - 1>([&](auto s_c) LINEAR_INLINE {
       constexpr int s = decltype(s_c)::value, part = decltype(first_c)::value && NBUF == 2 ? NONE : s + 1;
       slice(std::integral_constant<int, (s & 1)>{}, buf, std::integral_constant<int, s + 1>{}, std::integral_constant<int, part>{}, before);
     });

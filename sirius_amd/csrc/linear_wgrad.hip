@@ -1,0 +1,387 @@
+// Weight and bias gradients of linear layers in bf16: dw (+)= dy^T x over the rows, dbias (+)= column sums of dy, in fp32.
+//
+// One of the operands may come with a low part (what rounding to bf16 took off it: linear_epilogue.h, rounded_off); the gradient is
+// then that of the unrounded operand, in twice the multiplies.  Both parts add to the same accumulators, and share the other
+// operand's tile in LDS and in registers: a step moves 1.5 times the bytes for twice the multiplies.
+//
+// Both operands are contiguous along the output's axes and strided along the reduction, the opposite of what an MFMA operand wants:
+// tiles of 32 rows are kept as they come, [row][column], and read transposed (ds_read_b64_tr_b16: sixteen lanes fetch a patch of 4
+// rows x 16 columns, each keeps 4 rows of one column).  The 16-byte slot of a column is XOR-ed by four times the row, so that
+// the 64-byte patches of the eight rows of a read lie in different banks.  Element 4t + i of lane half h is row 8t + 4h + i of a
+// sixteen-row slice, for both operands alike.
+#include "direct_load.h"
+#include "fp32_split.h"
+#include "linear_epilogue.h"
+
+#include "context.h"
+#include "ops.h"
+
+namespace tch {
+namespace {
+
+struct LinearWgradArgs {
+  const void* a;        // dy [M][N]
+  const void* a_low;
+  const void* b;        // x [M][K]
+  const void* b_low;
+  float* out;           // dw [N][K], or partial sums [split][N][K]
+  float* bias;          // dbias [N], or partial sums [split][N]; may be null
+  int64_t M;
+  int N, K;
+  int rows_per_split;   // a multiple of 32
+  int tiles_k, tiles;   // column tiles; tiles of one split
+  int accumulate;       // without splits: out and bias are added to
+  FastDiv div_tiles, div_tiles_k;
+};
+
+enum Pair : int { kNoLow = 0, kLowA = 1, kLowB = 2 };
+constexpr int kRows = 32;   // of a reduction step
+
+// WM x WN wavefronts of TM x TN MFMA tiles (32 x 32).  NBUF tiles in LDS, one barrier per step; the sixteen-row slice that is multiplied
+// next is read while this one is multiplied, and the direct loads of the step NBUF - 1 ahead go out between the multiplies.
+// What bounds it is LDS: per slice of 256 x 256 with a low part 64 KB read and 24 KB written beside 1024 cycles of multiplies.
+template <int PAIR, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
+__global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_kernel(LinearWgradArgs p) {
+  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, NW = WM * WN;
+  constexpr int PA = PAIR == kLowA ? 2 : 1, PB = PAIR == kLowB ? 2 : 1;
+  constexpr int RA = BM * 2, RB = BN * 2;                       // bytes of an LDS row
+  constexpr int A_PLANE = kRows * RA, B_PLANE = kRows * RB, B_AT = PA * A_PLANE, BUF_BYTES = B_AT + PB * B_PLANE;
+  constexpr int A_LD = BM / 16 / NW, B_LD = BN / 16 / NW;       // direct loads (1 KB) per wavefront, plane and step
+  constexpr int LOADS = PA * A_LD + PB * B_LD, AHEAD = (NBUF - 2) * LOADS;
+  static_assert(BM % (16 * NW) == 0 && BN % (16 * NW) == 0 && AHEAD < 64 && NBUF >= 3, "tile/loader mismatch");
+  static_assert(BUF_BYTES <= 65536, "operand reads reach a buffer's planes with their immediate offset");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[NBUF * BUF_BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  uint32_t split, tile, tile_n, tile_k;
+  p.div_tiles.divmod(xcd_remap(blockIdx.x, gridDim.x), split, tile);
+  p.div_tiles_k.divmod(tile, tile_n, tile_k);
+  const int n0 = static_cast<int>(tile_n) * BM, k0 = static_cast<int>(tile_k) * BN;
+  const int64_t row0 = static_cast<int64_t>(split) * p.rows_per_split;
+  const int rows = static_cast<int>(p.M - row0 < p.rows_per_split ? p.M - row0 : p.rows_per_split);
+  const int steps = (rows + kRows - 1) / kRows;
+
+  // ---- the walk of the loads: the resources move down the rows, the lanes' offsets stay; rows behind the last one are outside ----
+  auto lane_offset = [&](int load, int row_bytes, int ld, int col0) {   // of 1 KB number `load` of a plane
+    const int per_row = row_bytes / 16, row = load * (1024 / row_bytes) + lane / per_row;
+    const int chunk = (lane % per_row) ^ ((row & 3) << 2);
+    return (row * ld + col0 + chunk * 8) * 2;
+  };
+  int a_off[A_LD], b_off[B_LD];
+#pragma unroll
+  for (int j = 0; j < A_LD; ++j) a_off[j] = lane_offset(wave * A_LD + j, RA, p.N, n0);
+#pragma unroll
+  for (int j = 0; j < B_LD; ++j) b_off[j] = lane_offset(wave * B_LD + j, RB, p.K, k0);
+  const int64_t a_step = static_cast<int64_t>(kRows) * p.N * 2, b_step = static_cast<int64_t>(kRows) * p.K * 2;
+  int64_t a_at = row0 * p.N * 2, b_at = row0 * p.K * 2;
+  int left = rows;
+  __amdgpu_buffer_rsrc_t rsrc_a[PA], rsrc_b[PB];
+  auto resources = [&]() LINEAR_INLINE {
+    const int here = left < 0 ? 0 : left < kRows ? left : kRows;
+    const uint32_t a_bytes = static_cast<uint32_t>(here) * static_cast<uint32_t>(p.N) * 2, b_bytes = static_cast<uint32_t>(here) * static_cast<uint32_t>(p.K) * 2;
+    rsrc_a[0] = make_rsrc(static_cast<const unsigned char*>(p.a) + a_at, a_bytes);
+    if constexpr (PA == 2) rsrc_a[1] = make_rsrc(static_cast<const unsigned char*>(p.a_low) + a_at, a_bytes);
+    rsrc_b[0] = make_rsrc(static_cast<const unsigned char*>(p.b) + b_at, b_bytes);
+    if constexpr (PB == 2) rsrc_b[1] = make_rsrc(static_cast<const unsigned char*>(p.b_low) + b_at, b_bytes);
+  };
+  auto next_step = [&]() LINEAR_INLINE {
+    left -= kRows;
+    if (left > 0) a_at += a_step, b_at += b_step;   // (behind the last row the resources are empty)
+    resources();
+  };
+  auto issue_load = [&](uint32_t buf, int j) LINEAR_INLINE {
+    if (j < PA * A_LD) {
+      const int plane = j / A_LD, i = j % A_LD;
+      load_to_lds(rsrc_a[plane], lds + buf + plane * A_PLANE + (wave * A_LD + i) * 1024, a_off[i], 0);
+    } else {
+      const int plane = (j - PA * A_LD) / B_LD, i = (j - PA * A_LD) % B_LD;
+      load_to_lds(rsrc_b[plane], lds + buf + B_AT + plane * B_PLANE + (wave * B_LD + i) * 1024, b_off[i], 0);
+    }
+  };
+
+  // ---- operand reads ----
+  const int half = lane >> 5, patch_row = (lane & 15) >> 2, patch_slot = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+  uint32_t rd[TM + TN];
+#pragma unroll
+  for (int i = 0; i < TM + TN; ++i) {
+    const bool is_a = i < TM;
+    const int ct = is_a ? wm * TM + i : wn * TN + i - TM;
+    rd[i] = lds_base + (is_a ? 0 : B_AT) + (4 * half + patch_row) * (is_a ? RA : RB) + (4 * (ct ^ patch_row) + patch_slot) * 16 + (lane & 1) * 8;
+  }
+  constexpr int FRAGS = PA * TM + PB * TN, READS = 2 * FRAGS;
+  uint2_t frag[2][FRAGS][2];   // [set][operand tile: A's planes, B's planes][rows 0-7, 8-15 of the slice]
+  auto read_one = [&](auto kk_c, uint32_t buf, auto set_c, auto i_c) LINEAR_INLINE {
+    constexpr int kk = decltype(kk_c)::value, set = decltype(set_c)::value, i = decltype(i_c)::value, f = i >> 1, t = i & 1;
+    constexpr bool is_a = f < PA * TM;
+    constexpr int plane = is_a ? f / TM : (f - PA * TM) / TN, which = is_a ? f % TM : TM + (f - PA * TM) % TN;
+    constexpr int ROW = kk * 16 + 8 * t, OFF = is_a ? plane * A_PLANE + ROW * RA : plane * B_PLANE + ROW * RB;
+    const uint32_t from = rd[which] + buf;
+    uint2_t v;
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(from), "n"(OFF));
+    frag[set][f][t] = v;
+  };
+  auto hold_set = [&](int set) LINEAR_INLINE {
+#pragma unroll
+    for (int f = 0; f < FRAGS; ++f)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(frag[set][f][t]));
+  };
+  auto operand = [&](int set, int f) LINEAR_INLINE {
+    Chunk c;
+    c.w[0] = frag[set][f][0][0];
+    c.w[1] = frag[set][f][0][1];
+    c.w[2] = frag[set][f][1][0];
+    c.w[3] = frag[set][f][1][1];
+    return c.h;
+  };
+
+  f32x16_t acc[TM][TN];
+  clear(acc);
+  // the bias gradient: the wavefronts of the first column of tiles add up the dy operands that they multiply anyway
+  const bool sums = p.bias && tile_k == 0 && wn == 0;
+  float col_sum[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) col_sum[i] = 0.f;
+
+  // multiplies the slice in `set`; meanwhile slice kk of the step in `buf` is read into the other set and half q of the loads goes
+  // to `ld_buf`
+  auto slice = [&](auto set_c, uint32_t buf, auto kk_c, auto q_c, uint32_t ld_buf) LINEAR_INLINE {
+    constexpr int set = decltype(set_c)::value, q = decltype(q_c)::value;
+    constexpr int PARTS = PA > PB ? PA : PB, MF = TM * TN * PARTS, FIRST = q * LOADS / 2, AUX = READS + (q + 1) * LOADS / 2 - FIRST;
+    constexpr int PER = (AUX + MF - 1) / MF;
+    unrolled<MF>([&](auto m_c) LINEAR_INLINE {
+      constexpr int m = decltype(m_c)::value, part = m / (TM * TN), tm = m % (TM * TN) / TN, tn = m % TN;
+      constexpr int fa = (PA == 2 ? part * TM : 0) + tm, fb = PA * TM + (PB == 2 ? part * TN : 0) + tn;
+      acc[tm][tn] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(set, fa), operand(set, fb), acc[tm][tn], 0, 0, 0);
+      unrolled<PER>([&](auto a_c) LINEAR_INLINE {
+        constexpr int a = m * PER + decltype(a_c)::value;
+        if constexpr (a < READS)
+          read_one(kk_c, buf, std::integral_constant<int, set ^ 1>{}, std::integral_constant<int, a>{});
+        else if constexpr (a < AUX)
+          issue_load(ld_buf, FIRST + a - READS);
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    hold_set(set ^ 1);
+    if (sums) {
+#pragma unroll
+      for (int f = 0; f < PA * TM; ++f)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t w = frag[set][f][t][i];
+            col_sum[f % TM] += __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u);
+          }
+    }
+  };
+
+  std::integral_constant<int, 0> zero;
+  std::integral_constant<int, 1> one;
+  resources();
+#pragma unroll
+  for (int s = 0; s < NBUF - 1; ++s) {
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) issue_load(s * BUF_BYTES, j);
+    next_step();
+  }
+#pragma unroll
+  for (int j = 0; j < LOADS / 2; ++j) issue_load((NBUF - 1) * BUF_BYTES, j);
+  wait_and_meet<AHEAD + LOADS / 2>();
+  unrolled<READS>([&](auto i_c) LINEAR_INLINE { read_one(zero, 0u, zero, i_c); });
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  hold_set(0);
+  uint32_t buf = 0, before = (NBUF - 1) * BUF_BYTES;
+  for (int s = 0; s < steps; ++s) {
+    slice(zero, buf, one, one, before);
+    next_step();
+    wait_and_meet<AHEAD>();
+    before = buf;
+    buf = buf == (NBUF - 1) * BUF_BYTES ? 0 : buf + BUF_BYTES;
+    slice(one, buf, zero, zero, before);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the zeros behind the last step land before the LDS goes
+
+  // ---- a lane's accumulators are one column of dw (x) and rows 8 (e / 4) + 4 half + e % 4: whole lines of 128 bytes a store ----
+  const int out_rows = min(BM, p.N - n0);
+  float* out = p.out + (static_cast<int64_t>(split) * p.N + n0) * p.K;
+  const __amdgpu_buffer_rsrc_t rsrc_out = make_rsrc(out, static_cast<uint32_t>(out_rows) * static_cast<uint32_t>(p.K) * 4);
+#pragma unroll
+  for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+    for (int tn = 0; tn < TN; ++tn) {
+      const int col = k0 + (wn * TN + tn) * 32 + (lane & 31), row = (wm * TM + tm) * 32 + 4 * half;
+      const int at = col < p.K ? (row * p.K + col) * 4 : static_cast<int>(kOutOfRange);
+      auto off = [&](int e) { return at + (8 * (e >> 2) + (e & 3)) * p.K * 4; };
+      if (p.accumulate) {
+        float old[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) old[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc_out, off(e), 0, 0));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[tm][tn][e] += old[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[tm][tn][e]), rsrc_out, off(e), 0, 0);
+    }
+  if (sums) {
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) {
+      const float s = col_sum[tm] + __shfl_xor(col_sum[tm], 32, 64);
+      const int n = n0 + (wm * TM + tm) * 32 + (lane & 31);
+      if (lane < 32 && n < p.N) {
+        float* b = p.bias + static_cast<int64_t>(split) * p.N + n;
+        *b = p.accumulate ? *b + s : s;
+      }
+    }
+  }
+}
+
+// out (+)= the sum of the splits' partial results, in their order, four at a time; the bias gradient's behind them
+struct WgradSumArgs {
+  const float* partial;
+  float* out;
+  const float* partial_bias;
+  float* bias;
+  int64_t quads, bias_quads;   // of one split
+  int splits, accumulate;
+};
+__global__ __launch_bounds__(256) void linear_wgrad_sum_kernel(WgradSumArgs p) {
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const float* from = p.partial;
+  float* to = p.out;
+  int64_t quads = p.quads;
+  if (i >= quads) {
+    i -= quads;
+    from = p.partial_bias, to = p.bias, quads = p.bias_quads;
+    if (i >= quads) return;
+  }
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < p.splits; ++k) {
+    const float4 v = load_streaming_f4(from + (k * quads + i) * 4);
+    s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+  }
+  if (p.accumulate) {
+    const float4 v = *reinterpret_cast<const float4*>(to + i * 4);
+    s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+  }
+  store_streaming_f4(to + i * 4, s);
+}
+
+int tiles_over(int n, int tile) { return (n + tile - 1) / tile; }
+
+// The tiling and the number of splits with the shortest estimate: rounds of workgroups, each of its steps and a start and end, and
+// the partial sums' way through memory.
+struct Choice {
+  bool big;
+  int splits, steps;   // reduction steps of a split
+};
+Choice choose(int64_t M, int N, int K, bool low) {
+  const int64_t steps = (M + kRows - 1) / kRows;
+  Choice best{false, 1, static_cast<int>(steps)};
+  float best_us = INFINITY;
+  for (int big = 0; big < 2; ++big) {
+    const int side = big ? 256 : 128;
+    const int64_t tiles = static_cast<int64_t>(tiles_over(N, side)) * tiles_over(K, side);
+    const float step_us = (big ? 1.0f : 0.30f) * (low ? 1.f : 0.55f), fixed_us = big ? 8.f : 5.f;
+    for (int64_t want = 1; want <= steps && want <= 64; ++want) {
+      const int64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+      if (splits != want || tiles * splits > 0x3fffffff) continue;
+      const int64_t slots = big ? 256 : 512, rounds = (tiles * splits + slots - 1) / slots;
+      // two workgroups of 128 x 128 share a compute unit: alone on it, one takes little more than half as long
+      const float share = !big && tiles * splits > 256 ? 1.75f : 1.f;
+      float us = rounds * (per * step_us * share + fixed_us);
+      if (splits > 1) us += 4.f + static_cast<float>(N) * K * (splits * 8.f + 4.f) / 4.5e6f;
+      if (us < best_us) {
+        best_us = us;
+        best = Choice{big != 0, static_cast<int>(splits), static_cast<int>(per)};
+      }
+    }
+  }
+  return best;
+}
+
+template <int PAIR>
+int launch_wgrad_pair(Context* ctx, const LinearWgradArgs& a, bool big, unsigned grid, double flops, double bytes) {
+  static const char* const names[2][3] = {
+      {"linear_wgrad_kernel<128x128>", "linear_wgrad_kernel<128x128,dy_low>", "linear_wgrad_kernel<128x128,x_low>"},
+      {"linear_wgrad_kernel<256x256>", "linear_wgrad_kernel<256x256,dy_low>", "linear_wgrad_kernel<256x256,x_low>"}};
+  const char* name = names[big][PAIR];
+  if (!big) return launch(ctx, linear_wgrad_kernel<PAIR, 2, 2, 2, 2, 3, 2>, dim3(grid), dim3(256), a, name, flops, 0, bytes);
+  if constexpr (PAIR == kLowB)
+    return launch(ctx, linear_wgrad_kernel<PAIR, 2, 4, 4, 2, 3, 1>, dim3(grid), dim3(512), a, name, flops, 0, bytes);
+  else
+    return launch(ctx, linear_wgrad_kernel<PAIR, 4, 2, 2, 4, 3, 1>, dim3(grid), dim3(512), a, name, flops, 0, bytes);
+}
+
+}  // namespace
+
+int64_t linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+  if (M <= 0 || K <= 0 || N <= 0 || K > INT32_MAX || N > INT32_MAX) return 0;
+  int64_t most = 0;
+  for (int low = 0; low < 2; ++low) {
+    const Choice c = choose(M, static_cast<int>(N), static_cast<int>(K), low != 0);
+    if (c.splits > 1 && c.splits * (N * K + N) * 4 > most) most = c.splits * (N * K + N) * 4;
+  }
+  return most;
+}
+
+int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy, const void* dy_low, float* dw, float* dbias, int accumulate, int64_t M,
+                 int64_t K, int64_t N, void* workspace, int64_t workspace_bytes) {
+  TCH_CHECK_ARG(M >= 0 && K > 0 && N > 0 && M <= INT32_MAX - 1024, "linear_wgrad: bad shape");
+  TCH_CHECK_ARG(K % 8 == 0 && N % 8 == 0, "linear_wgrad: the layer's sizes must be multiples of a 16-byte chunk");
+  TCH_CHECK_ARG(K < (1 << 21) && N < (1 << 21) && N * K < (1ll << 40), "linear_wgrad: layer too large");
+  TCH_CHECK_ARG(x && dy && dw, "linear_wgrad: null tensor");
+  TCH_CHECK_ARG(!x_low || !dy_low, "linear_wgrad: one low part at a time");
+  TCH_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(x_low) | reinterpret_cast<uintptr_t>(dy) |
+                  reinterpret_cast<uintptr_t>(dy_low) | reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(dbias) |
+                  reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
+                "linear_wgrad: tensors must start on 16-byte boundaries");
+  if (M == 0) {
+    if (accumulate) return 0;
+    if (int rc = fill_zero(ctx, dw, N * K * 4)) return rc;
+    return dbias ? fill_zero(ctx, dbias, N * 4) : 0;
+  }
+  const int n = static_cast<int>(N), k = static_cast<int>(K);
+  const bool low = x_low || dy_low;
+  Choice c = choose(M, n, k, low);
+  if (c.splits > 1 && (!workspace || workspace_bytes < c.splits * (N * K + N) * 4)) {
+    TCH_CHECK_ARG(!workspace, "linear_wgrad: workspace too small");
+    c.splits = 1;
+    c.steps = static_cast<int>((M + kRows - 1) / kRows);
+  }
+  const int side = c.big ? 256 : 128;
+  LinearWgradArgs a{};
+  a.a = dy, a.a_low = dy_low;
+  a.b = x, a.b_low = x_low;
+  a.M = M, a.N = n, a.K = k;
+  a.rows_per_split = c.steps * kRows;
+  a.tiles_k = tiles_over(k, side);
+  a.tiles = tiles_over(n, side) * a.tiles_k;
+  a.div_tiles = FastDiv(static_cast<uint32_t>(a.tiles));
+  a.div_tiles_k = FastDiv(static_cast<uint32_t>(a.tiles_k));
+  float* partial = static_cast<float*>(workspace);
+  const bool split = c.splits > 1;
+  a.out = split ? partial : dw;
+  a.bias = !dbias ? nullptr : split ? partial + c.splits * N * K : dbias;
+  a.accumulate = split ? 0 : accumulate;
+  TCH_CHECK_ARG(static_cast<int64_t>(a.tiles) * c.splits <= 0x3fffffff, "linear_wgrad: grid out of range");
+  const unsigned grid = static_cast<unsigned>(a.tiles * c.splits);
+  const double flops = 2.0 * M * N * K * (low ? 2.0 : 1.0);
+  const double bytes = 2.0 * M * (N * (dy_low ? 2 : 1) + K * (x_low ? 2 : 1)) + 4.0 * N * K;
+  int rc = dy_low   ? launch_wgrad_pair<kLowA>(ctx, a, c.big, grid, flops, bytes)
+           : x_low ? launch_wgrad_pair<kLowB>(ctx, a, c.big, grid, flops, bytes)
+                   : launch_wgrad_pair<kNoLow>(ctx, a, c.big, grid, flops, bytes);
+  if (rc || !split) return rc;
+  WgradSumArgs s{partial, dw, a.bias, dbias, N * K / 4, dbias ? N / 4 : 0, c.splits, accumulate};
+  const int64_t blocks = (s.quads + s.bias_quads + 255) / 256;
+  TCH_CHECK_ARG(blocks <= 0x7fffffff, "linear_wgrad: grid out of range");
+  return launch(ctx, linear_wgrad_sum_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), s, "linear_wgrad_sum_kernel",
+                4.0 * N * K * (c.splits + 1 + (accumulate ? 1 : 0)), 1);
+}
+
+}  // namespace tch

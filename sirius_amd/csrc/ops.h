@@ -204,6 +204,11 @@ int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, 
 int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, void* dz_low, const Rows& h, int gated, int act, int64_t M,
             int64_t N);
 
+// linear_wgrad.hip -- weight and bias gradients of bf16 linear layers, of an operand and its low part on request
+int64_t linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy, const void* dy_low, float* dw, float* dbias, int accumulate, int64_t M,
+                 int64_t K, int64_t N, void* workspace, int64_t workspace_bytes);
+
 // grad_norm.hip -- the global norm of many tensors, listed in pieces in device memory, and clipping by it
 int64_t grad_table_piece_elems();
 int64_t grad_norm_workspace_bytes(int64_t pieces);

@@ -1023,9 +1023,13 @@ def _wgrad_splits(x, K, N, rows):
 
 
 def linear_bwd_workspace_bytes(x, N):
-    """Bytes of workspace that linear_bwd (gated_linear_bwd: N = 2 F) wants for a layer with the input x [..., K] and N outputs."""
+    """Bytes of workspace that linear_wgrad and linear_bwd (gated_linear_bwd: N = 2 F) want for a layer with the input x [..., K]
+    and N outputs."""
     K = x.shape[-1]
-    blocks = {rows for _, rows in _wgrad_blocks(x.numel() // K, K, N, x.element_size())}
+    M = x.numel() // K
+    if x.dtype == torch.bfloat16:
+        return max(int(lib().tch_linear_wgrad_workspace_bytes(M, K, N)), 4)
+    blocks = {rows for _, rows in _wgrad_blocks(M, K, N, x.element_size())}
     return max([conv2d_wgrad_workspace_bytes(dtype_code(x), N, 1, 1, K, _wgrad_splits(x, K, N, rows)) for rows in blocks] + [4])
 
 
@@ -1047,18 +1051,15 @@ def linear_wgrad(ctx, x, dy, dw, dbias=None, accumulate=False, workspace=None, d
             if t is not None and not accumulate:
                 fill_zero(ctx, t)
         return
-    pairs = [(x, dy, dbias)]
-    if dy_low is not None:
-        pairs.append((x, dy_low, dbias))
-    if x_low is not None:
-        pairs.append((x_low, dy, None))
-    dw4 = dw.view(N, 1, 1, K)
-    for i, (a, g, db) in enumerate(pairs):
-        a, g = a.view(M, 1, 1, K), g.view(M, 1, 1, N)
-        for at, rows in _wgrad_blocks(M, K, N, a.element_size()):
-            splits = 1 if workspace is None else _wgrad_splits(a, K, N, rows)
-            conv2d_wgrad(ctx, a[at:at + rows], g[at:at + rows], dw4, 1, 0, workspace=workspace, splits=splits,
-                         accumulate=accumulate or at > 0 or i > 0, dbias=db)
+    if x.dtype == torch.bfloat16:
+        check(lib().tch_linear_wgrad(ctx.handle, _p(x), _p(x_low), _p(dy), _p(dy_low), _p(dw), _p(dbias), int(accumulate), M, K, N, _p(workspace),
+                                     0 if workspace is None else workspace.numel() * workspace.element_size()), "tch_linear_wgrad")
+        return
+    x, dy, dw = x.view(M, 1, 1, K), dy.view(M, 1, 1, N), dw.view(N, 1, 1, K)
+    for at, rows in _wgrad_blocks(M, K, N, x.element_size()):
+        splits = 1 if workspace is None else _wgrad_splits(x, K, N, rows)
+        conv2d_wgrad(ctx, x[at:at + rows], dy[at:at + rows], dw, 1, 0, workspace=workspace, splits=splits, accumulate=accumulate or at > 0,
+                     dbias=dbias)
 
 
 def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=None, residual=None, accumulate=False, workspace=None,

@@ -307,3 +307,39 @@ def test_feed_forward_block(ctx, M, C, F):
     ref = dy.double().t() @ (a * up)
     near(dwd, ref, dy.abs().double().t() @ eh + (2 * M + 64) * 2.0 ** -23 * (dy.abs().double().t() @ (a * up).abs()) + 2.0 ** -23 * ref.abs(), "dw_down")
     check_backward((dx, dw, db), exact, x, w, u, edp, residual=dy, low=True)
+
+
+@pytest.mark.parametrize("low", ["none", "dy", "x"])
+@pytest.mark.parametrize("M,K,N", [(1, 8, 8), (31, 264, 72), (33, 8, 520), (64, 136, 136), (1000, 256, 256), (3001, 776, 1288), (4100, 1032, 2056),
+                                   (9000, 264, 264), (70, 2056, 2312)])
+def test_linear_wgrad(ctx, M, K, N, low):
+    """bf16 weight gradients with and without a low part, rows split and not, added to what is there and not."""
+    from sirius_amd import ops
+    x, dy = rnd(M, K, dtype=BF16, seed=1), rnd(M, N, dtype=BF16, seed=2)
+    dy_low = rnd(M, N, dtype=BF16, seed=3, std=2.0 ** -9) if low == "dy" else None
+    x_low = rnd(M, K, dtype=BF16, seed=4, std=2.0 ** -9) if low == "x" else None
+    a = dy.double() + (0 if dy_low is None else dy_low.double())
+    b = x.double() + (0 if x_low is None else x_low.double())
+    for split, accumulate, with_bias in ((True, False, True), (False, True, True), (True, True, False)):
+        dw, db = Framed(N, K, F32, False), Framed(1, N, F32, False)
+        dw.view.copy_(rnd(N, K, dtype=F32, seed=5))
+        db.view.copy_(rnd(1, N, dtype=F32, seed=6))
+        dw0, db0 = dw.view.double(), db.view.double()
+        need = ops.linear_bwd_workspace_bytes(x, N)
+        ws = torch.full((need + 64,), 99, dtype=torch.uint8, device="cuda")
+        ops.linear_wgrad(ctx, x, dy, dw.view, dbias=db.view if with_bias else None, accumulate=accumulate,
+                         workspace=ws[:need] if split else None, dy_low=dy_low, x_low=x_low)
+        ref, tol = a.t() @ b, (2 * M + 64) * 2.0 ** -23 * (a.abs().t() @ b.abs())
+        if accumulate:
+            ref = ref + dw0
+        near(dw.view, ref, tol + 2.0 ** -22 * ref.abs() + 1e-30, "dw")
+        ref, tol = a.sum(0, keepdim=True), (2 * M + 64) * 2.0 ** -23 * a.abs().sum(0, keepdim=True)
+        if accumulate:
+            ref = ref + db0
+        if with_bias:
+            near(db.view, ref, tol + 2.0 ** -22 * ref.abs() + 1e-30, "db")
+        else:
+            assert torch.equal(db.view.double(), db0)
+        dw.check("dw")
+        db.check("db")
+        assert bool((ws[need:] == 99).all())
