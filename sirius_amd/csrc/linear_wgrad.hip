@@ -13,26 +13,33 @@
 #include "fp32_split.h"
 #include "linear_epilogue.h"
 
+#include <algorithm>
+
 #include "context.h"
 #include "ops.h"
 
 namespace tch {
 namespace {
 
+// All reduction steps of all output tiles are one sequence, tile by tile, and every workgroup takes an equal run of it: as many
+// workgroups as the chip holds finish together however many tiles there are.  A tile that lies within one run is stored; of a
+// tile that is cut, every workgroup leaves its part in the workspace (the first run of a workgroup in slot 2 g, the last in
+// 2 g + 1), and a second launch adds them up in the order of the workgroups.
 struct LinearWgradArgs {
   const void* a;        // dy [M][N]
   const void* a_low;
   const void* b;        // x [M][K]
   const void* b_low;
-  float* out;           // dw [N][K], or partial sums [split][N][K]
-  float* bias;          // dbias [N], or partial sums [split][N]; may be null
-  int64_t M;
+  float* out;           // dw [N][K]
+  float* bias;          // dbias [N]; may be null
+  float* slots;         // partial tiles [2 groups][tile]
+  float* bias_slots;    // and their column sums [2 groups][rows of a tile]
+  int64_t M, units;     // units: tiles * steps
   int N, K;
-  int rows_per_split;   // a multiple of 32
-  int tiles_k, tiles;   // column tiles; tiles of one split
-  int accumulate;       // without splits: out and bias are added to
-  FastDiv div_tiles, div_tiles_k;
+  int tiles_k, tiles, steps, groups;
+  int accumulate;       // out and bias are added to
 };
+__host__ __device__ inline int64_t run_start(int64_t units, int groups, int group) { return units * group / groups; }
 
 enum Pair : int { kNoLow = 0, kLowA = 1, kLowB = 2 };
 constexpr int kRows = 32;   // of a reduction step
@@ -55,13 +62,8 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  uint32_t split, tile, tile_n, tile_k;
-  p.div_tiles.divmod(xcd_remap(blockIdx.x, gridDim.x), split, tile);
-  p.div_tiles_k.divmod(tile, tile_n, tile_k);
-  const int n0 = static_cast<int>(tile_n) * BM, k0 = static_cast<int>(tile_k) * BN;
-  const int64_t row0 = static_cast<int64_t>(split) * p.rows_per_split;
-  const int rows = static_cast<int>(p.M - row0 < p.rows_per_split ? p.M - row0 : p.rows_per_split);
-  const int steps = (rows + kRows - 1) / kRows;
+  const int group = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x));
+  const int64_t run_end = run_start(p.units, p.groups, group + 1);
 
   // ---- the walk of the loads: the resources move down the rows, the lanes' offsets stay; rows behind the last one are outside ----
   auto lane_offset = [&](int load, int row_bytes, int ld, int col0) {   // of 1 KB number `load` of a plane
@@ -70,13 +72,9 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
     return (row * ld + col0 + chunk * 8) * 2;
   };
   int a_off[A_LD], b_off[B_LD];
-#pragma unroll
-  for (int j = 0; j < A_LD; ++j) a_off[j] = lane_offset(wave * A_LD + j, RA, p.N, n0);
-#pragma unroll
-  for (int j = 0; j < B_LD; ++j) b_off[j] = lane_offset(wave * B_LD + j, RB, p.K, k0);
   const int64_t a_step = static_cast<int64_t>(kRows) * p.N * 2, b_step = static_cast<int64_t>(kRows) * p.K * 2;
-  int64_t a_at = row0 * p.N * 2, b_at = row0 * p.K * 2;
-  int left = rows;
+  int64_t a_at = 0, b_at = 0;
+  int left = 0;
   __amdgpu_buffer_rsrc_t rsrc_a[PA], rsrc_b[PB];
   auto resources = [&]() LINEAR_INLINE {
     const int here = left < 0 ? 0 : left < kRows ? left : kRows;
@@ -139,12 +137,9 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
   };
 
   f32x16_t acc[TM][TN];
-  clear(acc);
   // the bias gradient: the wavefronts of the first column of tiles add up the dy operands that they multiply anyway
-  const bool sums = p.bias && tile_k == 0 && wn == 0;
+  bool sums = false;
   float col_sum[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) col_sum[i] = 0.f;
 
   // multiplies the slice in `set`; meanwhile slice kk of the step in `buf` is read into the other set and half q of the loads goes
   // to `ld_buf`
@@ -182,127 +177,175 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
 
   std::integral_constant<int, 0> zero;
   std::integral_constant<int, 1> one;
-  resources();
+  // behind the last barrier of a part nobody reads what counts, and every wavefront waits for its own loads: the next part's may
+  // go to the same buffers
+  int64_t unit = run_start(p.units, p.groups, group);
+  for (int part = 0; unit < run_end; ++part) {
+    const int tile = static_cast<int>(unit / p.steps), from = static_cast<int>(unit - static_cast<int64_t>(tile) * p.steps);
+    const int to = static_cast<int>(min(static_cast<int64_t>(p.steps), from + (run_end - unit)));
+    const int tile_n = tile / p.tiles_k, tile_k = tile - tile_n * p.tiles_k;
+    const int n0 = tile_n * BM, k0 = tile_k * BN;
+    const int64_t row0 = static_cast<int64_t>(from) * kRows;
+    unit += to - from;
 #pragma unroll
-  for (int s = 0; s < NBUF - 1; ++s) {
+    for (int j = 0; j < A_LD; ++j) a_off[j] = lane_offset(wave * A_LD + j, RA, p.N, n0);
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) issue_load(s * BUF_BYTES, j);
-    next_step();
-  }
+    for (int j = 0; j < B_LD; ++j) b_off[j] = lane_offset(wave * B_LD + j, RB, p.K, k0);
+    a_at = row0 * p.N * 2;
+    b_at = row0 * p.K * 2;
+    left = static_cast<int>(min(static_cast<int64_t>(to - from) * kRows, p.M - row0));
+    sums = p.bias && tile_k == 0 && wn == 0;
+    clear(acc);
 #pragma unroll
-  for (int j = 0; j < LOADS / 2; ++j) issue_load((NBUF - 1) * BUF_BYTES, j);
-  wait_and_meet<AHEAD + LOADS / 2>();
-  unrolled<READS>([&](auto i_c) LINEAR_INLINE { read_one(zero, 0u, zero, i_c); });
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  hold_set(0);
-  uint32_t buf = 0, before = (NBUF - 1) * BUF_BYTES;
-  for (int s = 0; s < steps; ++s) {
-    slice(zero, buf, one, one, before);
-    next_step();
-    wait_and_meet<AHEAD>();
-    before = buf;
-    buf = buf == (NBUF - 1) * BUF_BYTES ? 0 : buf + BUF_BYTES;
-    slice(one, buf, zero, zero, before);
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the zeros behind the last step land before the LDS goes
+    for (int i = 0; i < TM; ++i) col_sum[i] = 0.f;
 
-  // ---- a lane's accumulators are one column of dw (x) and rows 8 (e / 4) + 4 half + e % 4: whole lines of 128 bytes a store ----
-  const int out_rows = min(BM, p.N - n0);
-  float* out = p.out + (static_cast<int64_t>(split) * p.N + n0) * p.K;
-  const __amdgpu_buffer_rsrc_t rsrc_out = make_rsrc(out, static_cast<uint32_t>(out_rows) * static_cast<uint32_t>(p.K) * 4);
+    resources();
 #pragma unroll
-  for (int tm = 0; tm < TM; ++tm)
+    for (int s = 0; s < NBUF - 1; ++s) {
 #pragma unroll
-    for (int tn = 0; tn < TN; ++tn) {
-      const int col = k0 + (wn * TN + tn) * 32 + (lane & 31), row = (wm * TM + tm) * 32 + 4 * half;
-      const int at = col < p.K ? (row * p.K + col) * 4 : static_cast<int>(kOutOfRange);
-      auto off = [&](int e) { return at + (8 * (e >> 2) + (e & 3)) * p.K * 4; };
-      if (p.accumulate) {
-        float old[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) old[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc_out, off(e), 0, 0));
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[tm][tn][e] += old[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[tm][tn][e]), rsrc_out, off(e), 0, 0);
+      for (int j = 0; j < LOADS; ++j) issue_load(s * BUF_BYTES, j);
+      next_step();
     }
-  if (sums) {
 #pragma unroll
-    for (int tm = 0; tm < TM; ++tm) {
-      const float s = col_sum[tm] + __shfl_xor(col_sum[tm], 32, 64);
-      const int n = n0 + (wm * TM + tm) * 32 + (lane & 31);
-      if (lane < 32 && n < p.N) {
-        float* b = p.bias + static_cast<int64_t>(split) * p.N + n;
-        *b = p.accumulate ? *b + s : s;
+    for (int j = 0; j < LOADS / 2; ++j) issue_load((NBUF - 1) * BUF_BYTES, j);
+    wait_and_meet<AHEAD + LOADS / 2>();
+    unrolled<READS>([&](auto i_c) LINEAR_INLINE { read_one(zero, 0u, zero, i_c); });
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    hold_set(0);
+    uint32_t buf = 0, before = (NBUF - 1) * BUF_BYTES;
+    for (int s = from; s < to; ++s) {
+      slice(zero, buf, one, one, before);
+      next_step();
+      wait_and_meet<AHEAD>();
+      before = buf;
+      buf = buf == (NBUF - 1) * BUF_BYTES ? 0 : buf + BUF_BYTES;
+      slice(one, buf, zero, zero, before);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the zeros behind the last step have landed
+
+    // ---- a lane's accumulators are one column of dw (x) and rows 8 (e / 4) + 4 half + e % 4: whole lines of 128 bytes a store ----
+    const bool whole = to - from == p.steps;
+    const int slot = 2 * group + (part == 0 ? 0 : 1);
+    const int ld = whole ? p.K : BN;
+    const bool add = whole && p.accumulate;
+    float* out = whole ? p.out + static_cast<int64_t>(n0) * p.K + k0 : p.slots + static_cast<int64_t>(slot) * (BM * BN);
+    const int rows = whole ? min(BM, p.N - n0) : BM, cols = whole ? min(BN, p.K - k0) : BN;
+    const __amdgpu_buffer_rsrc_t rsrc_out = make_rsrc(out, static_cast<uint32_t>((rows - 1) * ld + cols) * 4u);
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+      for (int tn = 0; tn < TN; ++tn) {
+        const int col = (wn * TN + tn) * 32 + (lane & 31), row = (wm * TM + tm) * 32 + 4 * half;
+        const int at = col < cols ? (row * ld + col) * 4 : static_cast<int>(kOutOfRange);
+        auto off = [&](int e) { return at + (8 * (e >> 2) + (e & 3)) * ld * 4; };
+        if (add) {
+          float old[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) old[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc_out, off(e), 0, 0));
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[tm][tn][e] += old[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[tm][tn][e]), rsrc_out, off(e), 0, 0);
+      }
+    if (sums) {
+#pragma unroll
+      for (int tm = 0; tm < TM; ++tm) {
+        const float s = col_sum[tm] + __shfl_xor(col_sum[tm], 32, 64);
+        const int n = (wm * TM + tm) * 32 + (lane & 31);
+        if (lane < 32 && n < rows) {
+          float* b = whole ? p.bias + n0 + n : p.bias_slots + static_cast<int64_t>(slot) * BM + n;
+          *b = add ? *b + s : s;
+        }
       }
     }
   }
 }
 
-// out (+)= the sum of the splits' partial results, in their order, four at a time; the bias gradient's behind them
-struct WgradSumArgs {
-  const float* partial;
-  float* out;
-  const float* partial_bias;
-  float* bias;
-  int64_t quads, bias_quads;   // of one split
-  int splits, accumulate;
-};
-__global__ __launch_bounds__(256) void linear_wgrad_sum_kernel(WgradSumArgs p) {
-  int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const float* from = p.partial;
-  float* to = p.out;
-  int64_t quads = p.quads;
-  if (i >= quads) {
-    i -= quads;
-    from = p.partial_bias, to = p.bias, quads = p.bias_quads;
-    if (i >= quads) return;
+// The tiles that several workgroups had a part of: dw (+)= their sum in the workgroups' order.  A workgroup here has a band of 32
+// rows of a tile.
+template <int SIDE>
+__global__ __launch_bounds__(256) void linear_wgrad_sum_kernel(LinearWgradArgs p) {
+  constexpr int BANDS = SIDE / 32;
+  const int tile = blockIdx.x / BANDS, band = blockIdx.x % BANDS;
+  const int64_t first = static_cast<int64_t>(tile) * p.steps, behind = first + p.steps;
+  // the group that has the tile's first unit, and the slot of a group's part
+  int g0 = static_cast<int>(first * p.groups / p.units);
+  while (run_start(p.units, p.groups, g0 + 1) <= first) ++g0;
+  if (run_start(p.units, p.groups, g0 + 1) >= behind) return;   // one workgroup had all of it
+  int g1 = g0 + 1;
+  while (g1 + 1 < p.groups && run_start(p.units, p.groups, g1 + 1) < behind) ++g1;
+  auto slot_of = [&](int g) { return static_cast<int64_t>(2 * g + (run_start(p.units, p.groups, g) >= first ? 0 : 1)); };
+  const int tile_n = tile / p.tiles_k, tile_k = tile - tile_n * p.tiles_k;
+  const int n0 = tile_n * SIDE + band * 32, k0 = tile_k * SIDE;
+  for (int q = threadIdx.x; q < 32 * SIDE / 4; q += 256) {
+    const int row = q / (SIDE / 4), col = q % (SIDE / 4) * 4;
+    if (n0 + row >= p.N || k0 + col >= p.K) continue;
+    const int64_t in_tile = (band * 32 + row) * SIDE + col;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g = g0; g <= g1; ++g) {
+      const float4 v = load_streaming_f4(p.slots + slot_of(g) * (SIDE * SIDE) + in_tile);
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    float* to = p.out + static_cast<int64_t>(n0 + row) * p.K + k0 + col;
+    if (p.accumulate) {
+      const float4 v = *reinterpret_cast<const float4*>(to);
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    store_streaming_f4(to, s);
   }
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int k = 0; k < p.splits; ++k) {
-    const float4 v = load_streaming_f4(from + (k * quads + i) * 4);
-    s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+  if (p.bias && tile_k == 0 && threadIdx.x < 32 && n0 + static_cast<int>(threadIdx.x) < p.N) {
+    float s = 0.f;
+    for (int g = g0; g <= g1; ++g) s += p.bias_slots[slot_of(g) * SIDE + band * 32 + threadIdx.x];
+    float* to = p.bias + n0 + threadIdx.x;
+    *to = p.accumulate ? *to + s : s;
   }
-  if (p.accumulate) {
-    const float4 v = *reinterpret_cast<const float4*>(to + i * 4);
-    s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
-  }
-  store_streaming_f4(to + i * 4, s);
 }
 
 int tiles_over(int n, int tile) { return (n + tile - 1) / tile; }
 
-// The tiling and the number of splits with the shortest estimate: rounds of workgroups, each of its steps and a start and end, and
-// the partial sums' way through memory.
+// The tiling and the number of workgroups with the shortest estimate: the steps of a run, a start and an end, and the partial tiles'
+// way through memory.  Steps in microseconds, with a low part: 256 x 256 1.43; 128 x 128 0.95 alone on a compute unit, 0.97 where
+// two share it.
 struct Choice {
-  bool big;
-  int splits, steps;   // reduction steps of a split
+  bool big, cut;       // cut: some tiles are shared, the workspace is needed
+  int groups;
 };
-Choice choose(int64_t M, int N, int K, bool low) {
+Choice choose(int64_t M, int N, int K, bool low, bool may_cut) {
   const int64_t steps = (M + kRows - 1) / kRows;
-  Choice best{false, 1, static_cast<int>(steps)};
+  Choice best{false, false, 1};
   float best_us = INFINITY;
+  auto consider = [&](bool big, int64_t groups) {
+    const int side = big ? 256 : 128;
+    const int64_t tiles = static_cast<int64_t>(tiles_over(N, side)) * tiles_over(K, side), units = tiles * steps;
+    if (groups < 1 || groups > units || groups > 0x3fffffff) return;
+    const bool cut = groups % tiles != 0 && tiles % groups != 0 ? true : groups > tiles;
+    if (cut && (!may_cut || groups > (big ? 256 : 512))) return;
+    const int64_t slots = big ? 256 : 512, rounds = (groups + slots - 1) / slots, run = (units + groups - 1) / groups;
+    const float step_us = (big ? 1.43f : groups > 256 ? 0.97f : 0.95f) * (low ? 1.f : 0.6f);
+    float us = static_cast<float>(rounds) * (run * step_us + (big ? 8.f : 5.f) * ((run + steps - 1) / steps));
+    if (cut) {
+      const float parts = static_cast<float>(groups < tiles ? 2 * groups : groups + tiles);
+      us += 5.f + (parts * side * side * 8.f + static_cast<float>(N) * K * 4.f) / 5e6f;
+    }
+    if (us < best_us) {
+      best_us = us;
+      best = Choice{big, cut, static_cast<int>(groups)};
+    }
+  };
   for (int big = 0; big < 2; ++big) {
     const int side = big ? 256 : 128;
-    const int64_t tiles = static_cast<int64_t>(tiles_over(N, side)) * tiles_over(K, side);
-    const float step_us = (big ? 1.0f : 0.30f) * (low ? 1.f : 0.55f), fixed_us = big ? 8.f : 5.f;
-    for (int64_t want = 1; want <= steps && want <= 64; ++want) {
-      const int64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
-      if (splits != want || tiles * splits > 0x3fffffff) continue;
-      const int64_t slots = big ? 256 : 512, rounds = (tiles * splits + slots - 1) / slots;
-      // two workgroups of 128 x 128 share a compute unit: alone on it, one takes little more than half as long
-      const float share = !big && tiles * splits > 256 ? 1.75f : 1.f;
-      float us = rounds * (per * step_us * share + fixed_us);
-      if (splits > 1) us += 4.f + static_cast<float>(N) * K * (splits * 8.f + 4.f) / 4.5e6f;
-      if (us < best_us) {
-        best_us = us;
-        best = Choice{big != 0, static_cast<int>(splits), static_cast<int>(per)};
-      }
+    consider(big, static_cast<int64_t>(tiles_over(N, side)) * tiles_over(K, side));
+    for (int64_t groups = big ? 256 : 512; groups >= 8; groups /= 2) {
+      consider(big, groups);
+      consider(big, groups / 4 * 3);
     }
   }
   return best;
+}
+int64_t slot_floats(const Choice& c) {
+  const int64_t side = c.big ? 256 : 128;
+  return c.cut ? 2 * static_cast<int64_t>(c.groups) * (side * side + side) : 0;
 }
 
 template <int PAIR>
@@ -323,10 +366,7 @@ int launch_wgrad_pair(Context* ctx, const LinearWgradArgs& a, bool big, unsigned
 int64_t linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N) {
   if (M <= 0 || K <= 0 || N <= 0 || K > INT32_MAX || N > INT32_MAX) return 0;
   int64_t most = 0;
-  for (int low = 0; low < 2; ++low) {
-    const Choice c = choose(M, static_cast<int>(N), static_cast<int>(K), low != 0);
-    if (c.splits > 1 && c.splits * (N * K + N) * 4 > most) most = c.splits * (N * K + N) * 4;
-  }
+  for (int low = 0; low < 2; ++low) most = std::max(most, slot_floats(choose(M, static_cast<int>(N), static_cast<int>(K), low != 0, true)) * 4);
   return most;
 }
 
@@ -348,40 +388,36 @@ int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy,
   }
   const int n = static_cast<int>(N), k = static_cast<int>(K);
   const bool low = x_low || dy_low;
-  Choice c = choose(M, n, k, low);
-  if (c.splits > 1 && (!workspace || workspace_bytes < c.splits * (N * K + N) * 4)) {
-    TCH_CHECK_ARG(!workspace, "linear_wgrad: workspace too small");
-    c.splits = 1;
-    c.steps = static_cast<int>((M + kRows - 1) / kRows);
-  }
+  Choice c = choose(M, n, k, low, workspace != nullptr);
+  TCH_CHECK_ARG(slot_floats(c) * 4 <= (workspace ? workspace_bytes : 0), "linear_wgrad: workspace too small");
   const int side = c.big ? 256 : 128;
   LinearWgradArgs a{};
   a.a = dy, a.a_low = dy_low;
   a.b = x, a.b_low = x_low;
+  a.out = dw;
+  a.bias = dbias;
+  a.slots = static_cast<float*>(workspace);
+  a.bias_slots = a.slots + 2 * static_cast<int64_t>(c.groups) * side * side;
   a.M = M, a.N = n, a.K = k;
-  a.rows_per_split = c.steps * kRows;
   a.tiles_k = tiles_over(k, side);
+  TCH_CHECK_ARG(static_cast<int64_t>(tiles_over(n, side)) * a.tiles_k <= 0x3fffffff, "linear_wgrad: grid out of range");
   a.tiles = tiles_over(n, side) * a.tiles_k;
-  a.div_tiles = FastDiv(static_cast<uint32_t>(a.tiles));
-  a.div_tiles_k = FastDiv(static_cast<uint32_t>(a.tiles_k));
-  float* partial = static_cast<float*>(workspace);
-  const bool split = c.splits > 1;
-  a.out = split ? partial : dw;
-  a.bias = !dbias ? nullptr : split ? partial + c.splits * N * K : dbias;
-  a.accumulate = split ? 0 : accumulate;
-  TCH_CHECK_ARG(static_cast<int64_t>(a.tiles) * c.splits <= 0x3fffffff, "linear_wgrad: grid out of range");
-  const unsigned grid = static_cast<unsigned>(a.tiles * c.splits);
+  a.steps = static_cast<int>((M + kRows - 1) / kRows);
+  a.units = static_cast<int64_t>(a.tiles) * a.steps;
+  a.groups = c.groups;
+  a.accumulate = accumulate;
+  TCH_CHECK_ARG(a.units < (1ll << 62) / (c.groups + 1), "linear_wgrad: grid out of range");
+  const unsigned grid = static_cast<unsigned>(c.groups);
   const double flops = 2.0 * M * N * K * (low ? 2.0 : 1.0);
   const double bytes = 2.0 * M * (N * (dy_low ? 2 : 1) + K * (x_low ? 2 : 1)) + 4.0 * N * K;
   int rc = dy_low   ? launch_wgrad_pair<kLowA>(ctx, a, c.big, grid, flops, bytes)
            : x_low ? launch_wgrad_pair<kLowB>(ctx, a, c.big, grid, flops, bytes)
                    : launch_wgrad_pair<kNoLow>(ctx, a, c.big, grid, flops, bytes);
-  if (rc || !split) return rc;
-  WgradSumArgs s{partial, dw, a.bias, dbias, N * K / 4, dbias ? N / 4 : 0, c.splits, accumulate};
-  const int64_t blocks = (s.quads + s.bias_quads + 255) / 256;
-  TCH_CHECK_ARG(blocks <= 0x7fffffff, "linear_wgrad: grid out of range");
-  return launch(ctx, linear_wgrad_sum_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), s, "linear_wgrad_sum_kernel",
-                4.0 * N * K * (c.splits + 1 + (accumulate ? 1 : 0)), 1);
+  if (rc || !c.cut) return rc;
+  const dim3 blocks(static_cast<unsigned>(a.tiles * (side / 32)));
+  const double sum_bytes = 4.0 * (static_cast<double>(c.groups) + a.tiles) * side * side + 4.0 * N * K;
+  return c.big ? launch(ctx, linear_wgrad_sum_kernel<256>, blocks, dim3(256), a, "linear_wgrad_sum_kernel<256>", sum_bytes, 1)
+               : launch(ctx, linear_wgrad_sum_kernel<128>, blocks, dim3(256), a, "linear_wgrad_sum_kernel<128>", sum_bytes, 1);
 }
 
 }  // namespace tch
