@@ -481,16 +481,16 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
 // ---------------------------------------------------------------------------
 // few tiles: every wavefront of a workgroup has the whole tile for every KG-th reduction step
 // ---------------------------------------------------------------------------
-// Each wavefront has a ring of NBUF operand tiles (64-byte rows) of its own, filled with direct loads, and waits for its own loads
+// Each wavefront has a ring of NBUF operand tiles (rows of RB bytes) of its own, filled with direct loads, and waits for its own loads
 // only: no barrier before the partial tiles meet in LDS, where they are added in the order of the wavefronts.  What that buys
 // where workgroups are few: KG * (NBUF - 1) operand tiles in flight per compute unit and a chain of nk / KG steps instead of nk.
-template <typename T, int MODE, int TM, int TN, int KG, int NBUF>
-__global__ __launch_bounds__(KG * 64, KG / 4) void linear_split_kernel(LinearArgs p) {
-  constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), RB = 64, KS = RB / EB;
+template <typename T, int MODE, int TM, int TN, int KG, int NBUF, int RB>
+__global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
+  constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), KS = RB / EB, SL = RB / 32, SLOTS = RB / 16, LD_ROWS = 1024 / RB;
   constexpr bool GATED_FWD = MODE == kGatedFwd;
   constexpr int BM = TM * 32, BN = TN * 32, BN_OUT = GATED_FWD ? BN / 2 : BN;
   static_assert(!GATED_FWD || TN % 2 == 0, "gate and up tiles come in pairs");
-  constexpr int A_LD = BM / 16, B_LD = BN / 16, A_BYTES = BM * RB, BUF_BYTES = (BM + BN) * RB;
+  constexpr int A_LD = BM / LD_ROWS, B_LD = BN / LD_ROWS, A_BYTES = BM * RB, BUF_BYTES = (BM + BN) * RB;
   constexpr int NT = KG * 64, LD = BN + 4;
   constexpr int RED_BYTES = KG * BM * LD * 4, RING_BYTES = KG * NBUF * BUF_BYTES;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[RED_BYTES > RING_BYTES ? RED_BYTES : RING_BYTES];
@@ -505,16 +505,19 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void linear_split_kernel(LinearArg
   const int nk = (p.K + KS - 1) / KS;
   const int my_steps = nk > wave ? (nk - wave + KG - 1) / KG : 0;
 
-  const int sub_row = lane >> 2, slot = lane & 3;
-  const int chunk = slot ^ ((sub_row >> 2) & 3);
+  auto swizzle = [](int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
+  const int sub_row = lane / SLOTS, slot = lane % SLOTS;
+  int chunk[2];   // of an even and an odd direct load
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd) chunk[odd] = slot ^ swizzle(odd * LD_ROWS + sub_row);
   uint32_t a_off[A_LD], b_off[B_LD];
 #pragma unroll
-  for (int j = 0; j < A_LD; ++j) a_off[j] = (static_cast<uint32_t>(j * 16 + sub_row) * static_cast<uint32_t>(p.lda) + chunk * E) * EB;
+  for (int j = 0; j < A_LD; ++j) a_off[j] = (static_cast<uint32_t>(j * LD_ROWS + sub_row) * static_cast<uint32_t>(p.lda) + chunk[j & 1] * E) * EB;
 #pragma unroll
   for (int j = 0; j < B_LD; ++j) {
-    const int trow = j * 16 + sub_row, block = trow >> 5;
+    const int trow = j * LD_ROWS + sub_row, block = trow >> 5;
     const uint32_t row = GATED_FWD ? static_cast<uint32_t>((block & 1) * p.N + (block >> 1) * 32 + (trow & 31)) : static_cast<uint32_t>(trow);
-    b_off[j] = (row * static_cast<uint32_t>(p.K) + chunk * E) * EB;
+    b_off[j] = (row * static_cast<uint32_t>(p.K) + chunk[j & 1] * E) * EB;
   }
   const __amdgpu_buffer_rsrc_t rsrc_a =
       make_rsrc(static_cast<const T*>(p.a) + m0 * p.lda, static_cast<uint32_t>(((rows - 1) * p.lda + p.K) * EB));
@@ -524,19 +527,21 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void linear_split_kernel(LinearArg
   unsigned char* ring = lds + wave * (NBUF * BUF_BYTES);
   int ld_kt = wave;
   auto issue_loads = [&](int buf) {
-    const uint32_t behind = ld_kt * KS + chunk * E >= p.K ? kOutOfRange : 0u;   // the chunk lies behind K
+    uint32_t behind[2];   // the chunk lies behind K
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) behind[odd] = ld_kt * KS + chunk[odd] * E >= p.K ? kOutOfRange : 0u;
     unsigned char* dst = ring + buf * BUF_BYTES;
 #pragma unroll
-    for (int j = 0; j < A_LD; ++j) load_to_lds(rsrc_a, dst + j * 1024, static_cast<int>(a_off[j] | behind), ld_kt * RB);
+    for (int j = 0; j < A_LD; ++j) load_to_lds(rsrc_a, dst + j * 1024, static_cast<int>(a_off[j] | behind[j & 1]), ld_kt * RB);
 #pragma unroll
-    for (int j = 0; j < B_LD; ++j) load_to_lds(rsrc_b, dst + A_BYTES + j * 1024, static_cast<int>(b_off[j] | behind), ld_kt * RB);
+    for (int j = 0; j < B_LD; ++j) load_to_lds(rsrc_b, dst + A_BYTES + j * 1024, static_cast<int>(b_off[j] | behind[j & 1]), ld_kt * RB);
     ld_kt += KG;
   };
 
   f32x16_t acc[TM][TN];
   clear(acc);
   const int frag_row = lane & 31, frag_half = lane >> 5;
-  const uint32_t rd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring)) + frag_row * RB + ((frag_row >> 2) & 3) * 16;
+  const uint32_t rd = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ring)) + frag_row * RB + swizzle(frag_row) * 16;
   auto read_frags = [&](int buf, int kk, uint4_t* fa, uint4_t* fb) {
     const uint32_t pa = (rd ^ static_cast<uint32_t>((2 * kk + frag_half) * 16)) + buf * BUF_BYTES;
 #pragma unroll
@@ -564,13 +569,19 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void linear_split_kernel(LinearArg
     else
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (i + NBUF - 1 < my_steps) issue_loads((buf + NBUF - 1) % NBUF);
-    uint4_t fa0[TM], fb0[TN], fa1[TM], fb1[TN];
-    read_frags(buf, 0, fa0, fb0);
-    read_frags(buf, 1, fa1, fb1);
-    asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(TM + TN) : "memory");
-    multiply(fa0, fb0);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    multiply(fa1, fb1);
+    // a slice is read while the one before it is multiplied
+    uint4_t fa[2][TM], fb[2][TN];
+    read_frags(buf, 0, fa[0], fb[0]);
+#pragma unroll
+    for (int kk = 0; kk < SL; ++kk) {
+      if (kk + 1 < SL) {
+        read_frags(buf, kk + 1, fa[(kk + 1) & 1], fb[(kk + 1) & 1]);
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(TM + TN) : "memory");
+      } else {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      multiply(fa[kk & 1], fb[kk & 1]);
+    }
   };
 #pragma unroll
   for (int i = 0; i < NBUF - 1; ++i)
@@ -654,12 +665,13 @@ __global__ __launch_bounds__(KG * 64, KG / 4) void linear_split_kernel(LinearArg
 }
 
 // ---------------------------------------------------------------------------
-// up to 16 rows (tokens that decode together): the weights are read once, straight into registers
+// few rows (tokens that decode together), or few outputs: operands straight into registers
 // ---------------------------------------------------------------------------
-// A workgroup has 16 TN output columns; its KG wavefronts take 256-byte pieces of the reduction in turn.  Weight rows are the rows
-// and the tokens the columns of 16 x 16 MFMA tiles; lane l holds the 16-byte chunk l / 16 (of four) of row l % 16, so that a
-// load covers 64 neighbouring bytes of sixteen rows.  The next piece is requested before this one is multiplied.  Bound by the
-// bytes of the weights.
+// A workgroup has 16 rows and 16 output columns (of the gate and of the up projection); its KG wavefronts take 256-byte pieces of
+// the reduction in turn.  Weight rows are the rows and the tokens the columns of 16 x 16 MFMA tiles; lane l holds the 16-byte
+// chunk l / 16 (of four) of row l % 16, so that a load covers 64 neighbouring bytes of sixteen rows.  The next piece is
+// requested before this one is multiplied.  Up to 16 rows it is bound by the bytes of the weights; beyond, by what a compute unit
+// loads into registers (32 or 64 rows a workgroup, for fewer loads of the weights, were slower throughout).
 template <typename T>
 __device__ inline void mma16(const uint4_t& first, const uint4_t& second, f32x4_t& acc) {
   if constexpr (sizeof(T) == 2) {
@@ -682,35 +694,36 @@ __device__ inline void store_four(T* p, const float* v) {
   for (int e = 0; e < 4; ++e) Elem<T>::store(p + e, v[e]);
 }
 
-template <typename T, int MODE, int TN, int KG>
+template <typename T, int MODE, int KG>
 __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T);
   constexpr bool GATED_FWD = MODE == kGatedFwd;
-  constexpr int W = GATED_FWD ? 2 * TN : TN;   // weight tiles of 16 rows: gate and up next to each other
+  constexpr int W = GATED_FWD ? 2 : 1;         // weight tiles of 16 rows: gate and up next to each other
   constexpr int U = 4, PIECE = U * 4 * E;      // loads per piece and tile; elements of a piece
-  __shared__ float red[KG][W][16 * 20];
+  constexpr int LD = 20;                       // floats of a row of 16 partial sums
+  __shared__ float red[KG][W][16 * LD];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n0 = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x)) * (16 * TN);
+  // consecutive workgroups (one XCD) share the weights of a column tile
+  uint32_t tile_n, tile_m;
+  p.div_tiles_n.divmod(xcd_remap(blockIdx.x, gridDim.x), tile_n, tile_m);   // divided by the row tiles
+  const int n0 = static_cast<int>(tile_n) * 16, m0 = static_cast<int>(tile_m) * 16;
   const int pieces = (p.K + PIECE - 1) / PIECE;
   const int row16 = lane & 15, quarter = lane >> 4;
 
-  const __amdgpu_buffer_rsrc_t rsrc_a = rows_from<T>(p.a, p.lda, 0, p.M, p.K);
+  const __amdgpu_buffer_rsrc_t rsrc_a = rows_from<T>(p.a, p.lda, m0, min(16, p.M - m0), p.K);
   const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
   const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
   const uint32_t a_off = (static_cast<uint32_t>(row16) * static_cast<uint32_t>(p.lda) + quarter * E) * EB;
   uint32_t b_off[W];
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    const uint32_t row = GATED_FWD ? static_cast<uint32_t>((w & 1) * p.N + (w >> 1) * 16 + row16) : static_cast<uint32_t>(w * 16 + row16);
-    b_off[w] = (row * static_cast<uint32_t>(p.K) + quarter * E) * EB;
-  }
+  for (int w = 0; w < W; ++w) b_off[w] = (static_cast<uint32_t>(w * p.N + row16) * static_cast<uint32_t>(p.K) + quarter * E) * EB;
   f32x4_t acc[W];
 #pragma unroll
   for (int w = 0; w < W; ++w) acc[w] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
   uint4_t fa[2][U], fb[2][U][W];
-  auto request = [&](int piece, int set) {
+  auto request = [&](int piece, int set) LINEAR_INLINE {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = piece * PIECE + u * (4 * E);
@@ -720,7 +733,7 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
       fa[set][u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_a, static_cast<int>((a_off + from) | behind), 0, 0);
     }
   };
-  auto multiply = [&](int set) {
+  auto multiply = [&](int set) LINEAR_INLINE {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -735,20 +748,20 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
     multiply(1);
   }
 
-  // acc[w][i] is column 4 * quarter + i of the tile, token row16; the wavefronts' sums meet in LDS, added in their order
+  // acc[w][e] is column 4 * quarter + e of the tile, token row16; the wavefronts' sums meet in LDS, added in their order
 #pragma unroll
   for (int w = 0; w < W; ++w)
-    *reinterpret_cast<float4*>(&red[wave][w][row16 * 20 + quarter * 4]) = make_float4(acc[w][0], acc[w][1], acc[w][2], acc[w][3]);
+    *reinterpret_cast<float4*>(&red[wave][w][row16 * LD + quarter * 4]) = make_float4(acc[w][0], acc[w][1], acc[w][2], acc[w][3]);
   __syncthreads();
-  for (int q = tid; q < 64 * TN; q += KG * 64) {   // four columns of one token a thread
-    const int tile = q >> 6, row = (q >> 2) & 15, c = (q & 3) * 4, col = n0 + tile * 16 + c;
+  for (int q = tid; q < 64; q += KG * 64) {   // four columns of one token a thread
+    const int in_tile = q >> 2, row = m0 + in_tile, c = (q & 3) * 4, col = n0 + c;
     if (row >= p.M || col >= p.N) continue;
     auto total = [&](int w, float* v) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = 0.f;
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
-        const float4 s = *reinterpret_cast<const float4*>(&red[g][w][row * 20 + c]);
+        const float4 s = *reinterpret_cast<const float4*>(&red[g][w][in_tile * LD + c]);
         v[0] += s.x;
         v[1] += s.y;
         v[2] += s.z;
@@ -756,12 +769,8 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
       }
     };
     float v[4], u[4], zg[4], zu[4], o[4], h[4];
-    if constexpr (GATED_FWD) {
-      total(2 * tile, v);
-      total(2 * tile + 1, u);
-    } else {
-      total(tile, v);
-    }
+    total(0, v);
+    if constexpr (GATED_FWD) total(1, u);
     T* out = static_cast<T*>(p.out) + row * p.ldo + col;
     T* out2 = static_cast<T*>(p.out2) + row * p.ldo2 + col;
     if constexpr (MODE == kLinFwd || MODE == kGatedFwd) {
@@ -856,11 +865,11 @@ int launch_linear_tile(Context* ctx, LinearArgs& a) {
                 linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
 }
 
-template <typename T, int MODE, int TM, int TN, int KG, int NBUF>
+template <typename T, int MODE, int TM, int TN, int KG, int NBUF, int RB>
 int launch_linear_split(Context* ctx, LinearArgs& a) {
   constexpr int BM = TM * 32, BN = TN * 32, BN_OUT = MODE == kGatedFwd ? BN / 2 : BN;
   static const std::string name = std::string("linear_split_kernel<") + type_name<T>() + mode_name(MODE) + std::to_string(BM) + "x" +
-                                  std::to_string(BN) + "," + std::to_string(KG) + "way>";
+                                  std::to_string(BN) + "," + std::to_string(KG) + "way," + std::to_string(RB) + ">";
   a.tiles_m = tiles_over(a.M, BM);
   a.tiles_n = tiles_over(a.N, BN_OUT);
   const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
@@ -868,34 +877,102 @@ int launch_linear_split(Context* ctx, LinearArgs& a) {
   // the larger operand is the one an XCD should fetch once
   a.group_rows = (MODE == kGatedFwd ? 2.0 : 1.0) * a.N > a.M ? 1 : 0;
   a.div_tiles_n = FastDiv(a.group_rows ? a.tiles_m : a.tiles_n);
-  return launch(ctx, linear_split_kernel<T, MODE, TM, TN, KG, NBUF>, dim3(static_cast<unsigned>(tiles)), dim3(KG * 64), a, name.c_str(),
+  return launch(ctx, linear_split_kernel<T, MODE, TM, TN, KG, NBUF, RB>, dim3(static_cast<unsigned>(tiles)), dim3(KG * 64), a, name.c_str(),
                 linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
 }
 
-template <typename T, int MODE, int TN, int KG>
+template <typename T, int MODE, int KG>
 int launch_linear_rows(Context* ctx, LinearArgs& a) {
-  static const std::string name = std::string("linear_rows_kernel<") + type_name<T>() + mode_name(MODE) + std::to_string(16 * TN) + "," +
-                                  std::to_string(KG) + "way>";
-  return launch(ctx, linear_rows_kernel<T, MODE, TN, KG>, dim3(static_cast<unsigned>(tiles_over(a.N, 16 * TN))), dim3(KG * 64), a, name.c_str(),
-                linear_bytes(a, MODE, sizeof(T)), 1);
+  static const std::string name = std::string("linear_rows_kernel<") + type_name<T>() + mode_name(MODE) + "16x16," + std::to_string(KG) + "way>";
+  a.tiles_m = tiles_over(a.M, 16);
+  a.tiles_n = tiles_over(a.N, 16);
+  const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
+  TCH_CHECK_ARG(tiles <= 0x3fffffff, "linear: grid out of range");
+  a.div_tiles_n = FastDiv(static_cast<uint32_t>(a.tiles_m));
+  return launch(ctx, linear_rows_kernel<T, MODE, KG>, dim3(static_cast<unsigned>(tiles)), dim3(KG * 64), a, name.c_str(),
+                linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
+}
+
+// Which kernel: the one with the shortest estimate, (rounds of workgroups) x (reduction steps of a wavefront x microseconds a step +
+// start and end).  The constants are measured on products of 24-16384 rows, 64-11264 outputs and 256-11104 reduction elements, and
+// take the best kernel or one within 10 % of it for nearly all of them: bf16, M x N over K: 24 x 1024 over 4096 7.4 us as 32 x 32 (16-row
+// tiles 9.6, 64 x 64 14.1), 215 x 256 over 4296 8.4 with 16-row tiles (11.5 as 32 x 32, 22 as 64 x 64), 512 x 1024 over 8192 23 as 32 x 64
+// (30 as 64 x 64, 98 as 128 x 128), 1024 x 1024 over 1024 7.7 as 64 x 64 (14.1 as 128 x 128), 2048 x 2048 over 1024 15.3 as 128 x 128 (28 as
+// 64 x 64), 4096 x 4096 over 1024 36 as 256 x 256 (38 as 256 x 128, 40 as 128 x 128).
+enum Kernel : int { kRows16, kSplit32, kSplit32x64, kSplit64, kTile64x128, kTile128, kTile256x128, kTile256, kKernels };
+struct KernelCost {
+  int bm, bn;      // tile; gated forward: half as many output columns
+  int step;        // reduction bytes of a step
+  int ways;        // wavefronts that share a tile's steps
+  int per_cu;      // workgroups of it that a compute unit holds
+  float alone, shared, fixed;   // a step with one workgroup on the compute unit, with per_cu; start and end
+};
+template <typename T, bool GATED_FWD>
+Kernel choose_kernel(const LinearArgs& a) {
+  // (gated tiles of 16-row and 32 x 32 kernels have twice the weight rows)
+  static constexpr KernelCost kBf16[kKernels] = {
+      {16, GATED_FWD ? 32 : 16, 256, 8, 1, GATED_FWD ? 1.9f : 1.35f, 0.f, 1.2f},
+      {32, GATED_FWD ? 64 : 32, 128, 4, 1, GATED_FWD ? 0.72f : 0.48f, 0.f, 0.6f},
+      {GATED_FWD ? 0 : 32, 64, 128, 4, 1, 0.72f, 0.f, 0.6f},
+      {64, 64, 128, 3, 1, 0.78f, 0.f, 0.9f},
+      {0, 0, 0, 0, 0, 0.f, 0.f, 0.f},
+      {128, 128, 128, 1, 2, 0.78f, 1.08f, 2.5f},
+      {256, 128, 128, 1, 1, 0.92f, 0.f, 3.2f},
+      {256, 256, 128, 1, 1, 1.55f, 0.f, 6.f}};
+  static constexpr KernelCost kF32[kKernels] = {
+      {16, GATED_FWD ? 32 : 16, 256, 8, 1, GATED_FWD ? 2.2f : 1.45f, 0.f, 1.2f},
+      {32, GATED_FWD ? 64 : 32, 128, 4, 1, GATED_FWD ? 1.2f : 0.65f, 0.f, 0.8f},
+      {GATED_FWD ? 0 : 32, 64, 128, 4, 1, 1.2f, 0.f, 0.8f},
+      {64, 64, 64, 4, 1, 1.18f, 0.f, 1.2f},
+      {64, 128, 128, 1, 2, 1.03f, 1.95f, 2.5f},
+      {128, 128, 128, 1, 2, 1.95f, 3.75f, 2.5f},
+      {0, 0, 0, 0, 0, 0.f, 0.f, 0.f},
+      {0, 0, 0, 0, 0, 0.f, 0.f, 0.f}};
+  const KernelCost* costs = sizeof(T) == 2 ? kBf16 : kF32;
+  Kernel best = kSplit32;
+  float best_us = INFINITY;
+  for (int k = 0; k < kKernels; ++k) {
+    const KernelCost& c = costs[k];
+    if (!c.bm || (k == kTile256 && a.K * static_cast<int>(sizeof(T)) <= c.step)) continue;   // (256 x 256 takes two steps at least)
+    const double tiles = static_cast<double>(tiles_over(a.M, c.bm)) * tiles_over(a.N, GATED_FWD ? c.bn / 2 : c.bn);
+    const int steps = tiles_over(tiles_over(a.K * static_cast<int>(sizeof(T)), c.step), c.ways);
+    const bool alone = c.per_cu == 1 || tiles <= 256;
+    const double slots = alone ? 256.0 : 256.0 * c.per_cu, rounds = tiles > 8 * slots ? tiles / slots : ceil(tiles / slots);
+    const float us = static_cast<float>(rounds) * (steps * (alone ? c.alone : c.shared) + c.fixed);
+    if (us < best_us) {
+      best_us = us;
+      best = static_cast<Kernel>(k);
+    }
+  }
+  return best;
 }
 
 template <typename T, int MODE>
 int launch_linear_mode(Context* ctx, LinearArgs& a) {
-  constexpr bool kWide = MODE == kGatedFwd;
-  if (a.M <= 16) return launch_linear_rows<T, MODE, 1, 8>(ctx, a);
-  const int64_t tiles = static_cast<int64_t>(tiles_over(a.M, 128)) * tiles_over(a.N, kWide ? 64 : 128);
-  if (tiles >= 192) {
-    if constexpr (sizeof(T) == 2) {
-      if (tiles >= 1024 && a.K > 64) return launch_linear_tile<T, MODE, 2, 4, 4, 2, 2, 128, 1>(ctx, a);
-      if (tiles >= 512) return launch_linear_tile<T, MODE, 4, 2, 2, 2, 3, 128, 1>(ctx, a);
-      return launch_linear_tile<T, MODE, 2, 2, 2, 2, 2, 128, 2>(ctx, a);
-    } else {
-      return launch_linear_tile<T, MODE, 2, 2, 2, 2, 2, 128, 2>(ctx, a);
-    }
+  constexpr bool kWide = MODE == kGatedFwd, kBf = sizeof(T) == 2;
+  switch (choose_kernel<T, kWide>(a)) {
+    case kRows16: return launch_linear_rows<T, MODE, 8>(ctx, a);
+    case kSplit32: return launch_linear_split<T, MODE, 1, kWide ? 2 : 1, 4, 3, 128>(ctx, a);
+    case kSplit32x64:
+      if constexpr (!kWide) return launch_linear_split<T, MODE, 1, 2, 4, 3, 128>(ctx, a);
+      break;
+    case kSplit64:
+      if constexpr (kBf) return launch_linear_split<T, MODE, 2, 2, 3, 3, 128>(ctx, a);
+      else return launch_linear_split<T, MODE, 2, 2, 4, 4, 64>(ctx, a);
+    case kTile64x128:
+      if constexpr (!kBf) return launch_linear_tile<T, MODE, 2, 2, 1, 2, 2, 128, 2>(ctx, a);
+      break;
+    case kTile128: return launch_linear_tile<T, MODE, 2, 2, 2, 2, 2, 128, 2>(ctx, a);
+    case kTile256x128:
+      if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 2, 2, 2, 3, 128, 1>(ctx, a);
+      break;
+    case kTile256:
+      if constexpr (kBf) return launch_linear_tile<T, MODE, 2, 4, 4, 2, 2, 128, 1>(ctx, a);
+      break;
+    default: break;
   }
-  if (static_cast<int64_t>(tiles_over(a.M, 64)) * tiles_over(a.N, kWide ? 32 : 64) >= 256) return launch_linear_split<T, MODE, 2, 2, 4, 4>(ctx, a);
-  return launch_linear_split<T, MODE, 1, kWide ? 2 : 1, 8, kWide ? 3 : 4>(ctx, a);
+  set_error("linear: no kernel");
+  return -22;
 }
 
 template <typename T>

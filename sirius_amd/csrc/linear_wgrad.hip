@@ -278,16 +278,25 @@ __global__ __launch_bounds__(256) void linear_wgrad_sum_kernel(LinearWgradArgs p
   auto slot_of = [&](int g) { return static_cast<int64_t>(2 * g + (run_start(p.units, p.groups, g) >= first ? 0 : 1)); };
   const int tile_n = tile / p.tiles_k, tile_k = tile - tile_n * p.tiles_k;
   const int n0 = tile_n * SIDE + band * 32, k0 = tile_k * SIDE;
-  for (int q = threadIdx.x; q < 32 * SIDE / 4; q += 256) {
-    const int row = q / (SIDE / 4), col = q % (SIDE / 4) * 4;
+  // all quads of a thread at once: a band is a few KB, what counts is how many of its parts' loads are on their way
+  constexpr int QUADS = 32 * SIDE / 4 / 256;
+  float4 sum[QUADS];
+#pragma unroll
+  for (int i = 0; i < QUADS; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int g = g0; g <= g1; ++g) {
+    const float* from = p.slots + slot_of(g) * (SIDE * SIDE) + band * 32 * SIDE;
+    float4 v[QUADS];
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) v[i] = load_streaming_f4(from + (i * 256 + threadIdx.x) * 4);
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) sum[i] = make_float4(sum[i].x + v[i].x, sum[i].y + v[i].y, sum[i].z + v[i].z, sum[i].w + v[i].w);
+  }
+#pragma unroll
+  for (int i = 0; i < QUADS; ++i) {
+    const int q = i * 256 + threadIdx.x, row = q / (SIDE / 4), col = q % (SIDE / 4) * 4;
     if (n0 + row >= p.N || k0 + col >= p.K) continue;
-    const int64_t in_tile = (band * 32 + row) * SIDE + col;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int g = g0; g <= g1; ++g) {
-      const float4 v = load_streaming_f4(p.slots + slot_of(g) * (SIDE * SIDE) + in_tile);
-      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
-    }
     float* to = p.out + static_cast<int64_t>(n0 + row) * p.K + k0 + col;
+    float4 s = sum[i];
     if (p.accumulate) {
       const float4 v = *reinterpret_cast<const float4*>(to);
       s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
