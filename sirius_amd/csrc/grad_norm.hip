@@ -43,10 +43,11 @@ __device__ inline double group_sum_f64(double v, double* scratch) {
   return ((scratch[0] + scratch[1]) + scratch[2]) + scratch[3];
 }
 
-template <typename T>
+// LAST: nobody reads it again
+template <bool LAST, typename T>
 __device__ inline void load4(const T* p, int64_t i, float* v) {
   if constexpr (sizeof(T) == 4) {
-    const float4 f = reinterpret_cast<const float4*>(p)[i];
+    const float4 f = LAST ? load_streaming_f4(p + 4 * i) : reinterpret_cast<const float4*>(p)[i];
     v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
   } else {
     const uint2 u = reinterpret_cast<const uint2*>(p)[i];
@@ -67,7 +68,7 @@ __device__ inline double piece_squares(const Piece& piece) {
 #pragma unroll
   for (int i = 0; i < kVisits; ++i) {
     const int q = i * 256 + threadIdx.x;
-    if (q < quads) load4(src, q, v[i]);
+    if (q < quads) load4<false>(src, q, v[i]);
   }
 #pragma unroll
   for (int i = 0; i < kVisits; ++i) {
@@ -82,9 +83,11 @@ __device__ inline double piece_squares(const Piece& piece) {
 __global__ __launch_bounds__(256) void grad_norm_kernel(NormArgs p) {
   __shared__ double scratch[4];
   double s = 0.0;
+  Piece piece = p.pieces[blockIdx.x];
   for (int64_t i = blockIdx.x; i < p.count; i += gridDim.x) {
-    const Piece piece = p.pieces[i];
+    const Piece next = p.pieces[min(i + gridDim.x, p.count - 1)];   // on its way while this one is read
     s += piece.src_bf16 ? piece_squares<bf16>(piece) : piece_squares<float>(piece);
+    piece = next;
   }
   s = group_sum_f64(s, scratch);
   if (threadIdx.x == 0) p.partial[blockIdx.x] = s;
@@ -132,7 +135,7 @@ __device__ inline void scale_piece(const Piece& piece, float coef) {
 #pragma unroll
   for (int i = 0; i < kVisits; ++i) {
     const int q = i * 256 + threadIdx.x;
-    if (q < quads) load4(src, q, v[i]);
+    if (q < quads) load4<true>(src, q, v[i]);
   }
 #pragma unroll
   for (int i = 0; i < kVisits; ++i) {
@@ -154,14 +157,17 @@ __device__ inline void scale_piece(const Piece& piece, float coef) {
 
 __global__ __launch_bounds__(256) void grad_clip_kernel(ClipArgs p) {
   __shared__ double scratch[4];
+  Piece piece = p.pieces[p.count - 1 - blockIdx.x];
   const float coef = clip_coefficient(p, scratch);
   for (int64_t i = p.count - 1 - blockIdx.x; i >= 0; i -= gridDim.x) {
-    const Piece piece = p.pieces[i];
-    if (coef == 1.f && piece.src == piece.dst) continue;   // times one, in place
-    if (piece.src_bf16)
-      piece.dst_bf16 ? scale_piece<bf16, bf16>(piece, coef) : scale_piece<bf16, float>(piece, coef);
-    else
-      piece.dst_bf16 ? scale_piece<float, bf16>(piece, coef) : scale_piece<float, float>(piece, coef);
+    const Piece next = p.pieces[max(i - gridDim.x, static_cast<int64_t>(0))];
+    if (coef != 1.f || piece.src != piece.dst) {   // (times one, in place: nothing to do)
+      if (piece.src_bf16)
+        piece.dst_bf16 ? scale_piece<bf16, bf16>(piece, coef) : scale_piece<bf16, float>(piece, coef);
+      else
+        piece.dst_bf16 ? scale_piece<float, bf16>(piece, coef) : scale_piece<float, float>(piece, coef);
+    }
+    piece = next;
   }
 }
 

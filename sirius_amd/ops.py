@@ -706,7 +706,7 @@ class GradTable:
         assert tensors, "no tensors"
         self.device = tensors[0].device
         piece = int(lib().tch_grad_table_piece_elems())
-        rows, writes, reads = [], [], []
+        tables, writes, reads = [], [], []
         self.bytes_read = self.bytes_written = 0
         for t, o in zip(tensors, out):
             for x in (t, o):
@@ -723,9 +723,12 @@ class GradTable:
             writes.append((dst, dst + n * ob, src if eb == ob else None))
             reads.append((src, src + n * eb))
             aligned = int(src % (4 * eb) == 0 and dst % (4 * ob) == 0)
-            codes = dtype_code(t) << 32
-            for at in range(0, n, piece):
-                rows.append((src + at * eb, dst + at * ob, min(piece, n - at) | codes, dtype_code(o) | aligned << 32))
+            at = torch.arange(0, n, piece)
+            rows = torch.empty(at.numel(), 4, dtype=torch.int64)
+            rows[:, 0], rows[:, 1] = src + at * eb, dst + at * ob
+            rows[:, 2] = (n - at).clamp(max=piece) | dtype_code(t) << 32
+            rows[:, 3] = dtype_code(o) | aligned << 32
+            tables.append(rows)
         # an element may be written once, and read only where it is written from
         writes.sort()
         for (_, end, _), (start, _, _) in zip(writes, writes[1:]):
@@ -736,8 +739,9 @@ class GradTable:
             while i < len(writes) and writes[i][0] < hi:
                 assert writes[i][1] <= lo or (writes[i][0] == lo and writes[i][2] == lo), "an output overlaps another gradient"
                 i += 1
-        self.pieces = len(rows)
-        self.table = torch.tensor(rows if rows else [(0, 0, 0, 0)], dtype=torch.int64).to(self.device)
+        table = torch.cat(tables) if tables else torch.zeros(0, 4, dtype=torch.int64)
+        self.pieces = table.shape[0]
+        self.table = (table if tables else torch.zeros(1, 4, dtype=torch.int64)).to(self.device)
         self.tensors, self.out = tensors, out
 
 
