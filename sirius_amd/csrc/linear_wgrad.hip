@@ -77,7 +77,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
   int left = 0;
   __amdgpu_buffer_rsrc_t rsrc_a[PA], rsrc_b[PB];
   auto resources = [&]() LINEAR_INLINE {
-    const int here = left < 0 ? 0 : left < kRows ? left : kRows;
+    const int here = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : left < kRows ? left : kRows);
     const uint32_t a_bytes = static_cast<uint32_t>(here) * static_cast<uint32_t>(p.N) * 2, b_bytes = static_cast<uint32_t>(here) * static_cast<uint32_t>(p.K) * 2;
     rsrc_a[0] = make_rsrc(static_cast<const unsigned char*>(p.a) + a_at, a_bytes);
     if constexpr (PA == 2) rsrc_a[1] = make_rsrc(static_cast<const unsigned char*>(p.a_low) + a_at, a_bytes);
@@ -181,9 +181,11 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
   // go to the same buffers
   int64_t unit = run_start(p.units, p.groups, group);
   for (int part = 0; unit < run_end; ++part) {
-    const int tile = static_cast<int>(unit / p.steps), from = static_cast<int>(unit - static_cast<int64_t>(tile) * p.steps);
-    const int to = static_cast<int>(min(static_cast<int64_t>(p.steps), from + (run_end - unit)));
-    const int tile_n = tile / p.tiles_k, tile_k = tile - tile_n * p.tiles_k;
+    // (quotients and 64-bit minima come out of the vector unit: back in scalar registers, or every load of the loop becomes a loop over its resources)
+    const int tile = __builtin_amdgcn_readfirstlane(static_cast<int>(unit / p.steps));
+    const int from = __builtin_amdgcn_readfirstlane(static_cast<int>(unit - static_cast<int64_t>(tile) * p.steps));
+    const int to = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<int64_t>(p.steps), from + (run_end - unit))));
+    const int tile_n = __builtin_amdgcn_readfirstlane(tile / p.tiles_k), tile_k = tile - tile_n * p.tiles_k;
     const int n0 = tile_n * BM, k0 = tile_k * BN;
     const int64_t row0 = static_cast<int64_t>(from) * kRows;
     unit += to - from;
@@ -193,7 +195,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
     for (int j = 0; j < B_LD; ++j) b_off[j] = lane_offset(wave * B_LD + j, RB, p.K, k0);
     a_at = row0 * p.N * 2;
     b_at = row0 * p.K * 2;
-    left = static_cast<int>(min(static_cast<int64_t>(to - from) * kRows, p.M - row0));
+    left = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<int64_t>(to - from) * kRows, p.M - row0)));
     sums = p.bias && tile_k == 0 && wn == 0;
     clear(acc);
 #pragma unroll
