@@ -319,7 +319,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
     constexpr int COLS = GATED_FWD ? 32 : 64;             // output columns of a wavefront
     constexpr int LANES = COLS / E, ROWS = 64 / LANES;    // lanes per row, rows per pass
     constexpr int PASSES = 16 / ROWS, BLOCKS = TM * 2, TOTAL = BLOCKS * PASSES;
-    constexpr int DEPTH = TM > 2 ? 2 : 4;                 // passes whose operands are on their way, as the registers allow
+    constexpr int DEPTH = TM <= 2 ? 4 : MODE == kGatedBwd ? 1 : 2;                 // passes whose operands are on their way, as the registers allow
     const int lane_row = lane / LANES, lane_col = lane % LANES * E;
     const int col = n0 + wn * COLS + lane_col;
     ChunkOperands<T, MODE> operands[DEPTH];
