@@ -33,6 +33,8 @@ class EngineBase:
         self._acc_prog = None
         self._opt_global_prog = None
         self.global_grads = None
+        self.max_grad_norm = None
+        self._norms, self._last_norm = {}, None
 
     def plan(self, batch, loss_scale=1.0):
         key = (int(batch), float(loss_scale))
@@ -153,6 +155,37 @@ class EngineBase:
     def synchronize(self):
         self.ctx.synchronize()
 
+    # ------------------------------------------------------------------ gradient clipping
+    def set_grad_clip(self, max_norm):
+        """From the next optimizer step on, the gradients it consumes are scaled to a global norm of at most max_norm
+        (None: as they are): the step multiplies by the coefficient as it reads them, the buffers stay."""
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError("max_norm must not be negative")
+        self.ctx.synchronize()      # a step in flight still uses the old programs' memory
+        self.max_grad_norm = None if max_norm is None else float(max_norm)
+        self._opt_prog = self._opt_global_prog = None
+        self._norms, self._last_norm = {}, None
+
+    def last_grad_norm(self):
+        """The global norm, before clipping, of the gradients that the most recent optimizer step consumed (nan without
+        clipping)."""
+        if self._last_norm is None:
+            return float("nan")
+        self.ctx.synchronize()
+        return float(self._last_norm.item())
+
+    def _grad_scale(self, grads):
+        """Records the norm of a flat gradient buffer; returns the optimizer step's grad_scale (None without clipping)."""
+        if self.max_grad_norm is None:
+            return None
+        table = ops.GradTable([grads])
+        norm, coef = (self._alloc((4,), torch.float32).zero_()[:1] for _ in range(2))
+        scratch = self._alloc((ops.grad_norm_workspace_bytes(table) // 4,), torch.float32)
+        torch.cuda.synchronize()    # the zeros are there before a launch of this engine's own stream
+        self._norms[grads is self.global_grads] = (norm, coef, scratch, table)
+        ops.grad_norm(self.ctx, table, norm, scratch, max_norm=self.max_grad_norm, coef=coef)
+        return coef
+
     def zero_grad(self):
         ops.fill_zero(self.ctx, self.grads)
 
@@ -176,10 +209,12 @@ class EngineBase:
                 raise RuntimeError("optimizer_step(use_global=True) before any accumulate()")
             if self._opt_global_prog is None:
                 self._opt_global_prog = self._flat_prog(lambda: self._record_optimizer(self.global_grads))
+            self._last_norm = self._norms[True][0] if self.max_grad_norm is not None else None
             cut = self.ctx.run(self._opt_global_prog)
             if zero_global:
                 ops.fill_zero(self.ctx, self.global_grads)
             return cut
         if self._opt_prog is None:
             self._opt_prog = self._flat_prog(lambda: self._record_optimizer(self.grads))
+        self._last_norm = self._norms[False][0] if self.max_grad_norm is not None else None
         return self.ctx.run(self._opt_prog)

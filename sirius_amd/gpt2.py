@@ -46,8 +46,12 @@ class GPT2Engine(EngineBase):
     def __init__(self, vocab=50257, n_pos=1024, n_embd=768, n_layer=12, n_head=12, seq_len=1024, dtype=torch.bfloat16,
                  optimizer="adamw", lr=1e-3, weight_decay=0.01, betas=(0.9, 0.999), eps=1e-8, momentum=0.9,
                  stream=None, allocator=None, overlap_wgrad=True, fused_attention=True, trailing_wgrad=True,
-                 trailing_reduce=None):
+                 trailing_reduce=None, fused_mlp=False):
         self._init_engine(dtype, stream, allocator)
+        # fused_mlp: the activation rides the first MLP projection's launch, its derivative the second one's data gradient: no
+        # pass over the 4 C wide tensors in between.  The activation is then taken of the unrounded pre-activation, and the
+        # order of additions of small batches is the launch's choice: other roundings than without.
+        self.fused_mlp = bool(fused_mlp)
         # trailing_reduce: the split reduction of a weight gradient rides the next weight-gradient launch as extra
         # workgroups instead of being a launch of its own (same bits)
         self.trailing_reduce = (os.environ.get("TCH_TRAILING_REDUCE", "1") != "0") if trailing_reduce is None \
@@ -334,8 +338,12 @@ class GPT2Engine(EngineBase):
                 lin_fwd(pre + "attn.c_proj", o, h1, add=h)
                 m, f1, f2 = act(R, C), act(R, 4 * C), act(R, 4 * C)
                 ln_fwd(pre + "ln_2", 2 * i + 1, h1, m)
-                lin_fwd(pre + "mlp.c_fc", m, f1)
-                ops.gelu_fwd(ctx, f1, f2, tanh_form=True)
+                if self.fused_mlp:
+                    ops.linear_fwd(ctx, m, self._w(pre + "mlp.c_fc.weight").view(4 * C, C), f2,
+                                   bias=self._view(self.params, pre + "mlp.c_fc.bias"), act="gelu_tanh", pre=f1)
+                else:
+                    lin_fwd(pre + "mlp.c_fc", m, f1)
+                    ops.gelu_fwd(ctx, f1, f2, tanh_form=True)
                 h2 = act(R, C)
                 lin_fwd(pre + "mlp.c_proj", f2, h2, add=h1)
                 saved.append((h, a, qkv, P, o, h1, m, f1, f2))
@@ -361,7 +369,7 @@ class GPT2Engine(EngineBase):
             n_sets = 3 if self.trailing_wgrad else 1
             g_sets = [([act(R, C) for _ in range(4 if k == 0 else 3)], act(R, 4 * C), act(R, 3 * C)) for k in range(n_sets)]
             g_c = g_sets[0][0]
-            g_f2 = act(R, 4 * C)                      # main lane only
+            g_f2 = None if self.fused_mlp else act(R, 4 * C)   # main lane only
             dP = act(B * H, T, dtype=torch.float32) if fused else act(B, H, T, T)   # fused: the delta scratch
             d_hf, g = g_c[0], g_c[1]
             with side():
@@ -377,8 +385,14 @@ class GPT2Engine(EngineBase):
                 spare = [t for t in own_c if t is not g]
                 d_m, g1, d_o = spare[0], spare[1], spare[2]
                 # MLP
-                lin_bwd(pre + "mlp.c_proj", f2, g, g_f2)
-                ops.gelu_bwd(ctx, g_f2, f1, g_f1, tanh_form=True)
+                if self.fused_mlp:
+                    with side():
+                        wgrad(as4(f2), as4(g), self._view(self.grads, pre + "mlp.c_proj.weight"),
+                              self._view(self.grads, pre + "mlp.c_proj.bias"))
+                    ops.linear_dgrad(ctx, g, self._wt(pre + "mlp.c_proj.weight").view(4 * C, C), g_f1, act="gelu_tanh", pre=f1)
+                else:
+                    lin_bwd(pre + "mlp.c_proj", f2, g, g_f2)
+                    ops.gelu_bwd(ctx, g_f2, f1, g_f1, tanh_form=True)
                 lin_bwd(pre + "mlp.c_fc", m, g_f1, d_m)
                 ln_bwd(pre + "ln_2", 2 * i + 1, d_m, h1, g1, residual=g)
                 # attention
@@ -437,10 +451,10 @@ class GPT2Engine(EngineBase):
         if self.optimizer == "adamw":
             ops.adamw_step(self.ctx, self.params, grads, self.exp_avg, self.exp_avg_sq, self.step_dev, self.adam_scalars,
                            lr=self.lr, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps,
-                           weight_decay=self.weight_decay, shadow=self.shadow)
+                           weight_decay=self.weight_decay, shadow=self.shadow, grad_scale=self._grad_scale(grads))
         else:
             ops.sgd_momentum_step(self.ctx, self.params, grads, self.momentum_buf, self.lr, self.momentum,
-                                  self.weight_decay, shadow=self.shadow)
+                                  self.weight_decay, shadow=self.shadow, grad_scale=self._grad_scale(grads))
         # the transposed copies are read by the data gradients only: made on the second lane, beside the next
         # step's forward pass; the backward program joins the lanes before its first data gradient
         if self.overlap_wgrad:

@@ -879,7 +879,7 @@ class ResNetEngine(EngineBase):
 
     def _record_optimizer(self, grads):
         ops.sgd_momentum_step(self.ctx, self.params, grads, self.momentum_buf, self.lr, self.momentum,
-                              self.weight_decay, shadow=self.shadow)
+                              self.weight_decay, shadow=self.shadow, grad_scale=self._grad_scale(grads))
         # the transposed copies are read by the data gradients only: made on the second lane, beside the next
         # step's forward pass; the backward program joins the lanes before its first data gradient
         if self.overlap_wgrad:

@@ -667,7 +667,7 @@ class SwinEngine(EngineBase):
     def _record_optimizer(self, grads):
         ops.adamw_step(self.ctx, self.params, grads, self.exp_avg, self.exp_avg_sq, self.step_dev, self.adam_scalars,
                        lr=self.lr, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps,
-                       weight_decay=self.weight_decay, shadow=self.shadow)
+                       weight_decay=self.weight_decay, shadow=self.shadow, grad_scale=self._grad_scale(grads))
         # the transposed copies are read by the data gradients only: made on the second lane, beside the next
         # step's forward pass; the backward program joins the lanes before its first data gradient
         if self.overlap_wgrad:

@@ -22,7 +22,7 @@ from .common import PeerScript, attach_cu_partition, run_epochs, setup
 
 def train(num_epoch: int, batch_size: int, global_batch_size: Optional[int] = None, dataset_size: int = 500,
           seq_len: int = 256, dtype=torch.bfloat16, optimizer: str = "sgd", peer: Optional[PeerScript] = None,
-          num_distinct_samples: Optional[int] = 64, seed=0, **model_config):
+          num_distinct_samples: Optional[int] = 64, seed=0, max_grad_norm: Optional[float] = None, **model_config):
     stream = setup()
     torch_col.init_train_info(batch_size, batch_size, model_name='gpt2')
     train_mode = torch_col.get_colocate_train_mode()
@@ -35,6 +35,7 @@ def train(num_epoch: int, batch_size: int, global_batch_size: Optional[int] = No
     model = GPT2Engine(seq_len=seq_len, dtype=dtype, optimizer=optimizer, stream=stream, allocator=allocator, **hp,
                        **model_config)
     model.init_normal(seed)
+    model.set_grad_clip(max_grad_norm)
     print(f"Train params memory usage: {MemoryPool.get_memory_usage() * 1024:.2f}M")
 
     col_ctrl = torch_col.create_colocate_ctrl(train_mode, hook_mode, num_epoch, batch_size)
@@ -81,6 +82,8 @@ def main():
     parser.add_argument('--seq-len', type=int, default=256)
     parser.add_argument('--optimizer', choices=['sgd', 'adamw'], default='sgd')
     parser.add_argument('--fp32', action='store_true')
+    parser.add_argument('--fused-mlp', action='store_true', help="activation and its derivative in the MLP projections' launches")
+    parser.add_argument('--max-grad-norm', type=float, default=None, help="clip the gradients' global norm ahead of every step")
     parser.add_argument('--peer-script', type=str, default='',
                         help="e.g. '10:l1:2,20:exit:8' = at micro-batch 10 send AdjustL1 to 2, at 20 InferExit to 8")
     args = parser.parse_args()
@@ -96,7 +99,8 @@ def main():
     try:
         train(args.num_epoch, args.batch_size, global_batch_size=args.global_batch_size,
               dataset_size=args.dataset_size, seq_len=args.seq_len, optimizer=args.optimizer,
-              dtype=torch.float32 if args.fp32 else torch.bfloat16, peer=peer)
+              dtype=torch.float32 if args.fp32 else torch.bfloat16, peer=peer, max_grad_norm=args.max_grad_norm,
+              fused_mlp=args.fused_mlp)
     finally:
         if peer is not None:
             peer.stop()
