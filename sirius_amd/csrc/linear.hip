@@ -110,6 +110,17 @@ int linear_launch(Context* ctx, const char* what, int dtype, int mode, LinearArg
                     rows_fit(a.z, a.ldz, wide * N, eb) && rows_fit(a.out2, a.ldo2, mode == kGatedFwd ? 2 * N : N, eb) &&
                     rows_fit(a.low, a.ldo, 2 * N, eb) && rows_fit(a.low2, a.ldo2, N, eb),
                 name + ": rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
+  auto rows_of = [&](const void* t, int64_t ld, int64_t width) { return Span{t, ld * eb, width * eb, M}; };
+  const Span in[4] = {rows_of(a.a, a.lda, K), rows_of(a.add, a.ldadd, N), rows_of(a.z, a.ldz, wide * N), {a.b, K * eb, K * eb, weight_rows}};
+  const Span out[4] = {rows_of(a.out, a.ldo, mode == kGatedBwd ? 2 * N : N), rows_of(a.out2, a.ldo2, mode == kGatedFwd ? 2 * N : N),
+                       rows_of(a.low, a.ldo, 2 * N), rows_of(a.low2, a.ldo2, N)};
+  const Span bias{a.bias, weight_rows * 4, weight_rows * 4, 1};
+  for (int o = 0; o < 4; ++o) {
+    bool ok = apart(out[o], bias);
+    for (int i = 0; i < 4; ++i) ok = ok && apart(out[o], in[i], o == 0 && (i == 1 || i == 2));
+    for (int i = 0; i < o; ++i) ok = ok && apart(out[o], out[i]);
+    TCH_CHECK_ARG(ok, name + ": an output overlaps another tensor (it may be the residual or the pre-activations themselves)");
+  }
   a.M = static_cast<int>(M);
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
@@ -185,6 +196,13 @@ int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows
   TCH_CHECK_ARG(rows_fit(dy.ptr, dy.ld, N, eb) && rows_fit(pre.ptr, pre.ld, wide * N, eb) && rows_fit(dz.ptr, dz.ld, wide * N, eb) &&
                     rows_fit(h.ptr, h.ld, N, eb) && rows_fit(dz_low, dz.ld, wide * N, eb),
                 "act_bwd: rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
+  const Span in[2] = {{dy.ptr, dy.ld * eb, N * eb, M}, {pre.ptr, pre.ld * eb, wide * N * eb, M}};
+  const Span out[3] = {{dz.ptr, dz.ld * eb, wide * N * eb, M}, {h.ptr, h.ld * eb, N * eb, M}, {dz_low, dz.ld * eb, wide * N * eb, M}};
+  for (int o = 0; o < 3; ++o) {
+    bool ok = apart(out[o], in[0], o == 0) && apart(out[o], in[1], o == 0);
+    for (int i = 0; i < o; ++i) ok = ok && apart(out[o], out[i]);
+    TCH_CHECK_ARG(ok, "act_bwd: an output overlaps another tensor (the gradient may be the one it is made of, or the pre-activations)");
+  }
   const int row_chunks = static_cast<int>(N * eb / 16);
   TCH_CHECK_ARG(M * row_chunks < (1ll << 31), "act_bwd: tensor exceeds 2^31 chunks");
   ActBwdArgs a{dy.ptr, pre.ptr, dz.ptr, h.ptr, dz_low, dy.ld, pre.ld, dz.ld, h.ld, static_cast<uint32_t>(M * row_chunks), row_chunks, static_cast<int>(N), act,

@@ -9,6 +9,8 @@
 // unrounded product, not of the rounded copy that is kept in pre: one rounding less in y.
 #pragma once
 
+#include <cstdint>
+
 #include "kernels.h"
 
 namespace tch {
@@ -127,6 +129,23 @@ __device__ inline void combine(const float* v, float* u, const float* zg, const 
 __device__ inline float rounded_off(float v) {
   const float r = bf16_bits_to_float(float_to_bf16_bits(v));
   return fabsf(r) < INFINITY ? v - r : 0.f;
+}
+
+// What a call reads and writes: rows of `width` bytes, `ld` bytes apart.  A launch has no order among its tiles, so that what it
+// writes may not be what another tile reads; a chunk that is read by the lane that then writes it may (`in_place`).
+struct Span {
+  const void* at;
+  int64_t ld, width, rows;
+};
+inline bool apart(const Span& a, const Span& b, bool in_place = false) {
+  if (!a.at || !b.at || a.rows <= 0 || b.rows <= 0) return true;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.at), pb = reinterpret_cast<uintptr_t>(b.at);
+  if (pa + (a.rows - 1) * a.ld + a.width <= pb || pb + (b.rows - 1) * b.ld + b.width <= pa) return true;
+  const bool same_ld = a.ld == b.ld || (a.rows == 1 && b.rows == 1);
+  if (pa == pb && same_ld && a.width == b.width) return in_place;
+  if (a.ld != b.ld) return false;
+  const int64_t ld = a.ld, shift = ((static_cast<int64_t>(pb) - static_cast<int64_t>(pa)) % ld + ld) % ld;   // columns of one matrix?
+  return shift >= a.width && shift + b.width <= ld;
 }
 
 // fn with the activation as a constant

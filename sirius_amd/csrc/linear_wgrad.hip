@@ -401,6 +401,14 @@ int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy,
   const bool low = x_low || dy_low;
   Choice c = choose(M, n, k, low, workspace != nullptr);
   TCH_CHECK_ARG(slot_floats(c) * 4 <= (workspace ? workspace_bytes : 0), "linear_wgrad: workspace too small");
+  const Span in[4] = {{x, K * 2, K * 2, M}, {x_low, K * 2, K * 2, M}, {dy, N * 2, N * 2, M}, {dy_low, N * 2, N * 2, M}};
+  const Span out[3] = {{dw, K * 4, K * 4, N}, {dbias, N * 4, N * 4, 1}, {workspace, slot_floats(c) * 4, slot_floats(c) * 4, c.cut ? 1 : 0}};
+  for (int o = 0; o < 3; ++o) {
+    bool ok = true;
+    for (const Span& i : in) ok = ok && apart(out[o], i);
+    for (int i = 0; i < o; ++i) ok = ok && apart(out[o], out[i]);
+    TCH_CHECK_ARG(ok, "linear_wgrad: an output or the workspace overlaps another tensor");
+  }
   const int side = c.big ? 256 : 128;
   LinearWgradArgs a{};
   a.a = dy, a.a_low = dy_low;

@@ -972,7 +972,7 @@ def _weights(ctx, name, w, dtype):
 def linear_fwd(ctx, x, w, y, bias=None, act="none", residual=None, pre=None):
     """y = act(x w^T + bias) + residual in one launch: x [..., K], w [N, K], y [..., N], bias [N] fp32; pre (like y) keeps
     x w^T + bias for the backward pass.  Any number of rows; K and N multiples of a 16-byte chunk.  x, y, residual and pre may be
-    columns of wider tensors (rows on 16-byte boundaries); residual may be y itself.  act: one of ACTIVATIONS."""
+    columns of wider tensors (rows on 16-byte boundaries); residual may be y itself, nothing else may overlap an output.  act: one of ACTIVATIONS."""
     N, K = w.shape
     xp, ldx, M = _matrix(ctx, "x", x, K)
     yp, ldy, _ = _matrix(ctx, "y", y, N, M, x.dtype)
@@ -985,7 +985,7 @@ def linear_fwd(ctx, x, w, y, bias=None, act="none", residual=None, pre=None):
 def linear_dgrad(ctx, dy, wt, dx, act="none", pre=None, residual=None):
     """dx = (dy w) . act'(pre) + residual in one launch: wt [K, N] is the weight [N, K] transposed (as for conv2d_dgrad), dy [..., N],
     dx, pre and residual [..., K].  pre and act are those of the layer in FRONT of this one, whose output this layer read: dx is
-    then the gradient of that layer's pre-activation."""
+    then the gradient of that layer's pre-activation.  pre or residual may be dx itself."""
     K, N = wt.shape
     dyp, lddy, M = _matrix(ctx, "dy", dy, N)
     dxp, lddx, _ = _matrix(ctx, "dx", dx, K, M, dy.dtype)
@@ -1119,7 +1119,7 @@ def gated_act_bwd(ctx, dh, pre, dpre, act="silu", h=None, dpre_low=None):
 def linear_dgrad_gated(ctx, dy, wt, pre, dpre, act="silu", h=None, dpre_low=None, h_low=None):
     """The data gradient of a projection behind a gated layer, through that layer's product and activation, in one launch:
     dh = dy w stays on the chip, dpre = (dh . u . act'(g) | dh . act(g)) [..., 2F] is stored, and h = act(g) . u again where it is
-    asked for (the forward pass need not keep it).  wt [F, N] is the projection's weight [N, F] transposed, dy [..., N].
+    asked for (the forward pass need not keep it).  dpre may be pre.  wt [F, N] is the projection's weight [N, F] transposed, dy [..., N].
     dpre_low, h_low (bf16): what rounding took off dpre and h, for linear_wgrad."""
     F, N = wt.shape
     dyp, lddy, M = _matrix(ctx, "dy", dy, N)

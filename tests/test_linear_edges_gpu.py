@@ -321,6 +321,45 @@ def test_refusals(ctx):
         ops.linear_wgrad(ctx, big, dy, torch.empty(4096, 1024, device="cuda"), workspace=torch.empty(need // 2, dtype=torch.uint8, device="cuda"))
 
 
+def test_outputs_that_overlap_are_refused(ctx):
+    from sirius_amd import ops
+    from sirius_amd._lib import TorchColHipError
+
+    def new(*shape, dtype=BF16):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+    M, N = 40, 64
+    wide, w, pre = new(M, 4 * N), rnd(N, N, dtype=BF16, seed=1, std=0.1), rnd(M, 2 * N, dtype=BF16, seed=2)
+    wide.copy_(rnd(M, 4 * N, dtype=BF16, seed=3))
+    col = [wide[:, i * N:(i + 1) * N] for i in range(4)]
+    want = new(M, N)
+    ops.linear_fwd(ctx, col[0], w, want, residual=col[2])
+    ops.linear_fwd(ctx, col[0], w, col[1], residual=col[2], pre=col[3])      # columns of one matrix side by side are apart
+    assert torch.equal(want, col[1])
+    flat = new(M * N + 8)
+    shifted = flat[8:].view(M, N)
+    flat = flat[:M * N].view(M, N)
+    square = new(M, M)
+    for call in [
+            lambda: ops.linear_fwd(ctx, col[0], w, col[0]),
+            lambda: ops.linear_fwd(ctx, col[0], w, wide[:, 8:8 + N]),
+            lambda: ops.linear_fwd(ctx, col[0], w, flat, residual=shifted),
+            lambda: ops.linear_fwd(ctx, col[0], w, flat, pre=flat),
+            lambda: ops.linear_fwd(ctx, col[0], w, flat, residual=col[2], pre=shifted),
+            lambda: ops.linear_fwd(ctx, square, wide.view(-1)[:M * M].view(M, M), wide[:, :M]),       # over the weights
+            lambda: ops.linear_fwd(ctx, col[0], w, flat, residual=wide[:M // 4].view(M, N), pre=col[0]),
+            lambda: ops.linear_dgrad(ctx, flat, w, flat),
+            lambda: ops.linear_dgrad(ctx, flat, w, col[1], act="silu", pre=wide[:, N + 8:2 * N + 8]),
+            lambda: ops.linear_dgrad_gated(ctx, flat, w, pre, pre, h=pre[:, :N]),
+            lambda: ops.linear_dgrad_gated(ctx, flat, w, pre, wide[:, :2 * N], dpre_low=wide[:, N:3 * N]),
+            lambda: ops.linear_dgrad_gated(ctx, flat, w, pre, wide[:, :2 * N], dpre_low=pre),
+            lambda: ops.act_bwd(ctx, col[0], flat, wide[:, 8:8 + N], "silu"),
+            lambda: ops.act_bwd(ctx, col[0], flat, col[1], "silu", dz_low=col[1]),
+            lambda: ops.gated_act_bwd(ctx, pre[:, :N], wide[:, :2 * N], pre),
+            lambda: ops.linear_wgrad(ctx, flat, flat, wide.view(torch.float32).view(-1)[:N * N].view(N, N), x_low=wide.view(-1)[:M * N].view(M, N))]:
+        with pytest.raises((TorchColHipError, AssertionError)):
+            call()
+
+
 @pytest.mark.parametrize("act", ACTS[2:])
 @pytest.mark.parametrize("gated", [False, True], ids=["linear", "gated"])
 def test_gradients_against_differences(ctx, act, gated):

@@ -89,3 +89,17 @@ def test_gradient_norm():
     refused("tch_clip_grad_norm", None, A, 1, 4, 4, 1.0, B, ctypes.c_void_p(0x10004))
     refused("tch_adamw_step_scaled", None, A, A, A, A, None, 4, 0.1, 0.9, 0.99, 1e-8, 0.0, B, C, None)
     refused("tch_sgd_momentum_step_scaled", None, A, A, A, None, 4, 0.1, 0.9, 0.0, None)
+
+
+def test_outputs_that_overlap():
+    def at(byte):
+        return ctypes.c_void_p(0x100000 + byte)
+    assert "overlaps" in refused("tch_linear_fwd", *fwd(x=at(0), y=at(16), ldx=64, ldy=64))
+    assert "overlaps" in refused("tch_linear_fwd", *fwd(y=at(0), ldy=96, res=at(32), ldr=96))
+    assert "overlaps" in refused("tch_linear_fwd", *fwd(y=at(0), ldy=32, pre=at(0), ldp=32))
+    assert "overlaps" in refused("tch_linear_fwd", *fwd(y=at(0), ldy=32, bias=at(64)))
+    assert "overlaps" in refused("tch_linear_fwd", *fwd(w=at(0), y=at(32 * 64 * 2 - 16), ldy=32))
+    assert "overlaps" in refused("tch_linear_dgrad_gated", None, BF16, A, 64, B, at(0), 64, at(0), at(0), 64, None, None, 0, 4, 4, 64, 32)
+    assert "overlaps" in refused("tch_act_bwd", None, BF16, at(0), 32, B, 32, at(64), None, 32, 1, 4, 32)
+    assert "overlaps" in refused("tch_linear_wgrad", None, at(0), None, B, None, at(64 * 64 * 2 - 16), None, 0, 64, 64, 64, None, 0)
+    assert "overlaps" in refused("tch_linear_wgrad", None, A, None, B, None, at(0), at(16), 0, 64, 64, 64, None, 0)
