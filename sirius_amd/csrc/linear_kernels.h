@@ -2,7 +2,7 @@
 // feed-forward layer does to it in the epilogue (linear_epilogue.h).  A has its own row stride, B (the weights) is dense.
 // Compiled once per element type (linear_bf16.hip, linear_f32.hip).
 //
-// Gated modes multiply both projections in one tile: 32 (or 16) rows of the gate's weights lie next to the same rows of the up
+// Gated modes multiply both projections in one tile: 32 (in the narrowest tiles 16) rows of the gate's weights lie next to the same rows of the up
 // projection's, so that a lane ends up with both products of its columns and the epilogue needs nobody else's.
 #pragma once
 
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), KS = RB / EB, SL = RB / 32, SLOTS = RB / 16, LD_ROWS = 1024 / RB;
   constexpr bool GATED_FWD = MODE == kGatedFwd;
   constexpr int BM = TM * 32, BN = TN * 32, BN_OUT = GATED_FWD ? BN / 2 : BN;
-  static_assert(!GATED_FWD || TN % 2 == 0, "gate and up tiles come in pairs");
+  constexpr int HALF = TN == 1 ? 16 : 32;   // gated: columns of the gate that lie together, in front of the same of the up projection
   constexpr int A_LD = BM / LD_ROWS, B_LD = BN / LD_ROWS, A_BYTES = BM * RB, BUF_BYTES = (BM + BN) * RB;
   constexpr int NT = KG * 64, LD = BN + 4;
   constexpr int RED_BYTES = KG * BM * LD * 4, RING_BYTES = KG * NBUF * BUF_BYTES;
@@ -515,8 +515,8 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
   for (int j = 0; j < A_LD; ++j) a_off[j] = (static_cast<uint32_t>(j * LD_ROWS + sub_row) * static_cast<uint32_t>(p.lda) + chunk[j & 1] * E) * EB;
 #pragma unroll
   for (int j = 0; j < B_LD; ++j) {
-    const int trow = j * LD_ROWS + sub_row, block = trow >> 5;
-    const uint32_t row = GATED_FWD ? static_cast<uint32_t>((block & 1) * p.N + (block >> 1) * 32 + (trow & 31)) : static_cast<uint32_t>(trow);
+    const int trow = j * LD_ROWS + sub_row, block = trow / HALF;
+    const uint32_t row = GATED_FWD ? static_cast<uint32_t>((block & 1) * p.N + (block >> 1) * HALF + trow % HALF) : static_cast<uint32_t>(trow);
     b_off[j] = (row * static_cast<uint32_t>(p.K) + chunk[j & 1] * E) * EB;
   }
   const __amdgpu_buffer_rsrc_t rsrc_a =
@@ -648,8 +648,8 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
       if (q >= ITEMS || n0 + c >= p.N) continue;
       float v[E], u[E];
       if constexpr (GATED_FWD) {
-        total(row, (c >> 5) * 64 + (c & 31), v);
-        total(row, (c >> 5) * 64 + 32 + (c & 31), u);
+        total(row, c / HALF * (2 * HALF) + c % HALF, v);
+        total(row, c / HALF * (2 * HALF) + HALF + c % HALF, u);
       } else {
         total(row, c, v);
       }
@@ -667,11 +667,11 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
 // ---------------------------------------------------------------------------
 // few rows (tokens that decode together), or few outputs: operands straight into registers
 // ---------------------------------------------------------------------------
-// A workgroup has 16 rows and 16 output columns (of the gate and of the up projection); its KG wavefronts take 256-byte pieces of
-// the reduction in turn.  Weight rows are the rows and the tokens the columns of 16 x 16 MFMA tiles; lane l holds the 16-byte
+// A workgroup has 16 rows and 16 output columns; its KG wavefronts take 256-byte pieces of the reduction in turn.  Weight rows are the rows and the tokens the columns of 16 x 16 MFMA tiles; lane l holds the 16-byte
 // chunk l / 16 (of four) of row l % 16, so that a load covers 64 neighbouring bytes of sixteen rows.  The next piece is
 // requested before this one is multiplied.  Up to 16 rows it is bound by the bytes of the weights; beyond, by what a compute unit
-// loads into registers (32 or 64 rows a workgroup, for fewer loads of the weights, were slower throughout).
+// loads into registers (32 or 64 rows a workgroup, for fewer loads of the weights, were slower throughout, and so were gate and up tiles
+// next to each other against 32 x 32 tiles with a ring in LDS).  One token through 4096 x 4096 bf16: 7.6 us, 4.4 TB/s.
 template <typename T>
 __device__ inline void mma16(const uint4_t& first, const uint4_t& second, f32x4_t& acc) {
   if constexpr (sizeof(T) == 2) {
@@ -697,11 +697,10 @@ __device__ inline void store_four(T* p, const float* v) {
 template <typename T, int MODE, int KG>
 __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T);
-  constexpr bool GATED_FWD = MODE == kGatedFwd;
-  constexpr int W = GATED_FWD ? 2 : 1;         // weight tiles of 16 rows: gate and up next to each other
-  constexpr int U = 4, PIECE = U * 4 * E;      // loads per piece and tile; elements of a piece
-  constexpr int LD = 20;                       // floats of a row of 16 partial sums
-  __shared__ float red[KG][W][16 * LD];
+  static_assert(MODE != kGatedFwd, "gate and up projections need another layout");
+  constexpr int U = 4, PIECE = U * 4 * E;   // loads per piece and tile; elements of a piece
+  constexpr int LD = 20;                    // floats of a row of 16 partial sums
+  __shared__ float red[KG][16 * LD];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // consecutive workgroups (one XCD) share the weights of a column tile
@@ -715,29 +714,22 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
   const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
   const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
   const uint32_t a_off = (static_cast<uint32_t>(row16) * static_cast<uint32_t>(p.lda) + quarter * E) * EB;
-  uint32_t b_off[W];
-#pragma unroll
-  for (int w = 0; w < W; ++w) b_off[w] = (static_cast<uint32_t>(w * p.N + row16) * static_cast<uint32_t>(p.K) + quarter * E) * EB;
-  f32x4_t acc[W];
-#pragma unroll
-  for (int w = 0; w < W; ++w) acc[w] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const uint32_t b_off = (static_cast<uint32_t>(row16) * static_cast<uint32_t>(p.K) + quarter * E) * EB;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 
-  uint4_t fa[2][U], fb[2][U][W];
+  uint4_t fa[2][U], fb[2][U];
   auto request = [&](int piece, int set) LINEAR_INLINE {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = piece * PIECE + u * (4 * E);
       const uint32_t behind = k + quarter * E >= p.K ? kOutOfRange : 0u, from = static_cast<uint32_t>(k) * EB;
-#pragma unroll
-      for (int w = 0; w < W; ++w) fb[set][u][w] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_b, static_cast<int>((b_off[w] + from) | behind), 0, 0);
+      fb[set][u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_b, static_cast<int>((b_off + from) | behind), 0, 0);
       fa[set][u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_a, static_cast<int>((a_off + from) | behind), 0, 0);
     }
   };
   auto multiply = [&](int set) LINEAR_INLINE {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int w = 0; w < W; ++w) mma16<T>(fb[set][u][w], fa[set][u], acc[w]);
+    for (int u = 0; u < U; ++u) mma16<T>(fb[set][u], fa[set][u], acc);
   };
   // pieces behind the last one are requested out of range and add zeros: no branch around the loads in flight
   request(wave, 0);
@@ -748,47 +740,31 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
     multiply(1);
   }
 
-  // acc[w][e] is column 4 * quarter + e of the tile, token row16; the wavefronts' sums meet in LDS, added in their order
-#pragma unroll
-  for (int w = 0; w < W; ++w)
-    *reinterpret_cast<float4*>(&red[wave][w][row16 * LD + quarter * 4]) = make_float4(acc[w][0], acc[w][1], acc[w][2], acc[w][3]);
+  // acc[e] is column 4 * quarter + e of the tile, token row16; the wavefronts' sums meet in LDS, added in their order
+  *reinterpret_cast<float4*>(&red[wave][row16 * LD + quarter * 4]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
   for (int q = tid; q < 64; q += KG * 64) {   // four columns of one token a thread
     const int in_tile = q >> 2, row = m0 + in_tile, c = (q & 3) * 4, col = n0 + c;
     if (row >= p.M || col >= p.N) continue;
-    auto total = [&](int w, float* v) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f}, u[4], zg[4], zu[4], o[4], h[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = 0.f;
-#pragma unroll
-      for (int g = 0; g < KG; ++g) {
-        const float4 s = *reinterpret_cast<const float4*>(&red[g][w][in_tile * LD + c]);
-        v[0] += s.x;
-        v[1] += s.y;
-        v[2] += s.z;
-        v[3] += s.w;
-      }
-    };
-    float v[4], u[4], zg[4], zu[4], o[4], h[4];
-    total(0, v);
-    if constexpr (GATED_FWD) total(1, u);
+    for (int g = 0; g < KG; ++g) {
+      const float4 s = *reinterpret_cast<const float4*>(&red[g][in_tile * LD + c]);
+      v[0] += s.x;
+      v[1] += s.y;
+      v[2] += s.z;
+      v[3] += s.w;
+    }
     T* out = static_cast<T*>(p.out) + row * p.ldo + col;
     T* out2 = static_cast<T*>(p.out2) + row * p.ldo2 + col;
-    if constexpr (MODE == kLinFwd || MODE == kGatedFwd) {
+    if constexpr (MODE == kLinFwd) {
       if (p.bias) {
         float b[4];
         load_four(p.bias + col, b);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += b[e];
-        if constexpr (GATED_FWD) {
-          load_four(p.bias + p.N + col, b);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) u[e] += b[e];
-        }
       }
-      if (p.out2) {
-        store_four(out2, v);
-        if constexpr (GATED_FWD) store_four(out2 + p.N, u);
-      }
+      if (p.out2) store_four(out2, v);
     } else {
       const T* z = static_cast<const T*>(p.z) + row * p.ldz + col;
       if (MODE == kGatedBwd || p.act != kActNone) load_four(z, zg);
@@ -860,7 +836,10 @@ int launch_linear_tile(Context* ctx, LinearArgs& a) {
   a.div_tiles_n = FastDiv(a.tiles_n);
   a.div_group = FastDiv(static_cast<uint32_t>(a.group_rows > 1 ? a.group_rows * a.tiles_n : 1));
   a.div_rows = FastDiv(a.group_rows > 1 ? a.group_rows : 1);
-  const unsigned grid = static_cast<unsigned>(tiles < 256 * PER_CU ? tiles : 256 * PER_CU);
+  // bf16: the workgroups that the chip holds walk the tiles.  fp32 tiles take so long that their number per compute unit is what
+  // counts: a workgroup per tile, and who is done makes room (768 x 6216 over 3480: 319 us, walked 411)
+  const int64_t most = sizeof(T) == 2 ? 256 * PER_CU : tiles;
+  const unsigned grid = static_cast<unsigned>(tiles < most ? tiles : most);
   return launch(ctx, linear_tile_kernel<T, MODE, WM, WN, TM, TN, NBUF, RB, PER_CU>, dim3(grid), dim3(WM * WN * 64), a, name.c_str(),
                 linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
 }
@@ -894,40 +873,37 @@ int launch_linear_rows(Context* ctx, LinearArgs& a) {
 }
 
 // Which kernel: the one with the shortest estimate, (rounds of workgroups) x (reduction steps of a wavefront x microseconds a step +
-// start and end).  The constants are measured on products of 24-16384 rows, 64-11264 outputs and 256-11104 reduction elements, and
-// take the best kernel or one within 10 % of it for nearly all of them: bf16, M x N over K: 24 x 1024 over 4096 7.4 us as 32 x 32 (16-row
-// tiles 9.6, 64 x 64 14.1), 215 x 256 over 4296 8.4 with 16-row tiles (11.5 as 32 x 32, 22 as 64 x 64), 512 x 1024 over 8192 23 as 32 x 64
-// (30 as 64 x 64, 98 as 128 x 128), 1024 x 1024 over 1024 7.7 as 64 x 64 (14.1 as 128 x 128), 2048 x 2048 over 1024 15.3 as 128 x 128 (28 as
-// 64 x 64), 4096 x 4096 over 1024 36 as 256 x 256 (38 as 256 x 128, 40 as 128 x 128).
-enum Kernel : int { kRows16, kSplit32, kSplit32x64, kSplit64, kTile64x128, kTile128, kTile256x128, kTile256, kKernels };
+// start and end).  The constants are measured on products of 1-16384 rows, 64-11264 outputs and 256-11104 reduction elements, and
+// take the best kernel or one within 10 % of it for nearly all of them: bf16, M x N over K: 1 x 4096 over 4096 9.1 us with 16-row tiles (10.9
+// as 32 x 32), 17 x 1024 over 4096 7.3 as 32 x 32 (16-row tiles 9.8, 32 x 64 9.5), 512 x 1024 over 8192 23 as 32 x 64 (30 as 64 x 64),
+// 1024 x 1024 over 1024 7.7 as 64 x 64 (9.1 as 128 x 64, 10.8 as 128 x 128), 512 x 4096 over 4096 29 as 128 x 64 (37 as 128 x 128, 38 as
+// 64 x 64, 54 as 256 x 128), 512 x 8192 over 8192 76 as 128 x 128 (102 as 128 x 64, 103 as 256 x 128; 128 x 128 with two buffers 114),
+// 4096 x 4096 over 1024 36 as 256 x 256 (38 as 256 x 128, 40 as 128 x 128).  Gated, 7 rows, 2048 outputs over 8192: 19 as 32 x 32 (32 x 64
+// 25).  fp32: 8 x 4096 over 8192 33 with 16-row tiles (45 as 32 x 32), 768 x 6216 over 3480 319 as 128 x 64 (347 as 64 x 64, 420 as 128 x 128).
+enum Kernel : int { kRows16, kSplit32, kSplit32x64, kSplit64, kTile128x64, kTile128, kTile256x128, kTile256, kKernels };
 struct KernelCost {
   int bm, bn;      // tile; gated forward: half as many output columns
   int step;        // reduction bytes of a step
   int ways;        // wavefronts that share a tile's steps
-  int per_cu;      // workgroups of it that a compute unit holds
-  float alone, shared, fixed;   // a step with one workgroup on the compute unit, with per_cu; start and end
+  float step_us, full_us;   // a step where there is one workgroup; where there are 256 (16-row tiles: where 16 rows are filled)
+  float fixed_us, again_us; // start and end; what a further round costs beyond that
 };
 template <typename T, bool GATED_FWD>
 Kernel choose_kernel(const LinearArgs& a) {
-  // (gated tiles of 16-row and 32 x 32 kernels have twice the weight rows)
-  static constexpr KernelCost kBf16[kKernels] = {
-      {16, GATED_FWD ? 32 : 16, 256, 8, 1, GATED_FWD ? 1.9f : 1.35f, 0.f, 1.2f},
-      {32, GATED_FWD ? 64 : 32, 128, 4, 1, GATED_FWD ? 0.72f : 0.48f, 0.f, 0.6f},
-      {GATED_FWD ? 0 : 32, 64, 128, 4, 1, 0.72f, 0.f, 0.6f},
-      {64, 64, 128, 3, 1, 0.78f, 0.f, 0.9f},
-      {0, 0, 0, 0, 0, 0.f, 0.f, 0.f},
-      {128, 128, 128, 1, 2, 0.78f, 1.08f, 2.5f},
-      {256, 128, 128, 1, 1, 0.92f, 0.f, 3.2f},
-      {256, 256, 128, 1, 1, 1.55f, 0.f, 6.f}};
-  static constexpr KernelCost kF32[kKernels] = {
-      {16, GATED_FWD ? 32 : 16, 256, 8, 1, GATED_FWD ? 2.2f : 1.45f, 0.f, 1.2f},
-      {32, GATED_FWD ? 64 : 32, 128, 4, 1, GATED_FWD ? 1.2f : 0.65f, 0.f, 0.8f},
-      {GATED_FWD ? 0 : 32, 64, 128, 4, 1, 1.2f, 0.f, 0.8f},
-      {64, 64, 64, 4, 1, 1.18f, 0.f, 1.2f},
-      {64, 128, 128, 1, 2, 1.03f, 1.95f, 2.5f},
-      {128, 128, 128, 1, 2, 1.95f, 3.75f, 2.5f},
-      {0, 0, 0, 0, 0, 0.f, 0.f, 0.f},
-      {0, 0, 0, 0, 0, 0.f, 0.f, 0.f}};
+  static constexpr KernelCost kBf16[kKernels] = {{GATED_FWD ? 0 : 16, 16, 256, 8, 0.85f, 1.45f, 1.2f, 0.f},
+                                                 {32, 32, 128, 4, 0.22f, 0.45f, 0.6f, 0.f},
+                                                 {32, 64, 128, 4, 0.4f, 0.75f, 0.6f, 0.f},
+                                                 {64, 64, 128, 3, 0.78f, 0.78f, 0.9f, 0.f},
+                                                 {128, 64, 128, 1, 0.43f, 0.43f, 2.5f, 0.f},
+                                                 {128, 128, 128, 1, 0.56f, 0.56f, 3.5f, 0.f},
+                                                 {256, 128, 128, 1, 0.92f, 0.92f, 3.2f, 0.f},
+                                                 {256, 256, 128, 1, 1.55f, 1.55f, 6.f, 0.f}};
+  // (128 x 64: two share a compute unit at half the rate each)
+  static constexpr KernelCost kF32[kKernels] = {{GATED_FWD ? 0 : 16, 16, 256, 8, 1.45f, 1.45f, 1.2f, 0.f},
+                                                {32, 32, 128, 4, 0.65f, 0.65f, 0.8f, 2.f},
+                                                {32, 64, 128, 4, 1.2f, 1.2f, 0.8f, 3.5f},
+                                                {64, 64, 64, 4, 1.18f, 1.18f, 1.2f, 3.5f},
+                                                {128, 64, 128, 1, 1.f, 1.f, 2.8f, 0.f}};
   const KernelCost* costs = sizeof(T) == 2 ? kBf16 : kF32;
   Kernel best = kSplit32;
   float best_us = INFINITY;
@@ -936,9 +912,10 @@ Kernel choose_kernel(const LinearArgs& a) {
     if (!c.bm || (k == kTile256 && a.K * static_cast<int>(sizeof(T)) <= c.step)) continue;   // (256 x 256 takes two steps at least)
     const double tiles = static_cast<double>(tiles_over(a.M, c.bm)) * tiles_over(a.N, GATED_FWD ? c.bn / 2 : c.bn);
     const int steps = tiles_over(tiles_over(a.K * static_cast<int>(sizeof(T)), c.step), c.ways);
-    const bool alone = c.per_cu == 1 || tiles <= 256;
-    const double slots = alone ? 256.0 : 256.0 * c.per_cu, rounds = tiles > 8 * slots ? tiles / slots : ceil(tiles / slots);
-    const float us = static_cast<float>(rounds) * (steps * (alone ? c.alone : c.shared) + c.fixed);
+    const double rounds = tiles > 8 * 256 ? tiles / 256 : ceil(tiles / 256);
+    const float load = k == kRows16 ? static_cast<float>(min(a.M, 16)) / 16.f : tiles < 256 ? static_cast<float>(tiles) / 256.f : 1.f;
+    const float step_us = c.step_us + load * (c.full_us - c.step_us);
+    const float us = static_cast<float>(rounds) * (steps * step_us + c.fixed_us) + static_cast<float>(rounds - 1.0) * c.again_us;
     if (us < best_us) {
       best_us = us;
       best = static_cast<Kernel>(k);
@@ -951,18 +928,20 @@ template <typename T, int MODE>
 int launch_linear_mode(Context* ctx, LinearArgs& a) {
   constexpr bool kWide = MODE == kGatedFwd, kBf = sizeof(T) == 2;
   switch (choose_kernel<T, kWide>(a)) {
-    case kRows16: return launch_linear_rows<T, MODE, 8>(ctx, a);
-    case kSplit32: return launch_linear_split<T, MODE, 1, kWide ? 2 : 1, 4, 3, 128>(ctx, a);
-    case kSplit32x64:
-      if constexpr (!kWide) return launch_linear_split<T, MODE, 1, 2, 4, 3, 128>(ctx, a);
+    case kRows16:
+      if constexpr (!kWide) return launch_linear_rows<T, MODE, 8>(ctx, a);
       break;
+    case kSplit32: return launch_linear_split<T, MODE, 1, 1, 4, 3, 128>(ctx, a);
+    case kSplit32x64: return launch_linear_split<T, MODE, 1, 2, 4, 3, 128>(ctx, a);
     case kSplit64:
       if constexpr (kBf) return launch_linear_split<T, MODE, 2, 2, 3, 3, 128>(ctx, a);
       else return launch_linear_split<T, MODE, 2, 2, 4, 4, 64>(ctx, a);
-    case kTile64x128:
-      if constexpr (!kBf) return launch_linear_tile<T, MODE, 2, 2, 1, 2, 2, 128, 2>(ctx, a);
+    case kTile128x64:
+      if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 1, 1, 2, 4, 128, 1>(ctx, a);
+      else return launch_linear_tile<T, MODE, 4, 1, 1, 2, 2, 128, 2>(ctx, a);
+    case kTile128:
+      if constexpr (kBf) return launch_linear_tile<T, MODE, 2, 2, 2, 2, 3, 128, 1>(ctx, a);
       break;
-    case kTile128: return launch_linear_tile<T, MODE, 2, 2, 2, 2, 2, 128, 2>(ctx, a);
     case kTile256x128:
       if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 2, 2, 2, 3, 128, 1>(ctx, a);
       break;

@@ -264,34 +264,45 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
   }
 }
 
-// The tiles that several workgroups had a part of: dw (+)= their sum in the workgroups' order.  A workgroup here has a band of 32
-// rows of a tile.
+// The tiles that several workgroups had a part of: dw (+)= their sum in the workgroups' order.  A workgroup here has a band of
+// kBand rows of a tile; the loads of kPartsAtOnce parts are on their way together (few tiles have many parts each: 272 x 176 over 4115
+// rows 85, 33 us a part at a time in bands of 32 rows).
+constexpr int kBand = 8, kPartsAtOnce = 8;
 template <int SIDE>
 __global__ __launch_bounds__(256) void linear_wgrad_sum_kernel(LinearWgradArgs p) {
-  constexpr int BANDS = SIDE / 32;
+  constexpr int BANDS = SIDE / kBand;
   const int tile = blockIdx.x / BANDS, band = blockIdx.x % BANDS;
   const int64_t first = static_cast<int64_t>(tile) * p.steps, behind = first + p.steps;
   // the group that has the tile's first unit, and the slot of a group's part
   int g0 = static_cast<int>(first * p.groups / p.units);
   while (run_start(p.units, p.groups, g0 + 1) <= first) ++g0;
   if (run_start(p.units, p.groups, g0 + 1) >= behind) return;   // one workgroup had all of it
-  int g1 = g0 + 1;
-  while (g1 + 1 < p.groups && run_start(p.units, p.groups, g1 + 1) < behind) ++g1;
-  auto slot_of = [&](int g) { return static_cast<int64_t>(2 * g + (run_start(p.units, p.groups, g) >= first ? 0 : 1)); };
+  int g1 = static_cast<int>((behind - 1) * p.groups / p.units);
+  while (run_start(p.units, p.groups, g1 + 1) < behind) ++g1;
+  // (the first of them may have begun in the tile before: its part of this one is its second)
+  auto slot_of = [&](int g) { return static_cast<int64_t>(2 * g + (g > g0 || run_start(p.units, p.groups, g0) == first ? 0 : 1)); };
   const int tile_n = tile / p.tiles_k, tile_k = tile - tile_n * p.tiles_k;
-  const int n0 = tile_n * SIDE + band * 32, k0 = tile_k * SIDE;
-  // all quads of a thread at once: a band is a few KB, what counts is how many of its parts' loads are on their way
-  constexpr int QUADS = 32 * SIDE / 4 / 256;
+  const int n0 = tile_n * SIDE + band * kBand, k0 = tile_k * SIDE;
+  constexpr int QUADS = kBand * SIDE / 4 / 256;
   float4 sum[QUADS];
 #pragma unroll
   for (int i = 0; i < QUADS; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int g = g0; g <= g1; ++g) {
-    const float* from = p.slots + slot_of(g) * (SIDE * SIDE) + band * 32 * SIDE;
-    float4 v[QUADS];
+  for (int g = g0; g <= g1; g += kPartsAtOnce) {
+    float4 v[kPartsAtOnce][QUADS];
 #pragma unroll
-    for (int i = 0; i < QUADS; ++i) v[i] = load_streaming_f4(from + (i * 256 + threadIdx.x) * 4);
+    for (int b = 0; b < kPartsAtOnce; ++b) {
+      if (g + b > g1) continue;
+      const float* from = p.slots + slot_of(g + b) * (SIDE * SIDE) + band * kBand * SIDE;
 #pragma unroll
-    for (int i = 0; i < QUADS; ++i) sum[i] = make_float4(sum[i].x + v[i].x, sum[i].y + v[i].y, sum[i].z + v[i].z, sum[i].w + v[i].w);
+      for (int i = 0; i < QUADS; ++i) v[b][i] = load_streaming_f4(from + (i * 256 + threadIdx.x) * 4);
+    }
+#pragma unroll
+    for (int b = 0; b < kPartsAtOnce; ++b) {
+      if (g + b > g1) continue;
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i)
+        sum[i] = make_float4(sum[i].x + v[b][i].x, sum[i].y + v[b][i].y, sum[i].z + v[b][i].z, sum[i].w + v[b][i].w);
+    }
   }
 #pragma unroll
   for (int i = 0; i < QUADS; ++i) {
@@ -305,9 +316,10 @@ __global__ __launch_bounds__(256) void linear_wgrad_sum_kernel(LinearWgradArgs p
     }
     store_streaming_f4(to, s);
   }
-  if (p.bias && tile_k == 0 && threadIdx.x < 32 && n0 + static_cast<int>(threadIdx.x) < p.N) {
+  if (p.bias && tile_k == 0 && threadIdx.x < kBand && n0 + static_cast<int>(threadIdx.x) < p.N) {
     float s = 0.f;
-    for (int g = g0; g <= g1; ++g) s += p.bias_slots[slot_of(g) * SIDE + band * 32 + threadIdx.x];
+#pragma unroll 4
+    for (int g = g0; g <= g1; ++g) s += p.bias_slots[slot_of(g) * SIDE + band * kBand + threadIdx.x];
     float* to = p.bias + n0 + threadIdx.x;
     *to = p.accumulate ? *to + s : s;
   }
@@ -337,7 +349,7 @@ Choice choose(int64_t M, int N, int K, bool low, bool may_cut) {
     float us = static_cast<float>(rounds) * (run * step_us + (big ? 8.f : 5.f) * ((run + steps - 1) / steps));
     if (cut) {
       const float parts = static_cast<float>(groups < tiles ? 2 * groups : groups + tiles);
-      us += 5.f + (parts * side * side * 8.f + static_cast<float>(N) * K * 4.f) / 5e6f;
+      us += 5.f + 0.1f * parts / tiles + (parts * side * side * 8.f + static_cast<float>(N) * K * 4.f) / 5e6f;
     }
     if (us < best_us) {
       best_us = us;
@@ -433,7 +445,7 @@ int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy,
            : x_low ? launch_wgrad_pair<kLowB>(ctx, a, c.big, grid, flops, bytes)
                    : launch_wgrad_pair<kNoLow>(ctx, a, c.big, grid, flops, bytes);
   if (rc || !c.cut) return rc;
-  const dim3 blocks(static_cast<unsigned>(a.tiles * (side / 32)));
+  const dim3 blocks(static_cast<unsigned>(a.tiles * (side / kBand)));
   const double sum_bytes = 4.0 * (static_cast<double>(c.groups) + a.tiles) * side * side + 4.0 * N * K;
   return c.big ? launch(ctx, linear_wgrad_sum_kernel<256>, blocks, dim3(256), a, "linear_wgrad_sum_kernel<256>", sum_bytes, 1)
                : launch(ctx, linear_wgrad_sum_kernel<128>, blocks, dim3(256), a, "linear_wgrad_sum_kernel<128>", sum_bytes, 1);

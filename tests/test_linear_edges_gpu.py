@@ -9,8 +9,8 @@ from test_linear_gpu import ACTS, BF16, F32, half_step, near, product, rnd, slop
 
 pytestmark = pytest.mark.gpu
 
-# one per kernel: 16 x 16, dealt-out reductions of 32 and 64 rows, 128 x 128 (fp32: 64 x 128 too), 256 x 128, 256 x 256 tiles
-SHAPES = [(5, 72, 40), (70, 264, 136), (520, 72, 520), (1000, 136, 1032), (2040, 264, 1544), (4090, 520, 2056)]
+# among them every kernel's: 16 x 16, dealt-out reductions of 32 and 64 rows, 128 x 64, 128 x 128, 256 x 128, 256 x 256 tiles
+SHAPES = [(3, 4104, 4096), (5, 72, 40), (70, 264, 136), (520, 72, 520), (1000, 136, 1032), (2040, 264, 1544), (4090, 520, 2056)]
 
 
 def poisoned(rows, cols, dtype, seed):

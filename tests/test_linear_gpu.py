@@ -88,12 +88,12 @@ class Framed:
         assert bool((rest == SENTINEL).all()), f"{what}: wrote outside its output"
 
 
-# rows of every kernel: up to 16 tokens; reductions dealt to wavefronts; 128 x 128 and 128 x 256 tiles.  Sizes that end inside
+# rows of every kernel: up to 16 tokens; reductions dealt to wavefronts; tiles of 128 x 64 to 256 x 256.  Sizes that end inside
 # tiles, reductions shorter than a step, one step long, a chunk longer
-SHAPES = [(1, 8, 8), (1, 64, 24), (1, 4096, 104), (2, 72, 2056), (7, 1000, 64), (15, 520, 136), (16, 136, 1032),
+SHAPES = [(1, 8, 8), (1, 64, 24), (1, 4096, 104), (6, 4096, 4096), (2, 72, 2056), (7, 1000, 64), (15, 520, 136), (16, 136, 1032),
           (17, 8, 16), (31, 64, 64), (33, 72, 40), (65, 1000, 200), (128, 256, 512), (130, 2056, 96), (333, 200, 1032),
           (700, 40, 2056), (2050, 24, 1544), (1800, 200, 1928), (2049, 328, 1664), (1536, 1024, 2048),
-          (4100, 8, 2056), (4097, 72, 2104), (4096, 256, 2048), (130, 96, 66000)]
+          (100, 776, 4104), (4100, 8, 2056), (4097, 72, 2104), (4096, 256, 2048), (130, 96, 66000)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
