@@ -14,6 +14,7 @@
 #include "linear_epilogue.h"
 
 #include <algorithm>
+#include <numeric>
 
 #include "context.h"
 #include "ops.h"
@@ -21,10 +22,15 @@
 namespace tch {
 namespace {
 
-// All reduction steps of all output tiles are one sequence, tile by tile, and every workgroup takes an equal run of it: as many
-// workgroups as the chip holds finish together however many tiles there are.  A tile that lies within one run is stored; of a
-// tile that is cut, every workgroup leaves its part in the workspace (the first run of a workgroup in slot 2 g, the last in
-// 2 g + 1), and a second launch adds them up in the order of the workgroups.
+// As many workgroups as the chip holds, and all of them busy to the end however many tiles there are: each takes `rounds` whole
+// tiles, and an equal run of the steps of the tiles that are left, tile by tile.  A tile that lies within one run is stored; of a
+// tile that is cut, every workgroup leaves its part in the workspace (the first of its run in slot 2 g, the second in 2 g + 1), and a
+// second launch adds them up in the order of the runs.
+//
+// The operands come through L2 32 rows at a time, and what no neighbour on the XCD wants at about the same time is read again from
+// further away.  So whole tiles lie in blocks (locate_tile) that the workgroups of an XCD walk down together, and the runs are dealt
+// to the workgroups in the order of the row that they begin with: run r begins (left r mod runs) / runs of the way down a tile, so that
+// with g = gcd(left, runs) and q = runs / g the runs r = v inverse(left / g) mod q + c q, c < g, are those that begin v / q down.
 struct LinearWgradArgs {
   const void* a;        // dy [M][N]
   const void* a_low;
@@ -32,14 +38,22 @@ struct LinearWgradArgs {
   const void* b_low;
   float* out;           // dw [N][K]
   float* bias;          // dbias [N]; may be null
-  float* slots;         // partial tiles [2 groups][tile]
-  float* bias_slots;    // and their column sums [2 groups][rows of a tile]
-  int64_t M, units;     // units: tiles * steps
+  float* slots;         // partial tiles [2 runs][tile]
+  float* bias_slots;    // and their column sums [2 runs][rows of a tile]
+  int64_t M, units;     // units: steps of the tiles that are left
   int N, K;
-  int tiles_k, tiles, steps, groups;
+  int tiles_n, tiles_k, steps;
+  int groups, rounds, runs;   // tiles behind groups * rounds are left, for the first `runs` workgroups
   int accumulate;       // out and bias are added to
+  int same_start, period, inverse;   // g, q, inverse(left / g) mod q
 };
-__host__ __device__ inline int64_t run_start(int64_t units, int groups, int group) { return units * group / groups; }
+__host__ __device__ inline int64_t run_start(int64_t units, int runs, int run) { return units * run / runs; }
+// four tiles down, then one to the right
+__device__ inline void locate_tile(const LinearWgradArgs& p, int tile, int& tile_n, int& tile_k) {
+  const int band = tile / (4 * p.tiles_k), rest = tile - band * (4 * p.tiles_k), rows = min(4, p.tiles_n - 4 * band);
+  tile_k = rest / rows;
+  tile_n = 4 * band + rest - tile_k * rows;
+}
 
 enum Pair : int { kNoLow = 0, kLowA = 1, kLowB = 2 };
 constexpr int kRows = 32;   // of a reduction step
@@ -63,7 +77,9 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int group = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x));
-  const int64_t run_end = run_start(p.units, p.groups, group + 1);
+  const int run = __builtin_amdgcn_readfirstlane(group < p.runs ? group / p.same_start * p.inverse % p.period + group % p.same_start * p.period : 0);
+  int64_t unit = group < p.runs ? run_start(p.units, p.runs, run) : 0;
+  const int64_t run_end = group < p.runs ? run_start(p.units, p.runs, run + 1) : 0;
 
   // ---- the walk of the loads: the resources move down the rows, the lanes' offsets stay; rows behind the last one are outside ----
   auto lane_offset = [&](int load, int row_bytes, int ld, int col0) {   // of 1 KB number `load` of a plane
@@ -179,16 +195,23 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
   std::integral_constant<int, 1> one;
   // behind the last barrier of a part nobody reads what counts, and every wavefront waits for its own loads: the next part's may
   // go to the same buffers
-  int64_t unit = run_start(p.units, p.groups, group);
-  for (int part = 0; unit < run_end; ++part) {
-    // (quotients and 64-bit minima come out of the vector unit: back in scalar registers, or every load of the loop becomes a loop over its resources)
-    const int tile = __builtin_amdgcn_readfirstlane(static_cast<int>(unit / p.steps));
-    const int from = __builtin_amdgcn_readfirstlane(static_cast<int>(unit - static_cast<int64_t>(tile) * p.steps));
-    const int to = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<int64_t>(p.steps), from + (run_end - unit))));
-    const int tile_n = __builtin_amdgcn_readfirstlane(tile / p.tiles_k), tile_k = tile - tile_n * p.tiles_k;
+  int slot = 2 * run;
+  for (int round = 0; round < p.rounds || unit < run_end; ++round) {
+    int tile = round * p.groups + group, from = 0, to = p.steps;
+    if (round >= p.rounds) {
+      // (quotients and 64-bit minima come out of the vector unit: back in scalar registers, or every load of the loop becomes a
+      // loop over its resources)
+      const int left_tile = __builtin_amdgcn_readfirstlane(static_cast<int>(unit / p.steps));
+      tile = p.rounds * p.groups + left_tile;
+      from = __builtin_amdgcn_readfirstlane(static_cast<int>(unit - static_cast<int64_t>(left_tile) * p.steps));
+      to = __builtin_amdgcn_readfirstlane(static_cast<int>(min(static_cast<int64_t>(p.steps), from + (run_end - unit))));
+      unit += to - from;
+    }
+    int tile_n, tile_k;
+    locate_tile(p, tile, tile_n, tile_k);
+    tile_n = __builtin_amdgcn_readfirstlane(tile_n), tile_k = __builtin_amdgcn_readfirstlane(tile_k);
     const int n0 = tile_n * BM, k0 = tile_k * BN;
     const int64_t row0 = static_cast<int64_t>(from) * kRows;
-    unit += to - from;
 #pragma unroll
     for (int j = 0; j < A_LD; ++j) a_off[j] = lane_offset(wave * A_LD + j, RA, p.N, n0);
 #pragma unroll
@@ -227,7 +250,6 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
 
     // ---- a lane's accumulators are one column of dw (x) and rows 8 (e / 4) + 4 half + e % 4: whole lines of 128 bytes a store ----
     const bool whole = to - from == p.steps;
-    const int slot = 2 * group + (part == 0 ? 0 : 1);
     const int ld = whole ? p.K : BN;
     const bool add = whole && p.accumulate;
     float* out = whole ? p.out + static_cast<int64_t>(n0) * p.K + k0 : p.slots + static_cast<int64_t>(slot) * (BM * BN);
@@ -261,6 +283,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_
         }
       }
     }
+    if (round >= p.rounds) ++slot;
   }
 }
 
@@ -271,17 +294,18 @@ constexpr int kBand = 8, kPartsAtOnce = 8;
 template <int SIDE>
 __global__ __launch_bounds__(256) void linear_wgrad_sum_kernel(LinearWgradArgs p) {
   constexpr int BANDS = SIDE / kBand;
-  const int tile = blockIdx.x / BANDS, band = blockIdx.x % BANDS;
-  const int64_t first = static_cast<int64_t>(tile) * p.steps, behind = first + p.steps;
-  // the group that has the tile's first unit, and the slot of a group's part
-  int g0 = static_cast<int>(first * p.groups / p.units);
-  while (run_start(p.units, p.groups, g0 + 1) <= first) ++g0;
-  if (run_start(p.units, p.groups, g0 + 1) >= behind) return;   // one workgroup had all of it
-  int g1 = static_cast<int>((behind - 1) * p.groups / p.units);
-  while (run_start(p.units, p.groups, g1 + 1) < behind) ++g1;
+  const int left_tile = blockIdx.x / BANDS, band = blockIdx.x % BANDS;
+  const int64_t first = static_cast<int64_t>(left_tile) * p.steps, behind = first + p.steps;
+  // the runs that have the tile's first and its last step, and the slot of a run's part
+  int g0 = static_cast<int>(first * p.runs / p.units);
+  while (run_start(p.units, p.runs, g0 + 1) <= first) ++g0;
+  if (run_start(p.units, p.runs, g0 + 1) >= behind) return;   // one workgroup had all of it
+  int g1 = static_cast<int>((behind - 1) * p.runs / p.units);
+  while (run_start(p.units, p.runs, g1 + 1) < behind) ++g1;
   // (the first of them may have begun in the tile before: its part of this one is its second)
-  auto slot_of = [&](int g) { return static_cast<int64_t>(2 * g + (g > g0 || run_start(p.units, p.groups, g0) == first ? 0 : 1)); };
-  const int tile_n = tile / p.tiles_k, tile_k = tile - tile_n * p.tiles_k;
+  auto slot_of = [&](int g) { return static_cast<int64_t>(2 * g + (g > g0 || run_start(p.units, p.runs, g0) == first ? 0 : 1)); };
+  int tile_n, tile_k;
+  locate_tile(p, p.rounds * p.groups + left_tile, tile_n, tile_k);
   const int n0 = tile_n * SIDE + band * kBand, k0 = tile_k * SIDE;
   constexpr int QUADS = kBand * SIDE / 4 / 256;
   float4 sum[QUADS];
@@ -342,14 +366,14 @@ Choice choose(int64_t M, int N, int K, bool low, bool may_cut) {
     const int side = big ? 256 : 128;
     const int64_t tiles = static_cast<int64_t>(tiles_over(N, side)) * tiles_over(K, side), units = tiles * steps;
     if (groups < 1 || groups > units || groups > 0x3fffffff) return;
-    const bool cut = groups % tiles != 0 && tiles % groups != 0 ? true : groups > tiles;
+    const bool cut = tiles % groups != 0;
     if (cut && (!may_cut || groups > (big ? 256 : 512))) return;
     const int64_t slots = big ? 256 : 512, rounds = (groups + slots - 1) / slots, run = (units + groups - 1) / groups;
     const float step_us = (big ? 1.43f : groups > 256 ? 0.97f : 0.95f) * (low ? 1.f : 0.6f);
     float us = static_cast<float>(rounds) * (run * step_us + (big ? 8.f : 5.f) * ((run + steps - 1) / steps));
     if (cut) {
-      const float parts = static_cast<float>(groups < tiles ? 2 * groups : groups + tiles);
-      us += 5.f + 0.1f * parts / tiles + (parts * side * side * 8.f + static_cast<float>(N) * K * 4.f) / 5e6f;
+      const float parts = static_cast<float>(groups + tiles % groups);
+      us += 5.f + 0.1f * parts / (tiles % groups) + (parts * side * side * 8.f + static_cast<float>(N) * K * 4.f) / 5e6f;
     }
     if (us < best_us) {
       best_us = us;
@@ -430,14 +454,20 @@ int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy,
   a.slots = static_cast<float*>(workspace);
   a.bias_slots = a.slots + 2 * static_cast<int64_t>(c.groups) * side * side;
   a.M = M, a.N = n, a.K = k;
+  a.tiles_n = tiles_over(n, side);
   a.tiles_k = tiles_over(k, side);
-  TCH_CHECK_ARG(static_cast<int64_t>(tiles_over(n, side)) * a.tiles_k <= 0x3fffffff, "linear_wgrad: grid out of range");
-  a.tiles = tiles_over(n, side) * a.tiles_k;
+  const int64_t tiles = static_cast<int64_t>(a.tiles_n) * a.tiles_k;
+  TCH_CHECK_ARG(tiles <= 0x3fffffff, "linear_wgrad: grid out of range");
   a.steps = static_cast<int>((M + kRows - 1) / kRows);
-  a.units = static_cast<int64_t>(a.tiles) * a.steps;
   a.groups = c.groups;
+  a.rounds = static_cast<int>(tiles / c.groups);
+  const int left = static_cast<int>(tiles % c.groups);
+  a.units = static_cast<int64_t>(left) * a.steps;
+  a.runs = static_cast<int>(std::min<int64_t>(a.units, c.groups));   // (a run has a step at least)
+  a.same_start = std::max(std::gcd(left, a.runs), 1);
+  a.period = std::max(a.runs / a.same_start, 1);
+  while (a.period > 1 && static_cast<int64_t>(left / a.same_start) * a.inverse % a.period != 1) ++a.inverse;
   a.accumulate = accumulate;
-  TCH_CHECK_ARG(a.units < (1ll << 62) / (c.groups + 1), "linear_wgrad: grid out of range");
   const unsigned grid = static_cast<unsigned>(c.groups);
   const double flops = 2.0 * M * N * K * (low ? 2.0 : 1.0);
   const double bytes = 2.0 * M * (N * (dy_low ? 2 : 1) + K * (x_low ? 2 : 1)) + 4.0 * N * K;
@@ -445,8 +475,8 @@ int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy,
            : x_low ? launch_wgrad_pair<kLowB>(ctx, a, c.big, grid, flops, bytes)
                    : launch_wgrad_pair<kNoLow>(ctx, a, c.big, grid, flops, bytes);
   if (rc || !c.cut) return rc;
-  const dim3 blocks(static_cast<unsigned>(a.tiles * (side / kBand)));
-  const double sum_bytes = 4.0 * (static_cast<double>(c.groups) + a.tiles) * side * side + 4.0 * N * K;
+  const dim3 blocks(static_cast<unsigned>(left * (side / kBand)));
+  const double sum_bytes = 4.0 * (a.runs + 2.0 * left) * side * side;
   return c.big ? launch(ctx, linear_wgrad_sum_kernel<256>, blocks, dim3(256), a, "linear_wgrad_sum_kernel<256>", sum_bytes, 1)
                : launch(ctx, linear_wgrad_sum_kernel<128>, blocks, dim3(256), a, "linear_wgrad_sum_kernel<128>", sum_bytes, 1);
 }
