@@ -889,35 +889,42 @@ struct KernelCost {
   float fixed_us, again_us; // start and end; what a further round costs beyond that
 };
 template <typename T, bool GATED_FWD>
-Kernel choose_kernel(const LinearArgs& a) {
+const KernelCost* kernel_costs() {
   static constexpr KernelCost kBf16[kKernels] = {{GATED_FWD ? 0 : 16, 16, 256, 8, 0.85f, 1.45f, 1.2f, 0.f},
                                                  {32, 32, 128, 4, 0.22f, 0.45f, 0.6f, 0.f},
                                                  {32, 64, 128, 4, 0.4f, 0.75f, 0.6f, 0.f},
                                                  {64, 64, 128, 3, 0.78f, 0.78f, 0.9f, 0.f},
-                                                 {128, 64, 128, 1, 0.43f, 0.43f, 2.5f, 0.f},
-                                                 {128, 128, 128, 1, 0.56f, 0.56f, 3.5f, 0.f},
-                                                 {256, 128, 128, 1, 0.92f, 0.92f, 3.2f, 0.f},
-                                                 {256, 256, 128, 1, 1.55f, 1.55f, 6.f, 0.f}};
+                                                 {128, 64, 128, 1, 0.39f, 0.44f, 2.5f, 0.f},
+                                                 {128, 128, 128, 1, 0.5f, 0.58f, 3.5f, 0.f},
+                                                 {256, 128, 128, 1, 0.84f, 1.f, 3.2f, 0.f},
+                                                 {256, 256, 128, 1, 1.45f, 1.62f, 6.f, 0.f}};
   // (128 x 64: two share a compute unit at half the rate each)
   static constexpr KernelCost kF32[kKernels] = {{GATED_FWD ? 0 : 16, 16, 256, 8, 1.45f, 1.45f, 1.2f, 0.f},
                                                 {32, 32, 128, 4, 0.65f, 0.65f, 0.8f, 2.f},
                                                 {32, 64, 128, 4, 1.2f, 1.2f, 0.8f, 3.5f},
                                                 {64, 64, 64, 4, 1.18f, 1.18f, 1.2f, 3.5f},
                                                 {128, 64, 128, 1, 1.f, 1.f, 2.8f, 0.f}};
-  const KernelCost* costs = sizeof(T) == 2 ? kBf16 : kF32;
+  return sizeof(T) == 2 ? kBf16 : kF32;
+}
+template <typename T, bool GATED_FWD>
+float kernel_us(int kernel, int M, const LinearArgs& a) {
+  const KernelCost& c = kernel_costs<T, GATED_FWD>()[kernel];
+  if (!c.bm || (kernel == kTile256 && a.K * static_cast<int>(sizeof(T)) <= c.step)) return INFINITY;   // (256 x 256 takes two steps at least)
+  const double tiles = static_cast<double>(tiles_over(M, c.bm)) * tiles_over(a.N, GATED_FWD ? c.bn / 2 : c.bn);
+  const int steps = tiles_over(tiles_over(a.K * static_cast<int>(sizeof(T)), c.step), c.ways);
+  const double rounds = kernel < kTile128x64 && tiles > 8 * 256 ? tiles / 256 : ceil(tiles / 256);
+  const float load = kernel == kRows16 ? static_cast<float>(min(M, 16)) / 16.f : tiles < 256 ? static_cast<float>(tiles) / 256.f : 1.f;
+  const float step_us = c.step_us + load * (c.full_us - c.step_us);
+  return static_cast<float>(rounds) * (steps * step_us + c.fixed_us) + static_cast<float>(rounds - 1.0) * c.again_us;
+}
+template <typename T, bool GATED_FWD>
+Kernel choose_kernel(int M, const LinearArgs& a, float* us) {
   Kernel best = kSplit32;
-  float best_us = INFINITY;
+  *us = INFINITY;
   for (int k = 0; k < kKernels; ++k) {
-    const KernelCost& c = costs[k];
-    if (!c.bm || (k == kTile256 && a.K * static_cast<int>(sizeof(T)) <= c.step)) continue;   // (256 x 256 takes two steps at least)
-    const double tiles = static_cast<double>(tiles_over(a.M, c.bm)) * tiles_over(a.N, GATED_FWD ? c.bn / 2 : c.bn);
-    const int steps = tiles_over(tiles_over(a.K * static_cast<int>(sizeof(T)), c.step), c.ways);
-    const double rounds = tiles > 8 * 256 ? tiles / 256 : ceil(tiles / 256);
-    const float load = k == kRows16 ? static_cast<float>(min(a.M, 16)) / 16.f : tiles < 256 ? static_cast<float>(tiles) / 256.f : 1.f;
-    const float step_us = c.step_us + load * (c.full_us - c.step_us);
-    const float us = static_cast<float>(rounds) * (steps * step_us + c.fixed_us) + static_cast<float>(rounds - 1.0) * c.again_us;
-    if (us < best_us) {
-      best_us = us;
+    const float t = kernel_us<T, GATED_FWD>(k, M, a);
+    if (t < *us) {
+      *us = t;
       best = static_cast<Kernel>(k);
     }
   }
@@ -925,9 +932,9 @@ Kernel choose_kernel(const LinearArgs& a) {
 }
 
 template <typename T, int MODE>
-int launch_linear_mode(Context* ctx, LinearArgs& a) {
+int launch_linear_kernel(Context* ctx, Kernel kernel, LinearArgs& a) {
   constexpr bool kWide = MODE == kGatedFwd, kBf = sizeof(T) == 2;
-  switch (choose_kernel<T, kWide>(a)) {
+  switch (kernel) {
     case kRows16:
       if constexpr (!kWide) return launch_linear_rows<T, MODE, 8>(ctx, a);
       break;
@@ -952,6 +959,49 @@ int launch_linear_mode(Context* ctx, LinearArgs& a) {
   }
   set_error("linear: no kernel");
   return -22;
+}
+
+// Large tiles rarely fill their last round.  Where it is estimated to be shorter by more than the estimate is good for, the rows that
+// fill whole rounds are one launch and the others a second one, with tiles as small as suit them: bf16 9729 x 3456 over 15184 1217 ->
+// 1042 us, fp32 1568 x 4096 over 1024 151 -> 134.
+constexpr float kSecondLaunchUs = 3.f, kWorthwhile = 0.93f;
+template <typename T, int MODE>
+int launch_linear_mode(Context* ctx, LinearArgs& a) {
+  constexpr bool kWide = MODE == kGatedFwd;
+  float us;
+  Kernel kernel = choose_kernel<T, kWide>(a.M, a, &us), rest_kernel = kernel;
+  us *= kWorthwhile;
+  int rows = a.M;
+  for (int k = kTile128x64; k < kKernels; ++k) {
+    const KernelCost& c = kernel_costs<T, kWide>()[k];
+    if (!c.bm) continue;
+    const int64_t tiles_n = tiles_over(a.N, kWide ? c.bn / 2 : c.bn), rounds = tiles_over(a.M, c.bm) * tiles_n / 256;
+    const int64_t main_rows = rounds * 256 / tiles_n * c.bm;
+    if (main_rows <= 0 || main_rows >= a.M) continue;
+    float rest_us;
+    const Kernel rest = choose_kernel<T, kWide>(a.M - static_cast<int>(main_rows), a, &rest_us);
+    const float both_us = kernel_us<T, kWide>(k, static_cast<int>(main_rows), a) + rest_us + kSecondLaunchUs;
+    if (both_us < us) {
+      us = both_us;
+      kernel = static_cast<Kernel>(k);
+      rest_kernel = rest;
+      rows = static_cast<int>(main_rows);
+    }
+  }
+  if (rows == a.M) return launch_linear_kernel<T, MODE>(ctx, kernel, a);
+  LinearArgs rest = a;
+  auto skip = [&](const void* t, int64_t ld) -> const void* { return t ? static_cast<const T*>(t) + rows * ld : nullptr; };
+  rest.M = a.M - rows;
+  rest.a = skip(a.a, a.lda);
+  rest.add = skip(a.add, a.ldadd);
+  rest.z = skip(a.z, a.ldz);
+  rest.out = const_cast<void*>(skip(a.out, a.ldo));
+  rest.out2 = const_cast<void*>(skip(a.out2, a.ldo2));
+  rest.low = const_cast<void*>(skip(a.low, a.ldo));
+  rest.low2 = const_cast<void*>(skip(a.low2, a.ldo2));
+  a.M = rows;
+  if (int rc = launch_linear_kernel<T, MODE>(ctx, kernel, a)) return rc;
+  return launch_linear_kernel<T, MODE>(ctx, rest_kernel, rest);
 }
 
 template <typename T>

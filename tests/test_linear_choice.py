@@ -26,10 +26,12 @@ def launch(rec, op, dtype, M, K, N):  # noqa: F811
         check(L.tch_gated_linear_fwd(h, dtype, X, K, W, Y, N, None, 4, None, 0, M, K, N))
     else:
         check(L.tch_linear_dgrad_gated(h, dtype, X, K, W, PRE, 2 * N, Y, None, 2 * N, None, None, 0, 4, M, K, N))
-    (name, groups, _), = rec.end()
-    kind, mode, tile = re.match(r"linear_(\w+)_kernel<\w+,(\w+),(\d+x\d+)", name).groups()
-    assert mode == op
-    return f"{kind} {tile}", groups
+    out = []
+    for name, groups, _ in rec.end():
+        kind, mode, tile = re.match(r"linear_(\w+)_kernel<\w+,(\w+),(\d+x\d+)", name).groups()
+        assert mode == op
+        out.append((f"{kind} {tile}", groups))
+    return out
 
 
 @dtypes
@@ -38,18 +40,19 @@ def test_every_kernel_is_reached_and_tested(rec, op, dtype):  # noqa: F811
     want = set(KERNELS[dtype])
     if op == "gated_fwd":
         want.discard("rows 16x16")
-    reached = {launch(rec, op, dtype, M, K, N)[0] for M, K, N in SHAPES + EDGES + [(m, n, k) for m, k, n in BWD_SHAPES]}
-    assert reached == want
+    all_launches = [launch(rec, op, dtype, M, K, N) for M, K, N in SHAPES + EDGES + [(m, n, k) for m, k, n in BWD_SHAPES]]
+    assert {kernel for launches in all_launches for kernel, _ in launches} == want
+    assert max(len(launches) for launches in all_launches) == 2     # rows behind the last whole round
 
 
 def test_choice(rec):  # noqa: F811
     """Both sides of the rule, at sizes that were measured."""
-    assert launch(rec, "fwd", BF16, 1, 4096, 4096) == ("rows 16x16", 256)
-    assert launch(rec, "fwd", BF16, 512, 8192, 1024)[0] == "split 32x64"
-    assert launch(rec, "fwd", BF16, 1024, 1024, 1024)[0] == "split 64x64"
-    assert launch(rec, "fwd", BF16, 512, 4096, 4096) == ("tile 128x64", 256)
-    assert launch(rec, "fwd", BF16, 512, 8192, 8192) == ("tile 128x128", 256)
-    assert launch(rec, "fwd", BF16, 4096, 1024, 4096) == ("tile 256x256", 256)
-    assert launch(rec, "fwd", F32, 2048, 1024, 2048) == ("tile 128x64", 512)
-    assert launch(rec, "fwd", F32, 1568, 1024, 4096) == ("tile 128x64", 832)
-    assert launch(rec, "fwd", F32, 512, 2048, 1024) == ("split 32x64", 256)
+    assert launch(rec, "fwd", BF16, 1, 4096, 4096) == [("rows 16x16", 256)]
+    assert launch(rec, "fwd", BF16, 512, 8192, 1024)[0][0] == "split 32x64"
+    assert launch(rec, "fwd", BF16, 1024, 1024, 1024)[0][0] == "split 64x64"
+    assert launch(rec, "fwd", BF16, 512, 4096, 4096) == [("tile 128x64", 256)]
+    assert launch(rec, "fwd", BF16, 512, 8192, 8192) == [("tile 128x128", 256)]
+    assert launch(rec, "fwd", BF16, 4096, 1024, 4096) == [("tile 256x256", 256)]
+    assert launch(rec, "fwd", F32, 2048, 1024, 2048) == [("tile 128x64", 512)]
+    assert launch(rec, "fwd", F32, 1568, 1024, 4096) == [("tile 128x64", 768), ("split 32x32", 128)]
+    assert launch(rec, "fwd", F32, 512, 2048, 1024) == [("split 32x64", 256)]
