@@ -457,7 +457,7 @@ int tch_gelu_bwd(tch_context* ctx, int dtype, const void* dy, const void* x, voi
  *   fwd:    y = act(x w^T + bias) + residual; pre (may be NULL) = x w^T + bias.  x [M][K], w [N][K], y [M][N].
  *   dgrad:  dx = (dy w) . act'(pre) + residual, pre and act being those of the layer in FRONT of this one; wt [N][K] is
  *           this layer's weight transposed (tch_filter_transpose_batched), dy [M][K], dx [M][N].
- * A residual may be the output itself (in place); nothing else may overlap an output. */
+ * A residual, and the pre-activations of a dgrad, may be the output itself (in place); nothing else may overlap one. */
 int tch_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* y, int64_t ldy,
                    const float* bias, int act, const void* residual, int64_t ldr, void* pre, int64_t ldp, int64_t M,
                    int64_t K, int64_t N);
@@ -469,7 +469,7 @@ int tch_linear_dgrad(tch_context* ctx, int dtype, const void* dy, int64_t lddy, 
  * dgrad_gated: dh = dy w (wt [F][K] the down projection's weight transposed, dy [M][K]) goes straight into
  * dpre [M][2F] = (dh . u . act'(g) | dh . act(g)); h (may be NULL) [M][F] = act(g) . u again.  dpre may be pre itself.
  * dpre_low, h_low (bf16, may be NULL; laid out like dpre and h): what rounding took off.  A weight gradient of a bf16
- * gradient and its low part is that of the unrounded gradient, as exact as its fp32 sums. */
+ * gradient and its low part is that of the unrounded gradient, each element to 2^-18 of its size. */
 int tch_gated_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* h, int64_t ldh,
                          const float* bias, int act, void* pre, int64_t ldp, int64_t M, int64_t K, int64_t F);
 int tch_linear_dgrad_gated(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, const void* pre,

@@ -17,7 +17,8 @@ namespace {
 // ---------------------------------------------------------------------------
 // dz = dy * act'(z), and the gated form (dg, du, and h again on request) from dh and (g | u)
 // ---------------------------------------------------------------------------
-// Bound by memory: 6 (gated 10, with h 12) bytes per element in bf16.  A thread has kAtOnce chunks on their way at a time.
+// Bound by memory: 6 (gated 10, with h 12; with low parts 8 and 14) bytes per element in bf16.  A thread has kAtOnce chunks on their
+// way at a time.  8192 x 4096 with the low part: 46-51 us, 5.3-5.8 TB/s.
 struct ActBwdArgs {
   const void* dy;
   const void* z;

@@ -153,6 +153,11 @@ __device__ inline void mma32(const uint4_t& first, const uint4_t& second, f32x16
 // steps ahead go out between the multiplies.  The tiles of a workgroup are one sequence: the next tile's first loads are on
 // their way during this tile's last steps and its epilogue.  A row of the operands that does not exist is outside its buffer
 // resource and lands as zeros; a chunk behind K is turned away by its lane's offset in the last step of a tile.
+// Measured: gated forward 16384 x 11008 over 4096 2.18-2.21 ms, 1.34-1.36 PFLOP/s, bound by power (matrix pipes 79 % busy; a large library
+// product 1.33-1.37); data gradient 8192 x 2048 over 11264 292 us, 1.29.  Where the reduction is short the epilogue counts, in which the
+// matrix pipes stand: forward 8192 x 4096 over 1024 with GELU and the kept pre-activation 77 us, about 20 of them epilogue (vector
+// instructions: an exponential and a reciprocal per element); the gated data gradient 8192 x 5632 over 2048, five outputs of which
+// two are low parts, 287 us, half of them.  fp32 4096 x 4096 over 1024: 264 us, 0.130 of 0.157 PFLOP/s.
 template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int RB, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T);
@@ -484,6 +489,8 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
 // Each wavefront has a ring of NBUF operand tiles (rows of RB bytes) of its own, filled with direct loads, and waits for its own loads
 // only: no barrier before the partial tiles meet in LDS, where they are added in the order of the wavefronts.  What that buys
 // where workgroups are few: KG * (NBUF - 1) operand tiles in flight per compute unit and a chain of nk / KG steps instead of nk.
+// Bound by the bytes of the weights where there are many (7 rows through 2048 -> 2 x 5632 gated: 9.3 us, 5.0 TB/s; 32 through 8192 -> 8192:
+// 23 us, 5.8 TB/s), by the latency of a chain of steps where there are few.
 template <typename T, int MODE, int TM, int TN, int KG, int NBUF, int RB>
 __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), KS = RB / EB, SL = RB / 32, SLOTS = RB / 16, LD_ROWS = 1024 / RB;
