@@ -69,11 +69,11 @@ __device__ inline Chunk read_chunk(__amdgpu_buffer_rsrc_t rsrc, int off) {
   c.w[3] = v[3];
   return c;
 }
-template <typename T>
+template <typename T, int AUX = 0>
 __device__ inline void write_chunk(__amdgpu_buffer_rsrc_t rsrc, int off, const float* v) {
   const Chunk c = float_to_chunk<T>(v);
   const uint4_t w = {c.w[0], c.w[1], c.w[2], c.w[3]};
-  __builtin_amdgcn_raw_buffer_store_b128(w, rsrc, off, 0, 0);
+  __builtin_amdgcn_raw_buffer_store_b128(w, rsrc, off, 0, AUX);
 }
 
 // One 16-byte chunk of the output (E columns of a row) in two steps: what it reads, and the rest.
@@ -89,17 +89,19 @@ struct ChunkOperands {
     if constexpr (!is_gated(MODE))
       if (p.add) add = read_chunk(t.add, at<T>(row, p.ldadd, col, ok));
   }
-  template <int ACT>
+  // STREAM: forward outputs go past L2 (non-temporal) and leave it to the operands: the tile kernel, 8192 x 4096 over 1024 with the kept
+  // pre-activation 80 -> 76 us (the outputs of a gated data gradient that way 292 -> 310)
+  template <int ACT, bool STREAM>
   __device__ __forceinline__ void finish(const LinearArgs& p, const TileTensors& t, int row, int col, const float* v, float* u) {
-    constexpr int E = Elem<T>::kPerChunk;
+    constexpr int E = Elem<T>::kPerChunk, AUX = STREAM && (MODE == kLinFwd || MODE == kGatedFwd) ? 2 : 0;
     const bool ok = col < p.N;
     float fg[E], fu[E], o[E], h[E];
     if constexpr (MODE == kLinBwd || MODE == kGatedBwd) chunk_to_float<T>(zg, fg);
     if constexpr (MODE == kGatedBwd) chunk_to_float<T>(zu, fu);
     if constexpr (MODE == kLinFwd || MODE == kGatedFwd) {
       if (p.out2) {
-        write_chunk<T>(t.out2, at<T>(row, p.ldo2, col, ok), v);
-        if constexpr (MODE == kGatedFwd) write_chunk<T>(t.out2, at<T>(row, p.ldo2, p.N + col, ok), u);
+        write_chunk<T, AUX>(t.out2, at<T>(row, p.ldo2, col, ok), v);
+        if constexpr (MODE == kGatedFwd) write_chunk<T, AUX>(t.out2, at<T>(row, p.ldo2, p.N + col, ok), u);
       }
     }
     combine<T, MODE, ACT, E>(v, u, fg, fu, o, h);
@@ -111,7 +113,7 @@ struct ChunkOperands {
         for (int e = 0; e < E; ++e) o[e] += r[e];
       }
     }
-    write_chunk<T>(t.out, at<T>(row, p.ldo, col, ok), o);
+    write_chunk<T, AUX>(t.out, at<T>(row, p.ldo, col, ok), o);
     if constexpr (MODE == kGatedBwd) {
       write_chunk<T>(t.out, at<T>(row, p.ldo, p.N + col, ok), u);
       if (p.out2) write_chunk<T>(t.out2, at<T>(row, p.ldo2, col, ok), h);
@@ -155,9 +157,8 @@ __device__ inline void mma32(const uint4_t& first, const uint4_t& second, f32x16
 // resource and lands as zeros; a chunk behind K is turned away by its lane's offset in the last step of a tile.
 // Measured: gated forward 16384 x 11008 over 4096 2.18-2.21 ms, 1.34-1.36 PFLOP/s, bound by power (matrix pipes 79 % busy; a large library
 // product 1.33-1.37); data gradient 8192 x 2048 over 11264 292 us, 1.29.  Where the reduction is short the epilogue counts, in which the
-// matrix pipes stand: forward 8192 x 4096 over 1024 with GELU and the kept pre-activation 77 us, about 20 of them epilogue (vector
-// instructions: an exponential and a reciprocal per element); the gated data gradient 8192 x 5632 over 2048, five outputs of which
-// two are low parts, 287 us, half of them.  fp32 4096 x 4096 over 1024: 264 us, 0.130 of 0.157 PFLOP/s.
+// matrix pipes stand: forward 8192 x 4096 over 1024 with GELU and the kept pre-activation 75 us, about 25 of them epilogue (134 MB written);
+// the gated data gradient 8192 x 5632 over 2048 with its low parts 287 us, half of them (740 MB at 5.5 TB/s).  fp32 4096 x 4096 over 1024: 264 us, 0.130 of 0.157 PFLOP/s.
 template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int RB, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T);
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
               if constexpr (GATED_FWD) u[e] += bu[e];
             }
           }
-          operands[pass % DEPTH].template finish<ACT>(p, t, row_of(pass), col, v, u);
+          operands[pass % DEPTH].template finish<ACT, true>(p, t, row_of(pass), col, v, u);
           if (pass + DEPTH < TOTAL) request(pass + DEPTH);
           __builtin_amdgcn_sched_barrier(0);   // one pass at a time: the registers are the accumulators'
         }
@@ -666,7 +667,7 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
           if constexpr (GATED_FWD) add_bias(p.N + n0 + c, u);
         }
       }
-      operands[visit].template finish<ACT>(p, t, row, n0 + c, v, u);
+      operands[visit].template finish<ACT, false>(p, t, row, n0 + c, v, u);
     }
   });
 }
