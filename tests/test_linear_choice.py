@@ -56,3 +56,15 @@ def test_choice(rec):  # noqa: F811
     assert launch(rec, "fwd", F32, 2048, 1024, 2048) == [("tile 128x64", 512)]
     assert launch(rec, "fwd", F32, 1568, 1024, 4096) == [("tile 128x64", 768), ("split 32x32", 128)]
     assert launch(rec, "fwd", F32, 512, 2048, 1024) == [("split 32x64", 256)]
+
+
+def test_weight_gradients_are_cut_to_whole_rounds(rec):  # noqa: F811
+    def wgrad(M, K, N, low):
+        rec.begin()
+        need = lib().tch_linear_wgrad_workspace_bytes(M, K, N)
+        check(lib().tch_linear_wgrad(rec.ctx, X, None, Y, LOW if low else None, W, None, 0, M, K, N, WS, need))
+        return rec.end()
+    for M, K, N, tiles in ((1803, 5120, 3312, 260), (2319, 3976, 8736, 560)):
+        (name, groups, _), (add, parts, _) = wgrad(M, K, N, True)
+        assert "256x256" in name and "sum" in add and groups == 256 and parts == tiles % 256 * 32
+    assert len(wgrad(2048, 2048, 8192, True)) == len(wgrad(2048, 2048, 8192, False)) == 1          # 256 whole tiles

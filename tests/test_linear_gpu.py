@@ -311,7 +311,9 @@ def test_feed_forward_block(ctx, M, C, F):
 
 @pytest.mark.parametrize("low", ["none", "dy", "x"])
 @pytest.mark.parametrize("M,K,N", [(1, 8, 8), (31, 264, 72), (33, 8, 520), (64, 136, 136), (1000, 256, 256), (3001, 776, 1288), (4100, 1032, 2056),
-                                   (9000, 264, 264), (70, 2056, 2312)])
+                                   (9000, 264, 264), (70, 2056, 2312),
+                                   # whole rounds of tiles and a rest that fewer workgroups share; two rounds and a rest
+                                   (1803, 5120, 3312), (2319, 3976, 8736)])
 def test_linear_wgrad(ctx, M, K, N, low):
     """bf16 weight gradients with and without a low part, rows split and not, added to what is there and not."""
     from sirius_amd import ops
