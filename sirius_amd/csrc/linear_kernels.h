@@ -150,7 +150,7 @@ __device__ inline void mma32(const uint4_t& first, const uint4_t& second, f32x16
 // large products: a persistent grid whose workgroups walk output tiles as one sequence of reduction steps
 // ---------------------------------------------------------------------------
 // WM x WN wavefronts of TM x TN MFMA tiles (32 x 32).  Operand tiles go from global memory straight into LDS (16 bytes a lane,
-// rows of RB bytes, the 16-byte slot XOR-ed by the row so that an operand read touches every bank once), NBUF of them; the
+// rows of 128 bytes, the 16-byte slot XOR-ed by the row so that an operand read touches every bank once), NBUF of them; the
 // slice of 32 bytes that is multiplied next is read while this one is multiplied, and the direct loads of the tile NBUF - 1
 // steps ahead go out between the multiplies.  The tiles of a workgroup are one sequence: the next tile's first loads are on
 // their way during this tile's last steps and its epilogue.  A row of the operands that does not exist is outside its buffer
@@ -159,15 +159,15 @@ __device__ inline void mma32(const uint4_t& first, const uint4_t& second, f32x16
 // product 1.33-1.37); data gradient 8192 x 2048 over 11264 292 us, 1.29.  Where the reduction is short the epilogue counts, in which the
 // matrix pipes stand: forward 8192 x 4096 over 1024 with GELU and the kept pre-activation 75 us, about 25 of them epilogue (134 MB written);
 // the gated data gradient 8192 x 5632 over 2048 with its low parts 287 us, half of them (740 MB at 5.5 TB/s).  fp32 4096 x 4096 over 1024: 264 us, 0.130 of 0.157 PFLOP/s.
-template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int RB, int PER_CU>
+template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_kernel(LinearArgs p) {
-  constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T);
+  constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), RB = 128;
   constexpr int KS = RB / EB, SL = RB / 32, SLOTS = RB / 16, LD_ROWS = 1024 / RB;
   constexpr int BM = WM * TM * 32, BN = WN * TN * 32, NW = WM * WN;
   constexpr bool GATED_FWD = MODE == kGatedFwd;
   constexpr int BN_OUT = GATED_FWD ? BN / 2 : BN;
   static_assert(TN == 2, "a wavefront has 64 columns: gate and up tiles, or the whole lines of the epilogue");
-  static_assert((RB == 128 || RB == 64) && BM % (LD_ROWS * NW) == 0 && BN % (LD_ROWS * NW) == 0, "tile/loader mismatch");
+  static_assert(BM % (LD_ROWS * NW) == 0 && BN % (LD_ROWS * NW) == 0, "tile/loader mismatch");
   constexpr int A_LD = BM / LD_ROWS / NW, B_LD = BN / LD_ROWS / NW, LOADS = A_LD + B_LD;
   constexpr bool OWN_STAGE = NBUF == 2;   // the epilogue's staging has a place of its own
   static_assert(OWN_STAGE || A_LD >= 4, "4 KB of a wavefront's own loads stage its epilogue");
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   const int nk = (p.K + KS - 1) / KS;
   const int tiles = p.tiles_m * p.tiles_n;
   const int first = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x));
-  auto swizzle = [](int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
+  auto swizzle = [](int row) { return (row >> 1) & 7; };
 
   // consecutive tiles walk down group_rows row tiles before they move one column tile on: the tiles an XCD works on at one time
   // form a block, with fewer distinct operand rows through its L2
@@ -831,7 +831,7 @@ inline double linear_bytes(const LinearArgs& a, int mode, int eb) {
 }
 inline int tiles_over(int n, int tile) { return (n + tile - 1) / tile; }
 
-template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int RB, int PER_CU>
+template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
 int launch_linear_tile(Context* ctx, LinearArgs& a) {
   constexpr int BM = WM * TM * 32, BN = WN * TN * 32, BN_OUT = MODE == kGatedFwd ? BN / 2 : BN;
   static const std::string name = std::string("linear_tile_kernel<") + type_name<T>() + mode_name(MODE) + std::to_string(BM) + "x" +
@@ -848,7 +848,7 @@ int launch_linear_tile(Context* ctx, LinearArgs& a) {
   // counts: a workgroup per tile, and who is done makes room (768 x 6216 over 3480: 319 us, walked 411)
   const int64_t most = sizeof(T) == 2 ? 256 * PER_CU : tiles;
   const unsigned grid = static_cast<unsigned>(tiles < most ? tiles : most);
-  return launch(ctx, linear_tile_kernel<T, MODE, WM, WN, TM, TN, NBUF, RB, PER_CU>, dim3(grid), dim3(WM * WN * 64), a, name.c_str(),
+  return launch(ctx, linear_tile_kernel<T, MODE, WM, WN, TM, TN, NBUF, PER_CU>, dim3(grid), dim3(WM * WN * 64), a, name.c_str(),
                 linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
 }
 
@@ -952,16 +952,16 @@ int launch_linear_kernel(Context* ctx, Kernel kernel, LinearArgs& a) {
       if constexpr (kBf) return launch_linear_split<T, MODE, 2, 2, 3, 3, 128>(ctx, a);
       else return launch_linear_split<T, MODE, 2, 2, 4, 4, 64>(ctx, a);
     case kTile128x64:
-      if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 1, 1, 2, 4, 128, 1>(ctx, a);
-      else return launch_linear_tile<T, MODE, 4, 1, 1, 2, 2, 128, 2>(ctx, a);
+      if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 1, 1, 2, 4, 1>(ctx, a);
+      else return launch_linear_tile<T, MODE, 4, 1, 1, 2, 2, 2>(ctx, a);
     case kTile128:
-      if constexpr (kBf) return launch_linear_tile<T, MODE, 2, 2, 2, 2, 3, 128, 1>(ctx, a);
+      if constexpr (kBf) return launch_linear_tile<T, MODE, 2, 2, 2, 2, 3, 1>(ctx, a);
       break;
     case kTile256x128:
-      if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 2, 2, 2, 3, 128, 1>(ctx, a);
+      if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 2, 2, 2, 3, 1>(ctx, a);
       break;
     case kTile256:
-      if constexpr (kBf) return launch_linear_tile<T, MODE, 2, 4, 4, 2, 2, 128, 1>(ctx, a);
+      if constexpr (kBf) return launch_linear_tile<T, MODE, 2, 4, 4, 2, 2, 1>(ctx, a);
       break;
     default: break;
   }
