@@ -2,6 +2,11 @@
 // feed-forward layer does to it in the epilogue (linear_epilogue.h).  A has its own row stride, B (the weights) is dense.
 // Compiled once per element type (linear_bf16.hip, linear_f32.hip).
 //
+// LOW: a data gradient of bf16 gradients that come with what rounding took off them.  The product of the rounded gradient alone has an error of its
+// own of about 2^-9.3 of dx, next to the 2^-9.3 of rounding dx.  The reduction is walked twice, over a and then over its low part, into the
+// same accumulators: a tile's steps are twice as many, and so is its time where the multiplies bound it (8192 x 2048 over 11264 293 us, with the
+// low part 563; 8192 x 1024 over 4096 59 and 118; 392 x 512 over 2048 5.4 and 8.5).
+//
 // Gated modes multiply both projections in one tile: 32 (in the narrowest tiles 16) rows of the gate's weights lie next to the same rows of the up
 // projection's, so that a lane ends up with both products of its columns and the epilogue needs nobody else's.
 #pragma once
@@ -14,6 +19,7 @@ namespace tch {
 
 struct LinearArgs {
   const void* a;      // [M][K], row stride lda (elements)
+  const void* a_low;  // data gradient, bf16: what rounding took off a, laid out like it (may be null); both are multiplied
   const void* b;      // [N][K] dense; gated forward: [2N][K], gate rows first
   const float* bias;  // forward: [N] or [2N], may be null
   const void* add;    // residual, laid out by ldadd; may be null
@@ -159,7 +165,7 @@ __device__ inline void mma32(const uint4_t& first, const uint4_t& second, f32x16
 // product 1.33-1.37); data gradient 8192 x 2048 over 11264 292 us, 1.29.  Where the reduction is short the epilogue counts, in which the
 // matrix pipes stand: forward 8192 x 4096 over 1024 with GELU and the kept pre-activation 75 us, about 25 of them epilogue (134 MB written);
 // the gated data gradient 8192 x 5632 over 2048 with its low parts 287 us, half of them (740 MB at 5.5 TB/s).  fp32 4096 x 4096 over 1024: 264 us, 0.130 of 0.157 PFLOP/s.
-template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
+template <typename T, int MODE, bool LOW, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), RB = 128;
   constexpr int KS = RB / EB, SL = RB / 32, SLOTS = RB / 16, LD_ROWS = 1024 / RB;
@@ -183,7 +189,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int frag_row = lane & 31, frag_half = lane >> 5;
-  const int nk = (p.K + KS - 1) / KS;
+  const int nk = (p.K + KS - 1) / KS, steps = LOW && p.a_low ? 2 * nk : nk;   // the steps of a, and then those of its low part
   const int tiles = p.tiles_m * p.tiles_n;
   const int first = static_cast<int>(xcd_remap(blockIdx.x, gridDim.x));
   auto swizzle = [](int row) { return (row >> 1) & 7; };
@@ -229,18 +235,19 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b;
   const __amdgpu_buffer_rsrc_t rsrc_bias = make_rsrc(p.bias, BIAS && p.bias ? static_cast<uint32_t>(p.N) * (GATED_FWD ? 8u : 4u) : 0u);
   int ld_id = first, ld_kt = 0;
+  bool ld_low = false;   // the walk is in the low part
   auto mark_tail = [&]() LINEAR_INLINE {
 #pragma unroll
     for (int j = 0; j < A_LD; ++j) a_off[j] |= behind_k[(wave * A_LD + j) & 1];
 #pragma unroll
     for (int j = 0; j < B_LD; ++j) b_off[j] |= behind_k[(wave * B_LD + j) & 1];
   };
-  auto enter_tile = [&]() LINEAR_INLINE {
+  auto enter_tile = [&]() LINEAR_INLINE {   // or its low part
     int m0 = 0, n0 = 0;
     const bool any = ld_id < tiles;
     if (any) locate(ld_id, m0, n0);
     const int rows = min(BM, p.M - m0);
-    rsrc_a = make_rsrc(static_cast<const T*>(p.a) + m0 * p.lda, static_cast<uint32_t>(((rows - 1) * p.lda + p.K) * EB));
+    rsrc_a = make_rsrc(static_cast<const T*>(LOW && ld_low ? p.a_low : p.a) + m0 * p.lda, static_cast<uint32_t>(((rows - 1) * p.lda + p.K) * EB));
     const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
     rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
     if (ragged_k || !any) {   // behind the last tile every offset is out of range: zeros land
@@ -261,7 +268,8 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   auto next_step = [&]() LINEAR_INLINE {
     if (++ld_kt == nk) {
       ld_kt = 0;
-      ld_id += gridDim.x;
+      ld_low = LOW && p.a_low && !ld_low;
+      if (!ld_low) ld_id += gridDim.x;
       enter_tile();
     } else if (ragged_k && ld_kt == nk - 1) {
       mark_tail();
@@ -466,11 +474,11 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   const int outputs = p.out2 ? 2 : 1;
   int stored = 0;
   for (int id = first; id < tiles; id += gridDim.x) {
-    if (ONE_STEP && nk == 1) {
+    if (ONE_STEP && steps == 1) {
       step(stored, start, finish);
     } else {
       step(stored, start, middle);
-      for (int kt = 1; kt < nk - 1; ++kt) step(0, middle, middle);
+      for (int kt = 1; kt < steps - 1; ++kt) step(0, middle, middle);
       step(0, middle, finish);
     }
     if (NBUF == 2) next_step();
@@ -492,7 +500,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
 // where workgroups are few: KG * (NBUF - 1) operand tiles in flight per compute unit and a chain of nk / KG steps instead of nk.
 // Bound by the bytes of the weights where there are many (7 rows through 2048 -> 2 x 5632 gated: 9.3 us, 5.0 TB/s; 32 through 8192 -> 8192:
 // 23 us, 5.8 TB/s), by the latency of a chain of steps where there are few.
-template <typename T, int MODE, int TM, int TN, int KG, int NBUF, int RB>
+template <typename T, int MODE, bool LOW, int TM, int TN, int KG, int NBUF, int RB>
 __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), KS = RB / EB, SL = RB / 32, SLOTS = RB / 16, LD_ROWS = 1024 / RB;
   constexpr bool GATED_FWD = MODE == kGatedFwd;
@@ -510,8 +518,8 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
   p.div_tiles_n.divmod(xcd_remap(blockIdx.x, gridDim.x), slow, fast);
   const int m0 = static_cast<int>(p.group_rows ? fast : slow) * BM, n0 = static_cast<int>(p.group_rows ? slow : fast) * BN_OUT;
   const int rows = min(BM, p.M - m0);
-  const int nk = (p.K + KS - 1) / KS;
-  const int my_steps = nk > wave ? (nk - wave + KG - 1) / KG : 0;
+  const int nk = (p.K + KS - 1) / KS, steps = LOW && p.a_low ? 2 * nk : nk;   // the steps of a, and then those of its low part
+  const int my_steps = steps > wave ? (steps - wave + KG - 1) / KG : 0;
 
   auto swizzle = [](int row) { return RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3; };
   const int sub_row = lane / SLOTS, slot = lane % SLOTS;
@@ -527,22 +535,24 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
     const uint32_t row = GATED_FWD ? static_cast<uint32_t>((block & 1) * p.N + (block >> 1) * HALF + trow % HALF) : static_cast<uint32_t>(trow);
     b_off[j] = (row * static_cast<uint32_t>(p.K) + chunk[j & 1] * E) * EB;
   }
-  const __amdgpu_buffer_rsrc_t rsrc_a =
-      make_rsrc(static_cast<const T*>(p.a) + m0 * p.lda, static_cast<uint32_t>(((rows - 1) * p.lda + p.K) * EB));
   const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
   const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
 
   unsigned char* ring = lds + wave * (NBUF * BUF_BYTES);
   int ld_kt = wave;
   auto issue_loads = [&](int buf) {
+    const bool low = LOW && ld_kt >= nk;
+    const int kt = low ? ld_kt - nk : ld_kt;
+    const __amdgpu_buffer_rsrc_t rsrc_a =
+        make_rsrc(static_cast<const T*>(low ? p.a_low : p.a) + m0 * p.lda, static_cast<uint32_t>(((rows - 1) * p.lda + p.K) * EB));
     uint32_t behind[2];   // the chunk lies behind K
 #pragma unroll
-    for (int odd = 0; odd < 2; ++odd) behind[odd] = ld_kt * KS + chunk[odd] * E >= p.K ? kOutOfRange : 0u;
+    for (int odd = 0; odd < 2; ++odd) behind[odd] = kt * KS + chunk[odd] * E >= p.K ? kOutOfRange : 0u;
     unsigned char* dst = ring + buf * BUF_BYTES;
 #pragma unroll
-    for (int j = 0; j < A_LD; ++j) load_to_lds(rsrc_a, dst + j * 1024, static_cast<int>(a_off[j] | behind[j & 1]), ld_kt * RB);
+    for (int j = 0; j < A_LD; ++j) load_to_lds(rsrc_a, dst + j * 1024, static_cast<int>(a_off[j] | behind[j & 1]), kt * RB);
 #pragma unroll
-    for (int j = 0; j < B_LD; ++j) load_to_lds(rsrc_b, dst + A_BYTES + j * 1024, static_cast<int>(b_off[j] | behind[j & 1]), ld_kt * RB);
+    for (int j = 0; j < B_LD; ++j) load_to_lds(rsrc_b, dst + A_BYTES + j * 1024, static_cast<int>(b_off[j] | behind[j & 1]), kt * RB);
     ld_kt += KG;
   };
 
@@ -702,7 +712,7 @@ __device__ inline void store_four(T* p, const float* v) {
   for (int e = 0; e < 4; ++e) Elem<T>::store(p + e, v[e]);
 }
 
-template <typename T, int MODE, int KG>
+template <typename T, int MODE, bool LOW, int KG>
 __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T);
   static_assert(MODE != kGatedFwd, "gate and up projections need another layout");
@@ -715,10 +725,10 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
   uint32_t tile_n, tile_m;
   p.div_tiles_n.divmod(xcd_remap(blockIdx.x, gridDim.x), tile_n, tile_m);   // divided by the row tiles
   const int n0 = static_cast<int>(tile_n) * 16, m0 = static_cast<int>(tile_m) * 16;
-  const int pieces = (p.K + PIECE - 1) / PIECE;
+  const bool with_low = LOW && p.a_low;
+  const int nk = (p.K + PIECE - 1) / PIECE, pieces = with_low ? 2 * nk : nk;   // those of a, and then those of its low part
   const int row16 = lane & 15, quarter = lane >> 4;
 
-  const __amdgpu_buffer_rsrc_t rsrc_a = rows_from<T>(p.a, p.lda, m0, min(16, p.M - m0), p.K);
   const uint32_t skip = static_cast<uint32_t>(n0) * static_cast<uint32_t>(p.K) * EB;
   const __amdgpu_buffer_rsrc_t rsrc_b = make_rsrc(static_cast<const unsigned char*>(p.b) + skip, p.b_bytes - skip);
   const uint32_t a_off = (static_cast<uint32_t>(row16) * static_cast<uint32_t>(p.lda) + quarter * E) * EB;
@@ -727,9 +737,11 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
 
   uint4_t fa[2][U], fb[2][U];
   auto request = [&](int piece, int set) LINEAR_INLINE {
+    const bool low = with_low && piece >= nk;
+    const __amdgpu_buffer_rsrc_t rsrc_a = rows_from<T>(low ? p.a_low : p.a, p.lda, m0, min(16, p.M - m0), p.K);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = piece * PIECE + u * (4 * E);
+      const int k = (low ? piece - nk : piece) * PIECE + u * (4 * E);
       const uint32_t behind = k + quarter * E >= p.K ? kOutOfRange : 0u, from = static_cast<uint32_t>(k) * EB;
       fb[set][u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_b, static_cast<int>((b_off + from) | behind), 0, 0);
       fa[set][u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc_a, static_cast<int>((a_off + from) | behind), 0, 0);
@@ -814,14 +826,14 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
 // ---------------------------------------------------------------------------
 template <typename T>
 constexpr const char* type_name() { return sizeof(T) == 2 ? "bf16," : "f32,"; }
-inline std::string mode_name(int mode) {
+inline std::string mode_name(int mode, bool low) {
   static const char* const names[] = {"fwd,", "dgrad,", "gated_fwd,", "gated_dgrad,"};
-  return names[mode];
+  return low ? "dgrad_low," : names[mode];
 }
-inline double linear_flops(const LinearArgs& a, int mode) { return (mode == kGatedFwd ? 4.0 : 2.0) * a.M * a.N * a.K; }
+inline double linear_flops(const LinearArgs& a, int mode) { return (mode == kGatedFwd || a.a_low ? 4.0 : 2.0) * a.M * a.N * a.K; }
 inline double linear_bytes(const LinearArgs& a, int mode, int eb) {
   const double mn = static_cast<double>(a.M) * a.N, wide = is_gated(mode) ? 2.0 : 1.0;
-  double elems = static_cast<double>(a.M) * a.K + mn;
+  double elems = (a.a_low ? 2.0 : 1.0) * a.M * a.K + mn;
   if (a.add) elems += mn;
   if (mode == kLinBwd || mode == kGatedBwd) elems += a.z ? wide * mn : 0.0;
   if (mode == kGatedBwd) elems += mn;
@@ -831,10 +843,10 @@ inline double linear_bytes(const LinearArgs& a, int mode, int eb) {
 }
 inline int tiles_over(int n, int tile) { return (n + tile - 1) / tile; }
 
-template <typename T, int MODE, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
+template <typename T, int MODE, bool LOW, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
 int launch_linear_tile(Context* ctx, LinearArgs& a) {
   constexpr int BM = WM * TM * 32, BN = WN * TN * 32, BN_OUT = MODE == kGatedFwd ? BN / 2 : BN;
-  static const std::string name = std::string("linear_tile_kernel<") + type_name<T>() + mode_name(MODE) + std::to_string(BM) + "x" +
+  static const std::string name = std::string("linear_tile_kernel<") + type_name<T>() + mode_name(MODE, LOW) + std::to_string(BM) + "x" +
                                   std::to_string(BN) + "," + std::to_string(NBUF) + "buf>";
   a.tiles_m = tiles_over(a.M, BM);
   a.tiles_n = tiles_over(a.N, BN_OUT);
@@ -848,14 +860,14 @@ int launch_linear_tile(Context* ctx, LinearArgs& a) {
   // counts: a workgroup per tile, and who is done makes room (768 x 6216 over 3480: 319 us, walked 411)
   const int64_t most = sizeof(T) == 2 ? 256 * PER_CU : tiles;
   const unsigned grid = static_cast<unsigned>(tiles < most ? tiles : most);
-  return launch(ctx, linear_tile_kernel<T, MODE, WM, WN, TM, TN, NBUF, PER_CU>, dim3(grid), dim3(WM * WN * 64), a, name.c_str(),
+  return launch(ctx, linear_tile_kernel<T, MODE, LOW, WM, WN, TM, TN, NBUF, PER_CU>, dim3(grid), dim3(WM * WN * 64), a, name.c_str(),
                 linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
 }
 
-template <typename T, int MODE, int TM, int TN, int KG, int NBUF, int RB>
+template <typename T, int MODE, bool LOW, int TM, int TN, int KG, int NBUF, int RB>
 int launch_linear_split(Context* ctx, LinearArgs& a) {
   constexpr int BM = TM * 32, BN = TN * 32, BN_OUT = MODE == kGatedFwd ? BN / 2 : BN;
-  static const std::string name = std::string("linear_split_kernel<") + type_name<T>() + mode_name(MODE) + std::to_string(BM) + "x" +
+  static const std::string name = std::string("linear_split_kernel<") + type_name<T>() + mode_name(MODE, LOW) + std::to_string(BM) + "x" +
                                   std::to_string(BN) + "," + std::to_string(KG) + "way," + std::to_string(RB) + ">";
   a.tiles_m = tiles_over(a.M, BM);
   a.tiles_n = tiles_over(a.N, BN_OUT);
@@ -864,19 +876,19 @@ int launch_linear_split(Context* ctx, LinearArgs& a) {
   // the larger operand is the one an XCD should fetch once
   a.group_rows = (MODE == kGatedFwd ? 2.0 : 1.0) * a.N > a.M ? 1 : 0;
   a.div_tiles_n = FastDiv(a.group_rows ? a.tiles_m : a.tiles_n);
-  return launch(ctx, linear_split_kernel<T, MODE, TM, TN, KG, NBUF, RB>, dim3(static_cast<unsigned>(tiles)), dim3(KG * 64), a, name.c_str(),
+  return launch(ctx, linear_split_kernel<T, MODE, LOW, TM, TN, KG, NBUF, RB>, dim3(static_cast<unsigned>(tiles)), dim3(KG * 64), a, name.c_str(),
                 linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
 }
 
-template <typename T, int MODE, int KG>
+template <typename T, int MODE, bool LOW, int KG>
 int launch_linear_rows(Context* ctx, LinearArgs& a) {
-  static const std::string name = std::string("linear_rows_kernel<") + type_name<T>() + mode_name(MODE) + "16x16," + std::to_string(KG) + "way>";
+  static const std::string name = std::string("linear_rows_kernel<") + type_name<T>() + mode_name(MODE, LOW) + "16x16," + std::to_string(KG) + "way>";
   a.tiles_m = tiles_over(a.M, 16);
   a.tiles_n = tiles_over(a.N, 16);
   const int64_t tiles = static_cast<int64_t>(a.tiles_m) * a.tiles_n;
   TCH_CHECK_ARG(tiles <= 0x3fffffff, "linear: grid out of range");
   a.div_tiles_n = FastDiv(static_cast<uint32_t>(a.tiles_m));
-  return launch(ctx, linear_rows_kernel<T, MODE, KG>, dim3(static_cast<unsigned>(tiles)), dim3(KG * 64), a, name.c_str(),
+  return launch(ctx, linear_rows_kernel<T, MODE, LOW, KG>, dim3(static_cast<unsigned>(tiles)), dim3(KG * 64), a, name.c_str(),
                 linear_flops(a, MODE), 0, linear_bytes(a, MODE, sizeof(T)));
 }
 
@@ -917,9 +929,11 @@ const KernelCost* kernel_costs() {
 template <typename T, bool GATED_FWD>
 float kernel_us(int kernel, int M, const LinearArgs& a) {
   const KernelCost& c = kernel_costs<T, GATED_FWD>()[kernel];
-  if (!c.bm || (kernel == kTile256 && a.K * static_cast<int>(sizeof(T)) <= c.step)) return INFINITY;   // (256 x 256 takes two steps at least)
+  if (!c.bm) return INFINITY;
+  const int all_steps = tiles_over(a.K * static_cast<int>(sizeof(T)), c.step) * (a.a_low ? 2 : 1);
+  if (kernel == kTile256 && all_steps < 2) return INFINITY;   // (it takes two steps at least)
   const double tiles = static_cast<double>(tiles_over(M, c.bm)) * tiles_over(a.N, GATED_FWD ? c.bn / 2 : c.bn);
-  const int steps = tiles_over(tiles_over(a.K * static_cast<int>(sizeof(T)), c.step), c.ways);
+  const int steps = tiles_over(all_steps, c.ways);
   const double rounds = kernel < kTile128x64 && tiles > 8 * 256 ? tiles / 256 : ceil(tiles / 256);
   const float load = kernel == kRows16 ? static_cast<float>(min(M, 16)) / 16.f : tiles < 256 ? static_cast<float>(tiles) / 256.f : 1.f;
   const float step_us = c.step_us + load * (c.full_us - c.step_us);
@@ -939,29 +953,29 @@ Kernel choose_kernel(int M, const LinearArgs& a, float* us) {
   return best;
 }
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool LOW>
 int launch_linear_kernel(Context* ctx, Kernel kernel, LinearArgs& a) {
   constexpr bool kWide = MODE == kGatedFwd, kBf = sizeof(T) == 2;
   switch (kernel) {
     case kRows16:
-      if constexpr (!kWide) return launch_linear_rows<T, MODE, 8>(ctx, a);
+      if constexpr (!kWide) return launch_linear_rows<T, MODE, LOW, 8>(ctx, a);
       break;
-    case kSplit32: return launch_linear_split<T, MODE, 1, 1, 4, 3, 128>(ctx, a);
-    case kSplit32x64: return launch_linear_split<T, MODE, 1, 2, 4, 3, 128>(ctx, a);
+    case kSplit32: return launch_linear_split<T, MODE, LOW, 1, 1, 4, 3, 128>(ctx, a);
+    case kSplit32x64: return launch_linear_split<T, MODE, LOW, 1, 2, 4, 3, 128>(ctx, a);
     case kSplit64:
-      if constexpr (kBf) return launch_linear_split<T, MODE, 2, 2, 3, 3, 128>(ctx, a);
-      else return launch_linear_split<T, MODE, 2, 2, 4, 4, 64>(ctx, a);
+      if constexpr (kBf) return launch_linear_split<T, MODE, LOW, 2, 2, 3, 3, 128>(ctx, a);
+      else return launch_linear_split<T, MODE, LOW, 2, 2, 4, 4, 64>(ctx, a);
     case kTile128x64:
-      if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 1, 1, 2, 4, 1>(ctx, a);
-      else return launch_linear_tile<T, MODE, 4, 1, 1, 2, 2, 2>(ctx, a);
+      if constexpr (kBf) return launch_linear_tile<T, MODE, LOW, 4, 1, 1, 2, 4, 1>(ctx, a);
+      else return launch_linear_tile<T, MODE, LOW, 4, 1, 1, 2, 2, 2>(ctx, a);
     case kTile128:
-      if constexpr (kBf) return launch_linear_tile<T, MODE, 2, 2, 2, 2, 3, 1>(ctx, a);
+      if constexpr (kBf) return launch_linear_tile<T, MODE, LOW, 2, 2, 2, 2, 3, 1>(ctx, a);
       break;
     case kTile256x128:
-      if constexpr (kBf) return launch_linear_tile<T, MODE, 4, 2, 2, 2, 3, 1>(ctx, a);
+      if constexpr (kBf) return launch_linear_tile<T, MODE, LOW, 4, 2, 2, 2, 3, 1>(ctx, a);
       break;
     case kTile256:
-      if constexpr (kBf) return launch_linear_tile<T, MODE, 2, 4, 4, 2, 2, 1>(ctx, a);
+      if constexpr (kBf) return launch_linear_tile<T, MODE, LOW, 2, 4, 4, 2, 2, 1>(ctx, a);
       break;
     default: break;
   }
@@ -973,7 +987,7 @@ int launch_linear_kernel(Context* ctx, Kernel kernel, LinearArgs& a) {
 // fill whole rounds are one launch and the others a second one, with tiles as small as suit them: bf16 9729 x 3456 over 15184 1217 ->
 // 1042 us, fp32 1568 x 4096 over 1024 151 -> 134.
 constexpr float kSecondLaunchUs = 3.f, kWorthwhile = 0.93f;
-template <typename T, int MODE>
+template <typename T, int MODE, bool LOW = false>
 int launch_linear_mode(Context* ctx, LinearArgs& a) {
   constexpr bool kWide = MODE == kGatedFwd;
   float us;
@@ -996,11 +1010,12 @@ int launch_linear_mode(Context* ctx, LinearArgs& a) {
       rows = static_cast<int>(main_rows);
     }
   }
-  if (rows == a.M) return launch_linear_kernel<T, MODE>(ctx, kernel, a);
+  if (rows == a.M) return launch_linear_kernel<T, MODE, LOW>(ctx, kernel, a);
   LinearArgs rest = a;
   auto skip = [&](const void* t, int64_t ld) -> const void* { return t ? static_cast<const T*>(t) + rows * ld : nullptr; };
   rest.M = a.M - rows;
   rest.a = skip(a.a, a.lda);
+  rest.a_low = skip(a.a_low, a.lda);
   rest.add = skip(a.add, a.ldadd);
   rest.z = skip(a.z, a.ldz);
   rest.out = const_cast<void*>(skip(a.out, a.ldo));
@@ -1008,15 +1023,19 @@ int launch_linear_mode(Context* ctx, LinearArgs& a) {
   rest.low = const_cast<void*>(skip(a.low, a.ldo));
   rest.low2 = const_cast<void*>(skip(a.low2, a.ldo2));
   a.M = rows;
-  if (int rc = launch_linear_kernel<T, MODE>(ctx, kernel, a)) return rc;
-  return launch_linear_kernel<T, MODE>(ctx, rest_kernel, rest);
+  if (int rc = launch_linear_kernel<T, MODE, LOW>(ctx, kernel, a)) return rc;
+  return launch_linear_kernel<T, MODE, LOW>(ctx, rest_kernel, rest);
 }
 
 template <typename T>
 int launch_linear_typed(Context* ctx, int mode, LinearArgs& a) {
   switch (mode) {
     case kLinFwd: return launch_linear_mode<T, kLinFwd>(ctx, a);
-    case kLinBwd: return launch_linear_mode<T, kLinBwd>(ctx, a);
+    case kLinBwd:
+      // low parts have kernels of their own: with the choice at run time the others are slower (8192 x 4096 over 1024 81 -> 87 us)
+      if constexpr (sizeof(T) == 2)
+        if (a.a_low) return launch_linear_mode<T, kLinBwd, true>(ctx, a);
+      return launch_linear_mode<T, kLinBwd>(ctx, a);
     case kGatedFwd: return launch_linear_mode<T, kGatedFwd>(ctx, a);
     default: return launch_linear_mode<T, kGatedBwd>(ctx, a);
   }

@@ -982,17 +982,19 @@ def linear_fwd(ctx, x, w, y, bias=None, act="none", residual=None, pre=None):
                                _vector(ctx, "bias", bias, N), _act_code(act), rp, ldr, pp, ldp, M, K, N), "tch_linear_fwd")
 
 
-def linear_dgrad(ctx, dy, wt, dx, act="none", pre=None, residual=None):
+def linear_dgrad(ctx, dy, wt, dx, act="none", pre=None, residual=None, dy_low=None):
     """dx = (dy w) . act'(pre) + residual in one launch: wt [K, N] is the weight [N, K] transposed (as for conv2d_dgrad), dy [..., N],
     dx, pre and residual [..., K].  pre and act are those of the layer in FRONT of this one, whose output this layer read: dx is
-    then the gradient of that layer's pre-activation.  pre or residual may be dx itself."""
+    then the gradient of that layer's pre-activation.  pre or residual may be dx itself.  dy_low (bf16): the low part of dy (act_bwd,
+    linear_dgrad_gated): dx is then that of the unrounded gradient, in twice the products."""
     K, N = wt.shape
     dyp, lddy, M = _matrix(ctx, "dy", dy, N)
+    lowp = _low(ctx, "dy_low", dy_low, dy)
     dxp, lddx, _ = _matrix(ctx, "dx", dx, K, M, dy.dtype)
     pp, ldp, _ = _matrix(ctx, "pre", pre, K, M, dy.dtype)
     rp, ldr, _ = _matrix(ctx, "residual", residual, K, M, dy.dtype)
-    check(lib().tch_linear_dgrad(ctx.handle, dtype_code(dy), dyp, lddy, _weights(ctx, "wt", wt, dy.dtype), dxp, lddx, _act_code(act),
-                                 pp, ldp, rp, ldr, M, N, K), "tch_linear_dgrad")
+    check(lib().tch_linear_dgrad_low(ctx.handle, dtype_code(dy), dyp, lowp, lddy, _weights(ctx, "wt", wt, dy.dtype), dxp, lddx, _act_code(act),
+                                     pp, ldp, rp, ldr, M, N, K), "tch_linear_dgrad_low")
 
 
 def _low(ctx, name, low, high):
@@ -1071,8 +1073,9 @@ def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=No
     """The gradients of linear_fwd: dpre = dy . act'(pre) (act "none": dy itself, and dpre stays untouched), dx = dpre w + residual,
     dw (+)= dpre^T x and dbias (+)= column sums of dpre, both fp32.  The residual's own gradient is dy.  dx (with wt) or dw may be
     None.  x and the gradient it meets are contiguous; workspace: linear_bwd_workspace_bytes (without it the weight gradient
-    is not split over its rows).  bf16: dpre is rounded, and so are its products, except where dpre_low (like dpre) keeps what
-    rounding takes off it: dw and dbias are then those of the unrounded dpre.  dy_low, x_low: as for linear_wgrad."""
+    is not split over its rows).  bf16: dpre is rounded (2^-8 of each element at most), and dx, dw and dbias are those of the rounded
+    one, except where dpre_low (like dpre) keeps what rounding takes off it: all three are then those of the unrounded dpre (2^-16), in
+    twice the products.  dy_low (the low part of dy, act "none") does the same for all three, x_low (the low part of x) for dw."""
     N = dy.shape[-1]
     g, low = dy, dy_low
     if act != "none":
@@ -1081,7 +1084,7 @@ def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=No
         act_bwd(ctx, dy, pre, dpre, act, dz_low=dpre_low)
         g, low = dpre, dpre_low
     if dx is not None:
-        linear_dgrad(ctx, g, wt, dx, residual=residual)
+        linear_dgrad(ctx, g, wt, dx, residual=residual, dy_low=low)
     else:
         assert residual is None, "a residual without dx"
     if dw is not None:
@@ -1133,7 +1136,7 @@ def linear_dgrad_gated(ctx, dy, wt, pre, dpre, act="silu", h=None, dpre_low=None
 
 def gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=None, act="silu", residual=None, accumulate=False, workspace=None, dpre_low=None):
     """The gradients of gated_linear_fwd from dh [..., F]: dpre [..., 2F] as in gated_act_bwd, dx = dpre w + residual,
-    dw (+)= dpre^T x, dbias (+)= column sums of dpre.  wt [K, 2F] is w transposed; the rest as for linear_bwd."""
+    dw (+)= dpre^T x, dbias (+)= column sums of dpre.  wt [K, 2F] is w transposed; dpre_low and the rest as for linear_bwd."""
     gated_act_bwd(ctx, dh, pre, dpre, act, dpre_low=dpre_low)
     linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=dbias, residual=residual, accumulate=accumulate, workspace=workspace, dy_low=dpre_low)
 
