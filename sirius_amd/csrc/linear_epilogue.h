@@ -23,8 +23,8 @@ enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh =
 
 constexpr bool is_gated(int mode) { return mode == kGatedFwd || mode == kGatedBwd; }
 
-// T decides how exactly: bf16 results are rounded to 2^-9 of their size, so the hardware's exponential and reciprocal (a few
-// 2^-23) and an error function to 1.5e-7 do; fp32 results take the library's exponential and division.
+// T decides how exactly: bf16 results are off by up to 2^-8 of their size when they are stored (2^-16 in two parts), so the hardware's
+// exponential and reciprocal (2^-23 each) do; fp32 results take the library's exponential and division.
 template <typename T>
 __device__ inline float fast_exp(float x) {
   if constexpr (sizeof(T) == 2)
@@ -44,18 +44,23 @@ __device__ inline float sigmoid(float x) {
   return reciprocal<T>(1.f + fast_exp<T>(-x));   // x -> -inf: 1 / inf = 0
 }
 
-// The normal distribution's integral and density at z.  bf16: formula 7.1.26 of Abramowitz and Stegun for erfc(|z| / sqrt 2), whose
-// exponential is the density's as well.  fp32: erfc(x) = exp(-x^2) t Q(t) with t = 1 / (1 + 0.42 x) and Q the polynomial of degree 9 with the
-// smallest relative error (2.7e-9, an exchange over 0 <= x <= 10.5); what rounding takes off z^2 / 2 goes back into the exponential.  Within
-// 3.8e-7 of the value for all z, against a call of the library's erfc the epilogue of 1568 x 4096 over 1024 is 20 us shorter.
+// The normal distribution's integral and density at z.  Left of zero the integral is small and GELU is z times it, so it is its relative error
+// that counts: 0.5 erfc(m / sqrt 2) = exp(-m^2 / 2) t Q(t), m = |z|, t = 1 / (1 + a m), Q the polynomial with the smallest relative error; the
+// exponential is the density's as well.
+// bf16: degree 6, 7.1e-7 (a linear program over 0 <= m <= 13.3).  With the roundings of the exponential's argument the integral is within
+// (40 + 1.5 z^2) 2^-24 of its size: 1.1e-6 next to zero, 7.7e-6 at z = -13, behind which it is subnormal.
+// fp32: degree 9, 2.7e-9 (an exchange, x = m / sqrt 2 <= 10.5); what rounding takes off z^2 / 2 goes back into the exponential.  Within 12 x 2^-24 of its
+// size for z > -13 (4.5e-7 is the largest found); against a call of the library's erfc the epilogue of 1568 x 4096 over 1024 is 20 us shorter.
 template <typename T>
 __device__ inline void normal_cdf(float z, float& cdf, float& density) {
   if constexpr (sizeof(T) == 2) {
-    const float x = fabsf(z) * 0.7071067811865476f;
-    const float e = fast_exp<T>(-x * x);
-    const float t = reciprocal<T>(1.f + 0.3275911f * x);
-    const float half_erfc =
-        0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);   // log2(e) / 2
+    const float t = reciprocal<T>(fmaf(0.362f, fabsf(z), 1.f));
+    constexpr float kQ[7] = {0.14450584f, 0.14266214f, 0.13957834f, 0.028423097f, 0.17721444f, -0.18045251f, 0.048069008f};
+    float q = kQ[6];
+#pragma unroll
+    for (int i = 5; i >= 0; --i) q = fmaf(q, t, kQ[i]);
+    const float half_erfc = e * t * q;
     cdf = z < 0.f ? half_erfc : 1.f - half_erfc;
     density = 0.3989422804014327f * e;
   } else {
