@@ -168,7 +168,7 @@ class EngineBase:
 
     def last_grad_norm(self):
         """The global norm, before clipping, of the gradients that the most recent optimizer step consumed (nan without
-        clipping)."""
+        clipping, and before the first step).  A step whose launches were rejected consumed none."""
         if self._last_norm is None:
             return float("nan")
         self.ctx.synchronize()
@@ -209,12 +209,16 @@ class EngineBase:
                 raise RuntimeError("optimizer_step(use_global=True) before any accumulate()")
             if self._opt_global_prog is None:
                 self._opt_global_prog = self._flat_prog(lambda: self._record_optimizer(self.global_grads))
-            self._last_norm = self._norms[True][0] if self.max_grad_norm is not None else None
-            cut = self.ctx.run(self._opt_global_prog)
+            cut = self._run_step(self._opt_global_prog, True)
             if zero_global:
                 ops.fill_zero(self.ctx, self.global_grads)
             return cut
         if self._opt_prog is None:
             self._opt_prog = self._flat_prog(lambda: self._record_optimizer(self.grads))
-        self._last_norm = self._norms[False][0] if self.max_grad_norm is not None else None
-        return self.ctx.run(self._opt_prog)
+        return self._run_step(self._opt_prog, False)
+
+    def _run_step(self, prog, use_global):
+        cut = self.ctx.run(prog)
+        if not cut:
+            self._last_norm = self._norms[use_global][0] if self.max_grad_norm is not None else None
+        return cut
