@@ -458,7 +458,7 @@ int tch_gelu_bwd(tch_context* ctx, int dtype, const void* dy, const void* x, voi
  *   dgrad:  dx = (dy w) . act'(pre) + residual, pre and act being those of the layer in FRONT of this one; wt [N][K] is
  *           this layer's weight transposed (tch_filter_transpose_batched), dy [M][K], dx [M][N].
  * dgrad_low: dgrad of dy + dy_low (bf16; laid out like dy; NULL: of dy), both multiplied: the data gradient of a gradient
- *           that was not rounded, in twice the products.
+ *           that was not rounded, in twice the products.  dx_low (laid out like dx; may be NULL): what rounding took off dx.
  * A residual, and the pre-activations of a dgrad, may be the output itself (in place); nothing else may overlap one. */
 int tch_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* y, int64_t ldy,
                    const float* bias, int act, const void* residual, int64_t ldr, void* pre, int64_t ldp, int64_t M,
@@ -467,8 +467,8 @@ int tch_linear_dgrad(tch_context* ctx, int dtype, const void* dy, int64_t lddy, 
                      int act, const void* pre, int64_t ldp, const void* residual, int64_t ldr, int64_t M, int64_t K,
                      int64_t N);
 int tch_linear_dgrad_low(tch_context* ctx, int dtype, const void* dy, const void* dy_low, int64_t lddy, const void* wt,
-                         void* dx, int64_t lddx, int act, const void* pre, int64_t ldp, const void* residual,
-                         int64_t ldr, int64_t M, int64_t K, int64_t N);
+                         void* dx, void* dx_low, int64_t lddx, int act, const void* pre, int64_t ldp,
+                         const void* residual, int64_t ldr, int64_t M, int64_t K, int64_t N);
 /* Gated layer: g = x wg^T + bg, u = x wu^T + bu, h = act(g) . u.  w [2F][K] and bias [2F] hold the gate's rows first,
  * pre [M][2F] (may be NULL) = (g | u), h [M][F].
  * dgrad_gated: dh = dy w (wt [F][K] the down projection's weight transposed, dy [M][K]) goes straight into

@@ -368,12 +368,12 @@ int tch_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, cons
 
 int tch_linear_dgrad(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, void* dx, int64_t lddx, int act, const void* pre,
                      int64_t ldp, const void* residual, int64_t ldr, int64_t M, int64_t K, int64_t N) {
-  return linear_dgrad(C(ctx), dtype, rows(dy, lddy), nullptr, wt, rows(dx, lddx), act, rows(pre, ldp), rows(residual, ldr), M, K, N);
+  return linear_dgrad(C(ctx), dtype, rows(dy, lddy), nullptr, wt, rows(dx, lddx), nullptr, act, rows(pre, ldp), rows(residual, ldr), M, K, N);
 }
 
-int tch_linear_dgrad_low(tch_context* ctx, int dtype, const void* dy, const void* dy_low, int64_t lddy, const void* wt, void* dx, int64_t lddx, int act,
-                         const void* pre, int64_t ldp, const void* residual, int64_t ldr, int64_t M, int64_t K, int64_t N) {
-  return linear_dgrad(C(ctx), dtype, rows(dy, lddy), dy_low, wt, rows(dx, lddx), act, rows(pre, ldp), rows(residual, ldr), M, K, N);
+int tch_linear_dgrad_low(tch_context* ctx, int dtype, const void* dy, const void* dy_low, int64_t lddy, const void* wt, void* dx, void* dx_low, int64_t lddx,
+                         int act, const void* pre, int64_t ldp, const void* residual, int64_t ldr, int64_t M, int64_t K, int64_t N) {
+  return linear_dgrad(C(ctx), dtype, rows(dy, lddy), dy_low, wt, rows(dx, lddx), dx_low, act, rows(pre, ldp), rows(residual, ldr), M, K, N);
 }
 
 int tch_gated_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* h, int64_t ldh, const float* bias, int act,

@@ -109,13 +109,13 @@ int linear_launch(Context* ctx, const char* what, int dtype, int mode, LinearArg
                 name + ": weights and bias must start on a 16-byte boundary");
   TCH_CHECK_ARG(rows_fit(a.a, a.lda, K, eb) && rows_fit(a.a_low, a.lda, K, eb) && rows_fit(a.out, a.ldo, mode == kGatedBwd ? 2 * N : N, eb) && rows_fit(a.add, a.ldadd, N, eb) &&
                     rows_fit(a.z, a.ldz, wide * N, eb) && rows_fit(a.out2, a.ldo2, mode == kGatedFwd ? 2 * N : N, eb) &&
-                    rows_fit(a.low, a.ldo, 2 * N, eb) && rows_fit(a.low2, a.ldo2, N, eb),
+                    rows_fit(a.low, a.ldo, wide * N, eb) && rows_fit(a.low2, a.ldo2, N, eb),
                 name + ": rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
   auto rows_of = [&](const void* t, int64_t ld, int64_t width) { return Span{t, ld * eb, width * eb, M}; };
   const Span in[5] = {rows_of(a.a, a.lda, K), rows_of(a.add, a.ldadd, N), rows_of(a.z, a.ldz, wide * N), {a.b, K * eb, K * eb, weight_rows},
                       rows_of(a.a_low, a.lda, K)};
   const Span out[4] = {rows_of(a.out, a.ldo, mode == kGatedBwd ? 2 * N : N), rows_of(a.out2, a.ldo2, mode == kGatedFwd ? 2 * N : N),
-                       rows_of(a.low, a.ldo, 2 * N), rows_of(a.low2, a.ldo2, N)};
+                       rows_of(a.low, a.ldo, wide * N), rows_of(a.low2, a.ldo2, N)};
   const Span bias{a.bias, weight_rows * 4, weight_rows * 4, 1};
   for (int o = 0; o < 4; ++o) {
     bool ok = apart(out[o], bias);
@@ -145,10 +145,10 @@ int linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows
   return linear_launch(ctx, "linear_fwd", dtype, kLinFwd, a, M, K, N);
 }
 
-int linear_dgrad(Context* ctx, int dtype, const Rows& dy, const void* dy_low, const void* wt, const Rows& dx, int act, const Rows& pre,
-                 const Rows& residual, int64_t M, int64_t K, int64_t N) {
+int linear_dgrad(Context* ctx, int dtype, const Rows& dy, const void* dy_low, const void* wt, const Rows& dx, void* dx_low, int act,
+                 const Rows& pre, const Rows& residual, int64_t M, int64_t K, int64_t N) {
   TCH_CHECK_ARG(act == kActNone || pre.ptr || M == 0, "linear_dgrad: an activation's derivative needs its pre-activations");
-  TCH_CHECK_ARG(dtype == kBF16 || !dy_low, "linear_dgrad: fp32 gradients are not rounded: there is no low part");
+  TCH_CHECK_ARG(dtype == kBF16 || (!dy_low && !dx_low), "linear_dgrad: fp32 gradients are not rounded: there is no low part");
   LinearArgs a{};
   a.a = dy.ptr, a.lda = dy.ld;
   a.a_low = dy_low;
@@ -156,6 +156,7 @@ int linear_dgrad(Context* ctx, int dtype, const Rows& dy, const void* dy_low, co
   a.add = residual.ptr, a.ldadd = residual.ld;
   a.z = act == kActNone ? nullptr : pre.ptr, a.ldz = pre.ld;
   a.out = dx.ptr, a.ldo = dx.ld;
+  a.low = dx_low;
   a.act = act;
   return linear_launch(ctx, "linear_dgrad", dtype, kLinBwd, a, M, K, N);
 }

@@ -2,10 +2,10 @@
 // feed-forward layer does to it in the epilogue (linear_epilogue.h).  A has its own row stride, B (the weights) is dense.
 // Compiled once per element type (linear_bf16.hip, linear_f32.hip).
 //
-// LOW: a data gradient of bf16 gradients that come with what rounding took off them.  The product of the rounded gradient alone has an error of its
+// LOW: a data gradient of bf16 gradients that come with what rounding took off them, or one that keeps what rounding takes off its own.  The product of the rounded gradient alone has an error of its
 // own of about 2^-9.3 of dx, next to the 2^-9.3 of rounding dx.  The reduction is walked twice, over a and then over its low part, into the
 // same accumulators: a tile's steps are twice as many, and so is its time where the multiplies bound it (8192 x 2048 over 11264 293 us, with the
-// low part 563; 8192 x 1024 over 4096 59 and 118; 392 x 512 over 2048 5.4 and 8.5).
+// low part of a 563; 8192 x 1024 over 4096 59 and 118; 392 x 512 over 2048 5.4 and 8.5).
 //
 // Gated modes multiply both projections in one tile: 32 (in the narrowest tiles 16) rows of the gate's weights lie next to the same rows of the up
 // projection's, so that a lane ends up with both products of its columns and the epilogue needs nobody else's.
@@ -26,7 +26,7 @@ struct LinearArgs {
   const void* z;      // backward: pre-activations [M][N] or [M][2N]
   void* out;          // [M][N]; gated backward: [M][2N]
   void* out2;         // forward: pre (may be null); gated backward: h (may be null)
-  void* low;          // gated backward, bf16: what rounding took off out and out2 (may be null), laid out like them
+  void* low;          // data gradients, bf16: what rounding took off out and out2 (may be null), laid out like them
   void* low2;
   int64_t lda, ldadd, ldz, ldo, ldo2;
   int M, N, K, act;
@@ -47,7 +47,7 @@ __device__ inline __amdgpu_buffer_rsrc_t rows_from(const void* base, int64_t ld,
   const int64_t bytes = rows > 0 && base ? ((rows - 1) * ld + width) * static_cast<int64_t>(sizeof(T)) : 0;
   return make_rsrc(base ? static_cast<const T*>(base) + row0 * ld : nullptr, static_cast<uint32_t>(bytes));
 }
-template <typename T, int MODE>
+template <typename T, int MODE, bool LOW>
 __device__ inline TileTensors tile_tensors(const LinearArgs& p, int m0, int rows) {
   constexpr int kWide = is_gated(MODE) ? 2 : 1;
   TileTensors t;
@@ -55,10 +55,8 @@ __device__ inline TileTensors tile_tensors(const LinearArgs& p, int m0, int rows
   t.z = rows_from<T>(p.z, p.ldz, m0, rows, kWide * p.N);
   t.out = rows_from<T>(p.out, p.ldo, m0, rows, MODE == kGatedBwd ? 2 * p.N : p.N);
   t.out2 = rows_from<T>(p.out2, p.ldo2, m0, rows, MODE == kGatedFwd ? 2 * p.N : p.N);
-  if constexpr (MODE == kGatedBwd) {
-    t.low = rows_from<T>(p.low, p.ldo, m0, rows, 2 * p.N);
-    t.low2 = rows_from<T>(p.low2, p.ldo2, m0, rows, p.N);
-  }
+  if constexpr (LOW || MODE == kGatedBwd) t.low = rows_from<T>(p.low, p.ldo, m0, rows, kWide * p.N);
+  if constexpr (MODE == kGatedBwd) t.low2 = rows_from<T>(p.low2, p.ldo2, m0, rows, p.N);
   return t;
 }
 
@@ -83,7 +81,7 @@ __device__ inline void write_chunk(__amdgpu_buffer_rsrc_t rsrc, int off, const f
 }
 
 // One 16-byte chunk of the output (E columns of a row) in two steps: what it reads, and the rest.
-template <typename T, int MODE>
+template <typename T, int MODE, bool LOW>
 struct ChunkOperands {
   Chunk zg, zu, add;
   __device__ __forceinline__ void request(const LinearArgs& p, const TileTensors& t, int row, int col) {
@@ -120,6 +118,13 @@ struct ChunkOperands {
       }
     }
     write_chunk<T, AUX>(t.out, at<T>(row, p.ldo, col, ok), o);
+    if constexpr (LOW) {
+      if (p.low) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = rounded_off(o[e]);
+        write_chunk<T>(t.low, at<T>(row, p.ldo, col, ok), o);
+      }
+    }
     if constexpr (MODE == kGatedBwd) {
       write_chunk<T>(t.out, at<T>(row, p.ldo, p.N + col, ok), u);
       if (p.out2) write_chunk<T>(t.out2, at<T>(row, p.ldo2, col, ok), h);
@@ -329,14 +334,14 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   auto epilogue = [&](int id, uint32_t stage) LINEAR_INLINE {
     int m0, n0;
     locate(id, m0, n0);
-    const TileTensors t = tile_tensors<T, MODE>(p, m0, min(BM, p.M - m0));
+    const TileTensors t = tile_tensors<T, MODE, LOW>(p, m0, min(BM, p.M - m0));
     constexpr int COLS = GATED_FWD ? 32 : 64;             // output columns of a wavefront
     constexpr int LANES = COLS / E, ROWS = 64 / LANES;    // lanes per row, rows per pass
     constexpr int PASSES = 16 / ROWS, BLOCKS = TM * 2, TOTAL = BLOCKS * PASSES;
     constexpr int DEPTH = TM <= 2 ? 4 : MODE == kGatedBwd ? 1 : 2;                 // passes whose operands are on their way, as the registers allow
     const int lane_row = lane / LANES, lane_col = lane % LANES * E;
     const int col = n0 + wn * COLS + lane_col;
-    ChunkOperands<T, MODE> operands[DEPTH];
+    ChunkOperands<T, MODE, LOW> operands[DEPTH];
     auto row_of = [&](int pass) {
       int row = (wm * BLOCKS + pass / PASSES) * 16 + pass % PASSES * ROWS + lane_row;
       asm volatile("" : "+v"(row));   // offsets are made where they are used, not all of them ahead of the first
@@ -427,7 +432,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   // has to land: they are not waited for.  With two buffers all of that step is requested ahead of the epilogue for this.
   constexpr int STORES = TM * 32 * (GATED_FWD ? 32 : 64) / (64 * E);
   constexpr int NEWER = NBUF == 2 ? 0 : AHEAD;
-  constexpr int OUTPUTS = MODE == kGatedBwd ? 2 : 1, MORE = MODE == kGatedFwd ? 2 : MODE == kLinBwd ? 0 : 1;   // `out`, `out2`
+  constexpr int OUTPUTS = MODE == kGatedBwd ? 2 : 1, MORE = MODE == kGatedFwd ? 2 : MODE == kLinBwd && !LOW ? 0 : 1;   // `out`; `out2` or `low`
   constexpr int AFTER_ONE = NEWER + STORES * OUTPUTS < 63 ? NEWER + STORES * OUTPUTS : 63;
   constexpr int AFTER_BOTH = NEWER + STORES * (OUTPUTS + MORE) < 63 ? NEWER + STORES * (OUTPUTS + MORE) : 63;
   enter_tile();
@@ -471,7 +476,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
   std::integral_constant<int, 1> start;
   std::integral_constant<int, NBUF == 2 ? ALL : NONE> finish;
   constexpr bool ONE_STEP = TM <= 2;   // reductions of one step; with 128 accumulators the second way there costs registers (spilled)
-  const int outputs = p.out2 ? 2 : 1;
+  const int outputs = p.out2 || (LOW && p.low) ? 2 : 1;
   int stored = 0;
   for (int id = first; id < tiles; id += gridDim.x) {
     if (ONE_STEP && steps == 1) {
@@ -615,9 +620,9 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
 
   // ---- the partial tiles meet: [wave][BM][LD] fp32, over the rings ----
   float* red = reinterpret_cast<float*>(lds);
-  const TileTensors t = tile_tensors<T, MODE>(p, m0, rows);
+  const TileTensors t = tile_tensors<T, MODE, LOW>(p, m0, rows);
   constexpr int CH = BN_OUT / E, ITEMS = BM * CH, VISITS = (ITEMS + NT - 1) / NT;
-  ChunkOperands<T, MODE> operands[VISITS];
+  ChunkOperands<T, MODE, LOW> operands[VISITS];
 #pragma unroll
   for (int visit = 0; visit < VISITS; ++visit) {
     const int q = tid + visit * NT;
@@ -800,6 +805,13 @@ __global__ __launch_bounds__(KG * 64) void linear_rows_kernel(LinearArgs p) {
       }
     }
     store_four(out, o);
+    if constexpr (LOW) {
+      if (p.low) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = rounded_off(o[e]);
+        store_four(static_cast<T*>(p.low) + row * p.ldo + col, o);
+      }
+    }
     if constexpr (MODE == kGatedBwd) {
       store_four(out + p.N, u);
       if (p.out2) store_four(out2, h);
@@ -838,7 +850,7 @@ inline double linear_bytes(const LinearArgs& a, int mode, int eb) {
   if (mode == kLinBwd || mode == kGatedBwd) elems += a.z ? wide * mn : 0.0;
   if (mode == kGatedBwd) elems += mn;
   if (a.out2) elems += mode == kGatedFwd ? 2.0 * mn : mn;
-  elems += (a.low ? 2.0 * mn : 0.0) + (a.low2 ? mn : 0.0);
+  elems += (a.low ? wide * mn : 0.0) + (a.low2 ? mn : 0.0);
   return elems * eb + a.b_bytes;
 }
 inline int tiles_over(int n, int tile) { return (n + tile - 1) / tile; }
@@ -1034,7 +1046,7 @@ int launch_linear_typed(Context* ctx, int mode, LinearArgs& a) {
     case kLinBwd:
       // low parts have kernels of their own: with the choice at run time the others are slower (8192 x 4096 over 1024 81 -> 87 us)
       if constexpr (sizeof(T) == 2)
-        if (a.a_low) return launch_linear_mode<T, kLinBwd, true>(ctx, a);
+        if (a.a_low || a.low) return launch_linear_mode<T, kLinBwd, true>(ctx, a);
       return launch_linear_mode<T, kLinBwd>(ctx, a);
     case kGatedFwd: return launch_linear_mode<T, kGatedFwd>(ctx, a);
     default: return launch_linear_mode<T, kGatedBwd>(ctx, a);

@@ -195,8 +195,8 @@ struct Rows {   // a matrix whose rows lie ld elements apart; ptr may be null wh
 };
 int linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows& y, const float* bias, int act, const Rows& residual,
                const Rows& pre, int64_t M, int64_t K, int64_t N);
-int linear_dgrad(Context* ctx, int dtype, const Rows& dy, const void* dy_low, const void* wt, const Rows& dx, int act, const Rows& pre,
-                 const Rows& residual, int64_t M, int64_t K, int64_t N);
+int linear_dgrad(Context* ctx, int dtype, const Rows& dy, const void* dy_low, const void* wt, const Rows& dx, void* dx_low, int act,
+                 const Rows& pre, const Rows& residual, int64_t M, int64_t K, int64_t N);
 int gated_linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows& h, const float* bias, int act, const Rows& pre, int64_t M,
                      int64_t K, int64_t F);
 int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& pre, const Rows& dpre, void* dpre_low, const Rows& h,

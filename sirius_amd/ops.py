@@ -982,19 +982,20 @@ def linear_fwd(ctx, x, w, y, bias=None, act="none", residual=None, pre=None):
                                _vector(ctx, "bias", bias, N), _act_code(act), rp, ldr, pp, ldp, M, K, N), "tch_linear_fwd")
 
 
-def linear_dgrad(ctx, dy, wt, dx, act="none", pre=None, residual=None, dy_low=None):
+def linear_dgrad(ctx, dy, wt, dx, act="none", pre=None, residual=None, dy_low=None, dx_low=None):
     """dx = (dy w) . act'(pre) + residual in one launch: wt [K, N] is the weight [N, K] transposed (as for conv2d_dgrad), dy [..., N],
     dx, pre and residual [..., K].  pre and act are those of the layer in FRONT of this one, whose output this layer read: dx is
     then the gradient of that layer's pre-activation.  pre or residual may be dx itself.  dy_low (bf16): the low part of dy (act_bwd,
-    linear_dgrad_gated): dx is then that of the unrounded gradient, in twice the products."""
+    linear_dgrad_gated, dx_low): dx is then that of the unrounded gradient, in twice the products.  dx_low (bf16): what rounding took
+    off dx, for the layer in front."""
     K, N = wt.shape
     dyp, lddy, M = _matrix(ctx, "dy", dy, N)
     lowp = _low(ctx, "dy_low", dy_low, dy)
     dxp, lddx, _ = _matrix(ctx, "dx", dx, K, M, dy.dtype)
     pp, ldp, _ = _matrix(ctx, "pre", pre, K, M, dy.dtype)
     rp, ldr, _ = _matrix(ctx, "residual", residual, K, M, dy.dtype)
-    check(lib().tch_linear_dgrad_low(ctx.handle, dtype_code(dy), dyp, lowp, lddy, _weights(ctx, "wt", wt, dy.dtype), dxp, lddx, _act_code(act),
-                                     pp, ldp, rp, ldr, M, N, K), "tch_linear_dgrad_low")
+    check(lib().tch_linear_dgrad_low(ctx.handle, dtype_code(dy), dyp, lowp, lddy, _weights(ctx, "wt", wt, dy.dtype), dxp,
+                                     _low(ctx, "dx_low", dx_low, dx), lddx, _act_code(act), pp, ldp, rp, ldr, M, N, K), "tch_linear_dgrad_low")
 
 
 def _low(ctx, name, low, high):
