@@ -486,6 +486,16 @@ int tch_act_bwd(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const
                 void* dz_low, int64_t lddz, int act, int64_t M, int64_t N);
 int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp,
                       void* dpre, void* dpre_low, int64_t lddp, void* h, int64_t ldh, int act, int64_t M, int64_t F);
+/* The same passes with the bias gradient: dbias [N] (gated [2F]) (+)= the column sums of the gradients before they are
+ * rounded.  workspace: the sums of blocks of rows, at least tch_act_bwd_workspace_bytes; NULL: the rows are not split
+ * over workgroups. */
+int64_t tch_act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int gated);
+int tch_act_bwd_bias(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* pre, int64_t ldp, void* dz,
+                     void* dz_low, int64_t lddz, float* dbias, int accumulate, int act, int64_t M, int64_t N,
+                     void* workspace, int64_t workspace_bytes);
+int tch_gated_act_bwd_bias(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp,
+                           void* dpre, void* dpre_low, int64_t lddp, void* h, int64_t ldh, float* dbias, int accumulate,
+                           int act, int64_t M, int64_t F, void* workspace, int64_t workspace_bytes);
 /* Weight and bias gradients of a bf16 layer: dw [N][K] (+)= dy^T x, dbias [N] (may be NULL) (+)= column sums of dy, both
  * fp32; x [M][K] and dy [M][N] dense.  x_low or dy_low (one of them, or none): the low part of that operand; both parts
  * are multiplied.  workspace: partial sums where the rows are split, at least tch_linear_wgrad_workspace_bytes; NULL: the

@@ -396,6 +396,21 @@ int tch_gated_act_bwd(tch_context* ctx, int dtype, const void* dh, int64_t lddh,
   return act_bwd(C(ctx), dtype, rows(dh, lddh), rows(pre, ldp), rows(dpre, lddp), dpre_low, rows(h, ldh), 1, act, M, F);
 }
 
+int64_t tch_act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int gated) { return act_bwd_workspace_bytes(dtype, M, N, gated); }
+
+int tch_act_bwd_bias(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* pre, int64_t ldp, void* dz, void* dz_low, int64_t lddz,
+                     float* dbias, int accumulate, int act, int64_t M, int64_t N, void* workspace, int64_t workspace_bytes) {
+  return act_bwd(C(ctx), dtype, rows(dy, lddy), rows(pre, ldp), rows(dz, lddz), dz_low, rows(nullptr, 0), 0, act, M, N, dbias, accumulate, workspace,
+                 workspace_bytes);
+}
+
+int tch_gated_act_bwd_bias(tch_context* ctx, int dtype, const void* dh, int64_t lddh, const void* pre, int64_t ldp, void* dpre, void* dpre_low,
+                           int64_t lddp, void* h, int64_t ldh, float* dbias, int accumulate, int act, int64_t M, int64_t F, void* workspace,
+                           int64_t workspace_bytes) {
+  return act_bwd(C(ctx), dtype, rows(dh, lddh), rows(pre, ldp), rows(dpre, lddp), dpre_low, rows(h, ldh), 1, act, M, F, dbias, accumulate, workspace,
+                 workspace_bytes);
+}
+
 int64_t tch_linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N) { return linear_wgrad_workspace_bytes(M, K, N); }
 
 int tch_linear_wgrad(tch_context* ctx, const void* x, const void* x_low, const void* dy, const void* dy_low, float* dw, float* dbias, int accumulate,

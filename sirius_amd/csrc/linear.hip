@@ -6,6 +6,7 @@
 // (a projection, an activation, a projection and the residual).
 #include "linear_kernels.h"
 
+#include <algorithm>
 #include <climits>
 
 #include "context.h"
@@ -29,56 +30,169 @@ struct ActBwdArgs {
   uint32_t chunks;    // rows * row_chunks
   int row_chunks, N, act;
   FastDiv div;        // by row_chunks
+  // act_bwd_sum_kernel
+  float* sums;        // [row blocks][N, gated 2 N]; one row block: dbias itself
+  int64_t M, block_rows;
+  int lanes_log;      // 2^lanes_log threads of a workgroup share a row
+  int add;            // sums is added to
 };
 constexpr int kAtOnce = 4;
 
+// The chunks of one place: what is read, and the gradients from it, stored and (unrounded) returned in o and u.
+template <typename T, int GATED>
+struct ActBwdChunks {
+  static constexpr int E = Elem<T>::kPerChunk;
+  Chunk dy, zg, zu;
+  __device__ __forceinline__ void request(const ActBwdArgs& p, int64_t row, uint32_t col) {
+    dy.u = load_streaming_u4(static_cast<const T*>(p.dy) + row * p.lddy, col);
+    zg.u = load_streaming_u4(static_cast<const T*>(p.z) + row * p.ldz, col);
+    if (GATED) zu.u = load_streaming_u4(static_cast<const T*>(p.z) + row * p.ldz + p.N, col);
+  }
+  template <int ACT>
+  __device__ __forceinline__ void finish(const ActBwdArgs& p, int64_t row, uint32_t col, float* o, float* u) {
+    float v[E], fg[E], fu[E], h[E];
+    chunk_to_float<T>(dy, v);
+    chunk_to_float<T>(zg, fg);
+    if (GATED) chunk_to_float<T>(zu, fu);
+    combine<T, GATED ? kGatedBwd : kLinBwd, ACT, E>(v, u, fg, fu, o, h);
+    T* dz = static_cast<T*>(p.dz) + row * p.lddz;
+    reinterpret_cast<uint4*>(dz)[col] = float_to_chunk<T>(o).u;
+    if (GATED) {
+      reinterpret_cast<uint4*>(dz + p.N)[col] = float_to_chunk<T>(u).u;
+      if (p.h) reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row * p.ldh)[col] = float_to_chunk<T>(h).u;
+    }
+    if constexpr (sizeof(T) == 2) {
+      if (p.low) {
+        T* low = static_cast<T*>(p.low) + row * p.lddz;
+        float o_low[E], u_low[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          o_low[e] = rounded_off(o[e]);
+          if (GATED) u_low[e] = rounded_off(u[e]);
+        }
+        reinterpret_cast<uint4*>(low)[col] = float_to_chunk<T>(o_low).u;
+        if (GATED) reinterpret_cast<uint4*>(low + p.N)[col] = float_to_chunk<T>(u_low).u;
+      }
+    }
+  }
+};
+
 template <typename T, int GATED>
 __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
-  constexpr int E = Elem<T>::kPerChunk, MODE = GATED ? kGatedBwd : kLinBwd;
+  constexpr int E = Elem<T>::kPerChunk;
   with_activation(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * kAtOnce);
     for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * kAtOnce) + threadIdx.x; base < p.chunks; base += stride) {
-      Chunk dy[kAtOnce], zg[kAtOnce], zu[kAtOnce];
+      ActBwdChunks<T, GATED> c[kAtOnce];
       uint32_t row[kAtOnce], col[kAtOnce];
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
         const uint64_t q = base + 256 * i;
         if (q >= p.chunks) break;
         p.div.divmod(static_cast<uint32_t>(q), row[i], col[i]);
-        dy[i].u = load_streaming_u4(static_cast<const T*>(p.dy) + row[i] * p.lddy, col[i]);
-        zg[i].u = load_streaming_u4(static_cast<const T*>(p.z) + row[i] * p.ldz, col[i]);
-        if (GATED) zu[i].u = load_streaming_u4(static_cast<const T*>(p.z) + row[i] * p.ldz + p.N, col[i]);
+        c[i].request(p, row[i], col[i]);
       }
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
         if (base + 256 * i >= p.chunks) break;
-        float v[E], fg[E], fu[E], u[E], o[E], h[E];
-        chunk_to_float<T>(dy[i], v);
-        chunk_to_float<T>(zg[i], fg);
-        if (GATED) chunk_to_float<T>(zu[i], fu);
-        combine<T, MODE, ACT, E>(v, u, fg, fu, o, h);
-        T* dz = static_cast<T*>(p.dz) + row[i] * p.lddz;
-        reinterpret_cast<uint4*>(dz)[col[i]] = float_to_chunk<T>(o).u;
-        if (GATED) {
-          reinterpret_cast<uint4*>(dz + p.N)[col[i]] = float_to_chunk<T>(u).u;
-          if (p.h) reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row[i] * p.ldh)[col[i]] = float_to_chunk<T>(h).u;
-        }
-        if constexpr (sizeof(T) == 2) {
-          if (p.low) {
-            T* low = static_cast<T*>(p.low) + row[i] * p.lddz;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-              o[e] = rounded_off(o[e]);
-              if (GATED) u[e] = rounded_off(u[e]);
-            }
-            reinterpret_cast<uint4*>(low)[col[i]] = float_to_chunk<T>(o).u;
-            if (GATED) reinterpret_cast<uint4*>(low + p.N)[col[i]] = float_to_chunk<T>(u).u;
-          }
-        }
+        float o[E], u[E];
+        c[i].template finish<ACT>(p, row[i], col[i], o, u);
       }
     }
   });
+}
+
+// The same with the column sums of the unrounded gradients, which are the bias gradient: added up from their rounded parts they would be as far off
+// as the parts (8192 rows: 2.5e-6 of the result; this way 1.1e-7).  A workgroup has a block of rows and 2^lanes_log chunks of columns; a thread walks down the
+// rows of its chunk, the threads of a column meet in LDS in their order, and the row blocks' sums are added up by a second launch.
+template <typename T, int GATED>
+__global__ __launch_bounds__(256) void act_bwd_sum_kernel(ActBwdArgs p) {
+  constexpr int E = Elem<T>::kPerChunk, PARTS = GATED ? 2 : 1;
+  __shared__ float meet[PARTS][256 * E];
+  const int lanes = 1 << p.lanes_log, lane = threadIdx.x & (lanes - 1), line = threadIdx.x >> p.lanes_log, lines = 256 >> p.lanes_log;
+  const int col = blockIdx.x * lanes + lane;
+  const int64_t row0 = blockIdx.y * p.block_rows, behind = min(row0 + p.block_rows, p.M);
+  float sum[PARTS][E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) sum[0][e] = sum[PARTS - 1][e] = 0.f;
+  with_activation(p.act, [&](auto act_c) {
+    constexpr int ACT = decltype(act_c)::value;
+    if (col < p.row_chunks)
+      for (int64_t base = row0 + line; base < behind; base += kAtOnce * lines) {
+        ActBwdChunks<T, GATED> c[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+          if (base + i * lines < behind) c[i].request(p, base + i * lines, col);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          if (base + i * lines >= behind) break;
+          float o[E], u[E];
+          c[i].template finish<ACT>(p, base + i * lines, col, o, u);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            sum[0][e] += o[e];
+            if (GATED) sum[PARTS - 1][e] += u[e];
+          }
+        }
+      }
+  });
+  // [line][column] of the workgroup: thread t adds up columns t, t + 256, ...
+#pragma unroll
+  for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+    for (int e = 0; e < E; ++e) meet[part][(line * lanes + lane) * E + e] = sum[part][e];
+  __syncthreads();
+  const int cols = lanes * E, first = blockIdx.x * cols;
+#pragma unroll
+  for (int part = 0; part < PARTS; ++part)
+    for (int c = threadIdx.x; c < cols && first + c < p.N; c += 256) {
+      float s = 0.f;
+      for (int l = 0; l < lines; ++l) s += meet[part][l * cols + c];
+      float* to = p.sums + blockIdx.y * static_cast<int64_t>(PARTS * p.N) + part * p.N + first + c;
+      *to = p.add ? *to + s : s;
+    }
+}
+
+// dbias (+)= the sum of the row blocks' sums: 32 columns a workgroup, eight threads a column, in a fixed order
+struct BiasSumArgs {
+  const float* sums;
+  float* out;
+  int blocks, cols, add;
+};
+__global__ __launch_bounds__(256) void act_bwd_bias_kernel(BiasSumArgs p) {
+  __shared__ double meet[8][32];
+  const int lane = threadIdx.x & 31, line = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+  double s = 0.0;
+  if (col < p.cols) {
+#pragma unroll 8
+    for (int b = line; b < p.blocks; b += 8) s += p.sums[static_cast<int64_t>(b) * p.cols + col];
+  }
+  meet[line][lane] = s;
+  __syncthreads();
+  if (line != 0 || col >= p.cols) return;
+#pragma unroll
+  for (int l = 1; l < 8; ++l) s += meet[l][lane];
+  p.out[col] = p.add ? static_cast<float>(p.out[col] + s) : static_cast<float>(s);
+}
+
+// How the rows of a derivative pass with column sums are cut: enough workgroups for the chip, kAtOnce rows a thread at least.  `split`: there is a
+// workspace for the row blocks' sums; without it a workgroup has all rows, of one 128-byte line's columns.
+struct RowBlocks {
+  int lanes_log, col_blocks, blocks;
+  int64_t rows;
+};
+constexpr int kSumGroups = 1024;
+RowBlocks row_blocks(int64_t M, int row_chunks, bool split) {
+  RowBlocks r{split ? 6 : 3, 0, 1, M};
+  while (r.lanes_log > 0 && (1 << (r.lanes_log - 1)) >= row_chunks) --r.lanes_log;
+  r.col_blocks = (row_chunks + (1 << r.lanes_log) - 1) >> r.lanes_log;
+  if (!split) return r;
+  const int64_t lines = 256 >> r.lanes_log, want = std::max(kSumGroups / r.col_blocks, 1);
+  const int64_t each = std::max((M + want - 1) / want, kAtOnce * lines);
+  r.rows = (each + lines - 1) / lines * lines;
+  r.blocks = static_cast<int>((M + r.rows - 1) / r.rows);
+  return r;
 }
 
 // a tensor [M][width] with rows ld elements apart: aligned for 16-byte accesses, and within reach of a tile's 32-bit offsets
@@ -190,31 +304,64 @@ int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, 
   return linear_launch(ctx, "linear_dgrad_gated", dtype, kGatedBwd, a, M, K, F);
 }
 
+int64_t act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int gated) {
+  if ((dtype != kBF16 && dtype != kF32) || M <= 0 || N <= 0 || M > INT_MAX || N > INT_MAX) return 0;
+  const int E = dtype == kBF16 ? 8 : 4;
+  if (N % E != 0) return 0;   // no layer: the call is refused
+  const RowBlocks r = row_blocks(M, static_cast<int>(N / E), true);
+  return r.blocks > 1 ? r.blocks * N * (gated ? 2 : 1) * 4 : 0;
+}
+
 int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, void* dz_low, const Rows& h, int gated, int act, int64_t M,
-            int64_t N) {
+            int64_t N, float* dbias, int accumulate, void* workspace, int64_t workspace_bytes) {
   if (int rc = check_common("act_bwd", dtype, M, 16, N, act)) return rc;
   TCH_CHECK_ARG(dtype == kBF16 || !dz_low, "act_bwd: fp32 gradients are not rounded: there is no low part");
-  if (M == 0) return 0;
-  const int eb = dtype == kBF16 ? 2 : 4;
   const int64_t wide = gated ? 2 : 1;
+  if (M == 0) return dbias && !accumulate ? fill_zero(ctx, dbias, wide * N * 4) : 0;
+  const int eb = dtype == kBF16 ? 2 : 4;
   TCH_CHECK_ARG(dy.ptr && pre.ptr && dz.ptr, "act_bwd: null tensor");
   TCH_CHECK_ARG(rows_fit(dy.ptr, dy.ld, N, eb) && rows_fit(pre.ptr, pre.ld, wide * N, eb) && rows_fit(dz.ptr, dz.ld, wide * N, eb) &&
                     rows_fit(h.ptr, h.ld, N, eb) && rows_fit(dz_low, dz.ld, wide * N, eb),
                 "act_bwd: rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
+  TCH_CHECK_ARG(((reinterpret_cast<uintptr_t>(dbias) | reinterpret_cast<uintptr_t>(workspace)) & 3) == 0,
+                "act_bwd: dbias and the workspace must start on a 4-byte boundary");
+  const int row_chunks = static_cast<int>(N * eb / 16);
+  TCH_CHECK_ARG(M * row_chunks < (1ll << 31), "act_bwd: tensor exceeds 2^31 chunks");
+  const RowBlocks cut = row_blocks(M, row_chunks, workspace != nullptr);
+  const int64_t sums_bytes = dbias && cut.blocks > 1 ? cut.blocks * wide * N * 4 : 0;
+  TCH_CHECK_ARG(sums_bytes <= (workspace ? workspace_bytes : 0), "act_bwd: workspace too small");
   const Span in[2] = {{dy.ptr, dy.ld * eb, N * eb, M}, {pre.ptr, pre.ld * eb, wide * N * eb, M}};
-  const Span out[3] = {{dz.ptr, dz.ld * eb, wide * N * eb, M}, {h.ptr, h.ld * eb, N * eb, M}, {dz_low, dz.ld * eb, wide * N * eb, M}};
-  for (int o = 0; o < 3; ++o) {
+  const Span out[5] = {{dz.ptr, dz.ld * eb, wide * N * eb, M}, {h.ptr, h.ld * eb, N * eb, M}, {dz_low, dz.ld * eb, wide * N * eb, M},
+                       {dbias, wide * N * 4, wide * N * 4, 1}, {workspace, sums_bytes, sums_bytes, sums_bytes ? 1 : 0}};
+  for (int o = 0; o < 5; ++o) {
     bool ok = apart(out[o], in[0], o == 0) && apart(out[o], in[1], o == 0);
     for (int i = 0; i < o; ++i) ok = ok && apart(out[o], out[i]);
     TCH_CHECK_ARG(ok, "act_bwd: an output overlaps another tensor (the gradient may be the one it is made of, or the pre-activations)");
   }
-  const int row_chunks = static_cast<int>(N * eb / 16);
-  TCH_CHECK_ARG(M * row_chunks < (1ll << 31), "act_bwd: tensor exceeds 2^31 chunks");
   ActBwdArgs a{dy.ptr, pre.ptr, dz.ptr, h.ptr, dz_low, dy.ld, pre.ld, dz.ld, h.ld, static_cast<uint32_t>(M * row_chunks), row_chunks, static_cast<int>(N), act,
                FastDiv(static_cast<uint32_t>(row_chunks))};
+  const double bytes = static_cast<double>(M) * N * eb * ((gated ? (h.ptr ? 6.0 : 5.0) : 3.0) + (dz_low ? wide : 0));
+  if (dbias) {
+    const bool split = cut.blocks > 1;
+    a.sums = split ? static_cast<float*>(workspace) : dbias;
+    a.M = M, a.block_rows = cut.rows;
+    a.lanes_log = cut.lanes_log;
+    a.add = accumulate && !split;
+    const dim3 blocks(static_cast<unsigned>(cut.col_blocks), static_cast<unsigned>(cut.blocks));
+    int rc;
+    if (gated)
+      rc = dtype == kBF16 ? launch(ctx, act_bwd_sum_kernel<bf16, 1>, blocks, dim3(256), a, "act_bwd_sum_kernel<bf16,gated>", bytes, 1)
+                          : launch(ctx, act_bwd_sum_kernel<float, 1>, blocks, dim3(256), a, "act_bwd_sum_kernel<f32,gated>", bytes, 1);
+    else
+      rc = dtype == kBF16 ? launch(ctx, act_bwd_sum_kernel<bf16, 0>, blocks, dim3(256), a, "act_bwd_sum_kernel<bf16>", bytes, 1)
+                          : launch(ctx, act_bwd_sum_kernel<float, 0>, blocks, dim3(256), a, "act_bwd_sum_kernel<f32>", bytes, 1);
+    if (rc || !split) return rc;
+    const int cols = static_cast<int>(wide * N);
+    BiasSumArgs b{a.sums, dbias, cut.blocks, cols, accumulate};
+    return launch(ctx, act_bwd_bias_kernel, dim3(static_cast<unsigned>((cols + 31) / 32)), dim3(256), b, "act_bwd_bias_kernel", 4.0 * cut.blocks * cols, 1);
+  }
   const int64_t groups = (M * row_chunks + 256 * kAtOnce - 1) / (256 * kAtOnce);
   const dim3 grid(static_cast<unsigned>(groups < (1 << 20) ? groups : (1 << 20)));
-  const double bytes = static_cast<double>(M) * N * eb * ((gated ? (h.ptr ? 6.0 : 5.0) : 3.0) + (dz_low ? wide : 0));
   if (gated)
     return dtype == kBF16 ? launch(ctx, act_bwd_kernel<bf16, 1>, grid, dim3(256), a, "act_bwd_kernel<bf16,gated>", bytes, 1)
                           : launch(ctx, act_bwd_kernel<float, 1>, grid, dim3(256), a, "act_bwd_kernel<f32,gated>", bytes, 1);

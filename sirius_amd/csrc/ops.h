@@ -201,8 +201,9 @@ int gated_linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, cons
                      int64_t K, int64_t F);
 int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, const Rows& pre, const Rows& dpre, void* dpre_low, const Rows& h,
                        void* h_low, int act, int64_t M, int64_t K, int64_t F);
+int64_t act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int gated);
 int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, void* dz_low, const Rows& h, int gated, int act, int64_t M,
-            int64_t N);
+            int64_t N, float* dbias = nullptr, int accumulate = 0, void* workspace = nullptr, int64_t workspace_bytes = 0);
 
 // linear_wgrad.hip -- weight and bias gradients of bf16 linear layers, of an operand and its low part on request
 int64_t linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N);

@@ -1007,14 +1007,28 @@ def _low(ctx, name, low, high):
     return ctypes.c_void_p(low.data_ptr())
 
 
-def act_bwd(ctx, dy, pre, dz, act, dz_low=None):
-    """dz = dy . act'(pre), element by element; dz may be dy or pre.  dz_low (bf16): what rounding took off dz, for linear_wgrad."""
+def act_bwd_workspace_bytes(dy, gated=False):
+    """Bytes of workspace that act_bwd (gated_act_bwd) wants for the bias gradient behind dy [..., N]."""
+    N = dy.shape[-1]
+    return int(lib().tch_act_bwd_workspace_bytes(dtype_code(dy), dy.numel() // N, N, int(gated)))
+
+
+def _sums(ctx, name, dbias, numel, workspace):
+    assert workspace is None or workspace.device == ctx.stream.device, "workspace: on the context's device"
+    return _vector(ctx, name, dbias, numel), _p(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def act_bwd(ctx, dy, pre, dz, act, dz_low=None, dbias=None, accumulate=False, workspace=None):
+    """dz = dy . act'(pre), element by element; dz may be dy or pre.  dz_low (bf16): what rounding took off dz, for linear_wgrad and
+    linear_dgrad.  dbias [N] fp32 (+)= column sums of dz before it is rounded; workspace for it: act_bwd_workspace_bytes (without it
+    the rows are not split over workgroups)."""
     N = dy.shape[-1]
     dyp, lddy, M = _matrix(ctx, "dy", dy, N)
     pp, ldp, _ = _matrix(ctx, "pre", pre, N, M, dy.dtype)
     dzp, lddz, _ = _matrix(ctx, "dz", dz, N, M, dy.dtype)
-    check(lib().tch_act_bwd(ctx.handle, dtype_code(dy), dyp, lddy, pp, ldp, dzp, _low(ctx, "dz_low", dz_low, dz), lddz, _act_code(act), M, N),
-          "tch_act_bwd")
+    sums, ws, ws_bytes = _sums(ctx, "dbias", dbias, N, workspace)
+    check(lib().tch_act_bwd_bias(ctx.handle, dtype_code(dy), dyp, lddy, pp, ldp, dzp, _low(ctx, "dz_low", dz_low, dz), lddz, sums, int(accumulate),
+                                 _act_code(act), M, N, ws, ws_bytes), "tch_act_bwd_bias")
 
 
 def _wgrad_blocks(rows, K, N, element):
@@ -1035,7 +1049,9 @@ def linear_bwd_workspace_bytes(x, N):
     K = x.shape[-1]
     M = x.numel() // K
     if x.dtype == torch.bfloat16:
-        return max(int(lib().tch_linear_wgrad_workspace_bytes(M, K, N)), 4)
+        # one after the other: the bias gradient's sums (of either form of the derivative), the weight gradient's parts
+        sums = [int(lib().tch_act_bwd_workspace_bytes(dtype_code(x), M, N // (1 + gated), gated)) for gated in (0, 1)]
+        return max(int(lib().tch_linear_wgrad_workspace_bytes(M, K, N)), *sums, 4)
     blocks = {rows for _, rows in _wgrad_blocks(M, K, N, x.element_size())}
     return max([conv2d_wgrad_workspace_bytes(dtype_code(x), N, 1, 1, K, _wgrad_splits(x, K, N, rows)) for rows in blocks] + [4])
 
@@ -1069,20 +1085,30 @@ def linear_wgrad(ctx, x, dy, dw, dbias=None, accumulate=False, workspace=None, d
                      dbias=dbias)
 
 
+def _sums_ahead(dy):
+    """Whether the bias gradient of a layer with an activation is added up where the derivative is taken.  bf16: there the gradient is not
+    rounded yet.  fp32 gradients are not rounded, and the weight gradient adds them up on its way without a launch more."""
+    return dy.dtype == torch.bfloat16
+
+
 def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=None, residual=None, accumulate=False, workspace=None,
                dpre_low=None, dy_low=None, x_low=None):
     """The gradients of linear_fwd: dpre = dy . act'(pre) (act "none": dy itself, and dpre stays untouched), dx = dpre w + residual,
     dw (+)= dpre^T x and dbias (+)= column sums of dpre, both fp32.  The residual's own gradient is dy.  dx (with wt) or dw may be
     None.  x and the gradient it meets are contiguous; workspace: linear_bwd_workspace_bytes (without it the weight gradient
-    is not split over its rows).  bf16: dpre is rounded (2^-8 of each element at most), and dx, dw and dbias are those of the rounded
-    one, except where dpre_low (like dpre) keeps what rounding takes off it: all three are then those of the unrounded dpre (2^-16), in
-    twice the products.  dy_low (the low part of dy, act "none") does the same for all three, x_low (the low part of x) for dw."""
+    is not split over its rows).  bf16: dpre is rounded (2^-8 of each element at most), and dx and dw are those of the rounded one,
+    except where dpre_low (like dpre) keeps what rounding takes off it: both are then those of the unrounded dpre (2^-16), in twice the
+    products; behind an activation dbias is that of the unrounded dpre either way.  dy_low (the low part of dy, act "none") does the
+    same for dx, dw and dbias, x_low (the low part of x) for dw."""
     N = dy.shape[-1]
+    assert dw is not None or dbias is None, "dbias comes with dw"
     g, low = dy, dy_low
     if act != "none":
         assert pre is not None and dpre is not None, "an activation's derivative needs pre, and dpre to keep its result"
         assert dy_low is None, "dy_low goes with a gradient that is multiplied as it is"
-        act_bwd(ctx, dy, pre, dpre, act, dz_low=dpre_low)
+        here = dbias if _sums_ahead(dy) else None
+        act_bwd(ctx, dy, pre, dpre, act, dz_low=dpre_low, dbias=here, accumulate=accumulate, workspace=workspace if here is not None else None)
+        dbias = None if here is not None else dbias
         g, low = dpre, dpre_low
     if dx is not None:
         linear_dgrad(ctx, g, wt, dx, residual=residual, dy_low=low)
@@ -1090,8 +1116,6 @@ def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=No
         assert residual is None, "a residual without dx"
     if dw is not None:
         linear_wgrad(ctx, x, g, dw, dbias=dbias, accumulate=accumulate, workspace=workspace, dy_low=low, x_low=x_low)
-    else:
-        assert dbias is None, "dbias comes with dw"
 
 
 def gated_linear_fwd(ctx, x, w, h, bias=None, act="silu", pre=None):
@@ -1108,16 +1132,17 @@ def gated_linear_fwd(ctx, x, w, h, bias=None, act="silu", pre=None):
                                      _vector(ctx, "bias", bias, F2), _act_code(act), pp, ldp, M, K, F), "tch_gated_linear_fwd")
 
 
-def gated_act_bwd(ctx, dh, pre, dpre, act="silu", h=None, dpre_low=None):
+def gated_act_bwd(ctx, dh, pre, dpre, act="silu", h=None, dpre_low=None, dbias=None, accumulate=False, workspace=None):
     """dpre = (dh . u . act'(g) | dh . act(g)) from pre = (g | u), element by element; h = act(g) . u again.  dpre may be pre.
-    dpre_low (bf16): what rounding took off dpre, for linear_wgrad."""
+    dpre_low, dbias [2F], workspace: as for act_bwd."""
     F = dh.shape[-1]
     dhp, lddh, M = _matrix(ctx, "dh", dh, F)
     pp, ldp, _ = _matrix(ctx, "pre", pre, 2 * F, M, dh.dtype)
     dpp, lddp, _ = _matrix(ctx, "dpre", dpre, 2 * F, M, dh.dtype)
     hp, ldh, _ = _matrix(ctx, "h", h, F, M, dh.dtype)
-    check(lib().tch_gated_act_bwd(ctx.handle, dtype_code(dh), dhp, lddh, pp, ldp, dpp, _low(ctx, "dpre_low", dpre_low, dpre), lddp, hp, ldh,
-                                  _act_code(act), M, F), "tch_gated_act_bwd")
+    sums, ws, ws_bytes = _sums(ctx, "dbias", dbias, 2 * F, workspace)
+    check(lib().tch_gated_act_bwd_bias(ctx.handle, dtype_code(dh), dhp, lddh, pp, ldp, dpp, _low(ctx, "dpre_low", dpre_low, dpre), lddp, hp, ldh,
+                                       sums, int(accumulate), _act_code(act), M, F, ws, ws_bytes), "tch_gated_act_bwd_bias")
 
 
 def linear_dgrad_gated(ctx, dy, wt, pre, dpre, act="silu", h=None, dpre_low=None, h_low=None):
@@ -1138,8 +1163,10 @@ def linear_dgrad_gated(ctx, dy, wt, pre, dpre, act="silu", h=None, dpre_low=None
 def gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=None, act="silu", residual=None, accumulate=False, workspace=None, dpre_low=None):
     """The gradients of gated_linear_fwd from dh [..., F]: dpre [..., 2F] as in gated_act_bwd, dx = dpre w + residual,
     dw (+)= dpre^T x, dbias (+)= column sums of dpre.  wt [K, 2F] is w transposed; dpre_low and the rest as for linear_bwd."""
-    gated_act_bwd(ctx, dh, pre, dpre, act, dpre_low=dpre_low)
-    linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=dbias, residual=residual, accumulate=accumulate, workspace=workspace, dy_low=dpre_low)
+    assert dw is not None or dbias is None, "dbias comes with dw"
+    here = dbias if _sums_ahead(dh) else None
+    gated_act_bwd(ctx, dh, pre, dpre, act, dpre_low=dpre_low, dbias=here, accumulate=accumulate, workspace=workspace if here is not None else None)
+    linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=None if here is not None else dbias, residual=residual, accumulate=accumulate, workspace=workspace, dy_low=dpre_low)
 
 
 def attn_softmax_fwd(ctx, scores, probs, scale=1.0, bias=None, mask=None, causal=False):
