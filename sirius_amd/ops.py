@@ -1085,10 +1085,11 @@ def linear_wgrad(ctx, x, dy, dw, dbias=None, accumulate=False, workspace=None, d
                      dbias=dbias)
 
 
-def _sums_ahead(dy):
+def _sums_ahead(dy, workspace):
     """Whether the bias gradient of a layer with an activation is added up where the derivative is taken.  bf16: there the gradient is not
-    rounded yet.  fp32 gradients are not rounded, and the weight gradient adds them up on its way without a launch more."""
-    return dy.dtype == torch.bfloat16
+    rounded yet.  fp32 gradients are not rounded, and the weight gradient adds them up on its way without a launch more; so it does
+    without a workspace, where a pass that does not split its rows would take as long again."""
+    return dy.dtype == torch.bfloat16 and workspace is not None
 
 
 def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=None, residual=None, accumulate=False, workspace=None,
@@ -1098,7 +1099,7 @@ def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=No
     None.  x and the gradient it meets are contiguous; workspace: linear_bwd_workspace_bytes (without it the weight gradient
     is not split over its rows).  bf16: dpre is rounded (2^-8 of each element at most), and dx and dw are those of the rounded one,
     except where dpre_low (like dpre) keeps what rounding takes off it: both are then those of the unrounded dpre (2^-16), in twice the
-    products; behind an activation dbias is that of the unrounded dpre either way.  dy_low (the low part of dy, act "none") does the
+    products; behind an activation and with a workspace dbias is that of the unrounded dpre either way.  dy_low (the low part of dy, act "none") does the
     same for dx, dw and dbias, x_low (the low part of x) for dw."""
     N = dy.shape[-1]
     assert dw is not None or dbias is None, "dbias comes with dw"
@@ -1106,8 +1107,8 @@ def linear_bwd(ctx, dy, x, wt, dx, dw, dbias=None, act="none", pre=None, dpre=No
     if act != "none":
         assert pre is not None and dpre is not None, "an activation's derivative needs pre, and dpre to keep its result"
         assert dy_low is None, "dy_low goes with a gradient that is multiplied as it is"
-        here = dbias if _sums_ahead(dy) else None
-        act_bwd(ctx, dy, pre, dpre, act, dz_low=dpre_low, dbias=here, accumulate=accumulate, workspace=workspace if here is not None else None)
+        here = dbias if _sums_ahead(dy, workspace) else None
+        act_bwd(ctx, dy, pre, dpre, act, dz_low=dpre_low, dbias=here, accumulate=accumulate, workspace=workspace)
         dbias = None if here is not None else dbias
         g, low = dpre, dpre_low
     if dx is not None:
@@ -1164,8 +1165,8 @@ def gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=None, act="silu", 
     """The gradients of gated_linear_fwd from dh [..., F]: dpre [..., 2F] as in gated_act_bwd, dx = dpre w + residual,
     dw (+)= dpre^T x, dbias (+)= column sums of dpre.  wt [K, 2F] is w transposed; dpre_low and the rest as for linear_bwd."""
     assert dw is not None or dbias is None, "dbias comes with dw"
-    here = dbias if _sums_ahead(dh) else None
-    gated_act_bwd(ctx, dh, pre, dpre, act, dpre_low=dpre_low, dbias=here, accumulate=accumulate, workspace=workspace if here is not None else None)
+    here = dbias if _sums_ahead(dh, workspace) else None
+    gated_act_bwd(ctx, dh, pre, dpre, act, dpre_low=dpre_low, dbias=here, accumulate=accumulate, workspace=workspace)
     linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=None if here is not None else dbias, residual=residual, accumulate=accumulate, workspace=workspace, dy_low=dpre_low)
 
 

@@ -67,7 +67,7 @@ def test_whole_numbers(ctx, M, N, dtype):
 @pytest.mark.parametrize("with_low", [True, False], ids=["low", "rounded"])
 @pytest.mark.parametrize("M,K,N", [(1023, 64, 2736), (2000, 72, 520), (4096, 64, 1024)])
 def test_backward_passes(ctx, M, K, N, with_low):
-    """linear_bwd and gated_linear_bwd in bf16: dbias is that of the unrounded gradient, whether dw is or not."""
+    """linear_bwd and gated_linear_bwd in bf16, with a workspace: dbias is that of the unrounded gradient, whether dw is or not."""
     from sirius_amd import ops
     x, w = rnd(M, K, dtype=BF16, seed=1), rnd(2 * N, K, dtype=BF16, seed=2, std=1 / math.sqrt(K))
     dy, pre = rnd(M, N, dtype=BF16, seed=3), rnd(M, 2 * N, dtype=BF16, seed=4, std=0.5)

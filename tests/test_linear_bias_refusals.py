@@ -48,7 +48,7 @@ def test_rows_are_cut_for_the_chip(rec, dtype, gated):  # noqa: F811
             name, groups, _ = launches[0]
             assert name.startswith("act_bwd_sum_kernel")
             chunks = N // E
-            lanes = min(1 << max(chunks - 1, 0).bit_length(), 64 if ws else 8)
+            lanes = min(1 << max(chunks - 1, 0).bit_length(), 32 if ws else 8)
             col_blocks = -(-chunks // lanes)
             blocks = groups // col_blocks
             assert groups == col_blocks * blocks and blocks <= 1024
