@@ -474,7 +474,7 @@ int tch_linear_dgrad_low(tch_context* ctx, int dtype, const void* dy, const void
  * dgrad_gated: dh = dy w (wt [F][K] the down projection's weight transposed, dy [M][K]) goes straight into
  * dpre [M][2F] = (dh . u . act'(g) | dh . act(g)); h (may be NULL) [M][F] = act(g) . u again.  dpre may be pre itself.
  * dpre_low, h_low (bf16, may be NULL; laid out like dpre and h): what rounding took off.  A weight gradient of a bf16
- * gradient and its low part is that of the unrounded gradient, each element to 2^-18 of its size. */
+ * gradient and its low part is that of the unrounded gradient, each element to 2^-16 of its size (2.5e-6 of the result). */
 int tch_gated_linear_fwd(tch_context* ctx, int dtype, const void* x, int64_t ldx, const void* w, void* h, int64_t ldh,
                          const float* bias, int act, void* pre, int64_t ldp, int64_t M, int64_t K, int64_t F);
 int tch_linear_dgrad_gated(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* wt, const void* pre,

@@ -5,7 +5,8 @@
 // LOW: a data gradient of bf16 gradients that come with what rounding took off them, or one that keeps what rounding takes off its own.  The product of the rounded gradient alone has an error of its
 // own of about 2^-9.3 of dx, next to the 2^-9.3 of rounding dx.  The reduction is walked twice, over a and then over its low part, into the
 // same accumulators: a tile's steps are twice as many, and so is its time where the multiplies bound it (8192 x 2048 over 11264 293 us, with the
-// low part of a 563; 8192 x 1024 over 4096 59 and 118; 392 x 512 over 2048 5.4 and 8.5).
+// low part of a 551-566; 8192 x 1024 over 4096 59 and 117; 1023 x 1024 over 5472 25 and 45).  A low part that is stored: 8192 x 4096 over 1024
+// through GELU 80 and 96.
 //
 // Gated modes multiply both projections in one tile: 32 (in the narrowest tiles 16) rows of the gate's weights lie next to the same rows of the up
 // projection's, so that a lane ends up with both products of its columns and the epilogue needs nobody else's.
@@ -94,7 +95,7 @@ struct ChunkOperands {
       if (p.add) add = read_chunk(t.add, at<T>(row, p.ldadd, col, ok));
   }
   // STREAM: forward outputs go past L2 (non-temporal) and leave it to the operands: the tile kernel, 8192 x 4096 over 1024 with the kept
-  // pre-activation 80 -> 76 us (the outputs of a gated data gradient that way 292 -> 310)
+  // pre-activation 78 -> 74 us (the outputs of a gated data gradient that way are 6 % slower)
   template <int ACT, bool STREAM>
   __device__ __forceinline__ void finish(const LinearArgs& p, const TileTensors& t, int row, int col, const float* v, float* u) {
     constexpr int E = Elem<T>::kPerChunk, AUX = STREAM && (MODE == kLinFwd || MODE == kGatedFwd) ? 2 : 0;
@@ -166,10 +167,10 @@ __device__ inline void mma32(const uint4_t& first, const uint4_t& second, f32x16
 // steps ahead go out between the multiplies.  The tiles of a workgroup are one sequence: the next tile's first loads are on
 // their way during this tile's last steps and its epilogue.  A row of the operands that does not exist is outside its buffer
 // resource and lands as zeros; a chunk behind K is turned away by its lane's offset in the last step of a tile.
-// Measured: gated forward 16384 x 11008 over 4096 2.18-2.21 ms, 1.34-1.36 PFLOP/s, bound by power (matrix pipes 79 % busy; a large library
-// product 1.33-1.37); data gradient 8192 x 2048 over 11264 292 us, 1.29.  Where the reduction is short the epilogue counts, in which the
-// matrix pipes stand: forward 8192 x 4096 over 1024 with GELU and the kept pre-activation 75 us, about 25 of them epilogue (134 MB written);
-// the gated data gradient 8192 x 5632 over 2048 with its low parts 287 us, half of them (740 MB at 5.5 TB/s).  fp32 4096 x 4096 over 1024: 264 us, 0.130 of 0.157 PFLOP/s.
+// Measured: gated forward 16384 x 11008 over 4096 2.12-2.27 ms, 1.30-1.39 PFLOP/s, bound by power (matrix pipes 79 % busy; a library product
+// of this size 1.35); data gradient 8192 x 2048 over 11264 293 us, 1.29.  Where the reduction is short the epilogue counts, in which the
+// matrix pipes stand: forward 8192 x 4096 over 1024 with GELU and the kept pre-activation 72-74 us, about 25 of them epilogue (134 MB written);
+// the gated data gradient 8192 x 5632 over 2048 with its low parts 287-293 us, half of them (740 MB at 5.5 TB/s).  fp32 4096 x 4096 over 1024: 247 us, 0.139 of 0.157 PFLOP/s.
 template <typename T, int MODE, bool LOW, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), RB = 128;
@@ -504,7 +505,7 @@ __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_tile_k
 // only: no barrier before the partial tiles meet in LDS, where they are added in the order of the wavefronts.  What that buys
 // where workgroups are few: KG * (NBUF - 1) operand tiles in flight per compute unit and a chain of nk / KG steps instead of nk.
 // Bound by the bytes of the weights where there are many (7 rows through 2048 -> 2 x 5632 gated: 9.3 us, 5.0 TB/s; 32 through 8192 -> 8192:
-// 23 us, 5.8 TB/s), by the latency of a chain of steps where there are few.
+// 23.6 us, 5.7 TB/s), by the latency of a chain of steps where there are few.
 template <typename T, int MODE, bool LOW, int TM, int TN, int KG, int NBUF, int RB>
 __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
   constexpr int E = Elem<T>::kPerChunk, EB = sizeof(T), KS = RB / EB, SL = RB / 32, SLOTS = RB / 16, LD_ROWS = 1024 / RB;
@@ -694,7 +695,7 @@ __global__ __launch_bounds__(KG * 64) void linear_split_kernel(LinearArgs p) {
 // chunk l / 16 (of four) of row l % 16, so that a load covers 64 neighbouring bytes of sixteen rows.  The next piece is
 // requested before this one is multiplied.  Up to 16 rows it is bound by the bytes of the weights; beyond, by what a compute unit
 // loads into registers (32 or 64 rows a workgroup, for fewer loads of the weights, were slower throughout, and so were gate and up tiles
-// next to each other against 32 x 32 tiles with a ring in LDS).  One token through 4096 x 4096 bf16: 7.6 us, 4.4 TB/s.
+// next to each other against 32 x 32 tiles with a ring in LDS).  One token through 4096 x 4096 bf16: 7.4 us, 4.5 TB/s.
 template <typename T>
 __device__ inline void mma16(const uint4_t& first, const uint4_t& second, f32x4_t& acc) {
   if constexpr (sizeof(T) == 2) {
@@ -869,7 +870,7 @@ int launch_linear_tile(Context* ctx, LinearArgs& a) {
   a.div_group = FastDiv(static_cast<uint32_t>(a.group_rows > 1 ? a.group_rows * a.tiles_n : 1));
   a.div_rows = FastDiv(a.group_rows > 1 ? a.group_rows : 1);
   // bf16: the workgroups that the chip holds walk the tiles.  fp32 tiles take so long that their number per compute unit is what
-  // counts: a workgroup per tile, and who is done makes room (768 x 6216 over 3480: 319 us, walked 411)
+  // counts: a workgroup per tile, and who is done makes room (768 x 6216 over 3480: 308 us, walked 404)
   const int64_t most = sizeof(T) == 2 ? 256 * PER_CU : tiles;
   const unsigned grid = static_cast<unsigned>(tiles < most ? tiles : most);
   return launch(ctx, linear_tile_kernel<T, MODE, LOW, WM, WN, TM, TN, NBUF, PER_CU>, dim3(grid), dim3(WM * WN * 64), a, name.c_str(),
@@ -906,12 +907,12 @@ int launch_linear_rows(Context* ctx, LinearArgs& a) {
 
 // Which kernel: the one with the shortest estimate, (rounds of workgroups) x (reduction steps of a wavefront x microseconds a step +
 // start and end).  The constants are measured on products of 1-16384 rows, 64-11264 outputs and 256-11104 reduction elements, and
-// take the best kernel or one within 10 % of it for nearly all of them: bf16, M x N over K: 1 x 4096 over 4096 9.1 us with 16-row tiles (10.9
-// as 32 x 32), 17 x 1024 over 4096 7.3 as 32 x 32 (16-row tiles 9.8, 32 x 64 9.5), 512 x 1024 over 8192 23 as 32 x 64 (30 as 64 x 64),
-// 1024 x 1024 over 1024 7.7 as 64 x 64 (9.1 as 128 x 64, 10.8 as 128 x 128), 512 x 4096 over 4096 29 as 128 x 64 (37 as 128 x 128, 38 as
-// 64 x 64, 54 as 256 x 128), 512 x 8192 over 8192 76 as 128 x 128 (102 as 128 x 64, 103 as 256 x 128; 128 x 128 with two buffers 114),
-// 4096 x 4096 over 1024 36 as 256 x 256 (38 as 256 x 128, 40 as 128 x 128).  Gated, 7 rows, 2048 outputs over 8192: 19 as 32 x 32 (32 x 64
-// 25).  fp32: 8 x 4096 over 8192 33 with 16-row tiles (45 as 32 x 32), 768 x 6216 over 3480 319 as 128 x 64 (347 as 64 x 64, 420 as 128 x 128).
+// take the best kernel or one within 10 % of it for nearly all of them: bf16, M x N over K: 1 x 4096 over 4096 7.4 us with 16-row tiles (7.6
+// as 32 x 32), 17 x 1024 over 4096 6.7 as 32 x 32 (16-row tiles 9.2, 32 x 64 8.9), 512 x 1024 over 8192 20 as 32 x 64 (27 as 64 x 64),
+// 1024 x 1024 over 1024 7.9 as 64 x 64 (8.3 as 128 x 64, 10.2 as 128 x 128), 512 x 4096 over 4096 23 as 128 x 64 (25 as 128 x 128, 29 as
+// 64 x 64, 38 as 256 x 128), 512 x 8192 over 8192 73 as 128 x 128 (97 as 128 x 64, 93 as 256 x 128), 4096 x 4096 over 1024 31 as 256 x 256
+// (33 as 256 x 128, 37 as 128 x 128).  Gated, 7 rows, 2048 outputs over 8192: 11.8 as 32 x 32 (32 x 64 15.0).  fp32: 8 x 4096 over 8192 27
+// with 16-row tiles (40 as 32 x 32), 4096 x 4096 over 1024 247 as 128 x 64 (314 as 64 x 64).  (One run of replayed programs on warm operands.)
 enum Kernel : int { kRows16, kSplit32, kSplit32x64, kSplit64, kTile128x64, kTile128, kTile256x128, kTile256, kKernels };
 struct KernelCost {
   int bm, bn;      // tile; gated forward: half as many output columns
@@ -996,8 +997,8 @@ int launch_linear_kernel(Context* ctx, Kernel kernel, LinearArgs& a) {
 }
 
 // Large tiles rarely fill their last round.  Where it is estimated to be shorter by more than the estimate is good for, the rows that
-// fill whole rounds are one launch and the others a second one, with tiles as small as suit them: bf16 9729 x 3456 over 15184 1217 ->
-// 1042 us, fp32 1568 x 4096 over 1024 151 -> 134.
+// fill whole rounds are one launch and the others a second one, with tiles as small as suit them: bf16 9729 x 3456 over 15184 1128 ->
+// 990 us, fp32 1568 x 4096 over 1024 124 -> 103, 768 x 6216 over 3480 297 -> 268.
 constexpr float kSecondLaunchUs = 3.f, kWorthwhile = 0.93f;
 template <typename T, int MODE, bool LOW = false>
 int launch_linear_mode(Context* ctx, LinearArgs& a) {

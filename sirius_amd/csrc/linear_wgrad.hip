@@ -60,8 +60,8 @@ constexpr int kRows = 32;   // of a reduction step
 
 // WM x WN wavefronts of TM x TN MFMA tiles (32 x 32).  NBUF tiles in LDS, one barrier per step; the sixteen-row slice that is multiplied
 // next is read while this one is multiplied, and the direct loads of the step NBUF - 1 ahead go out between the multiplies.
-// 2048 x 11264 over 8192 rows with a low part: 547 us, 1.38 PFLOP/s, which is what the chip's power allows (a large library product:
-// 1.33-1.37); with runs dealt out as they come, 4 GB through L2 in 661 us.  4096 x 1024: 135 us and 18 to add up four parts a tile.
+// 2048 x 11264 over 8192 rows with a low part: 548-576 us, 1.31-1.38 PFLOP/s, which is what the chip's power allows; with runs dealt out as they
+// come, 4 GB through L2 in 661 us.  4096 x 1024: 110-116 us and 17 to add up four parts a tile.
 template <int PAIR, int WM, int WN, int TM, int TN, int NBUF, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU* WM* WN / 4) void linear_wgrad_kernel(LinearWgradArgs p) {
   constexpr int BM = WM * TM * 32, BN = WN * TN * 32, NW = WM * WN;

@@ -697,7 +697,9 @@ def sgd_momentum_step(ctx, param, grad, buf, lr, momentum, weight_decay, shadow=
 class GradTable:
     """Device table of gradient tensors (fp32 or bf16, contiguous, any number and sizes, empty ones too) for grad_norm and
     clip_grad_norm; `out`: tensors of the same sizes that clip_grad_norm writes instead of the gradients themselves.  It holds
-    the tensors' addresses, and the tensors."""
+    the tensors' addresses, and the tensors.  Made on the host, with a copy: 20 us a tensor (148 tensors of 124 million numbers 2.9 ms),
+    for gradients that stay where they are; whoever has new addresses every step pays it every step.  No element may be written
+    twice, so a tensor given twice needs an `out`, for grad_norm too."""
 
     def __init__(self, tensors, out=None):
         tensors = list(tensors)
