@@ -504,6 +504,15 @@ int64_t tch_linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int tch_linear_wgrad(tch_context* ctx, const void* x, const void* x_low, const void* dy, const void* dy_low, float* dw,
                      float* dbias, int accumulate, int64_t M, int64_t K, int64_t N, void* workspace,
                      int64_t workspace_bytes);
+/* Rotary positions: x [rows][heads * head_dim] (rows ldx elements apart) -> y (ldy).  The first rot elements of a head are
+ * rot / 2 pairs, (i, i + rot / 2) or with interleaved (2 i, 2 i + 1); pair i of a row at position p is turned by p freqs[i]
+ * (freqs [rot / 2] in device memory, radians) and multiplied by scale; the other elements are copied.  back: turned back,
+ * which is the gradient.  positions [rows] (wide_positions: int64, else int32) in device memory, or NULL: row r stands at
+ * start + r % seq.  y may be x (rows as far apart); otherwise they may not overlap.  Any alignment of whole elements, whole
+ * 16-byte chunks where heads, halves and rows allow it run fastest. */
+int tch_rotary(tch_context* ctx, int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, const double* freqs,
+               const void* positions, int wide_positions, int64_t start, int64_t seq, int64_t rows, int heads,
+               int head_dim, int rot, int interleaved, float scale, int back);
 /* probs = softmax over the last dimension of scale * scores[batch, heads, Lq, Lk] + bias[heads, Lq, Lk]
  * + mask[windows, Lq, Lk] (window = batch index % windows); bias and mask may be NULL; causal != 0 keeps keys
  * j <= i only (Lq == Lk).  In place (probs == scores) is allowed. */

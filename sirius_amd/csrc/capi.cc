@@ -418,6 +418,12 @@ int tch_linear_wgrad(tch_context* ctx, const void* x, const void* x_low, const v
   return linear_wgrad(C(ctx), x, x_low, dy, dy_low, dw, dbias, accumulate, M, K, N, workspace, workspace_bytes);
 }
 
+int tch_rotary(tch_context* ctx, int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, const double* freqs, const void* positions,
+               int wide_positions, int64_t start, int64_t seq, int64_t rows, int heads, int head_dim, int rot, int interleaved, float scale, int back) {
+  return rotary(C(ctx), dtype, {const_cast<void*>(x), ldx}, {y, ldy}, freqs, positions, wide_positions, start, seq, rows, heads, head_dim, rot,
+                interleaved, scale, back);
+}
+
 int64_t tch_grad_table_piece_elems(void) { return grad_table_piece_elems(); }
 int64_t tch_grad_norm_workspace_bytes(int64_t pieces) { return grad_norm_workspace_bytes(pieces); }
 

@@ -210,6 +210,10 @@ int64_t linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy, const void* dy_low, float* dw, float* dbias, int accumulate, int64_t M,
                  int64_t K, int64_t N, void* workspace, int64_t workspace_bytes);
 
+// rotary.hip -- rotary positions of the heads of queries and keys, and the rotation back
+int rotary(Context* ctx, int dtype, const Rows& x, const Rows& y, const double* freqs, const void* positions, int wide_positions, int64_t start,
+           int64_t seq, int64_t rows, int heads, int head_dim, int rot, int interleaved, float scale, int back);
+
 // grad_norm.hip -- the global norm of many tensors, listed in pieces in device memory, and clipping by it
 int64_t grad_table_piece_elems();
 int64_t grad_norm_workspace_bytes(int64_t pieces);

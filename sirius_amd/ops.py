@@ -8,6 +8,7 @@ filters are [K, R, S, C].
 import bisect
 import contextlib
 import ctypes
+import math
 import time
 
 import torch
@@ -1170,6 +1171,57 @@ def gated_linear_bwd(ctx, dh, x, wt, dx, dw, pre, dpre, dbias=None, act="silu", 
     here = dbias if _sums_ahead(dh, workspace) else None
     gated_act_bwd(ctx, dh, pre, dpre, act, dpre_low=dpre_low, dbias=here, accumulate=accumulate, workspace=workspace)
     linear_bwd(ctx, dpre, x, wt, dx, dw, dbias=None if here is not None else dbias, residual=residual, accumulate=accumulate, workspace=workspace, dy_low=dpre_low)
+
+
+def rotary_freqs(rot, base=10000.0, factor=1.0, trained=None, slow=1.0, fast=32.0):
+    """Radians per position of the rot / 2 pairs of a rotated head, fp64 on the CPU: base^(-2 i / rot).  For contexts `factor` times
+    as long as a model was trained on: without `trained` every pair is slowed down by the factor; with it (that length in tokens)
+    pairs that turn over `fast` times or more within it stay, those that turn over `slow` times or less are slowed down, and in
+    between the one goes over into the other."""
+    if rot <= 0 or rot % 2:
+        raise ValueError("an even number of elements is rotated")
+    if not factor > 0 or not base > 0 or (trained is not None and not (trained > 0 and fast > slow)):
+        raise ValueError("base, factor and trained are positive, fast is above slow")
+    f = torch.pow(torch.tensor(float(base), dtype=torch.float64), -2.0 * torch.arange(rot // 2, dtype=torch.float64) / rot)
+    if trained is None:
+        return f / factor
+    kept = ((trained * f / (2.0 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+    return f * (kept + (1.0 - kept) / factor)
+
+
+def rotary_fwd(ctx, x, y, freqs, head_dim, layout="half", positions=None, start=0, seq=None, scale=1.0):
+    """Rotary positions of every head of x [..., heads * head_dim] (queries and keys side by side in the packed projection are one
+    call), for flash_attn_fwd: the first 2 * freqs.numel() elements of a head are pairs (i, i + half) ("half") or (2 i, 2 i + 1)
+    ("interleaved"); pair i of a row at position p is turned by p * freqs[i] and multiplied by scale, the rest of the head is copied.
+    freqs: rotary_freqs on the GPU.  positions: int32 or int64, one a row, as deep in a cache as they like; None: row r stands at
+    start + r % seq (seq: the second to last size of x).  x and y are rows of any type and alignment, y may be x."""
+    _rotary(ctx, x, y, freqs, head_dim, layout, positions, start, seq, scale, False)
+
+
+def rotary_bwd(ctx, dy, dx, freqs, head_dim, layout="half", positions=None, start=0, seq=None, scale=1.0):
+    """The gradient of rotary_fwd: dx is dy turned back, with the same arguments.  dx may be dy."""
+    _rotary(ctx, dy, dx, freqs, head_dim, layout, positions, start, seq, scale, True)
+
+
+def _rotary(ctx, x, y, freqs, head_dim, layout, positions, start, seq, scale, back):
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"unknown layout {layout!r}: half or interleaved")
+    width = x.shape[-1]
+    assert head_dim > 0 and width % head_dim == 0, f"rows of {width} elements are not whole heads of {head_dim}"
+    xp, ldx, rows = _matrix(ctx, "x", x, width)
+    yp, ldy, _ = _matrix(ctx, "y", y, width, rows, x.dtype)
+    assert freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.device == ctx.stream.device, "freqs: fp64 numbers on the context's device"
+    assert 2 * freqs.numel() <= head_dim, f"{freqs.numel()} pairs in heads of {head_dim} elements"
+    if positions is not None:
+        assert positions.dtype in (torch.int32, torch.int64) and positions.numel() == rows and positions.device == ctx.stream.device, \
+            f"positions: {rows} int32 or int64 numbers"
+        seq = 1
+    elif seq is None:
+        assert x.dim() >= 2, "the length of a sequence"
+        seq = x.shape[-2]
+    check(lib().tch_rotary(ctx.handle, dtype_code(x), xp, ldx, yp, ldy, _p(freqs), _p(positions),
+                           int(positions is not None and positions.dtype == torch.int64), int(start), max(int(seq), 1), rows, width // head_dim,
+                           head_dim, 2 * freqs.numel(), int(layout == "interleaved"), float(scale), int(back)), "tch_rotary")
 
 
 def attn_softmax_fwd(ctx, scores, probs, scale=1.0, bias=None, mask=None, causal=False):
