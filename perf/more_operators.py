@@ -210,9 +210,9 @@ def _record(s, case):
         return None if s[name] is None else torch.empty_like(s[name])
     if op == "rotary":
         y = new(*s["x"].shape)
-        call = ops.rotary_bwd if case["back"] else ops.rotary_fwd
-        calls = [lambda: call(ctx, s["x"], y, s["freqs"], case["head_dim"], layout=case["layout"], positions=s["positions"],
-                              seq=case["tokens"], scale=_rotary_scale(case))]
+        rotary = ops.rotary_bwd if case["back"] else ops.rotary_fwd
+        calls = [lambda: rotary(ctx, s["x"], y, s["freqs"], case["head_dim"], layout=case["layout"], positions=s["positions"],
+                                seq=case["tokens"], scale=_rotary_scale(case))]
         s["out"] = [y]
     elif op == "norm_fwd":
         total, y, stats = new(*s["x"].shape), new(*s["x"].shape), new(s["x"].shape[0], 4, dtype=torch.float32)
