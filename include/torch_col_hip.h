@@ -513,6 +513,39 @@ int tch_linear_wgrad(tch_context* ctx, const void* x, const void* x_low, const v
 int tch_rotary(tch_context* ctx, int dtype, const void* x, int64_t ldx, void* y, int64_t ldy, const double* freqs,
                const void* positions, int wide_positions, int64_t start, int64_t seq, int64_t rows, int heads,
                int head_dim, int rot, int interleaved, float scale, int back);
+/* The boundary between two blocks of a transformer in one pass: total = scale * x + gate . post(branch), y = norm(total).
+ * All tensors [rows][C] with rows ld elements apart (16-byte boundaries; C at most 8192, whole 16-byte chunks).  layer != 0:
+ * LayerNorm, else RMS (no mean).  post_weight [C] NULL: no norm of the branch; weight NULL: no norm behind the sum, y NULL;
+ * branch and total NULL: y = norm(x), with no post norm and no gate and scale 1.  Biases [C] may be NULL.  gate (may be NULL): [gates][C],
+ * row r has gate r / (rows / gates), fp32 (gate_f32) or of the tensors' type.  The norm is that of the sum as it is stored.
+ * stats [rows][4] fp32 receives mean and 1 / deviation of the branch and of the sum (0 where there is no such norm; RMS: mean 0).
+ * packed, packed_scales (may be NULL): y in 8 bits as well (tch_pack8).  total and y may be x or branch. */
+int tch_residual_norm_fwd(tch_context* ctx, int dtype, int layer, const void* x, int64_t ldx, const void* branch,
+                          int64_t ldb, void* total, int64_t ldt, void* y, int64_t ldy, float* stats,
+                          const float* weight, const float* bias, const float* post_weight, const float* post_bias,
+                          const void* gate, int gate_f32, int64_t gates, float scale, float eps, void* packed,
+                          void* packed_scales, int packed_format, int64_t rows, int64_t C);
+/* Its gradients from dy and dtotal (the gradient that the sum has from elsewhere; may be NULL where dy is given): dx and dbranch in
+ * the tensors' type (dx may be NULL with a branch), dweight, dbias, dpost_weight, dpost_bias [C] and dgate [gates][C] fp32, each may be NULL,
+ * (+)= with accumulate, the same bits every run.  total, branch and stats are those of the forward call (without a branch, total is its
+ * x).  dx and dbranch may be dy, dtotal, total or branch.  workspace: at least tch_residual_norm_bwd_workspace_bytes. */
+int64_t tch_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t C, int64_t gates);
+int tch_residual_norm_bwd(tch_context* ctx, int dtype, int layer, const void* dy, int64_t lddy, const void* dtotal,
+                          int64_t lddt, const void* total, int64_t ldt, const void* branch, int64_t ldb, void* dx,
+                          int64_t lddx, void* dbranch, int64_t lddb, const float* stats, const float* weight,
+                          const float* post_weight, const float* post_bias, const void* gate, int gate_f32,
+                          int64_t gates, float scale, float* dweight, float* dbias, float* dpost_weight,
+                          float* dpost_bias, float* dgate, int accumulate, int64_t rows, int64_t C, void* workspace,
+                          int64_t workspace_bytes);
+/* Activations in 8 bits for the backward pass: x [M][C] (rows ldx elements apart) -> data [M][C], a byte each, and scales
+ * [M][(C + 31) / 32]: 32 neighbours of a row are multiples of 2^(scale - 127), the smallest power of two with which none of them is
+ * beyond 127 (format 0, int8) or 448 (format 1, fp8 e4m3), rounded to nearest even.  Scales lie between 10 and 248 (int8) or 246 (e4m3),
+ * beyond which numbers saturate; 255: an infinity or a NaN among the 32, which all come back as NaN.  What comes back is exact in
+ * bf16.  h (may be NULL, may be x): act(x) [M][C] (rows ldh apart) of the unrounded x, in the same pass; act as for tch_linear_fwd. */
+int tch_pack8(tch_context* ctx, int dtype, const void* x, int64_t ldx, void* data, void* scales, int format, void* h,
+              int64_t ldh, int act, int64_t M, int64_t C);
+int tch_unpack8(tch_context* ctx, int dtype, const void* data, const void* scales, int format, void* x, int64_t ldx,
+                int64_t M, int64_t C);
 /* probs = softmax over the last dimension of scale * scores[batch, heads, Lq, Lk] + bias[heads, Lq, Lk]
  * + mask[windows, Lq, Lk] (window = batch index % windows); bias and mask may be NULL; causal != 0 keeps keys
  * j <= i only (Lq == Lk).  In place (probs == scores) is allowed. */

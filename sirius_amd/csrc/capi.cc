@@ -424,6 +424,37 @@ int tch_rotary(tch_context* ctx, int dtype, const void* x, int64_t ldx, void* y,
                 interleaved, scale, back);
 }
 
+int tch_residual_norm_fwd(tch_context* ctx, int dtype, int layer, const void* x, int64_t ldx, const void* branch, int64_t ldb, void* total,
+                          int64_t ldt, void* y, int64_t ldy, float* stats, const float* weight, const float* bias, const float* post_weight,
+                          const float* post_bias, const void* gate, int gate_f32, int64_t gates, float scale, float eps, void* packed,
+                          void* packed_scales, int packed_format, int64_t rows, int64_t Cc) {
+  const ResidualNorm n{weight, bias, post_weight, post_bias, gate, gate_f32, gates, layer, scale, eps};
+  return residual_norm_fwd(C(ctx), dtype, n, {const_cast<void*>(x), ldx}, {const_cast<void*>(branch), ldb}, {total, ldt}, {y, ldy}, stats, packed,
+                           packed_scales, packed_format, rows, Cc);
+}
+
+int64_t tch_residual_norm_bwd_workspace_bytes(int64_t rows, int64_t Cc, int64_t gates) { return residual_norm_bwd_workspace_bytes(rows, Cc, gates); }
+
+int tch_residual_norm_bwd(tch_context* ctx, int dtype, int layer, const void* dy, int64_t lddy, const void* dtotal, int64_t lddt, const void* total,
+                          int64_t ldt, const void* branch, int64_t ldb, void* dx, int64_t lddx, void* dbranch, int64_t lddb, const float* stats,
+                          const float* weight, const float* post_weight, const float* post_bias, const void* gate, int gate_f32, int64_t gates,
+                          float scale, float* dweight, float* dbias, float* dpost_weight, float* dpost_bias, float* dgate, int accumulate,
+                          int64_t rows, int64_t Cc, void* workspace, int64_t workspace_bytes) {
+  const ResidualNorm n{weight, nullptr, post_weight, post_bias, gate, gate_f32, gates, layer, scale, 0.f};
+  return residual_norm_bwd(C(ctx), dtype, n, {const_cast<void*>(dy), lddy}, {const_cast<void*>(dtotal), lddt}, {const_cast<void*>(total), ldt},
+                           {const_cast<void*>(branch), ldb}, {dx, lddx}, {dbranch, lddb}, stats, {dweight, dbias, dpost_weight, dpost_bias, dgate},
+                           accumulate, rows, Cc, workspace, workspace_bytes);
+}
+
+int tch_pack8(tch_context* ctx, int dtype, const void* x, int64_t ldx, void* data, void* scales, int format, void* h, int64_t ldh, int act,
+              int64_t M, int64_t Cc) {
+  return pack8(C(ctx), dtype, {const_cast<void*>(x), ldx}, data, scales, format, {h, ldh}, act, M, Cc);
+}
+
+int tch_unpack8(tch_context* ctx, int dtype, const void* data, const void* scales, int format, void* x, int64_t ldx, int64_t M, int64_t Cc) {
+  return unpack8(C(ctx), dtype, data, scales, format, {x, ldx}, M, Cc);
+}
+
 int64_t tch_grad_table_piece_elems(void) { return grad_table_piece_elems(); }
 int64_t tch_grad_norm_workspace_bytes(int64_t pieces) { return grad_norm_workspace_bytes(pieces); }
 

@@ -214,6 +214,36 @@ int linear_wgrad(Context* ctx, const void* x, const void* x_low, const void* dy,
 int rotary(Context* ctx, int dtype, const Rows& x, const Rows& y, const double* freqs, const void* positions, int wide_positions, int64_t start,
            int64_t seq, int64_t rows, int heads, int head_dim, int rot, int interleaved, float scale, int back);
 
+// residual_norm.hip -- the boundary between two blocks: total = scale x + gate . norm(branch), y = norm(total), and its gradients
+struct ResidualNorm {
+  const float* weight;        // null: no norm behind the sum
+  const float* bias;
+  const float* post_weight;   // null: no norm of the branch
+  const float* post_bias;
+  const void* gate;           // [gates][C]; null: none
+  int gate_f32;               // else of the tensors' type
+  int64_t gates;              // each of rows / gates rows
+  int layer;                  // else RMS
+  float scale, eps;
+};
+struct ResidualNormGrads {    // fp32; any may be null
+  float* weight;
+  float* bias;
+  float* post_weight;
+  float* post_bias;
+  float* gate;
+};
+int residual_norm_fwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows& x, const Rows& branch, const Rows& total, const Rows& y, float* stats,
+                      void* packed, void* codes, int format, int64_t rows, int64_t C);
+int64_t residual_norm_bwd_workspace_bytes(int64_t rows, int64_t C, int64_t gates);
+int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows& dy, const Rows& dtotal, const Rows& total, const Rows& branch, const Rows& dx,
+                      const Rows& dbranch, const float* stats, const ResidualNormGrads& g, int accumulate, int64_t rows, int64_t C, void* workspace,
+                      int64_t workspace_bytes);
+
+// pack8.hip -- activations in 8 bits: kept (with h = act(x) on request), and fetched
+int pack8(Context* ctx, int dtype, const Rows& x, void* data, void* codes, int format, const Rows& h, int act, int64_t M, int64_t C);
+int unpack8(Context* ctx, int dtype, const void* data, const void* codes, int format, const Rows& x, int64_t M, int64_t C);
+
 // grad_norm.hip -- the global norm of many tensors, listed in pieces in device memory, and clipping by it
 int64_t grad_table_piece_elems();
 int64_t grad_norm_workspace_bytes(int64_t pieces);

@@ -1,0 +1,194 @@
+// Activations in 8 bits for the backward pass (pack8.h): kept, fetched, and kept by the pass that takes an activation of them.
+// Bound by memory: an element is 2 or 4 bytes on one side and 1 + 1 / 32 on the other.
+//
+// Reference call sites: what the backward pass of train/gpt2.py:90 and train/swin_b.py:118 finds of the forward pass, all of it in the types it was computed in.
+#include <algorithm>
+#include <climits>
+
+#include "context.h"
+#include "linear_epilogue.h"
+#include "ops.h"
+#include "pack8.h"
+
+namespace tch {
+namespace {
+
+constexpr int kPackAtOnce = 4;   // eights of a thread, on their way together
+
+struct PackArgs {
+  const void* x;          // kept: rows ldx apart
+  void* h;                // act(x); may be null
+  void* out;              // fetched: rows ldx apart
+  unsigned char* data;    // [M][C]
+  unsigned char* codes;   // [M][groups of 32]
+  int64_t ldx, ldh;
+  uint64_t total;         // rows * eights of a row, whole groups
+  int C, groups, act;
+  FastDiv eights;
+};
+
+template <typename T>
+struct EightOf {
+  static constexpr int N = sizeof(T) / 2;
+  Chunk c[N];
+  __device__ __forceinline__ void load(const T* from, int live) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      c[i] = zero_chunk();
+      if (i * (8 / N) < live) c[i].u = load_streaming_u4(from, i);
+    }
+  }
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) chunk_to_float<T>(c[i], v + i * (8 / N));
+  }
+  __device__ __forceinline__ static void store(T* to, const float* v, int live) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * (8 / N) < live) reinterpret_cast<uint4*>(to)[i] = float_to_chunk<T>(v + i * (8 / N)).u;
+  }
+};
+
+struct At {
+  int64_t row;
+  int col, live;
+};
+__device__ __forceinline__ At place(const PackArgs& p, uint64_t q) {
+  At a{0, 0, 0};
+  if (q >= p.total) return a;
+  uint32_t row, eight;
+  p.eights.divmod(static_cast<uint32_t>(q), row, eight);
+  a.row = row;
+  a.col = static_cast<int>(eight) * 8;
+  a.live = max(0, min(p.C - a.col, 8));
+  return a;
+}
+
+// The four lanes of a group are neighbours (a row has whole groups of them), and all lanes of a wavefront go round together.
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void pack8_kernel(PackArgs p) {
+  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * kPackAtOnce);
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * kPackAtOnce); base < p.total; base += stride) {
+    EightOf<T> x[kPackAtOnce];
+    At at[kPackAtOnce];
+#pragma unroll
+    for (int i = 0; i < kPackAtOnce; ++i) {
+      at[i] = place(p, base + 256 * i + threadIdx.x);
+      x[i].load(static_cast<const T*>(p.x) + at[i].row * p.ldx + at[i].col, at[i].live);
+    }
+    with_activation(p.act, [&](auto act_c) {
+      constexpr int ACT = decltype(act_c)::value;
+#pragma unroll
+      for (int i = 0; i < kPackAtOnce; ++i) {
+        float v[8];
+        uint32_t words[2];
+        x[i].get(v);
+        const uint32_t code = pack8_lane<FMT>(v, at[i].live, words);
+        uint32_t* to = reinterpret_cast<uint32_t*>(p.data + at[i].row * p.C + at[i].col);
+        if (at[i].live > 0) to[0] = words[0];
+        if (at[i].live > 4) to[1] = words[1];
+        if (at[i].live > 0 && threadIdx.x % 4 == 0) p.codes[at[i].row * p.groups + at[i].col / kPackGroup] = static_cast<unsigned char>(code);
+        if (p.h) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = act_value<T, ACT>(v[e]);
+          EightOf<T>::store(static_cast<T*>(p.h) + at[i].row * p.ldh + at[i].col, v, at[i].live);
+        }
+      }
+    });
+  }
+}
+
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void unpack8_kernel(PackArgs p) {
+  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * kPackAtOnce);
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * kPackAtOnce) + threadIdx.x; base < p.total; base += stride) {
+    At at[kPackAtOnce];
+    uint32_t words[kPackAtOnce][2], code[kPackAtOnce];
+#pragma unroll
+    for (int i = 0; i < kPackAtOnce; ++i) {
+      at[i] = place(p, base + 256 * i);
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(p.data + at[i].row * p.C + at[i].col);
+      words[i][0] = at[i].live > 0 ? from[0] : 0;
+      words[i][1] = at[i].live > 4 ? from[1] : 0;
+      code[i] = at[i].live > 0 ? p.codes[at[i].row * p.groups + at[i].col / kPackGroup] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kPackAtOnce; ++i) {
+      float v[8];
+      const float unit = pack8_unit(code[i]);
+      unpack8_word<FMT>(words[i][0], unit, v);
+      unpack8_word<FMT>(words[i][1], unit, v + 4);
+      EightOf<T>::store(static_cast<T*>(p.out) + at[i].row * p.ldx + at[i].col, v, at[i].live);
+    }
+  }
+}
+
+int bind(const char* what, PackArgs& a, int dtype, void* data, void* codes, int format, int64_t M, int64_t C, dim3* grid) {
+  const std::string name(what);
+  TCH_CHECK_ARG(dtype == kBF16 || dtype == kF32, name + ": dtype must be f32(0) or bf16(1)");
+  TCH_CHECK_ARG(format >= 0 && format < kPackFormats, name + ": unknown 8-bit format");
+  TCH_CHECK_ARG(M >= 0 && M <= INT_MAX && C > 0 && C < (1 << 30), name + ": bad shape");
+  TCH_CHECK_ARG(C % (dtype == kBF16 ? 8 : 4) == 0, name + ": rows must be whole 16-byte chunks");
+  if (M == 0) return 0;
+  TCH_CHECK_ARG(data && codes, name + ": null tensor");
+  TCH_CHECK_ARG((reinterpret_cast<uintptr_t>(data) & 15) == 0, name + ": the kept numbers must start on a 16-byte boundary");
+  a.data = static_cast<unsigned char*>(data), a.codes = static_cast<unsigned char*>(codes);
+  a.C = static_cast<int>(C);
+  a.groups = static_cast<int>((C + kPackGroup - 1) / kPackGroup);
+  const int64_t eights = a.groups * 4ll;
+  TCH_CHECK_ARG(M * eights < (1ll << 31), name + ": tensor exceeds 2^34 elements");
+  a.total = static_cast<uint64_t>(M * eights);
+  a.eights = FastDiv(static_cast<uint32_t>(eights));
+  *grid = dim3(static_cast<unsigned>(std::min<uint64_t>((a.total + 256 * kPackAtOnce - 1) / (256 * kPackAtOnce), 1 << 20)));
+  return 0;
+}
+bool rows_ok(const void* t, int64_t ld, int64_t C, int eb) {
+  return ld >= C && ld % (16 / eb) == 0 && ld <= (1ll << 31) && (reinterpret_cast<uintptr_t>(t) & 15) == 0;
+}
+
+}  // namespace
+
+int pack8(Context* ctx, int dtype, const Rows& x, void* data, void* codes, int format, const Rows& h, int act, int64_t M, int64_t C) {
+  PackArgs a{};
+  dim3 grid;
+  if (int rc = bind("pack8", a, dtype, data, codes, format, M, C, &grid)) return rc;
+  TCH_CHECK_ARG(act >= 0 && act < kActCount, "pack8: unknown activation");
+  if (M == 0) return 0;
+  const int eb = dtype == kBF16 ? 2 : 4;
+  TCH_CHECK_ARG(x.ptr, "pack8: null tensor");
+  TCH_CHECK_ARG(rows_ok(x.ptr, x.ld, C, eb) && (!h.ptr || rows_ok(h.ptr, h.ld, C, eb)), "pack8: rows must start on 16-byte boundaries and not overlap");
+  const Span in{x.ptr, x.ld * eb, C * eb, M};
+  const Span out[3] = {{h.ptr, h.ld * eb, C * eb, M}, {data, C, C, M}, {codes, a.groups, a.groups, M}};
+  TCH_CHECK_ARG(apart(out[0], in, true) && apart(out[1], in) && apart(out[2], in) && apart(out[0], out[1]) && apart(out[0], out[2]) && apart(out[1], out[2]),
+                "pack8: an output overlaps another tensor (the activations may be written over what they are taken of)");
+  a.x = x.ptr, a.ldx = x.ld;
+  a.h = h.ptr, a.ldh = h.ld;
+  a.act = h.ptr ? act : kActNone;
+  const double bytes = static_cast<double>(M) * C * (eb * (h.ptr ? 2.0 : 1.0) + 33.0 / 32);
+  if (dtype == kBF16)
+    return format == kPackInt8 ? launch(ctx, pack8_kernel<bf16, kPackInt8>, grid, dim3(256), a, "pack8_kernel<bf16,int8>", bytes, 1)
+                               : launch(ctx, pack8_kernel<bf16, kPackE4m3>, grid, dim3(256), a, "pack8_kernel<bf16,e4m3>", bytes, 1);
+  return format == kPackInt8 ? launch(ctx, pack8_kernel<float, kPackInt8>, grid, dim3(256), a, "pack8_kernel<f32,int8>", bytes, 1)
+                             : launch(ctx, pack8_kernel<float, kPackE4m3>, grid, dim3(256), a, "pack8_kernel<f32,e4m3>", bytes, 1);
+}
+
+int unpack8(Context* ctx, int dtype, const void* data, const void* codes, int format, const Rows& x, int64_t M, int64_t C) {
+  PackArgs a{};
+  dim3 grid;
+  if (int rc = bind("unpack8", a, dtype, const_cast<void*>(data), const_cast<void*>(codes), format, M, C, &grid)) return rc;
+  if (M == 0) return 0;
+  const int eb = dtype == kBF16 ? 2 : 4;
+  TCH_CHECK_ARG(x.ptr, "unpack8: null tensor");
+  TCH_CHECK_ARG(rows_ok(x.ptr, x.ld, C, eb), "unpack8: rows must start on 16-byte boundaries and not overlap");
+  const Span out{x.ptr, x.ld * eb, C * eb, M};
+  TCH_CHECK_ARG(apart(out, {data, C, C, M}) && apart(out, {codes, a.groups, a.groups, M}), "unpack8: the output overlaps what is kept");
+  a.out = x.ptr, a.ldx = x.ld;
+  const double bytes = static_cast<double>(M) * C * (eb + 33.0 / 32);
+  if (dtype == kBF16)
+    return format == kPackInt8 ? launch(ctx, unpack8_kernel<bf16, kPackInt8>, grid, dim3(256), a, "unpack8_kernel<bf16,int8>", bytes, 1)
+                               : launch(ctx, unpack8_kernel<bf16, kPackE4m3>, grid, dim3(256), a, "unpack8_kernel<bf16,e4m3>", bytes, 1);
+  return format == kPackInt8 ? launch(ctx, unpack8_kernel<float, kPackInt8>, grid, dim3(256), a, "unpack8_kernel<f32,int8>", bytes, 1)
+                             : launch(ctx, unpack8_kernel<float, kPackE4m3>, grid, dim3(256), a, "unpack8_kernel<f32,e4m3>", bytes, 1);
+}
+
+}  // namespace tch

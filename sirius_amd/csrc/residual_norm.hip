@@ -1,0 +1,723 @@
+// The boundary between two blocks of a transformer, in one pass: the norm behind a block, its gate, the residual and its scale, and
+// the norm in front of the next block.
+//   n = pw . b^ + pb      b^ = (b - mean) / deviation of the block's output b (post norm; without one n = b)
+//   t = s x + g . n       g: none, a vector, or a vector per sample
+//   y = w . t^ + c        t^ = (t - mean) / deviation of t as it is stored
+// with the mean and the deviation of a row (LayerNorm), or a mean of 0 (RMS).  Backward, from dy and the gradient dt0 that t has from
+// elsewhere, with k = w . dy:
+//   dt = dt0 + (k - mean(k) - t^ mean(k t^)) / deviation,   dx = s dt,   dn = g . dt,   db: through the post norm likewise
+//   dw = sum dy t^,  dc = sum dy;  over the rows of a gate A = sum dt b^, B = sum dt:  dg = pw A + pb B,  dpw = sum g A,  dpb = sum g B
+//
+// Bound by memory: four tensors forward, six backward.  A lane has eight neighbours of a row, a row as many wavefronts as that takes (short
+// rows share one), the vectors stay in registers while a workgroup walks its rows, and the next row is on its way while this one is
+// worked on.  Means, deviations and sums are fp32 in registers; a wavefront's part of a deviation is taken about its own mean, and the
+// parts are joined about the row's.  What a workgroup adds up over its rows goes to the workspace, where a second launch adds the
+// workgroups up in fp64 in their order: the same bits every run.
+//
+// Reference call sites: the blocks that train/gpt2.py:26 and train/swin_b.py:38 build have a LayerNorm in front of each half and a
+// plain residual.
+#include <algorithm>
+#include <climits>
+
+#include "context.h"
+#include "linear_epilogue.h"
+#include "ops.h"
+#include "pack8.h"
+
+namespace tch {
+namespace {
+
+constexpr int kEach = 8;             // neighbours of a lane
+constexpr int kMaxWidth = 8192;      // sixteen wavefronts a row
+enum Branch : int { kNoBranch = 0, kBranch = 1, kPostNorm = 2 };
+
+struct RowsPtr {
+  void* at;
+  int64_t ld;   // elements
+};
+
+struct NormArgs {
+  RowsPtr x, branch, total, y;            // forward
+  RowsPtr dy, dtotal, dx, dbranch;        // backward, with total and branch
+  float4* stats;                          // [rows] mean and 1 / deviation of the branch, of the total
+  const float* weight;                    // null: there is no norm behind the sum
+  const float* bias;
+  const float* post_weight;
+  const float* post_bias;
+  const void* gate;
+  unsigned char* packed;                  // forward: y in 8 bits too
+  unsigned char* codes;
+  int64_t rows, gate_rows;                // gate_rows: rows that share a gate
+  int64_t group_rows;                     // backward: of a workgroup
+  int C, waves, groups;                   // wavefronts of a row, rows at a time of a workgroup
+  int layer, gate_f32, format;
+  float scale, eps;
+  // backward
+  float* sums;                            // [workgroups][planes][C]
+  float* gate_sums;                       // [workgroups][C], or the gradient of the gates itself
+  int planes, plane_of[4];                // -1: nobody wants it
+  int split_gates;                        // several workgroups have a part of a gate's rows
+  int gates_each;                         // otherwise: gates of a workgroup
+  int gates, add_gates;
+};
+
+// the sum over the L lanes of a row, in every lane of it; L = 64: over the wavefront
+template <int L>
+__device__ __forceinline__ float lane_sum(float v) {
+  auto plus = [&](auto ctrl) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  plus(std::integral_constant<int, 0xb1>{});     // lane ^ 1
+  plus(std::integral_constant<int, 0x4e>{});     // lane ^ 2
+  plus(std::integral_constant<int, 0x141>{});    // the other half of eight
+  plus(std::integral_constant<int, 0x140>{});    // the other half of sixteen
+  if constexpr (L > 16) v += __shfl_xor(v, 16, 64);
+  if constexpr (L > 32) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+
+// What the wavefronts of a row tell each other: two numbers each, in turn in two places, so that one barrier a time is enough.
+struct Meeting {
+  float2 (*said)[16];
+  int turn, first, waves, lane, wave;
+  __device__ __forceinline__ const float2* say(float a, float b) {
+    float2* here = said[turn];
+    turn ^= 1;
+    if (lane == 0) here[wave] = make_float2(a, b);
+    __syncthreads();
+    return here + first;
+  }
+  // both sums over the row, of sums over the wavefronts
+  __device__ __forceinline__ void add(float& a, float& b) {
+    if (waves == 1) return;
+    const float2* h = say(a, b);
+    a = b = 0.f;
+    for (int w = 0; w < waves; ++w) a += h[w].x, b += h[w].y;
+  }
+};
+
+// mean and 1 / deviation of a row
+template <int L>
+__device__ __forceinline__ float2 row_stats(const float* v, int live, int layer, const NormArgs& p, Meeting& meet, int row_wave) {
+  const float inv = 1.f / static_cast<float>(p.C);
+  if (!layer) {
+    float q = 0.f, none = 0.f;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) q = e < live ? fmaf(v[e], v[e], q) : q;
+    q = lane_sum<L>(q);
+    meet.add(q, none);
+    return make_float2(0.f, 1.f / sqrtf(q * inv + p.eps));
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) s += e < live ? v[e] : 0.f;
+  s = lane_sum<L>(s);
+  auto elements = [&](int w) { return static_cast<float>(min(p.C - w * 64 * kEach, 64 * kEach)); };   // of a wavefront
+  const float n = L < 64 ? static_cast<float>(p.C) : elements(row_wave), mine = s / n;
+  float q = 0.f;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const float d = v[e] - mine;
+    q = e < live ? fmaf(d, d, q) : q;
+  }
+  q = lane_sum<L>(q);
+  if (meet.waves == 1) return make_float2(mine, 1.f / sqrtf(q * inv + p.eps));
+  const float2* h = meet.say(s, q);
+  float mean = 0.f;
+  for (int w = 0; w < meet.waves; ++w) mean += h[w].x;
+  mean *= inv;
+  q = 0.f;
+  for (int w = 0; w < meet.waves; ++w) {
+    const float m = elements(w), d = h[w].x / m - mean;
+    q += fmaf(m * d, d, h[w].y);
+  }
+  return make_float2(mean, 1.f / sqrtf(q * inv + p.eps));
+}
+
+// Eight neighbours as they lie in memory; `live`: 8, 4 (fp32) or 0 of them.
+template <typename T>
+struct Eight {
+  static constexpr int N = sizeof(T) / 2;   // chunks
+  Chunk c[N];
+  __device__ __forceinline__ void load(const RowsPtr& t, int64_t row, int col, int live) {
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(t.at) + row * t.ld + col);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      c[i] = zero_chunk();
+      if (i * (kEach / N) < live) c[i].u = from[i];
+    }
+  }
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) chunk_to_float<T>(c[i], v + i * (kEach / N));
+  }
+  __device__ __forceinline__ void set(const float* v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) c[i] = float_to_chunk<T>(v + i * (kEach / N));
+  }
+  __device__ __forceinline__ void store(const RowsPtr& t, int64_t row, int col, int live) const {
+    uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(t.at) + row * t.ld + col);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i * (kEach / N) < live) to[i] = c[i].u;
+  }
+};
+
+__device__ __forceinline__ void load_vector(const float* from, int col, int live, float otherwise, float* v) {
+#pragma unroll
+  for (int i = 0; i < kEach; i += 4) {
+    float4 f = make_float4(otherwise, otherwise, otherwise, otherwise);
+    if (from && i < live) f = *reinterpret_cast<const float4*>(from + col + i);
+    v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load_gate(const NormArgs& p, int64_t gate, int col, int live, float* v) {
+  if (!p.gate || p.gate_f32) {
+    load_vector(static_cast<const float*>(p.gate) + (p.gate ? gate * p.C : 0), col, live, 1.f, v);
+  } else {
+    Eight<T> g;
+    g.load({const_cast<void*>(p.gate), p.C}, gate, col, live);
+    g.get(v);
+  }
+}
+
+struct Place {   // of a lane
+  int lane, wave, row_wave, group, col, live;
+};
+template <int L>
+__device__ __forceinline__ Place place(const NormArgs& p) {
+  Place a;
+  a.lane = threadIdx.x & 63;
+  a.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int sub;
+  if (L < 64) {
+    a.row_wave = 0;
+    a.group = threadIdx.x / L;
+    sub = threadIdx.x % L;
+  } else {
+    a.group = a.wave / p.waves;
+    a.row_wave = a.wave - a.group * p.waves;
+    sub = a.row_wave * 64 + a.lane;
+  }
+  a.col = sub * kEach;
+  a.live = max(0, min(p.C - a.col, kEach));
+  return a;
+}
+
+template <typename T, int L, int BR>
+__global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_fwd_kernel(NormArgs p) {
+  __shared__ float2 said[2][16];
+  const Place at = place<L>(p);
+  Meeting meet{said, 0, at.group * p.waves, p.waves, at.lane, at.wave};
+  const bool samples = p.gate_rows < p.rows;
+  float w[kEach], c[kEach], pw[kEach], pb[kEach], g[kEach];
+  load_vector(p.weight, at.col, at.live, 1.f, w);
+  load_vector(p.bias, at.col, at.live, 0.f, c);
+  if constexpr (BR != kNoBranch) load_gate<T>(p, 0, at.col, at.live, g);
+  if constexpr (BR == kPostNorm) {
+    load_vector(p.post_weight, at.col, at.live, 1.f, pw);
+    load_vector(p.post_bias, at.col, at.live, 0.f, pb);
+  }
+  const int64_t step = static_cast<int64_t>(gridDim.x) * p.groups;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * p.groups + at.group;
+  Eight<T> x, b;
+  auto request = [&](int64_t r) {
+    const int live = r < p.rows ? at.live : 0;
+    x.load(p.x, r, at.col, live);
+    if constexpr (BR != kNoBranch) b.load(p.branch, r, at.col, live);
+  };
+  request(row);
+  // (every wavefront of the workgroup makes as many rounds: they meet in each)
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * p.groups; first < p.rows; first += step, row += step) {
+    const int live = row < p.rows ? at.live : 0;
+    float t[kEach], n[kEach];
+    x.get(t);
+    if constexpr (BR != kNoBranch) b.get(n);
+    if (BR != kNoBranch && samples && row < p.rows) load_gate<T>(p, row / p.gate_rows, at.col, live, g);
+    request(row + step);
+    float4 stats = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (BR == kPostNorm) {
+      const float2 s = row_stats<L>(n, at.live, p.layer, p, meet, at.row_wave);
+      stats.x = s.x, stats.y = s.y;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) n[e] = fmaf((n[e] - s.x) * s.y, pw[e], pb[e]);
+    }
+    if constexpr (BR != kNoBranch) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) t[e] = fmaf(g[e], n[e], p.scale * t[e]);
+      Eight<T> sum;
+      sum.set(t);
+      sum.store(p.total, row, at.col, live);
+      sum.get(t);
+    }
+    if (p.weight) {
+      const float2 s = row_stats<L>(t, at.live, p.layer, p, meet, at.row_wave);
+      stats.z = s.x, stats.w = s.y;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) t[e] = fmaf((t[e] - s.x) * s.y, w[e], c[e]);
+      Eight<T> y;
+      y.set(t);
+      y.store(p.y, row, at.col, live);
+      if (p.packed) {   // what is kept is y as it is stored
+        y.get(t);
+        uint32_t words[2];
+        const uint32_t code = p.format == kPackInt8 ? pack8_lane<kPackInt8>(t, live, words) : pack8_lane<kPackE4m3>(t, live, words);
+        uint32_t* to = reinterpret_cast<uint32_t*>(p.packed + row * p.C + at.col);
+        if (live > 0) to[0] = words[0];
+        if (live > 4) to[1] = words[1];
+        if (live > 0 && at.lane % 4 == 0) p.codes[row * ((p.C + kPackGroup - 1) / kPackGroup) + at.col / kPackGroup] = static_cast<unsigned char>(code);
+      }
+    }
+    if (row < p.rows && at.col == 0) p.stats[row] = stats;
+  }
+}
+
+// SAMPLES: gates of their own for runs of rows
+template <typename T, int L, int BR, bool SAMPLES>
+__global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_bwd_kernel(NormArgs p) {
+  constexpr int kLds = L < 64 ? 256 * kEach : 512 * kEach;   // (more threads have one row at a time, and nothing to add up here)
+  __shared__ float2 said[2][16];
+  __shared__ float lds[kLds];
+  const Place at = place<L>(p);
+  Meeting meet{said, 0, at.group * p.waves, p.waves, at.lane, at.wave};
+  const float inv = 1.f / static_cast<float>(p.C);
+  float w[kEach], pw[kEach], g[kEach];
+  load_vector(p.weight, at.col, at.live, 0.f, w);
+  if constexpr (BR == kPostNorm) load_vector(p.post_weight, at.col, at.live, 0.f, pw);
+  if constexpr (BR != kNoBranch) load_gate<T>(p, 0, at.col, at.live, g);
+  float sum[4][kEach], gated[2][kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) sum[0][e] = sum[1][e] = sum[2][e] = sum[3][e] = gated[0][e] = gated[1][e] = 0.f;
+
+  // The lanes' eight sums over the row groups of the workgroup, to `to` [C].
+  auto add_up = [&](const float* v, float* to, bool add) {
+    if (p.groups == 1) {
+#pragma unroll
+      for (int i = 0; i < kEach; i += 4) {
+        if (i >= at.live) break;
+        float4* out = reinterpret_cast<float4*>(to + at.col + i);
+        float4 s = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        if (add) {
+          const float4 old = *out;
+          s = make_float4(s.x + old.x, s.y + old.y, s.z + old.z, s.w + old.w);
+        }
+        *out = s;
+      }
+      return;
+    }
+    const int span = (L < 64 ? L : p.waves * 64) * kEach;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) lds[at.group * span + at.col + e] = v[e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
+      float s = 0.f;
+      for (int q = 0; q < p.groups; ++q) s += lds[q * span + c];
+      to[c] = add ? to[c] + s : s;
+    }
+  };
+
+  int gate = 0, behind_gate = 1;
+  int64_t offset = 0;
+  if (p.split_gates) {
+    const int pieces = static_cast<int>((p.gate_rows + p.group_rows - 1) / p.group_rows);
+    gate = blockIdx.x / pieces;
+    behind_gate = gate + 1;
+    offset = static_cast<int64_t>(blockIdx.x - gate * pieces) * p.group_rows;
+  } else {
+    gate = blockIdx.x * p.gates_each;
+    behind_gate = min(gate + p.gates_each, p.gates);
+  }
+  for (; gate < behind_gate; ++gate) {
+    const int64_t r0 = gate * p.gate_rows + offset;
+    const int64_t r1 = min(p.split_gates ? r0 + p.group_rows : r0 + p.gate_rows, min((gate + 1) * p.gate_rows, p.rows));
+    if constexpr (SAMPLES) load_gate<T>(p, gate, at.col, at.live, g);
+    Eight<T> dy, d0, t, b;
+    float4 stats, next_stats;
+    auto request = [&](int64_t row) {
+      const int live = row < r1 ? at.live : 0;
+      if (p.weight) {
+        dy.load(p.dy, row, at.col, live);
+        t.load(p.total, row, at.col, live);
+      }
+      if (p.dtotal.at) d0.load(p.dtotal, row, at.col, live);
+      if constexpr (BR != kNoBranch) b.load(p.branch, row, at.col, live);
+      next_stats = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < r1) next_stats = p.stats[row];
+    };
+    request(r0 + at.group);
+    for (int64_t first = r0; first < r1; first += p.groups) {
+      const int64_t row = first + at.group;
+      const int live = row < r1 ? at.live : 0;
+      stats = next_stats;
+      float d[kEach], h[kEach], k[kEach], bh[kEach];
+      if (p.dtotal.at)
+        d0.get(d);
+      else
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) d[e] = 0.f;
+      if (p.weight) {
+        dy.get(k);
+        t.get(h);
+      }
+      if constexpr (BR != kNoBranch) b.get(bh);
+      request(row + p.groups);
+      if (p.weight) {
+        float a = 0.f, q = 0.f;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          h[e] = (h[e] - stats.z) * stats.w;
+          sum[0][e] = fmaf(k[e], h[e], sum[0][e]);      // (rows and columns that are not there have a gradient of 0)
+          sum[1][e] += k[e];
+          k[e] *= w[e];
+          a += k[e];
+          q = fmaf(k[e], h[e], q);
+        }
+        if (p.layer) a = lane_sum<L>(a);
+        q = lane_sum<L>(q);
+        meet.add(a, q);
+        a = p.layer ? a * inv : 0.f;
+        q *= inv;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) d[e] = fmaf(stats.w, k[e] - a - h[e] * q, d[e]);
+      }
+      if (p.dx.at) {
+        Eight<T> dx;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) h[e] = p.scale * d[e];
+        dx.set(h);
+        dx.store(p.dx, row, at.col, live);
+      }
+      if constexpr (BR != kNoBranch) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          if (e >= live) d[e] = 0.f;
+          if constexpr (BR == kPostNorm) bh[e] = (bh[e] - stats.x) * stats.y;
+          sum[2][e] = fmaf(d[e], bh[e], sum[2][e]);
+          sum[3][e] += d[e];
+          k[e] = d[e] * g[e];
+        }
+        if constexpr (BR == kPostNorm) {
+          float a = 0.f, q = 0.f;
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) {
+            k[e] *= pw[e];
+            a += k[e];
+            q = fmaf(k[e], bh[e], q);
+          }
+          if (p.layer) a = lane_sum<L>(a);
+          q = lane_sum<L>(q);
+          meet.add(a, q);
+          a = p.layer ? a * inv : 0.f;
+          q *= inv;
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) k[e] = stats.y * (k[e] - a - bh[e] * q);
+        }
+        Eight<T> db;
+        db.set(k);
+        db.store(p.dbranch, row, at.col, live);
+      }
+    }
+    if constexpr (SAMPLES) {
+      // dg of these rows, and what the post norm's gradients have from them
+      float dg[kEach], post[kEach];
+      load_vector(p.post_bias, at.col, at.live, 0.f, post);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        dg[e] = BR == kPostNorm ? fmaf(pw[e], sum[2][e], post[e] * sum[3][e]) : sum[2][e];
+        gated[0][e] = fmaf(g[e], sum[2][e], gated[0][e]);
+        gated[1][e] = fmaf(g[e], sum[3][e], gated[1][e]);
+        sum[2][e] = sum[3][e] = 0.f;
+      }
+      if (p.gate_sums) add_up(dg, p.gate_sums + static_cast<int64_t>(p.split_gates ? static_cast<int>(blockIdx.x) : gate) * p.C, p.add_gates);
+    }
+  }
+  if constexpr (SAMPLES) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sum[2][e] = gated[0][e], sum[3][e] = gated[1][e];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (p.plane_of[i] >= 0) add_up(sum[i], p.sums + (static_cast<int64_t>(blockIdx.x) * p.planes + p.plane_of[i]) * p.C, false);
+}
+
+// The workgroups' sums added up: 32 columns a workgroup, eight threads a column, in fp64 in a fixed order.  blockIdx.y 0: the norm's two
+// gradients; 1: those of the post norm, and of a gate that all rows share; 2 and on: of a sample's gate.
+struct NormSumArgs {
+  const float* sums;
+  const float* gate_sums;
+  const float* post_weight;
+  const float* post_bias;
+  const void* gate;         // shared by all rows, or null
+  float* dweight;
+  float* dbias;
+  float* dpost_weight;
+  float* dpost_bias;
+  float* dgate;
+  int C, blocks, planes, plane_of[4];
+  int pieces;               // of a sample's gate
+  int post, shared_gate, gate_f32, add;
+};
+__global__ __launch_bounds__(256) void residual_norm_sum_kernel(NormSumArgs p) {
+  __shared__ double meet[2][8][32];
+  const int lane = threadIdx.x & 31, line = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, job = blockIdx.y;
+  double s[2] = {0.0, 0.0};
+  if (c < p.C) {
+    if (job < 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int plane = p.plane_of[2 * job + i];
+        if (plane < 0) continue;
+        const float* from = p.sums + static_cast<int64_t>(plane) * p.C + c;
+        const int64_t ld = static_cast<int64_t>(p.planes) * p.C;
+#pragma unroll 8
+        for (int b = line; b < p.blocks; b += 8) s[i] += from[b * ld];
+      }
+    } else {
+      const float* from = p.gate_sums + static_cast<int64_t>(job - 2) * p.pieces * p.C + c;
+#pragma unroll 8
+      for (int b = line; b < p.pieces; b += 8) s[0] += from[static_cast<int64_t>(b) * p.C];
+    }
+  }
+  meet[0][line][lane] = s[0];
+  meet[1][line][lane] = s[1];
+  __syncthreads();
+  if (line != 0 || c >= p.C) return;
+#pragma unroll
+  for (int l = 1; l < 8; ++l) s[0] += meet[0][l][lane], s[1] += meet[1][l][lane];
+  auto put = [&](float* to, int64_t i, double v) {
+    if (to) to[i] = p.add ? static_cast<float>(to[i] + v) : static_cast<float>(v);
+  };
+  if (job == 0) {
+    put(p.dweight, c, s[0]);
+    put(p.dbias, c, s[1]);
+  } else if (job == 1) {
+    double g = 1.0;
+    if (p.shared_gate) {
+      if (p.gate) g = p.gate_f32 ? static_cast<const float*>(p.gate)[c] : Elem<bf16>::load(static_cast<const bf16*>(p.gate) + c);
+      const double w = p.post ? p.post_weight[c] : 1.0, b = p.post_bias ? p.post_bias[c] : 0.0;
+      put(p.dgate, c, w * s[0] + b * s[1]);
+    }
+    put(p.dpost_weight, c, g * s[0]);
+    put(p.dpost_bias, c, g * s[1]);
+  } else {
+    put(p.dgate, static_cast<int64_t>(job - 2) * p.C + c, s[0]);
+  }
+}
+
+struct Shape {
+  int lanes, waves, groups, threads;   // lanes: 16, 32, or 64 (as many wavefronts as it takes)
+};
+// As many rows at a time as make eight wavefronts, where there are that many.
+Shape shape_of(int64_t rows, int C) {
+  if (C <= 16 * kEach) return {16, 1, 16, 256};
+  if (C <= 32 * kEach) return {32, 1, 8, 256};
+  const int waves = (C + 64 * kEach - 1) / (64 * kEach);
+  const int groups = static_cast<int>(std::min<int64_t>(std::max(8 / waves, 1), std::max<int64_t>(rows, 1)));
+  return {64, waves, groups, waves * groups * 64};
+}
+
+// The backward's workgroups: about sixteen wavefronts a compute unit in all.
+struct Cut {
+  Shape shape;
+  int64_t group_rows, blocks, pieces;   // pieces: of a gate's rows
+  int gates_each;
+  bool split;
+};
+Cut cut_rows(int64_t rows, int C, int64_t gates) {
+  Cut c{};
+  c.shape = shape_of(rows, C);
+  const int64_t gate_rows = rows / gates, want = 4096 / (c.shape.threads / 64);
+  const int64_t each = (rows + want - 1) / want;
+  c.group_rows = (each + c.shape.groups - 1) / c.shape.groups * c.shape.groups;
+  c.split = gates == 1 || gate_rows >= c.group_rows;
+  c.pieces = c.split ? (gate_rows + c.group_rows - 1) / c.group_rows : 1;
+  c.gates_each = c.split ? 1 : static_cast<int>(std::max<int64_t>(c.group_rows / gate_rows, 1));
+  c.blocks = c.split ? gates * c.pieces : (gates + c.gates_each - 1) / c.gates_each;
+  return c;
+}
+
+int check_shape(const char* what, int dtype, int64_t rows, int64_t C, int64_t gates) {
+  const std::string name(what);
+  TCH_CHECK_ARG(dtype == kBF16 || dtype == kF32, name + ": dtype must be f32(0) or bf16(1)");
+  TCH_CHECK_ARG(rows >= 0 && rows <= INT_MAX && C > 0 && C <= kMaxWidth, name + ": rows of 1 to 8192 elements");
+  TCH_CHECK_ARG(C % (dtype == kBF16 ? 8 : 4) == 0, name + ": rows must be whole 16-byte chunks");
+  TCH_CHECK_ARG(gates >= 1 && (rows == 0 || (gates <= rows && rows % gates == 0)), name + ": every gate is shared by as many rows");
+  return 0;
+}
+bool fits(const Rows& t, int64_t C, int eb) {
+  return !t.ptr || (t.ld >= C && t.ld % (16 / eb) == 0 && t.ld <= (1ll << 31) && (reinterpret_cast<uintptr_t>(t.ptr) & 15) == 0);
+}
+bool aligned(std::initializer_list<const void*> all) {
+  uintptr_t bits = 0;
+  for (const void* p : all) bits |= reinterpret_cast<uintptr_t>(p);
+  return (bits & 15) == 0;
+}
+
+template <typename T, int L>
+int launch_fwd(Context* ctx, const NormArgs& a, int br, dim3 grid, dim3 block, const char* name, double bytes) {
+  if (br == kNoBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, kNoBranch>, grid, block, a, name, bytes, 1);
+  if (br == kBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, kBranch>, grid, block, a, name, bytes, 1);
+  return launch(ctx, residual_norm_fwd_kernel<T, L, kPostNorm>, grid, block, a, name, bytes, 1);
+}
+template <typename T, int L>
+int launch_bwd(Context* ctx, const NormArgs& a, int br, bool samples, dim3 grid, dim3 block, const char* name, double bytes) {
+  if (br == kNoBranch) return launch(ctx, residual_norm_bwd_kernel<T, L, kNoBranch, false>, grid, block, a, name, bytes, 1);
+  if (br == kBranch)
+    return samples ? launch(ctx, residual_norm_bwd_kernel<T, L, kBranch, true>, grid, block, a, name, bytes, 1)
+                   : launch(ctx, residual_norm_bwd_kernel<T, L, kBranch, false>, grid, block, a, name, bytes, 1);
+  return samples ? launch(ctx, residual_norm_bwd_kernel<T, L, kPostNorm, true>, grid, block, a, name, bytes, 1)
+                 : launch(ctx, residual_norm_bwd_kernel<T, L, kPostNorm, false>, grid, block, a, name, bytes, 1);
+}
+
+}  // namespace
+
+int residual_norm_fwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows& x, const Rows& branch, const Rows& total, const Rows& y, float* stats,
+                      void* packed, void* codes, int format, int64_t rows, int64_t C) {
+  if (int rc = check_shape("residual_norm_fwd", dtype, rows, C, n.gates)) return rc;
+  if (rows == 0) return 0;
+  const int eb = dtype == kBF16 ? 2 : 4;
+  TCH_CHECK_ARG(x.ptr && stats, "residual_norm_fwd: null tensor");
+  TCH_CHECK_ARG((branch.ptr != nullptr) == (total.ptr != nullptr), "residual_norm_fwd: a branch and the sum come together");
+  TCH_CHECK_ARG((n.weight != nullptr) == (y.ptr != nullptr), "residual_norm_fwd: a norm's weight and its output come together");
+  TCH_CHECK_ARG(branch.ptr || n.weight, "residual_norm_fwd: nothing to do");
+  TCH_CHECK_ARG(branch.ptr || (!n.post_weight && !n.gate && n.scale == 1.f), "residual_norm_fwd: a post norm, a gate and a scale go with a branch");
+  TCH_CHECK_ARG((n.weight || !n.bias) && (n.post_weight || !n.post_bias), "residual_norm_fwd: a bias goes with a weight");
+  TCH_CHECK_ARG((packed != nullptr) == (codes != nullptr) && (!packed || (y.ptr && format >= 0 && format < kPackFormats)),
+                "residual_norm_fwd: what is kept of y in 8 bits comes with its scales, and with y");
+  TCH_CHECK_ARG(n.gate || n.gates == 1, "residual_norm_fwd: gates without their values");
+  TCH_CHECK_ARG(n.eps >= 0.f, "residual_norm_fwd: eps must not be negative");
+  TCH_CHECK_ARG(fits(x, C, eb) && fits(branch, C, eb) && fits(total, C, eb) && fits(y, C, eb), "residual_norm_fwd: rows must start on 16-byte boundaries and not overlap");
+  TCH_CHECK_ARG(aligned({n.weight, n.bias, n.post_weight, n.post_bias, n.gate, stats, packed}),
+                "residual_norm_fwd: vectors, statistics and kept activations must start on a 16-byte boundary");
+  const int64_t gate_bytes = n.gates * C * (n.gate_f32 ? 4 : eb), groups32 = (C + kPackGroup - 1) / kPackGroup;
+  const Span in[7] = {{x.ptr, x.ld * eb, C * eb, rows}, {branch.ptr, branch.ld * eb, C * eb, rows}, {n.weight, C * 4, C * 4, 1}, {n.bias, C * 4, C * 4, 1},
+                      {n.post_weight, C * 4, C * 4, 1}, {n.post_bias, C * 4, C * 4, 1}, {n.gate, gate_bytes, gate_bytes, 1}};
+  const Span out[5] = {{total.ptr, total.ld * eb, C * eb, rows}, {y.ptr, y.ld * eb, C * eb, rows}, {stats, 16, 16, rows}, {packed, C, C, rows},
+                       {codes, groups32, groups32, rows}};
+  for (int o = 0; o < 5; ++o) {
+    bool ok = true;
+    for (int i = 0; i < 7; ++i) ok = ok && apart(out[o], in[i], o < 2 && i < 2);
+    for (int i = 0; i < o; ++i) ok = ok && apart(out[o], out[i]);
+    TCH_CHECK_ARG(ok, "residual_norm_fwd: an output overlaps another tensor (the sum and y may be x or the branch)");
+  }
+  const Shape s = shape_of(rows, static_cast<int>(C));
+  NormArgs a{};
+  a.x = {x.ptr, x.ld}, a.branch = {branch.ptr, branch.ld}, a.total = {total.ptr, total.ld}, a.y = {y.ptr, y.ld};
+  a.stats = reinterpret_cast<float4*>(stats);
+  a.weight = n.weight, a.bias = n.bias, a.post_weight = n.post_weight, a.post_bias = n.post_bias;
+  a.gate = n.gate, a.gate_f32 = n.gate_f32 || dtype == kF32, a.gate_rows = rows / n.gates;
+  a.packed = static_cast<unsigned char*>(packed), a.codes = static_cast<unsigned char*>(codes), a.format = format;
+  a.rows = rows, a.C = static_cast<int>(C);
+  a.waves = s.waves, a.groups = s.groups;
+  a.layer = n.layer, a.scale = n.scale, a.eps = n.eps;
+  const int64_t blocks = (rows + s.groups - 1) / s.groups;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 8192 / (s.threads / 64)))), block(s.threads);
+  const int br = !branch.ptr ? kNoBranch : n.post_weight ? kPostNorm : kBranch;
+  const double bytes = static_cast<double>(rows) * C * (eb * (1.0 + (branch.ptr ? 2 : 0) + (y.ptr ? 1 : 0)) + (packed ? 33.0 / 32 : 0));
+  if (dtype == kBF16)
+    return s.lanes == 16   ? launch_fwd<bf16, 16>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<bf16,16>", bytes)
+           : s.lanes == 32 ? launch_fwd<bf16, 32>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<bf16,32>", bytes)
+                           : launch_fwd<bf16, 64>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<bf16>", bytes);
+  return s.lanes == 16   ? launch_fwd<float, 16>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<f32,16>", bytes)
+         : s.lanes == 32 ? launch_fwd<float, 32>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<f32,32>", bytes)
+                         : launch_fwd<float, 64>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<f32>", bytes);
+}
+
+int64_t residual_norm_bwd_workspace_bytes(int64_t rows, int64_t C, int64_t gates) {
+  if (rows <= 0 || rows > INT_MAX || C <= 0 || C > kMaxWidth || gates < 1 || gates > rows || rows % gates != 0) return 0;
+  const Cut c = cut_rows(rows, static_cast<int>(C), gates);
+  return c.blocks * C * (gates > 1 && c.pieces > 1 ? 5 : 4) * 4;
+}
+
+int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows& dy, const Rows& dtotal, const Rows& total, const Rows& branch, const Rows& dx,
+                      const Rows& dbranch, const float* stats, const ResidualNormGrads& g, int accumulate, int64_t rows, int64_t C, void* workspace,
+                      int64_t workspace_bytes) {
+  if (int rc = check_shape("residual_norm_bwd", dtype, rows, C, n.gates)) return rc;
+  const int eb = dtype == kBF16 ? 2 : 4;
+  const int64_t grads[5] = {C, C, C, C, C * n.gates};
+  float* const grad[5] = {g.weight, g.bias, g.post_weight, g.post_bias, g.gate};
+  TCH_CHECK_ARG(aligned({n.weight, n.post_weight, n.post_bias, n.gate, stats, g.weight, g.bias, g.post_weight, g.post_bias, g.gate, workspace}),
+                "residual_norm_bwd: vectors, statistics and the workspace must start on a 16-byte boundary");
+  if (rows == 0) {
+    if (!accumulate)
+      for (int i = 0; i < 5; ++i)
+        if (grad[i])
+          if (int rc = fill_zero(ctx, grad[i], grads[i] * 4)) return rc;
+    return 0;
+  }
+  TCH_CHECK_ARG(stats && (n.weight != nullptr) == (dy.ptr != nullptr) && (!n.weight || total.ptr), "residual_norm_bwd: a norm's weight, the gradient of its output and the sum come together");
+  TCH_CHECK_ARG(n.weight || dtotal.ptr, "residual_norm_bwd: no gradient");
+  TCH_CHECK_ARG((branch.ptr != nullptr) == (dbranch.ptr != nullptr), "residual_norm_bwd: a branch and its gradient come together");
+  TCH_CHECK_ARG(branch.ptr || dx.ptr, "residual_norm_bwd: nothing to do");
+  TCH_CHECK_ARG(branch.ptr || (!n.post_weight && !n.gate && n.scale == 1.f), "residual_norm_bwd: a post norm, a gate and a scale go with a branch");
+  TCH_CHECK_ARG(n.gate || n.gates == 1, "residual_norm_bwd: gates without their values");
+  TCH_CHECK_ARG((n.weight || (!g.weight && !g.bias)) && (n.post_weight || (!g.post_weight && !g.post_bias && !n.post_bias)) && (n.gate || !g.gate),
+                "residual_norm_bwd: a gradient of what is not there");
+  TCH_CHECK_ARG(fits(dy, C, eb) && fits(dtotal, C, eb) && fits(total, C, eb) && fits(branch, C, eb) && fits(dx, C, eb) && fits(dbranch, C, eb),
+                "residual_norm_bwd: rows must start on 16-byte boundaries and not overlap");
+  const Cut cut = cut_rows(rows, static_cast<int>(C), n.gates);
+  const Shape& s = cut.shape;
+  const bool samples = n.gates > 1;
+  NormArgs a{};
+  a.planes = 0;
+  const bool shared = n.gate && !samples && g.gate;
+  const bool wanted[4] = {g.weight != nullptr, g.bias != nullptr, g.post_weight || shared, g.post_bias || (shared && n.post_bias)};
+  for (int i = 0; i < 4; ++i) a.plane_of[i] = wanted[i] ? a.planes++ : -1;
+  const bool gate_parts = samples && g.gate && cut.pieces > 1;
+  TCH_CHECK_ARG(n.gates <= 65533 || !gate_parts, "residual_norm_bwd: too many gates");
+  const int64_t sums_bytes = cut.blocks * C * 4 * a.planes, need = sums_bytes + (gate_parts ? cut.blocks * C * 4 : 0);
+  TCH_CHECK_ARG(need <= (workspace ? workspace_bytes : 0), "residual_norm_bwd: workspace too small");
+  const int64_t gate_bytes = n.gates * C * (n.gate_f32 ? 4 : eb);
+  auto rows_of = [&](const Rows& t) { return Span{t.ptr, t.ld * eb, C * eb, rows}; };
+  const Span in[9] = {rows_of(dy), rows_of(dtotal), rows_of(total), rows_of(branch), {n.weight, C * 4, C * 4, 1}, {n.post_weight, C * 4, C * 4, 1},
+                      {n.post_bias, C * 4, C * 4, 1}, {n.gate, gate_bytes, gate_bytes, 1}, {stats, 16, 16, rows}};
+  const Span out[8] = {rows_of(dx), rows_of(dbranch), {g.weight, C * 4, C * 4, 1}, {g.bias, C * 4, C * 4, 1}, {g.post_weight, C * 4, C * 4, 1},
+                       {g.post_bias, C * 4, C * 4, 1}, {g.gate, C * 4, C * 4, n.gates}, {workspace, need, need, need ? 1 : 0}};
+  for (int o = 0; o < 8; ++o) {
+    bool ok = true;
+    for (int i = 0; i < 9; ++i) ok = ok && apart(out[o], in[i], o < 2 && i < 4);
+    for (int i = 0; i < o; ++i) ok = ok && apart(out[o], out[i]);
+    TCH_CHECK_ARG(ok, "residual_norm_bwd: an output or the workspace overlaps another tensor (dx and dbranch may be dy, dtotal, the sum or the branch)");
+  }
+  a.dy = {dy.ptr, dy.ld}, a.dtotal = {dtotal.ptr, dtotal.ld}, a.total = {total.ptr, total.ld}, a.branch = {branch.ptr, branch.ld};
+  a.dx = {dx.ptr, dx.ld}, a.dbranch = {dbranch.ptr, dbranch.ld};
+  a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats));
+  a.weight = n.weight, a.post_weight = n.post_weight, a.post_bias = n.post_bias;
+  a.gate = n.gate, a.gate_f32 = n.gate_f32 || dtype == kF32, a.gate_rows = rows / n.gates;
+  a.gates = static_cast<int>(n.gates);
+  a.rows = rows, a.C = static_cast<int>(C);
+  a.group_rows = cut.group_rows, a.split_gates = cut.split, a.gates_each = cut.gates_each;
+  a.waves = s.waves, a.groups = s.groups;
+  a.layer = n.layer, a.scale = n.scale, a.eps = n.eps;
+  a.sums = static_cast<float*>(workspace);
+  float* const gate_parts_at = a.sums + sums_bytes / 4;
+  a.gate_sums = !samples || !g.gate ? nullptr : gate_parts ? gate_parts_at : g.gate;
+  a.add_gates = accumulate && !gate_parts;
+  const int br = !branch.ptr ? kNoBranch : n.post_weight ? kPostNorm : kBranch;
+  const double bytes = static_cast<double>(rows) * C * eb * ((dy.ptr ? 2.0 : 0) + (dtotal.ptr ? 1 : 0) + (dx.ptr ? 1 : 0) + (branch.ptr ? 2 : 0)) + need;
+  const dim3 grid(static_cast<unsigned>(cut.blocks)), block(s.threads);
+  int rc;
+  if (dtype == kBF16)
+    rc = s.lanes == 16   ? launch_bwd<bf16, 16>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<bf16,16>", bytes)
+         : s.lanes == 32 ? launch_bwd<bf16, 32>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<bf16,32>", bytes)
+                         : launch_bwd<bf16, 64>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<bf16>", bytes);
+  else
+    rc = s.lanes == 16   ? launch_bwd<float, 16>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<f32,16>", bytes)
+         : s.lanes == 32 ? launch_bwd<float, 32>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<f32,32>", bytes)
+                         : launch_bwd<float, 64>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<f32>", bytes);
+  if (rc || (a.planes == 0 && !gate_parts)) return rc;
+  NormSumArgs f{};
+  f.sums = a.sums, f.gate_sums = gate_parts_at;
+  f.post_weight = n.post_weight, f.post_bias = n.post_bias, f.post = n.post_weight != nullptr;
+  f.gate = samples ? nullptr : n.gate, f.gate_f32 = a.gate_f32;
+  f.dweight = g.weight, f.dbias = g.bias, f.dpost_weight = g.post_weight, f.dpost_bias = g.post_bias, f.dgate = g.gate;
+  f.C = static_cast<int>(C), f.blocks = static_cast<int>(cut.blocks), f.planes = a.planes;
+  for (int i = 0; i < 4; ++i) f.plane_of[i] = a.plane_of[i];
+  f.pieces = static_cast<int>(cut.pieces), f.shared_gate = !samples && n.gate != nullptr, f.add = accumulate;
+  const dim3 blocks(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(2 + (gate_parts ? n.gates : 0)));
+  return launch(ctx, residual_norm_sum_kernel, blocks, dim3(256), f, "residual_norm_sum_kernel", static_cast<double>(need), 1);
+}
+
+}  // namespace tch

@@ -1224,6 +1224,126 @@ def _rotary(ctx, x, y, freqs, head_dim, layout, positions, start, seq, scale, ba
                            head_dim, 2 * freqs.numel(), int(layout == "interleaved"), float(scale), int(back)), "tch_rotary")
 
 
+class Packed8:
+    """A tensor [rows, width] kept in 8 bits: data [rows, width] and scales [rows, ceil(width / 32)], uint8 on the GPU, contiguous.  32
+    neighbours of a row are multiples of 2^(scale - 127), as int8 or fp8 e4m3 numbers ("int8", "e4m3"); what comes back is exact in
+    bf16.  |x - kept| is at most half of 2^(scale - 127) for int8 (with the largest of the 32 above 63.5 of those), and for e4m3 the larger of
+    |x| / 16 and 2^(scale - 137).  A tensor's own buffers, so that whoever has a pool takes them from there; empty() makes new ones."""
+    FORMATS = {"int8": 0, "e4m3": 1}
+    GROUP = 32
+
+    def __init__(self, data, scales, format="int8"):
+        if format not in self.FORMATS:
+            raise ValueError(f"unknown 8-bit format {format!r}: one of {', '.join(self.FORMATS)}")
+        assert data.dim() == 2 and scales.dim() == 2 and data.dtype == scales.dtype == torch.uint8, "data and scales: matrices of uint8"
+        assert tuple(scales.shape) == (data.shape[0], -(-data.shape[1] // self.GROUP)), "a scale for every 32 neighbours of a row"
+        assert data.is_contiguous() and scales.is_contiguous() and data.device == scales.device, "data and scales: contiguous, on one device"
+        self.data, self.scales, self.format = data, scales, format
+
+    @classmethod
+    def empty(cls, rows, width, format="int8", device="cuda"):
+        new = lambda *shape: torch.empty(shape, dtype=torch.uint8, device=device)  # noqa: E731
+        return cls(new(rows, width), new(rows, -(-width // cls.GROUP)), format)
+
+    @property
+    def shape(self):
+        return self.data.shape
+
+    def nbytes(self):
+        return self.data.numel() + self.scales.numel()
+
+    def _args(self, ctx, name, rows, width):
+        assert tuple(self.data.shape) == (rows, width), f"{name}: {tuple(self.data.shape)} kept, {(rows, width)} wanted"
+        assert self.data.device == ctx.stream.device, f"{name} is not on the context's device"
+        return _p(self.data), _p(self.scales), self.FORMATS[self.format]
+
+
+def pack8(ctx, x, packed):
+    """packed = x [..., width] in 8 bits (Packed8): for what the backward pass reads again, in half or a quarter of its room."""
+    C = x.shape[-1]
+    xp, ldx, M = _matrix(ctx, "x", x, C)
+    check(lib().tch_pack8(ctx.handle, dtype_code(x), xp, ldx, *packed._args(ctx, "packed", M, C), None, 0, 0, M, C), "tch_pack8")
+
+
+def unpack8(ctx, packed, x):
+    """x = what is kept."""
+    C = x.shape[-1]
+    xp, ldx, M = _matrix(ctx, "x", x, C)
+    check(lib().tch_unpack8(ctx.handle, dtype_code(x), *packed._args(ctx, "packed", M, C), xp, ldx, M, C), "tch_unpack8")
+
+
+def act_fwd_pack8(ctx, pre, h, packed, act):
+    """h = act(pre) of the pre-activations as they are, and packed = pre in 8 bits for act_bwd_packed, in one pass.  h may be pre."""
+    C = pre.shape[-1]
+    pp, ldp, M = _matrix(ctx, "pre", pre, C)
+    hp, ldh, _ = _matrix(ctx, "h", h, C, M, pre.dtype)
+    assert h is not None, "h (pack8 keeps without an activation)"
+    check(lib().tch_pack8(ctx.handle, dtype_code(pre), pp, ldp, *packed._args(ctx, "packed", M, C), hp, ldh, _act_code(act), M, C), "tch_pack8")
+
+
+NORMS = {"rms": 0, "layer": 1}
+
+
+def _norm_args(ctx, kind, C, rows, dtype, gate):
+    if kind not in NORMS:
+        raise ValueError(f"unknown norm {kind!r}: one of {', '.join(NORMS)}")
+    if gate is None:
+        return None, 1, 1
+    gates = gate.numel() // C
+    assert gate.is_contiguous() and gate.numel() == gates * C and gate.shape[-1] == C and gates > 0, f"gate: rows of {C} numbers"
+    assert gate.dtype in (torch.float32, dtype) and gate.device == ctx.stream.device, f"gate: fp32 or {dtype}"
+    assert rows % gates == 0, f"gate: {rows} rows cannot share {gates} gates evenly"
+    return _p(gate), int(gate.dtype == torch.float32), gates
+
+
+def residual_norm_fwd(ctx, x, branch, total, y, stats, kind="rms", weight=None, bias=None, post_weight=None, post_bias=None, gate=None,
+                      scale=1.0, eps=1e-5, packed=None):
+    """The boundary between two blocks in one pass: total = scale * x + gate . post(branch), y = norm(total).  x, branch, total, y
+    [..., C]; kind: "rms" or "layer", of both norms; weight, bias, post_weight, post_bias [C] fp32.  Without post_weight the branch
+    is added as it is, without weight (and y) there is no norm behind the sum; branch and total None: y = norm(x).  gate: [C], or [samples, C]
+    where every sample has as many rows, fp32 or of x's type.  stats [rows, 4] fp32 is kept for residual_norm_bwd, as are branch and
+    total; packed (Packed8): y in 8 bits as well, for linear_wgrad_packed.  total and y may be x or branch."""
+    C = x.shape[-1]
+    xp, ldx, M = _matrix(ctx, "x", x, C)
+    bp, ldb, _ = _matrix(ctx, "branch", branch, C, M, x.dtype)
+    tp, ldt, _ = _matrix(ctx, "total", total, C, M, x.dtype)
+    yp, ldy, _ = _matrix(ctx, "y", y, C, M, x.dtype)
+    gp, gate_f32, gates = _norm_args(ctx, kind, C, M, x.dtype, gate)
+    kept = (None, None, 0) if packed is None else packed._args(ctx, "packed", M, C)
+    check(lib().tch_residual_norm_fwd(ctx.handle, dtype_code(x), NORMS[kind], xp, ldx, bp, ldb, tp, ldt, yp, ldy,
+                                      _vector(ctx, "stats", stats, 4 * M), _vector(ctx, "weight", weight, C), _vector(ctx, "bias", bias, C),
+                                      _vector(ctx, "post_weight", post_weight, C), _vector(ctx, "post_bias", post_bias, C), gp, gate_f32, gates,
+                                      float(scale), float(eps), *kept, M, C), "tch_residual_norm_fwd")
+
+
+def residual_norm_bwd_workspace_bytes(total, gate=None):
+    """Bytes of workspace of residual_norm_bwd for total [..., C] (the forward's x where there is no branch)."""
+    C = total.shape[-1]
+    gates = 1 if gate is None else gate.numel() // C
+    return max(int(lib().tch_residual_norm_bwd_workspace_bytes(total.numel() // C, C, gates)), 16)
+
+
+def residual_norm_bwd(ctx, dy, dtotal, total, branch, dx, dbranch, stats, kind="rms", weight=None, post_weight=None, post_bias=None, gate=None,
+                      scale=1.0, dweight=None, dbias=None, dpost_weight=None, dpost_bias=None, dgate=None, accumulate=False, workspace=None):
+    """The gradients of residual_norm_fwd from dy and dtotal (what the sum receives from elsewhere; either may be None): dx and
+    dbranch like x and branch, dweight, dbias, dpost_weight, dpost_bias [C] and dgate (like gate) fp32, each on request and (+)= with
+    accumulate; the same bits every run.  total: the forward's x where there is no branch.  dx and dbranch may be dy, dtotal, total or
+    branch.  workspace: residual_norm_bwd_workspace_bytes."""
+    shaped = next(t for t in (total, dy, dtotal) if t is not None)
+    C = shaped.shape[-1]
+    M = _matrix(ctx, "total", shaped, C)[2]
+    t = {name: _matrix(ctx, name, v, C, M, shaped.dtype)[:2]
+         for name, v in (("dy", dy), ("dtotal", dtotal), ("total", total), ("branch", branch), ("dx", dx), ("dbranch", dbranch))}
+    gp, gate_f32, gates = _norm_args(ctx, kind, C, M, shaped.dtype, gate)
+    ws, ws_bytes = _sums(ctx, "workspace", None, 0, workspace)[1:]
+    check(lib().tch_residual_norm_bwd(ctx.handle, dtype_code(shaped), NORMS[kind], *t["dy"], *t["dtotal"], *t["total"], *t["branch"], *t["dx"],
+                                      *t["dbranch"], _vector(ctx, "stats", stats, 4 * M), _vector(ctx, "weight", weight, C),
+                                      _vector(ctx, "post_weight", post_weight, C), _vector(ctx, "post_bias", post_bias, C), gp, gate_f32, gates,
+                                      float(scale), _vector(ctx, "dweight", dweight, C), _vector(ctx, "dbias", dbias, C),
+                                      _vector(ctx, "dpost_weight", dpost_weight, C), _vector(ctx, "dpost_bias", dpost_bias, C),
+                                      _vector(ctx, "dgate", dgate, gates * C), int(accumulate), M, C, ws, ws_bytes), "tch_residual_norm_bwd")
+
+
 def attn_softmax_fwd(ctx, scores, probs, scale=1.0, bias=None, mask=None, causal=False):
     """scores / probs [batch, heads, Lq, Lk]; bias [heads, Lq, Lk] fp32; mask [windows, Lq, Lk] fp32."""
     Bn, Hn, Lq, Lk = scores.shape

@@ -36,7 +36,7 @@ def oracle(x, freqs, head_dim, layout, positions, scale, back=False):
 
 def close(got, ref, tol, dtype):
     got = got.double().cpu()
-    bad = (got - ref).abs() > tol + ref.abs() * (torch.finfo(dtype).eps / 2) + torch.finfo(dtype).tiny
+    bad = ~((got - ref).abs() <= tol + ref.abs() * (torch.finfo(dtype).eps / 2) + torch.finfo(dtype).tiny)
     assert not bad.any(), (int(bad.sum()), float((got - ref).abs().max()))
 
 
