@@ -546,6 +546,13 @@ int tch_pack8(tch_context* ctx, int dtype, const void* x, int64_t ldx, void* dat
               int64_t ldh, int act, int64_t M, int64_t C);
 int tch_unpack8(tch_context* ctx, int dtype, const void* data, const void* scales, int format, void* x, int64_t ldx,
                 int64_t M, int64_t C);
+/* tch_act_bwd_bias (gated: tch_gated_act_bwd_bias with F = N, dy = dh, dz = dpre) from pre-activations kept in 8 bits: data [M][N]
+ * (gated [M][2N]) and scales as tch_pack8 leaves them.  h (may be NULL) [M][N] = act(pre), gated act(g) . u, of what is kept: the
+ * forward pass need not keep it.  dz may be dy.  Low parts, dbias and workspace as there. */
+int tch_act_bwd_packed(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* data, const void* scales,
+                       int format, void* dz, void* dz_low, int64_t lddz, void* h, int64_t ldh, float* dbias,
+                       int accumulate, int gated, int act, int64_t M, int64_t N, void* workspace,
+                       int64_t workspace_bytes);
 /* probs = softmax over the last dimension of scale * scores[batch, heads, Lq, Lk] + bias[heads, Lq, Lk]
  * + mask[windows, Lq, Lk] (window = batch index % windows); bias and mask may be NULL; causal != 0 keeps keys
  * j <= i only (Lq == Lk).  In place (probs == scores) is allowed. */

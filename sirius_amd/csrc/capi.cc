@@ -455,6 +455,13 @@ int tch_unpack8(tch_context* ctx, int dtype, const void* data, const void* scale
   return unpack8(C(ctx), dtype, data, scales, format, {x, ldx}, M, Cc);
 }
 
+int tch_act_bwd_packed(tch_context* ctx, int dtype, const void* dy, int64_t lddy, const void* data, const void* scales, int format, void* dz,
+                       void* dz_low, int64_t lddz, void* h, int64_t ldh, float* dbias, int accumulate, int gated, int act, int64_t M, int64_t N,
+                       void* workspace, int64_t workspace_bytes) {
+  return act_bwd_packed(C(ctx), dtype, {const_cast<void*>(dy), lddy}, data, scales, format, {dz, lddz}, dz_low, {h, ldh}, gated, act, M, N, dbias,
+                        accumulate, workspace, workspace_bytes);
+}
+
 int64_t tch_grad_table_piece_elems(void) { return grad_table_piece_elems(); }
 int64_t tch_grad_norm_workspace_bytes(int64_t pieces) { return grad_norm_workspace_bytes(pieces); }
 

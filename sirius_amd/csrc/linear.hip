@@ -11,6 +11,7 @@
 
 #include "context.h"
 #include "ops.h"
+#include "pack8.h"
 
 namespace tch {
 namespace {
@@ -35,31 +36,68 @@ struct ActBwdArgs {
   int64_t M, block_rows;
   int lanes_log;      // 2^lanes_log threads of a workgroup share a row
   int add;            // sums is added to
+  // pre-activations kept in 8 bits (pack8.h): z is [M][ldz] bytes
+  const unsigned char* codes;
+  int64_t code_groups;   // of a row
 };
 constexpr int kAtOnce = 4;
+constexpr int kDense = -1;   // z is of the tensors' type; otherwise a Pack8Format
+
+// the pre-activations of a chunk of dy
+template <typename T, int FORMAT>
+struct ActBwdZ {
+  static constexpr int E = Elem<T>::kPerChunk;
+  Chunk z;
+  __device__ __forceinline__ void request(const ActBwdArgs& p, int64_t row, uint32_t col, int64_t from) {
+    z.u = load_streaming_u4(static_cast<const T*>(p.z) + row * p.ldz + from, col);
+  }
+  __device__ __forceinline__ void get(float* v) const { chunk_to_float<T>(z, v); }
+};
+template <typename T, int FORMAT>
+struct ActBwdKept {
+  static constexpr int E = Elem<T>::kPerChunk;
+  uint32_t words[E / 4], code;
+  __device__ __forceinline__ void request(const ActBwdArgs& p, int64_t row, uint32_t col, int64_t from) {
+    const int64_t at = from + static_cast<int64_t>(col) * E;
+    const uint32_t* data = reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(p.z) + row * p.ldz + at);
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) words[i] = data[i];
+    code = p.codes[row * p.code_groups + at / kPackGroup];
+  }
+  __device__ __forceinline__ void get(float* v) const {
+    const float unit = pack8_unit(code);
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) unpack8_word<FORMAT>(words[i], unit, v + 4 * i);
+  }
+};
 
 // The chunks of one place: what is read, and the gradients from it, stored and (unrounded) returned in o and u.
-template <typename T, int GATED>
+template <typename T, int GATED, int FORMAT>
 struct ActBwdChunks {
   static constexpr int E = Elem<T>::kPerChunk;
-  Chunk dy, zg, zu;
+  Chunk dy;
+  std::conditional_t<FORMAT == kDense, ActBwdZ<T, FORMAT>, ActBwdKept<T, FORMAT>> zg, zu;
   __device__ __forceinline__ void request(const ActBwdArgs& p, int64_t row, uint32_t col) {
     dy.u = load_streaming_u4(static_cast<const T*>(p.dy) + row * p.lddy, col);
-    zg.u = load_streaming_u4(static_cast<const T*>(p.z) + row * p.ldz, col);
-    if (GATED) zu.u = load_streaming_u4(static_cast<const T*>(p.z) + row * p.ldz + p.N, col);
+    zg.request(p, row, col, 0);
+    if (GATED) zu.request(p, row, col, p.N);
   }
   template <int ACT>
   __device__ __forceinline__ void finish(const ActBwdArgs& p, int64_t row, uint32_t col, float* o, float* u) {
     float v[E], fg[E], fu[E], h[E];
     chunk_to_float<T>(dy, v);
-    chunk_to_float<T>(zg, fg);
-    if (GATED) chunk_to_float<T>(zu, fu);
+    zg.get(fg);
+    if (GATED) zu.get(fu);
     combine<T, GATED ? kGatedBwd : kLinBwd, ACT, E>(v, u, fg, fu, o, h);
     T* dz = static_cast<T*>(p.dz) + row * p.lddz;
     reinterpret_cast<uint4*>(dz)[col] = float_to_chunk<T>(o).u;
     if (GATED) {
       reinterpret_cast<uint4*>(dz + p.N)[col] = float_to_chunk<T>(u).u;
       if (p.h) reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row * p.ldh)[col] = float_to_chunk<T>(h).u;
+    } else if (FORMAT != kDense && p.h) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) h[e] = act_value<T, ACT>(fg[e]);
+      reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row * p.ldh)[col] = float_to_chunk<T>(h).u;
     }
     if constexpr (sizeof(T) == 2) {
       if (p.low) {
@@ -77,14 +115,14 @@ struct ActBwdChunks {
   }
 };
 
-template <typename T, int GATED>
+template <typename T, int GATED, int FORMAT = kDense>
 __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
   constexpr int E = Elem<T>::kPerChunk;
   with_activation(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * kAtOnce);
     for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * kAtOnce) + threadIdx.x; base < p.chunks; base += stride) {
-      ActBwdChunks<T, GATED> c[kAtOnce];
+      ActBwdChunks<T, GATED, FORMAT> c[kAtOnce];
       uint32_t row[kAtOnce], col[kAtOnce];
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
@@ -106,7 +144,7 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
 // The same with the column sums of the unrounded gradients, which are the bias gradient: added up from their rounded parts they would be as far off
 // as the parts (8192 rows: 2.5e-6 of the result; this way 1.1e-7).  A workgroup has a block of rows and 2^lanes_log chunks of columns; a thread walks down the
 // rows of its chunk, the threads of a column meet in LDS in their order, and the row blocks' sums are added up by a second launch.
-template <typename T, int GATED>
+template <typename T, int GATED, int FORMAT = kDense>
 __global__ __launch_bounds__(256) void act_bwd_sum_kernel(ActBwdArgs p) {
   constexpr int E = Elem<T>::kPerChunk, PARTS = GATED ? 2 : 1;
   __shared__ float meet[PARTS][256 * E];
@@ -120,7 +158,7 @@ __global__ __launch_bounds__(256) void act_bwd_sum_kernel(ActBwdArgs p) {
     constexpr int ACT = decltype(act_c)::value;
     if (col < p.row_chunks)
       for (int64_t base = row0 + line; base < behind; base += kAtOnce * lines) {
-        ActBwdChunks<T, GATED> c[kAtOnce];
+        ActBwdChunks<T, GATED, FORMAT> c[kAtOnce];
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
           if (base + i * lines < behind) c[i].request(p, base + i * lines, col);
@@ -246,6 +284,37 @@ int linear_launch(Context* ctx, const char* what, int dtype, int mode, LinearArg
   return dtype == kBF16 ? launch_linear_bf16(ctx, mode, a) : launch_linear_f32(ctx, mode, a);
 }
 
+// a derivative pass, with (SUMS) or without the column sums
+template <bool SUMS, typename T, int GATED, int FORMAT>
+int launch_act_bwd_of(Context* ctx, dim3 grid, const ActBwdArgs& a, double bytes) {
+  static const char* const names[2][2][2][3] = {
+      {{{"act_bwd_kernel<f32>", "act_bwd_kernel<f32,int8>", "act_bwd_kernel<f32,e4m3>"},
+        {"act_bwd_kernel<f32,gated>", "act_bwd_kernel<f32,gated,int8>", "act_bwd_kernel<f32,gated,e4m3>"}},
+       {{"act_bwd_kernel<bf16>", "act_bwd_kernel<bf16,int8>", "act_bwd_kernel<bf16,e4m3>"},
+        {"act_bwd_kernel<bf16,gated>", "act_bwd_kernel<bf16,gated,int8>", "act_bwd_kernel<bf16,gated,e4m3>"}}},
+      {{{"act_bwd_sum_kernel<f32>", "act_bwd_sum_kernel<f32,int8>", "act_bwd_sum_kernel<f32,e4m3>"},
+        {"act_bwd_sum_kernel<f32,gated>", "act_bwd_sum_kernel<f32,gated,int8>", "act_bwd_sum_kernel<f32,gated,e4m3>"}},
+       {{"act_bwd_sum_kernel<bf16>", "act_bwd_sum_kernel<bf16,int8>", "act_bwd_sum_kernel<bf16,e4m3>"},
+        {"act_bwd_sum_kernel<bf16,gated>", "act_bwd_sum_kernel<bf16,gated,int8>", "act_bwd_sum_kernel<bf16,gated,e4m3>"}}}};
+  const char* name = names[SUMS][sizeof(T) == 2][GATED][FORMAT + 1];
+  if constexpr (SUMS)
+    return launch(ctx, act_bwd_sum_kernel<T, GATED, FORMAT>, grid, dim3(256), a, name, bytes, 1);
+  else
+    return launch(ctx, act_bwd_kernel<T, GATED, FORMAT>, grid, dim3(256), a, name, bytes, 1);
+}
+template <bool SUMS, typename T, int GATED>
+int launch_act_bwd_format(Context* ctx, int format, dim3 grid, const ActBwdArgs& a, double bytes) {
+  if (format == kPackInt8) return launch_act_bwd_of<SUMS, T, GATED, kPackInt8>(ctx, grid, a, bytes);
+  if (format == kPackE4m3) return launch_act_bwd_of<SUMS, T, GATED, kPackE4m3>(ctx, grid, a, bytes);
+  return launch_act_bwd_of<SUMS, T, GATED, kDense>(ctx, grid, a, bytes);
+}
+template <bool SUMS>
+int launch_act_bwd(Context* ctx, int dtype, int gated, int format, dim3 grid, const ActBwdArgs& a, double bytes) {
+  if (dtype == kBF16)
+    return gated ? launch_act_bwd_format<SUMS, bf16, 1>(ctx, format, grid, a, bytes) : launch_act_bwd_format<SUMS, bf16, 0>(ctx, format, grid, a, bytes);
+  return gated ? launch_act_bwd_format<SUMS, float, 1>(ctx, format, grid, a, bytes) : launch_act_bwd_format<SUMS, float, 0>(ctx, format, grid, a, bytes);
+}
+
 }  // namespace
 
 int linear_fwd(Context* ctx, int dtype, const Rows& x, const void* w, const Rows& y, const float* bias, int act, const Rows& residual,
@@ -314,15 +383,21 @@ int64_t act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int gated) {
   return r.blocks > 1 ? r.blocks * N * (gated ? 2 : 1) * 4 : 0;
 }
 
-int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, void* dz_low, const Rows& h, int gated, int act, int64_t M,
-            int64_t N, float* dbias, int accumulate, void* workspace, int64_t workspace_bytes) {
+namespace {
+
+// pre: [M][N, gated 2 N] of the tensors' type, or kept in 8 bits (format >= 0: pre.ptr the numbers, dense, and `codes`)
+int act_bwd_launch(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const void* codes, int format, const Rows& dz, void* dz_low, const Rows& h,
+                   int gated, int act, int64_t M, int64_t N, float* dbias, int accumulate, void* workspace, int64_t workspace_bytes) {
   if (int rc = check_common("act_bwd", dtype, M, 16, N, act)) return rc;
   TCH_CHECK_ARG(dtype == kBF16 || !dz_low, "act_bwd: fp32 gradients are not rounded: there is no low part");
+  const bool kept = format != kDense;
   const int64_t wide = gated ? 2 : 1;
   if (M == 0) return dbias && !accumulate ? fill_zero(ctx, dbias, wide * N * 4) : 0;
   const int eb = dtype == kBF16 ? 2 : 4;
   TCH_CHECK_ARG(dy.ptr && pre.ptr && dz.ptr, "act_bwd: null tensor");
-  TCH_CHECK_ARG(rows_fit(dy.ptr, dy.ld, N, eb) && rows_fit(pre.ptr, pre.ld, wide * N, eb) && rows_fit(dz.ptr, dz.ld, wide * N, eb) &&
+  TCH_CHECK_ARG(!kept || (codes && (reinterpret_cast<uintptr_t>(pre.ptr) & 15) == 0 && wide * N < (1ll << 31)),
+                "act_bwd: kept pre-activations need their scales, and start on a 16-byte boundary");
+  TCH_CHECK_ARG(rows_fit(dy.ptr, dy.ld, N, eb) && (kept || rows_fit(pre.ptr, pre.ld, wide * N, eb)) && rows_fit(dz.ptr, dz.ld, wide * N, eb) &&
                     rows_fit(h.ptr, h.ld, N, eb) && rows_fit(dz_low, dz.ld, wide * N, eb),
                 "act_bwd: rows must start on 16-byte boundaries, not overlap, and be less than 4 MiB apart");
   TCH_CHECK_ARG(((reinterpret_cast<uintptr_t>(dbias) | reinterpret_cast<uintptr_t>(workspace)) & 3) == 0,
@@ -332,17 +407,25 @@ int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows
   const RowBlocks cut = row_blocks(M, row_chunks, workspace != nullptr);
   const int64_t sums_bytes = dbias && cut.blocks > 1 ? cut.blocks * wide * N * 4 : 0;
   TCH_CHECK_ARG(sums_bytes <= (workspace ? workspace_bytes : 0), "act_bwd: workspace too small");
-  const Span in[2] = {{dy.ptr, dy.ld * eb, N * eb, M}, {pre.ptr, pre.ld * eb, wide * N * eb, M}};
+  const int64_t groups = (wide * N + kPackGroup - 1) / kPackGroup;
+  const Span in[3] = {{dy.ptr, dy.ld * eb, N * eb, M},
+                      kept ? Span{pre.ptr, wide * N, wide * N, M} : Span{pre.ptr, pre.ld * eb, wide * N * eb, M},
+                      {codes, groups, groups, kept ? M : 0}};
   const Span out[5] = {{dz.ptr, dz.ld * eb, wide * N * eb, M}, {h.ptr, h.ld * eb, N * eb, M}, {dz_low, dz.ld * eb, wide * N * eb, M},
                        {dbias, wide * N * 4, wide * N * 4, 1}, {workspace, sums_bytes, sums_bytes, sums_bytes ? 1 : 0}};
   for (int o = 0; o < 5; ++o) {
-    bool ok = apart(out[o], in[0], o == 0) && apart(out[o], in[1], o == 0);
+    bool ok = apart(out[o], in[0], o == 0) && apart(out[o], in[1], o == 0 && !kept) && apart(out[o], in[2]);
     for (int i = 0; i < o; ++i) ok = ok && apart(out[o], out[i]);
     TCH_CHECK_ARG(ok, "act_bwd: an output overlaps another tensor (the gradient may be the one it is made of, or the pre-activations)");
   }
   ActBwdArgs a{dy.ptr, pre.ptr, dz.ptr, h.ptr, dz_low, dy.ld, pre.ld, dz.ld, h.ld, static_cast<uint32_t>(M * row_chunks), row_chunks, static_cast<int>(N), act,
                FastDiv(static_cast<uint32_t>(row_chunks))};
-  const double bytes = static_cast<double>(M) * N * eb * ((gated ? (h.ptr ? 6.0 : 5.0) : 3.0) + (dz_low ? wide : 0));
+  if (kept) {
+    a.ldz = wide * N;
+    a.codes = static_cast<const unsigned char*>(codes), a.code_groups = groups;
+  }
+  const double z_bytes = wide * (kept ? 33.0 / 32 : eb);
+  const double bytes = static_cast<double>(M) * N * (z_bytes + eb * (1.0 + wide + (h.ptr ? 1 : 0) + (dz_low ? wide : 0)));
   if (dbias) {
     const bool split = cut.blocks > 1;
     a.sums = split ? static_cast<float*>(workspace) : dbias;
@@ -350,25 +433,29 @@ int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows
     a.lanes_log = cut.lanes_log;
     a.add = accumulate && !split;
     const dim3 blocks(static_cast<unsigned>(cut.col_blocks), static_cast<unsigned>(cut.blocks));
-    int rc;
-    if (gated)
-      rc = dtype == kBF16 ? launch(ctx, act_bwd_sum_kernel<bf16, 1>, blocks, dim3(256), a, "act_bwd_sum_kernel<bf16,gated>", bytes, 1)
-                          : launch(ctx, act_bwd_sum_kernel<float, 1>, blocks, dim3(256), a, "act_bwd_sum_kernel<f32,gated>", bytes, 1);
-    else
-      rc = dtype == kBF16 ? launch(ctx, act_bwd_sum_kernel<bf16, 0>, blocks, dim3(256), a, "act_bwd_sum_kernel<bf16>", bytes, 1)
-                          : launch(ctx, act_bwd_sum_kernel<float, 0>, blocks, dim3(256), a, "act_bwd_sum_kernel<f32>", bytes, 1);
+    const int rc = launch_act_bwd<true>(ctx, dtype, gated, format, blocks, a, bytes);
     if (rc || !split) return rc;
     const int cols = static_cast<int>(wide * N);
     BiasSumArgs b{a.sums, dbias, cut.blocks, cols, accumulate};
     return launch(ctx, act_bwd_bias_kernel, dim3(static_cast<unsigned>((cols + 31) / 32)), dim3(256), b, "act_bwd_bias_kernel", 4.0 * cut.blocks * cols, 1);
   }
-  const int64_t groups = (M * row_chunks + 256 * kAtOnce - 1) / (256 * kAtOnce);
-  const dim3 grid(static_cast<unsigned>(groups < (1 << 20) ? groups : (1 << 20)));
-  if (gated)
-    return dtype == kBF16 ? launch(ctx, act_bwd_kernel<bf16, 1>, grid, dim3(256), a, "act_bwd_kernel<bf16,gated>", bytes, 1)
-                          : launch(ctx, act_bwd_kernel<float, 1>, grid, dim3(256), a, "act_bwd_kernel<f32,gated>", bytes, 1);
-  return dtype == kBF16 ? launch(ctx, act_bwd_kernel<bf16, 0>, grid, dim3(256), a, "act_bwd_kernel<bf16>", bytes, 1)
-                        : launch(ctx, act_bwd_kernel<float, 0>, grid, dim3(256), a, "act_bwd_kernel<f32>", bytes, 1);
+  const int64_t workgroups = (M * row_chunks + 256 * kAtOnce - 1) / (256 * kAtOnce);
+  const dim3 grid(static_cast<unsigned>(workgroups < (1 << 20) ? workgroups : (1 << 20)));
+  return launch_act_bwd<false>(ctx, dtype, gated, format, grid, a, bytes);
+}
+
+}  // namespace
+
+int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, void* dz_low, const Rows& h, int gated, int act, int64_t M,
+            int64_t N, float* dbias, int accumulate, void* workspace, int64_t workspace_bytes) {
+  return act_bwd_launch(ctx, dtype, dy, pre, nullptr, kDense, dz, dz_low, h, gated, act, M, N, dbias, accumulate, workspace, workspace_bytes);
+}
+
+int act_bwd_packed(Context* ctx, int dtype, const Rows& dy, const void* data, const void* codes, int format, const Rows& dz, void* dz_low, const Rows& h,
+                   int gated, int act, int64_t M, int64_t N, float* dbias, int accumulate, void* workspace, int64_t workspace_bytes) {
+  TCH_CHECK_ARG(format >= 0 && format < kPackFormats, "act_bwd_packed: unknown 8-bit format");
+  return act_bwd_launch(ctx, dtype, dy, {const_cast<void*>(data), 0}, codes, format, dz, dz_low, h, gated, act, M, N, dbias, accumulate, workspace,
+                        workspace_bytes);
 }
 
 }  // namespace tch

@@ -204,6 +204,9 @@ int linear_dgrad_gated(Context* ctx, int dtype, const Rows& dy, const void* wt, 
 int64_t act_bwd_workspace_bytes(int dtype, int64_t M, int64_t N, int gated);
 int act_bwd(Context* ctx, int dtype, const Rows& dy, const Rows& pre, const Rows& dz, void* dz_low, const Rows& h, int gated, int act, int64_t M,
             int64_t N, float* dbias = nullptr, int accumulate = 0, void* workspace = nullptr, int64_t workspace_bytes = 0);
+// the same from pre-activations kept in 8 bits (pack8), with h = act(pre) again on request for the layer that is not gated too
+int act_bwd_packed(Context* ctx, int dtype, const Rows& dy, const void* data, const void* codes, int format, const Rows& dz, void* dz_low, const Rows& h,
+                   int gated, int act, int64_t M, int64_t N, float* dbias, int accumulate, void* workspace, int64_t workspace_bytes);
 
 // linear_wgrad.hip -- weight and bias gradients of bf16 linear layers, of an operand and its low part on request
 int64_t linear_wgrad_workspace_bytes(int64_t M, int64_t K, int64_t N);

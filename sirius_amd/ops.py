@@ -1281,6 +1281,55 @@ def act_fwd_pack8(ctx, pre, h, packed, act):
     check(lib().tch_pack8(ctx.handle, dtype_code(pre), pp, ldp, *packed._args(ctx, "packed", M, C), hp, ldh, _act_code(act), M, C), "tch_pack8")
 
 
+def act_bwd_packed(ctx, dy, packed, dz, act, h=None, dz_low=None, dbias=None, accumulate=False, workspace=None):
+    """act_bwd from pre-activations kept in 8 bits (act_fwd_pack8): dz = dy . act'(kept); h (like dy): act(kept), where the forward
+    pass did not keep it.  dz may be dy; the rest as for act_bwd."""
+    _act_bwd_packed(ctx, dy, packed, dz, act, h, dz_low, dbias, accumulate, workspace, 0)
+
+
+def gated_act_bwd_packed(ctx, dh, packed, dpre, act="silu", h=None, dpre_low=None, dbias=None, accumulate=False, workspace=None):
+    """gated_act_bwd from (g | u) kept in 8 bits (pack8 of gated_linear_fwd's pre): dpre [..., 2F] from dh [..., F], h = act(g) . u
+    again; the rest as there."""
+    _act_bwd_packed(ctx, dh, packed, dpre, act, h, dpre_low, dbias, accumulate, workspace, 1)
+
+
+def _act_bwd_packed(ctx, dy, packed, dz, act, h, dz_low, dbias, accumulate, workspace, gated):
+    N = dy.shape[-1]
+    wide = N * (1 + gated)
+    dyp, lddy, M = _matrix(ctx, "dy", dy, N)
+    dzp, lddz, _ = _matrix(ctx, "dz", dz, wide, M, dy.dtype)
+    hp, ldh, _ = _matrix(ctx, "h", h, N, M, dy.dtype)
+    sums, ws, ws_bytes = _sums(ctx, "dbias", dbias, wide, workspace)
+    check(lib().tch_act_bwd_packed(ctx.handle, dtype_code(dy), dyp, lddy, *packed._args(ctx, "packed", M, wide), dzp, _low(ctx, "dz_low", dz_low, dz),
+                                   lddz, hp, ldh, sums, int(accumulate), gated, _act_code(act), M, N, ws, ws_bytes), "tch_act_bwd_packed")
+
+
+def _unpacked_bytes(packed, dy):
+    return -(-packed.data.numel() * dy.element_size() // 256) * 256
+
+
+def linear_wgrad_packed_workspace_bytes(packed, dy):
+    """Bytes of workspace that linear_wgrad_packed wants."""
+    M, K = packed.shape
+    N = dy.shape[-1]
+    like = torch.empty(1, dtype=dy.dtype).expand(M, K)
+    return _unpacked_bytes(packed, dy) + linear_bwd_workspace_bytes(like, N)
+
+
+def linear_wgrad_packed(ctx, packed, dy, dw, dbias=None, accumulate=False, workspace=None, dy_low=None):
+    """linear_wgrad from a layer's input kept in 8 bits (pack8, or residual_norm_fwd's packed): dw (+)= dy^T kept and dbias (+)= column
+    sums of dy, both fp32, dy [..., N] contiguous.  What is kept is exact in bf16: dw is the gradient for the kept input, no rounding
+    added.  workspace: linear_wgrad_packed_workspace_bytes; dy_low as for linear_wgrad."""
+    M, K = packed.shape
+    room = _unpacked_bytes(packed, dy)
+    assert workspace is not None and workspace.is_contiguous() and workspace.device == ctx.stream.device, "workspace: contiguous, on the context's device"
+    space = workspace.view(-1).view(torch.uint8)
+    assert space.numel() >= linear_wgrad_packed_workspace_bytes(packed, dy), "linear_wgrad_packed workspace too small"
+    x = space[:M * K * dy.element_size()].view(dy.dtype).view(M, K)
+    unpack8(ctx, packed, x)
+    linear_wgrad(ctx, x, dy, dw, dbias=dbias, accumulate=accumulate, workspace=space[room:], dy_low=dy_low)
+
+
 NORMS = {"rms": 0, "layer": 1}
 
 

@@ -52,3 +52,34 @@ def test_wrapper():
             ops.Packed8(data, scales)
     p = ops.Packed8.empty(3, 70, "e4m3", device="cpu")
     assert p.scales.shape == (3, 3) and p.nbytes() == 219 and tuple(p.shape) == (3, 70)
+
+
+def act(dtype=BF16, dy=A, lddy=64, data=B, scales=C, format=0, dz=D, dz_low=None, lddz=64, h=None, ldh=0, dbias=None, accumulate=0, gated=0, act=4, M=4, N=64,
+        ws=None, ws_bytes=0):
+    from sirius_amd._lib import lib
+    return lib().tch_act_bwd_packed(None, dtype, dy, lddy, data, scales, format, dz, dz_low, lddz, h, ldh, dbias, accumulate, gated, act, M, N, ws, ws_bytes)
+
+
+@pytest.mark.parametrize("change", [
+    dict(dtype=2), dict(format=2), dict(format=-1), dict(act=7), dict(M=-1), dict(N=60), dict(N=0), dict(dy=None), dict(data=None), dict(scales=None), dict(dz=None),
+    dict(dtype=F32, dz_low=ctypes.c_void_p(0x5000000)), dict(dy=ODD), dict(data=ODD), dict(dz=ODD), dict(lddy=56), dict(gated=1), dict(h=ODD, ldh=64), dict(h=D, ldh=64),
+    dict(dz=B), dict(dz=C), dict(h=B, ldh=64), dict(h=A, ldh=64), dict(dbias=B), dict(M=1 << 30, N=1024, lddy=1024, lddz=1024)], ids=str)
+def test_derivatives(change):
+    assert act(**change) == -22 and "act_bwd" in last()
+
+
+def test_weight_gradient_wrapper():
+    from sirius_amd import ops
+    packed, dy = ops.Packed8.empty(16, 64, device="cpu"), torch.zeros(16, 32, dtype=torch.bfloat16)
+    assert ops.linear_wgrad_packed_workspace_bytes(packed, dy) >= 4
+    assert ops.linear_wgrad_packed_workspace_bytes(ops.Packed8.empty(0, 64, device="cpu"), dy[:0]) >= 4
+
+    class Here:
+        handle = None
+
+        class stream:
+            device = torch.device("cpu")
+    with pytest.raises(AssertionError, match="workspace"):
+        ops.linear_wgrad_packed(Here, packed, dy, torch.zeros(32, 64))
+    with pytest.raises(AssertionError, match="workspace"):
+        ops.linear_wgrad_packed(Here, packed, dy, torch.zeros(32, 64), workspace=torch.zeros(2, dtype=torch.uint8))
