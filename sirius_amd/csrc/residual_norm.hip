@@ -54,7 +54,7 @@ struct NormArgs {
   float scale, eps;
   // backward
   float* sums;                            // [workgroups][planes][C]
-  float* gate_sums;                       // [workgroups][C], or the gradient of the gates itself
+  float* dgate;                           // [gates][C]: written here where a workgroup has all rows of its gates
   int planes, plane_of[4];                // -1: nobody wants it
   int split_gates;                        // several workgroups have a part of a gate's rows
   int gates_each;                         // otherwise: gates of a workgroup
@@ -71,8 +71,9 @@ __device__ __forceinline__ float lane_sum(float v) {
   plus(std::integral_constant<int, 0x4e>{});     // lane ^ 2
   plus(std::integral_constant<int, 0x141>{});    // the other half of eight
   plus(std::integral_constant<int, 0x140>{});    // the other half of sixteen
-  if constexpr (L > 16) v += __shfl_xor(v, 16, 64);
-  if constexpr (L > 32) v += __shfl_xor(v, 32, 64);
+  auto both = [&](auto r) { v = __uint_as_float(r[0]) + __uint_as_float(r[1]); };
+  if constexpr (L > 16) both(__builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  if constexpr (L > 32) both(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
   return v;
 }
 
@@ -80,37 +81,44 @@ __device__ __forceinline__ float lane_sum(float v) {
 struct Meeting {
   float2 (*said)[16];
   int turn, first, waves, lane, wave;
-  __device__ __forceinline__ const float2* say(float a, float b) {
+  // what wavefront lane % 16 of the row said; 0 of one that is not there
+  __device__ __forceinline__ float2 say(float a, float b) {
     float2* here = said[turn];
     turn ^= 1;
     if (lane == 0) here[wave] = make_float2(a, b);
     __syncthreads();
-    return here + first;
+    return (lane & 15) < waves ? here[first + (lane & 15)] : make_float2(0.f, 0.f);
   }
   // both sums over the row, of sums over the wavefronts
   __device__ __forceinline__ void add(float& a, float& b) {
     if (waves == 1) return;
-    const float2* h = say(a, b);
-    a = b = 0.f;
-    for (int w = 0; w < waves; ++w) a += h[w].x, b += h[w].y;
+    const float2 h = say(a, b);
+    a = lane_sum<16>(h.x);
+    b = lane_sum<16>(h.y);
   }
 };
 
+// Whether element e of a lane's eight is there: bf16 rows are whole eights, fp32 rows whole fours.
+template <typename T>
+__device__ __forceinline__ bool there(int live, int e) {
+  return live > (sizeof(T) == 2 || e < 4 ? 0 : 4);
+}
+
 // mean and 1 / deviation of a row
-template <int L>
+template <typename T, int L>
 __device__ __forceinline__ float2 row_stats(const float* v, int live, int layer, const NormArgs& p, Meeting& meet, int row_wave) {
   const float inv = 1.f / static_cast<float>(p.C);
   if (!layer) {
     float q = 0.f, none = 0.f;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) q = e < live ? fmaf(v[e], v[e], q) : q;
+    for (int e = 0; e < kEach; ++e) q = there<T>(live, e) ? fmaf(v[e], v[e], q) : q;
     q = lane_sum<L>(q);
     meet.add(q, none);
     return make_float2(0.f, 1.f / sqrtf(q * inv + p.eps));
   }
   float s = 0.f;
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) s += e < live ? v[e] : 0.f;
+  for (int e = 0; e < kEach; ++e) s += there<T>(live, e) ? v[e] : 0.f;
   s = lane_sum<L>(s);
   auto elements = [&](int w) { return static_cast<float>(min(p.C - w * 64 * kEach, 64 * kEach)); };   // of a wavefront
   const float n = L < 64 ? static_cast<float>(p.C) : elements(row_wave), mine = s / n;
@@ -118,19 +126,15 @@ __device__ __forceinline__ float2 row_stats(const float* v, int live, int layer,
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const float d = v[e] - mine;
-    q = e < live ? fmaf(d, d, q) : q;
+    q = there<T>(live, e) ? fmaf(d, d, q) : q;
   }
   q = lane_sum<L>(q);
   if (meet.waves == 1) return make_float2(mine, 1.f / sqrtf(q * inv + p.eps));
-  const float2* h = meet.say(s, q);
-  float mean = 0.f;
-  for (int w = 0; w < meet.waves; ++w) mean += h[w].x;
-  mean *= inv;
-  q = 0.f;
-  for (int w = 0; w < meet.waves; ++w) {
-    const float m = elements(w), d = h[w].x / m - mean;
-    q += fmaf(m * d, d, h[w].y);
-  }
+  const float2 h = meet.say(s, q);
+  const float mean = lane_sum<16>(h.x) * inv;
+  const int w = meet.lane & 15;
+  const float m = elements(w), d = h.x / m - mean;
+  q = lane_sum<16>(w < meet.waves ? fmaf(m * d, d, h.y) : 0.f);
   return make_float2(mean, 1.f / sqrtf(q * inv + p.eps));
 }
 
@@ -205,8 +209,9 @@ __device__ __forceinline__ Place place(const NormArgs& p) {
   return a;
 }
 
-template <typename T, int L, int BR>
-__global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_fwd_kernel(NormArgs p) {
+// WIDE: rows of more than eight wavefronts
+template <typename T, int L, bool WIDE, int BR>
+__global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_norm_fwd_kernel(NormArgs p) {
   __shared__ float2 said[2][16];
   const Place at = place<L>(p);
   Meeting meet{said, 0, at.group * p.waves, p.waves, at.lane, at.wave};
@@ -238,7 +243,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_fwd_kernel(
     request(row + step);
     float4 stats = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (BR == kPostNorm) {
-      const float2 s = row_stats<L>(n, at.live, p.layer, p, meet, at.row_wave);
+      const float2 s = row_stats<T, L>(n, at.live, p.layer, p, meet, at.row_wave);
       stats.x = s.x, stats.y = s.y;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) n[e] = fmaf((n[e] - s.x) * s.y, pw[e], pb[e]);
@@ -252,7 +257,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_fwd_kernel(
       sum.get(t);
     }
     if (p.weight) {
-      const float2 s = row_stats<L>(t, at.live, p.layer, p, meet, at.row_wave);
+      const float2 s = row_stats<T, L>(t, at.live, p.layer, p, meet, at.row_wave);
       stats.z = s.x, stats.w = s.y;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) t[e] = fmaf((t[e] - s.x) * s.y, w[e], c[e]);
@@ -273,26 +278,25 @@ __global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_fwd_kernel(
   }
 }
 
-// SAMPLES: gates of their own for runs of rows
-template <typename T, int L, int BR, bool SAMPLES>
-__global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_bwd_kernel(NormArgs p) {
-  constexpr int kLds = L < 64 ? 256 * kEach : 512 * kEach;   // (more threads have one row at a time, and nothing to add up here)
+// MANY: several gates' rows in a workgroup, so that what each gate has to itself is taken here.  Otherwise a workgroup's rows have one gate,
+// and the sums of dt and dt b^ go out as they are: what a gate makes of them the second launch does, once for all of a gate's rows.
+template <typename T, int L, bool WIDE, int BR, bool MANY>
+__global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_norm_bwd_kernel(NormArgs p) {
+  constexpr int kLds = L < 64 ? 256 * kEach : WIDE ? 1 : 512 * kEach;   // (a wide row's workgroup has one row at a time, and nothing to add up here)
   __shared__ float2 said[2][16];
   __shared__ float lds[kLds];
   const Place at = place<L>(p);
   Meeting meet{said, 0, at.group * p.waves, p.waves, at.lane, at.wave};
   const float inv = 1.f / static_cast<float>(p.C);
-  float w[kEach], pw[kEach], g[kEach];
+  float w[kEach], k2[kEach];   // k2: what dt is multiplied by in front of the post norm, g . pw; the gate where there is none
   load_vector(p.weight, at.col, at.live, 0.f, w);
-  if constexpr (BR == kPostNorm) load_vector(p.post_weight, at.col, at.live, 0.f, pw);
-  if constexpr (BR != kNoBranch) load_gate<T>(p, 0, at.col, at.live, g);
   float sum[4][kEach], gated[2][kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) sum[0][e] = sum[1][e] = sum[2][e] = sum[3][e] = gated[0][e] = gated[1][e] = 0.f;
 
   // The lanes' eight sums over the row groups of the workgroup, to `to` [C].
   auto add_up = [&](const float* v, float* to, bool add) {
-    if (p.groups == 1) {
+    if (WIDE || p.groups == 1) {
 #pragma unroll
       for (int i = 0; i < kEach; i += 4) {
         if (i >= at.live) break;
@@ -332,7 +336,15 @@ __global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_bwd_kernel(
   for (; gate < behind_gate; ++gate) {
     const int64_t r0 = gate * p.gate_rows + offset;
     const int64_t r1 = min(p.split_gates ? r0 + p.group_rows : r0 + p.gate_rows, min((gate + 1) * p.gate_rows, p.rows));
-    if constexpr (SAMPLES) load_gate<T>(p, gate, at.col, at.live, g);
+    if constexpr (BR != kNoBranch) {
+      load_gate<T>(p, gate, at.col, at.live, k2);
+      if constexpr (BR == kPostNorm) {
+        float pw[kEach];
+        load_vector(p.post_weight, at.col, at.live, 0.f, pw);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) k2[e] *= pw[e];
+      }
+    }
     Eight<T> dy, d0, t, b;
     float4 stats, next_stats;
     auto request = [&](int64_t row) {
@@ -392,17 +404,16 @@ __global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_bwd_kernel(
       if constexpr (BR != kNoBranch) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-          if (e >= live) d[e] = 0.f;
+          if (!there<T>(live, e)) d[e] = 0.f;
           if constexpr (BR == kPostNorm) bh[e] = (bh[e] - stats.x) * stats.y;
           sum[2][e] = fmaf(d[e], bh[e], sum[2][e]);
           sum[3][e] += d[e];
-          k[e] = d[e] * g[e];
+          k[e] = d[e] * k2[e];
         }
         if constexpr (BR == kPostNorm) {
           float a = 0.f, q = 0.f;
 #pragma unroll
           for (int e = 0; e < kEach; ++e) {
-            k[e] *= pw[e];
             a += k[e];
             q = fmaf(k[e], bh[e], q);
           }
@@ -419,21 +430,23 @@ __global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_bwd_kernel(
         db.store(p.dbranch, row, at.col, live);
       }
     }
-    if constexpr (SAMPLES) {
+    if constexpr (MANY) {
       // dg of these rows, and what the post norm's gradients have from them
-      float dg[kEach], post[kEach];
-      load_vector(p.post_bias, at.col, at.live, 0.f, post);
+      float g[kEach], dg[kEach], pw[kEach], pb[kEach];
+      load_gate<T>(p, gate, at.col, at.live, g);
+      load_vector(p.post_weight, at.col, at.live, 1.f, pw);
+      load_vector(p.post_bias, at.col, at.live, 0.f, pb);
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
-        dg[e] = BR == kPostNorm ? fmaf(pw[e], sum[2][e], post[e] * sum[3][e]) : sum[2][e];
+        dg[e] = fmaf(pw[e], sum[2][e], pb[e] * sum[3][e]);
         gated[0][e] = fmaf(g[e], sum[2][e], gated[0][e]);
         gated[1][e] = fmaf(g[e], sum[3][e], gated[1][e]);
         sum[2][e] = sum[3][e] = 0.f;
       }
-      if (p.gate_sums) add_up(dg, p.gate_sums + static_cast<int64_t>(p.split_gates ? static_cast<int>(blockIdx.x) : gate) * p.C, p.add_gates);
+      if (p.dgate) add_up(dg, p.dgate + static_cast<int64_t>(gate) * p.C, p.add_gates);
     }
   }
-  if constexpr (SAMPLES) {
+  if constexpr (MANY) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) sum[2][e] = gated[0][e], sum[3][e] = gated[1][e];
   }
@@ -443,41 +456,44 @@ __global__ __launch_bounds__(L < 64 ? 256 : 1024) void residual_norm_bwd_kernel(
 }
 
 // The workgroups' sums added up: 32 columns a workgroup, eight threads a column, in fp64 in a fixed order.  blockIdx.y 0: the norm's two
-// gradients; 1: those of the post norm, and of a gate that all rows share; 2 and on: of a sample's gate.
+// gradients; 1: those of the post norm; 2 and on: of gate blockIdx.y - 2.
 struct NormSumArgs {
   const float* sums;
-  const float* gate_sums;
   const float* post_weight;
   const float* post_bias;
-  const void* gate;         // shared by all rows, or null
+  const void* gate;         // [gates][C] where the sums are still without it, or null
   float* dweight;
   float* dbias;
   float* dpost_weight;
   float* dpost_bias;
   float* dgate;
   int C, blocks, planes, plane_of[4];
-  int pieces;               // of a sample's gate
-  int post, shared_gate, gate_f32, add;
+  int pieces;               // workgroups of a gate's rows
+  int gate_f32, add;
 };
 __global__ __launch_bounds__(256) void residual_norm_sum_kernel(NormSumArgs p) {
   __shared__ double meet[2][8][32];
   const int lane = threadIdx.x & 31, line = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, job = blockIdx.y;
   double s[2] = {0.0, 0.0};
   if (c < p.C) {
-    if (job < 2) {
+    const int first = job < 2 ? 0 : (job - 2) * p.pieces, behind = job < 2 ? p.blocks : first + p.pieces;
+    const int64_t ld = static_cast<int64_t>(p.planes) * p.C;
+    auto gate_of = [&](int b) {
+      const int64_t i = static_cast<int64_t>(b / p.pieces) * p.C + c;
+      return p.gate_f32 ? static_cast<const float*>(p.gate)[i] : Elem<bf16>::load(static_cast<const bf16*>(p.gate) + i);
+    };
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int plane = p.plane_of[2 * job + i];
-        if (plane < 0) continue;
-        const float* from = p.sums + static_cast<int64_t>(plane) * p.C + c;
-        const int64_t ld = static_cast<int64_t>(p.planes) * p.C;
+    for (int i = 0; i < 2; ++i) {
+      const int plane = p.plane_of[(job == 0 ? 0 : 2) + i];
+      if (plane < 0) continue;
+      const float* from = p.sums + static_cast<int64_t>(plane) * p.C + c;
+      if (job == 1 && p.gate) {
 #pragma unroll 8
-        for (int b = line; b < p.blocks; b += 8) s[i] += from[b * ld];
+        for (int b = first + line; b < behind; b += 8) s[i] += static_cast<double>(gate_of(b)) * from[b * ld];
+      } else {
+#pragma unroll 8
+        for (int b = first + line; b < behind; b += 8) s[i] += from[b * ld];
       }
-    } else {
-      const float* from = p.gate_sums + static_cast<int64_t>(job - 2) * p.pieces * p.C + c;
-#pragma unroll 8
-      for (int b = line; b < p.pieces; b += 8) s[0] += from[static_cast<int64_t>(b) * p.C];
     }
   }
   meet[0][line][lane] = s[0];
@@ -493,28 +509,23 @@ __global__ __launch_bounds__(256) void residual_norm_sum_kernel(NormSumArgs p) {
     put(p.dweight, c, s[0]);
     put(p.dbias, c, s[1]);
   } else if (job == 1) {
-    double g = 1.0;
-    if (p.shared_gate) {
-      if (p.gate) g = p.gate_f32 ? static_cast<const float*>(p.gate)[c] : Elem<bf16>::load(static_cast<const bf16*>(p.gate) + c);
-      const double w = p.post ? p.post_weight[c] : 1.0, b = p.post_bias ? p.post_bias[c] : 0.0;
-      put(p.dgate, c, w * s[0] + b * s[1]);
-    }
-    put(p.dpost_weight, c, g * s[0]);
-    put(p.dpost_bias, c, g * s[1]);
+    put(p.dpost_weight, c, s[0]);
+    put(p.dpost_bias, c, s[1]);
   } else {
-    put(p.dgate, static_cast<int64_t>(job - 2) * p.C + c, s[0]);
+    const double w = p.post_weight ? p.post_weight[c] : 1.0, b = p.post_bias ? p.post_bias[c] : 0.0;
+    put(p.dgate, static_cast<int64_t>(job - 2) * p.C + c, w * s[0] + b * s[1]);
   }
 }
 
 struct Shape {
   int lanes, waves, groups, threads;   // lanes: 16, 32, or 64 (as many wavefronts as it takes)
 };
-// As many rows at a time as make eight wavefronts, where there are that many.
+// As many rows at a time as make four wavefronts, where there are that many.
 Shape shape_of(int64_t rows, int C) {
   if (C <= 16 * kEach) return {16, 1, 16, 256};
   if (C <= 32 * kEach) return {32, 1, 8, 256};
   const int waves = (C + 64 * kEach - 1) / (64 * kEach);
-  const int groups = static_cast<int>(std::min<int64_t>(std::max(8 / waves, 1), std::max<int64_t>(rows, 1)));
+  const int groups = static_cast<int>(std::min<int64_t>(std::max(4 / waves, 1), std::max<int64_t>(rows, 1)));
   return {64, waves, groups, waves * groups * 64};
 }
 
@@ -555,21 +566,42 @@ bool aligned(std::initializer_list<const void*> all) {
   return (bits & 15) == 0;
 }
 
-template <typename T, int L>
+template <typename T, int L, bool WIDE>
 int launch_fwd(Context* ctx, const NormArgs& a, int br, dim3 grid, dim3 block, const char* name, double bytes) {
-  if (br == kNoBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, kNoBranch>, grid, block, a, name, bytes, 1);
-  if (br == kBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, kBranch>, grid, block, a, name, bytes, 1);
-  return launch(ctx, residual_norm_fwd_kernel<T, L, kPostNorm>, grid, block, a, name, bytes, 1);
+  if (br == kNoBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kNoBranch>, grid, block, a, name, bytes, 1);
+  if (br == kBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kBranch>, grid, block, a, name, bytes, 1);
+  return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kPostNorm>, grid, block, a, name, bytes, 1);
 }
-template <typename T, int L>
-int launch_bwd(Context* ctx, const NormArgs& a, int br, bool samples, dim3 grid, dim3 block, const char* name, double bytes) {
-  if (br == kNoBranch) return launch(ctx, residual_norm_bwd_kernel<T, L, kNoBranch, false>, grid, block, a, name, bytes, 1);
+template <typename T>
+int launch_fwd_of(Context* ctx, const NormArgs& a, const Shape& s, int br, dim3 grid, const char* const* names, double bytes) {
+  const dim3 block(s.threads);
+  if (s.lanes == 16) return launch_fwd<T, 16, false>(ctx, a, br, grid, block, names[0], bytes);
+  if (s.lanes == 32) return launch_fwd<T, 32, false>(ctx, a, br, grid, block, names[1], bytes);
+  return s.waves > 8 ? launch_fwd<T, 64, true>(ctx, a, br, grid, block, names[3], bytes) : launch_fwd<T, 64, false>(ctx, a, br, grid, block, names[2], bytes);
+}
+template <typename T, int L, bool WIDE>
+int launch_bwd(Context* ctx, const NormArgs& a, int br, bool many, dim3 grid, dim3 block, const char* name, double bytes) {
+  if (br == kNoBranch) return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kNoBranch, false>, grid, block, a, name, bytes, 1);
   if (br == kBranch)
-    return samples ? launch(ctx, residual_norm_bwd_kernel<T, L, kBranch, true>, grid, block, a, name, bytes, 1)
-                   : launch(ctx, residual_norm_bwd_kernel<T, L, kBranch, false>, grid, block, a, name, bytes, 1);
-  return samples ? launch(ctx, residual_norm_bwd_kernel<T, L, kPostNorm, true>, grid, block, a, name, bytes, 1)
-                 : launch(ctx, residual_norm_bwd_kernel<T, L, kPostNorm, false>, grid, block, a, name, bytes, 1);
+    return many ? launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kBranch, true>, grid, block, a, name, bytes, 1)
+                : launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kBranch, false>, grid, block, a, name, bytes, 1);
+  return many ? launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kPostNorm, true>, grid, block, a, name, bytes, 1)
+              : launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kPostNorm, false>, grid, block, a, name, bytes, 1);
 }
+template <typename T>
+int launch_bwd_of(Context* ctx, const NormArgs& a, const Shape& s, int br, bool many, dim3 grid, const char* const* names, double bytes) {
+  const dim3 block(s.threads);
+  if (s.lanes == 16) return launch_bwd<T, 16, false>(ctx, a, br, many, grid, block, names[0], bytes);
+  if (s.lanes == 32) return launch_bwd<T, 32, false>(ctx, a, br, many, grid, block, names[1], bytes);
+  return s.waves > 8 ? launch_bwd<T, 64, true>(ctx, a, br, many, grid, block, names[3], bytes)
+                     : launch_bwd<T, 64, false>(ctx, a, br, many, grid, block, names[2], bytes);
+}
+const char* const kFwdNames[2][4] = {
+    {"residual_norm_fwd_kernel<f32,16>", "residual_norm_fwd_kernel<f32,32>", "residual_norm_fwd_kernel<f32>", "residual_norm_fwd_kernel<f32,wide>"},
+    {"residual_norm_fwd_kernel<bf16,16>", "residual_norm_fwd_kernel<bf16,32>", "residual_norm_fwd_kernel<bf16>", "residual_norm_fwd_kernel<bf16,wide>"}};
+const char* const kBwdNames[2][4] = {
+    {"residual_norm_bwd_kernel<f32,16>", "residual_norm_bwd_kernel<f32,32>", "residual_norm_bwd_kernel<f32>", "residual_norm_bwd_kernel<f32,wide>"},
+    {"residual_norm_bwd_kernel<bf16,16>", "residual_norm_bwd_kernel<bf16,32>", "residual_norm_bwd_kernel<bf16>", "residual_norm_bwd_kernel<bf16,wide>"}};
 
 }  // namespace
 
@@ -613,22 +645,16 @@ int residual_norm_fwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
   a.waves = s.waves, a.groups = s.groups;
   a.layer = n.layer, a.scale = n.scale, a.eps = n.eps;
   const int64_t blocks = (rows + s.groups - 1) / s.groups;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 8192 / (s.threads / 64)))), block(s.threads);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 8192 / (s.threads / 64))));
   const int br = !branch.ptr ? kNoBranch : n.post_weight ? kPostNorm : kBranch;
   const double bytes = static_cast<double>(rows) * C * (eb * (1.0 + (branch.ptr ? 2 : 0) + (y.ptr ? 1 : 0)) + (packed ? 33.0 / 32 : 0));
-  if (dtype == kBF16)
-    return s.lanes == 16   ? launch_fwd<bf16, 16>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<bf16,16>", bytes)
-           : s.lanes == 32 ? launch_fwd<bf16, 32>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<bf16,32>", bytes)
-                           : launch_fwd<bf16, 64>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<bf16>", bytes);
-  return s.lanes == 16   ? launch_fwd<float, 16>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<f32,16>", bytes)
-         : s.lanes == 32 ? launch_fwd<float, 32>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<f32,32>", bytes)
-                         : launch_fwd<float, 64>(ctx, a, br, grid, block, "residual_norm_fwd_kernel<f32>", bytes);
+  return dtype == kBF16 ? launch_fwd_of<bf16>(ctx, a, s, br, grid, kFwdNames[1], bytes) : launch_fwd_of<float>(ctx, a, s, br, grid, kFwdNames[0], bytes);
 }
 
 int64_t residual_norm_bwd_workspace_bytes(int64_t rows, int64_t C, int64_t gates) {
   if (rows <= 0 || rows > INT_MAX || C <= 0 || C > kMaxWidth || gates < 1 || gates > rows || rows % gates != 0) return 0;
   const Cut c = cut_rows(rows, static_cast<int>(C), gates);
-  return c.blocks * C * (gates > 1 && c.pieces > 1 ? 5 : 4) * 4;
+  return c.blocks * C * 4 * 4;
 }
 
 int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows& dy, const Rows& dtotal, const Rows& total, const Rows& branch, const Rows& dx,
@@ -659,15 +685,13 @@ int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
                 "residual_norm_bwd: rows must start on 16-byte boundaries and not overlap");
   const Cut cut = cut_rows(rows, static_cast<int>(C), n.gates);
   const Shape& s = cut.shape;
-  const bool samples = n.gates > 1;
+  const bool many = cut.gates_each > 1;      // (and the gates' gradients are written where the rows are)
   NormArgs a{};
-  a.planes = 0;
-  const bool shared = n.gate && !samples && g.gate;
-  const bool wanted[4] = {g.weight != nullptr, g.bias != nullptr, g.post_weight || shared, g.post_bias || (shared && n.post_bias)};
+  const bool gates_later = g.gate && !many;
+  const bool wanted[4] = {g.weight != nullptr, g.bias != nullptr, g.post_weight || gates_later, g.post_bias || (gates_later && n.post_bias)};
   for (int i = 0; i < 4; ++i) a.plane_of[i] = wanted[i] ? a.planes++ : -1;
-  const bool gate_parts = samples && g.gate && cut.pieces > 1;
-  TCH_CHECK_ARG(n.gates <= 65533 || !gate_parts, "residual_norm_bwd: too many gates");
-  const int64_t sums_bytes = cut.blocks * C * 4 * a.planes, need = sums_bytes + (gate_parts ? cut.blocks * C * 4 : 0);
+  TCH_CHECK_ARG(n.gates <= 65533 || !gates_later, "residual_norm_bwd: too many gates");
+  const int64_t need = cut.blocks * C * 4 * a.planes;
   TCH_CHECK_ARG(need <= (workspace ? workspace_bytes : 0), "residual_norm_bwd: workspace too small");
   const int64_t gate_bytes = n.gates * C * (n.gate_f32 ? 4 : eb);
   auto rows_of = [&](const Rows& t) { return Span{t.ptr, t.ld * eb, C * eb, rows}; };
@@ -692,31 +716,23 @@ int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
   a.waves = s.waves, a.groups = s.groups;
   a.layer = n.layer, a.scale = n.scale, a.eps = n.eps;
   a.sums = static_cast<float*>(workspace);
-  float* const gate_parts_at = a.sums + sums_bytes / 4;
-  a.gate_sums = !samples || !g.gate ? nullptr : gate_parts ? gate_parts_at : g.gate;
-  a.add_gates = accumulate && !gate_parts;
+  a.dgate = g.gate;
+  a.add_gates = accumulate;
   const int br = !branch.ptr ? kNoBranch : n.post_weight ? kPostNorm : kBranch;
   const double bytes = static_cast<double>(rows) * C * eb * ((dy.ptr ? 2.0 : 0) + (dtotal.ptr ? 1 : 0) + (dx.ptr ? 1 : 0) + (branch.ptr ? 2 : 0)) + need;
-  const dim3 grid(static_cast<unsigned>(cut.blocks)), block(s.threads);
-  int rc;
-  if (dtype == kBF16)
-    rc = s.lanes == 16   ? launch_bwd<bf16, 16>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<bf16,16>", bytes)
-         : s.lanes == 32 ? launch_bwd<bf16, 32>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<bf16,32>", bytes)
-                         : launch_bwd<bf16, 64>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<bf16>", bytes);
-  else
-    rc = s.lanes == 16   ? launch_bwd<float, 16>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<f32,16>", bytes)
-         : s.lanes == 32 ? launch_bwd<float, 32>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<f32,32>", bytes)
-                         : launch_bwd<float, 64>(ctx, a, br, samples, grid, block, "residual_norm_bwd_kernel<f32>", bytes);
-  if (rc || (a.planes == 0 && !gate_parts)) return rc;
+  const dim3 grid(static_cast<unsigned>(cut.blocks));
+  const int rc = dtype == kBF16 ? launch_bwd_of<bf16>(ctx, a, s, br, many, grid, kBwdNames[1], bytes)
+                                : launch_bwd_of<float>(ctx, a, s, br, many, grid, kBwdNames[0], bytes);
+  if (rc || a.planes == 0) return rc;
   NormSumArgs f{};
-  f.sums = a.sums, f.gate_sums = gate_parts_at;
-  f.post_weight = n.post_weight, f.post_bias = n.post_bias, f.post = n.post_weight != nullptr;
-  f.gate = samples ? nullptr : n.gate, f.gate_f32 = a.gate_f32;
+  f.sums = a.sums;
+  f.post_weight = n.post_weight, f.post_bias = n.post_bias;
+  f.gate = many ? nullptr : n.gate, f.gate_f32 = a.gate_f32;
   f.dweight = g.weight, f.dbias = g.bias, f.dpost_weight = g.post_weight, f.dpost_bias = g.post_bias, f.dgate = g.gate;
   f.C = static_cast<int>(C), f.blocks = static_cast<int>(cut.blocks), f.planes = a.planes;
   for (int i = 0; i < 4; ++i) f.plane_of[i] = a.plane_of[i];
-  f.pieces = static_cast<int>(cut.pieces), f.shared_gate = !samples && n.gate != nullptr, f.add = accumulate;
-  const dim3 blocks(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(2 + (gate_parts ? n.gates : 0)));
+  f.pieces = static_cast<int>(cut.pieces), f.add = accumulate;
+  const dim3 blocks(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(gates_later ? 2 + n.gates : 2));
   return launch(ctx, residual_norm_sum_kernel, blocks, dim3(256), f, "residual_norm_sum_kernel", static_cast<double>(need), 1);
 }
 
