@@ -60,8 +60,12 @@ struct ActBwdKept {
   __device__ __forceinline__ void request(const ActBwdArgs& p, int64_t row, uint32_t col, int64_t from) {
     const int64_t at = from + static_cast<int64_t>(col) * E;
     const uint32_t* data = reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(p.z) + row * p.ldz + at);
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i) words[i] = data[i];
+    if constexpr (E == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(data);
+      words[0] = v.x, words[1] = v.y;
+    } else {
+      words[0] = data[0];
+    }
     code = p.codes[row * p.code_groups + at / kPackGroup];
   }
   __device__ __forceinline__ void get(float* v) const {

@@ -84,9 +84,7 @@ __global__ __launch_bounds__(256) void pack8_kernel(PackArgs p) {
         uint32_t words[2];
         x[i].get(v);
         const uint32_t code = pack8_lane<FMT>(v, at[i].live, words);
-        uint32_t* to = reinterpret_cast<uint32_t*>(p.data + at[i].row * p.C + at[i].col);
-        if (at[i].live > 0) to[0] = words[0];
-        if (at[i].live > 4) to[1] = words[1];
+        pack8_store<T>(p.data + at[i].row * p.C + at[i].col, words, at[i].live, p.C);
         if (at[i].live > 0 && threadIdx.x % 4 == 0) p.codes[at[i].row * p.groups + at[i].col / kPackGroup] = static_cast<unsigned char>(code);
         if (p.h) {
 #pragma unroll
@@ -107,9 +105,7 @@ __global__ __launch_bounds__(256) void unpack8_kernel(PackArgs p) {
 #pragma unroll
     for (int i = 0; i < kPackAtOnce; ++i) {
       at[i] = place(p, base + 256 * i);
-      const uint32_t* from = reinterpret_cast<const uint32_t*>(p.data + at[i].row * p.C + at[i].col);
-      words[i][0] = at[i].live > 0 ? from[0] : 0;
-      words[i][1] = at[i].live > 4 ? from[1] : 0;
+      pack8_load<T>(p.data + at[i].row * p.C + at[i].col, words[i], at[i].live, p.C);
       code[i] = at[i].live > 0 ? p.codes[at[i].row * p.groups + at[i].col / kPackGroup] : 0;
     }
 #pragma unroll

@@ -48,7 +48,6 @@ struct NormArgs {
   unsigned char* packed;                  // forward: y in 8 bits too
   unsigned char* codes;
   int64_t rows, gate_rows;                // gate_rows: rows that share a gate
-  int64_t group_rows;                     // backward: of a workgroup
   int C, waves, groups;                   // wavefronts of a row, rows at a time of a workgroup
   int layer, gate_f32, format;
   float scale, eps;
@@ -56,7 +55,7 @@ struct NormArgs {
   float* sums;                            // [workgroups][planes][C]
   float* dgate;                           // [gates][C]: written here where a workgroup has all rows of its gates
   int planes, plane_of[4];                // -1: nobody wants it
-  int split_gates;                        // several workgroups have a part of a gate's rows
+  int split_gates, pieces;                // several workgroups have a part of a gate's rows: so many
   int gates_each;                         // otherwise: gates of a workgroup
   int gates, add_gates;
 };
@@ -268,9 +267,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
         y.get(t);
         uint32_t words[2];
         const uint32_t code = p.format == kPackInt8 ? pack8_lane<kPackInt8>(t, live, words) : pack8_lane<kPackE4m3>(t, live, words);
-        uint32_t* to = reinterpret_cast<uint32_t*>(p.packed + row * p.C + at.col);
-        if (live > 0) to[0] = words[0];
-        if (live > 4) to[1] = words[1];
+        pack8_store<T>(p.packed + row * p.C + at.col, words, live, p.C);
         if (live > 0 && at.lane % 4 == 0) p.codes[row * ((p.C + kPackGroup - 1) / kPackGroup) + at.col / kPackGroup] = static_cast<unsigned char>(code);
       }
     }
@@ -278,11 +275,19 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
   }
 }
 
-// MANY: several gates' rows in a workgroup, so that what each gate has to itself is taken here.  Otherwise a workgroup's rows have one gate,
-// and the sums of dt and dt b^ go out as they are: what a gate makes of them the second launch does, once for all of a gate's rows.
-template <typename T, int L, bool WIDE, int BR, bool MANY>
+// What a call asks for, as far as it is worth a kernel of its own: kFullRms and kFullLayer have the norm behind the sum with dtotal and dx, and
+// a workgroup's rows have one gate, whose sums of dt b^ and dt go out as they are (what the gate makes of them the second launch does,
+// once for all of its rows); kFullRms adds no rows of dy and dt up (there are no biases).  kAnything is told the rest by its arguments:
+// among it several gates in a workgroup, where what each has to itself is taken here.  (Flags in registers and accumulators that nobody
+// asked for cost 16 x 1024 rows of 8192 in bf16 spills, 330 us.)
+enum BwdMode : int { kAnything = 0, kFullRms = 1, kFullLayer = 2 };
+template <typename T, int L, bool WIDE, int BR, int MODE>
 __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_norm_bwd_kernel(NormArgs p) {
   constexpr int kLds = L < 64 ? 256 * kEach : WIDE ? 1 : 512 * kEach;   // (a wide row's workgroup has one row at a time, and nothing to add up here)
+  const bool has_norm = MODE != kAnything || p.weight, has_dtotal = MODE != kAnything || p.dtotal.at, has_dx = MODE != kAnything || p.dx.at;
+  const bool layer = MODE == kAnything ? p.layer != 0 : MODE == kFullLayer;
+  const bool many = MODE == kAnything && p.gates_each > 1;
+  const bool rows_of_dy = MODE == kAnything ? p.plane_of[1] >= 0 : MODE == kFullLayer, rows_of_dt = MODE == kAnything || MODE == kFullLayer;
   __shared__ float2 said[2][16];
   __shared__ float lds[kLds];
   const Place at = place<L>(p);
@@ -322,20 +327,21 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
     }
   };
 
+  // The workgroups of a gate's rows take them in turn, so that what the chip works on at a time lies together (each with a run of its
+  // own rows the 16384 x 8192 case runs at 5.1 TB/s).
   int gate = 0, behind_gate = 1;
-  int64_t offset = 0;
+  int64_t offset = 0, step = p.groups;
   if (p.split_gates) {
-    const int pieces = static_cast<int>((p.gate_rows + p.group_rows - 1) / p.group_rows);
-    gate = blockIdx.x / pieces;
+    gate = blockIdx.x / p.pieces;
     behind_gate = gate + 1;
-    offset = static_cast<int64_t>(blockIdx.x - gate * pieces) * p.group_rows;
+    offset = static_cast<int64_t>(blockIdx.x - gate * p.pieces) * p.groups;
+    step *= p.pieces;
   } else {
     gate = blockIdx.x * p.gates_each;
     behind_gate = min(gate + p.gates_each, p.gates);
   }
   for (; gate < behind_gate; ++gate) {
-    const int64_t r0 = gate * p.gate_rows + offset;
-    const int64_t r1 = min(p.split_gates ? r0 + p.group_rows : r0 + p.gate_rows, min((gate + 1) * p.gate_rows, p.rows));
+    const int64_t r0 = gate * p.gate_rows + offset, r1 = min((gate + 1) * p.gate_rows, p.rows);
     if constexpr (BR != kNoBranch) {
       load_gate<T>(p, gate, at.col, at.live, k2);
       if constexpr (BR == kPostNorm) {
@@ -349,88 +355,114 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
     float4 stats, next_stats;
     auto request = [&](int64_t row) {
       const int live = row < r1 ? at.live : 0;
-      if (p.weight) {
+      if (has_norm) {
         dy.load(p.dy, row, at.col, live);
         t.load(p.total, row, at.col, live);
       }
-      if (p.dtotal.at) d0.load(p.dtotal, row, at.col, live);
+      if (has_dtotal) d0.load(p.dtotal, row, at.col, live);
       if constexpr (BR != kNoBranch) b.load(p.branch, row, at.col, live);
       next_stats = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < r1) next_stats = p.stats[row];
     };
     request(r0 + at.group);
-    for (int64_t first = r0; first < r1; first += p.groups) {
+    for (int64_t first = r0; first < r1; first += step) {
       const int64_t row = first + at.group;
       const int live = row < r1 ? at.live : 0;
       stats = next_stats;
       float d[kEach], h[kEach], k[kEach], bh[kEach];
-      if (p.dtotal.at)
+      if (has_dtotal)
         d0.get(d);
       else
 #pragma unroll
         for (int e = 0; e < kEach; ++e) d[e] = 0.f;
-      if (p.weight) {
+      if (has_norm) {
         dy.get(k);
         t.get(h);
       }
       if constexpr (BR != kNoBranch) b.get(bh);
-      request(row + p.groups);
-      if (p.weight) {
+      request(row + step);
+      if (has_norm) {
         float a = 0.f, q = 0.f;
+        if (layer)
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) h[e] -= stats.z;
+        if (rows_of_dy)
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) sum[1][e] += k[e];      // (rows and columns that are not there have a gradient of 0)
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-          h[e] = (h[e] - stats.z) * stats.w;
-          sum[0][e] = fmaf(k[e], h[e], sum[0][e]);      // (rows and columns that are not there have a gradient of 0)
-          sum[1][e] += k[e];
+          h[e] *= stats.w;
+          sum[0][e] = fmaf(k[e], h[e], sum[0][e]);
           k[e] *= w[e];
-          a += k[e];
           q = fmaf(k[e], h[e], q);
         }
-        if (p.layer) a = lane_sum<L>(a);
+        if (layer) {
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) a += k[e];
+          a = lane_sum<L>(a);
+        }
         q = lane_sum<L>(q);
         meet.add(a, q);
-        a = p.layer ? a * inv : 0.f;
         q *= inv;
+        if (layer) {
+          a *= inv;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) d[e] = fmaf(stats.w, k[e] - a - h[e] * q, d[e]);
+          for (int e = 0; e < kEach; ++e) k[e] -= a;
+        }
+        const float r_lo = live > 0 ? stats.w : 0.f, r_hi = there<T>(live, 4) ? stats.w : 0.f;   // (d stays 0 where nothing is)
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) d[e] = fmaf(e < 4 ? r_lo : r_hi, fmaf(-h[e], q, k[e]), d[e]);
       }
-      if (p.dx.at) {
+      if (has_dx) {
         Eight<T> dx;
+        if (p.scale != 1.f) {
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) h[e] = p.scale * d[e];
-        dx.set(h);
+          for (int e = 0; e < kEach; ++e) h[e] = p.scale * d[e];
+          dx.set(h);
+        } else {
+          dx.set(d);
+        }
         dx.store(p.dx, row, at.col, live);
       }
       if constexpr (BR != kNoBranch) {
+        if (BR == kPostNorm && layer)
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) bh[e] -= stats.x;
+        if (rows_of_dt)
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) sum[3][e] += d[e];
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-          if (!there<T>(live, e)) d[e] = 0.f;
-          if constexpr (BR == kPostNorm) bh[e] = (bh[e] - stats.x) * stats.y;
+          if constexpr (BR == kPostNorm) bh[e] *= stats.y;
           sum[2][e] = fmaf(d[e], bh[e], sum[2][e]);
-          sum[3][e] += d[e];
           k[e] = d[e] * k2[e];
         }
         if constexpr (BR == kPostNorm) {
           float a = 0.f, q = 0.f;
 #pragma unroll
-          for (int e = 0; e < kEach; ++e) {
-            a += k[e];
-            q = fmaf(k[e], bh[e], q);
+          for (int e = 0; e < kEach; ++e) q = fmaf(k[e], bh[e], q);
+          if (layer) {
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) a += k[e];
+            a = lane_sum<L>(a);
           }
-          if (p.layer) a = lane_sum<L>(a);
           q = lane_sum<L>(q);
           meet.add(a, q);
-          a = p.layer ? a * inv : 0.f;
           q *= inv;
+          if (layer) {
+            a *= inv;
 #pragma unroll
-          for (int e = 0; e < kEach; ++e) k[e] = stats.y * (k[e] - a - bh[e] * q);
+            for (int e = 0; e < kEach; ++e) k[e] -= a;
+          }
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) k[e] = stats.y * fmaf(-bh[e], q, k[e]);
         }
         Eight<T> db;
         db.set(k);
         db.store(p.dbranch, row, at.col, live);
       }
     }
-    if constexpr (MANY) {
+    if (many) {
       // dg of these rows, and what the post norm's gradients have from them
       float g[kEach], dg[kEach], pw[kEach], pb[kEach];
       load_gate<T>(p, gate, at.col, at.live, g);
@@ -446,7 +478,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
       if (p.dgate) add_up(dg, p.dgate + static_cast<int64_t>(gate) * p.C, p.add_gates);
     }
   }
-  if constexpr (MANY) {
+  if (many) {
 #pragma unroll
     for (int e = 0; e < kEach; ++e) sum[2][e] = gated[0][e], sum[3][e] = gated[1][e];
   }
@@ -455,7 +487,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
     if (p.plane_of[i] >= 0) add_up(sum[i], p.sums + (static_cast<int64_t>(blockIdx.x) * p.planes + p.plane_of[i]) * p.C, false);
 }
 
-// The workgroups' sums added up: 32 columns a workgroup, eight threads a column, in fp64 in a fixed order.  blockIdx.y 0: the norm's two
+// The workgroups' sums added up: 32 columns a workgroup, kLines threads a column, in fp64 in a fixed order.  blockIdx.y 0: the norm's two
 // gradients; 1: those of the post norm; 2 and on: of gate blockIdx.y - 2.
 struct NormSumArgs {
   const float* sums;
@@ -469,39 +501,63 @@ struct NormSumArgs {
   float* dgate;
   int C, blocks, planes, plane_of[4];
   int pieces;               // workgroups of a gate's rows
+  FastDiv div;              // by them
   int gate_f32, add;
 };
-__global__ __launch_bounds__(256) void residual_norm_sum_kernel(NormSumArgs p) {
-  __shared__ double meet[2][8][32];
+template <int kLines>
+__global__ __launch_bounds__(32 * kLines) void residual_norm_sum_kernel(NormSumArgs p) {
+  __shared__ double meet[2][kLines][32];
   const int lane = threadIdx.x & 31, line = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, job = blockIdx.y;
   double s[2] = {0.0, 0.0};
   if (c < p.C) {
     const int first = job < 2 ? 0 : (job - 2) * p.pieces, behind = job < 2 ? p.blocks : first + p.pieces;
     const int64_t ld = static_cast<int64_t>(p.planes) * p.C;
-    auto gate_of = [&](int b) {
-      const int64_t i = static_cast<int64_t>(b / p.pieces) * p.C + c;
-      return p.gate_f32 ? static_cast<const float*>(p.gate)[i] : Elem<bf16>::load(static_cast<const bf16*>(p.gate) + i);
-    };
+    constexpr int U = 8;   // workgroups of a thread, on their way together; behind the last one it is read again, for nothing
+    const int plane0 = p.plane_of[job == 0 ? 0 : 2], plane1 = p.plane_of[job == 0 ? 1 : 3];
+    auto add_up = [&](auto planes_c, int plane, int other, double* sum, auto weight_of) {
+      constexpr int N = decltype(planes_c)::value;
+      const float* at[2] = {p.sums + static_cast<int64_t>(plane) * p.C + c, p.sums + static_cast<int64_t>(other) * p.C + c};
+      for (int b = first + line; b < behind; b += U * kLines) {
+        float v[U][N], g[U];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int plane = p.plane_of[(job == 0 ? 0 : 2) + i];
-      if (plane < 0) continue;
-      const float* from = p.sums + static_cast<int64_t>(plane) * p.C + c;
-      if (job == 1 && p.gate) {
-#pragma unroll 8
-        for (int b = first + line; b < behind; b += 8) s[i] += static_cast<double>(gate_of(b)) * from[b * ld];
-      } else {
-#pragma unroll 8
-        for (int b = first + line; b < behind; b += 8) s[i] += from[b * ld];
+        for (int u = 0; u < U; ++u) {
+          const int block = min(b + u * kLines, behind - 1);
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[u][i] = at[i][block * ld];
+          g[u] = weight_of(block);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < N; ++i) sum[i] += b + u * kLines < behind ? static_cast<double>(g[u]) * v[u][i] : 0.0;
       }
-    }
+    };
+    auto with_weight = [&](auto weight_of) {
+      if (plane0 >= 0 && plane1 >= 0)
+        add_up(std::integral_constant<int, 2>{}, plane0, plane1, s, weight_of);
+      else if (plane0 >= 0)
+        add_up(std::integral_constant<int, 1>{}, plane0, plane0, s, weight_of);
+      else if (plane1 >= 0)
+        add_up(std::integral_constant<int, 1>{}, plane1, plane1, s + 1, weight_of);
+    };
+    auto gate_at = [&](int block) { return static_cast<int64_t>(p.div.div(static_cast<uint32_t>(block))) * p.C + c; };
+    if (job != 1 || !p.gate)
+      with_weight([](int) { return 1.f; });
+    else if (p.gate_f32)
+      with_weight([&](int block) { return static_cast<const float*>(p.gate)[gate_at(block)]; });
+    else
+      with_weight([&](int block) { return Elem<bf16>::load(static_cast<const bf16*>(p.gate) + gate_at(block)); });
   }
   meet[0][line][lane] = s[0];
   meet[1][line][lane] = s[1];
-  __syncthreads();
-  if (line != 0 || c >= p.C) return;
+  for (int half = kLines / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (line < half)
 #pragma unroll
-  for (int l = 1; l < 8; ++l) s[0] += meet[0][l][lane], s[1] += meet[1][l][lane];
+      for (int i = 0; i < 2; ++i) meet[i][line][lane] += meet[i][line + half][lane];
+  }
+  if (line != 0 || c >= p.C) return;
+  s[0] = meet[0][0][lane], s[1] = meet[1][0][lane];
   auto put = [&](float* to, int64_t i, double v) {
     if (to) to[i] = p.add ? static_cast<float>(to[i] + v) : static_cast<float>(v);
   };
@@ -529,23 +585,28 @@ Shape shape_of(int64_t rows, int C) {
   return {64, waves, groups, waves * groups * 64};
 }
 
-// The backward's workgroups: about sixteen wavefronts a compute unit in all.
+// The backward's workgroups: as many as the chip holds (three of four wavefronts a compute unit, one of a wide row), with equally many rounds each.
 struct Cut {
   Shape shape;
-  int64_t group_rows, blocks, pieces;   // pieces: of a gate's rows
-  int gates_each;
+  int64_t blocks, pieces;   // pieces: workgroups of a gate's rows
+  int gates_each;           // gates of a workgroup, where there are more gates than workgroups
   bool split;
 };
 Cut cut_rows(int64_t rows, int C, int64_t gates) {
   Cut c{};
   c.shape = shape_of(rows, C);
-  const int64_t gate_rows = rows / gates, want = 4096 / (c.shape.threads / 64);
-  const int64_t each = (rows + want - 1) / want;
-  c.group_rows = (each + c.shape.groups - 1) / c.shape.groups * c.shape.groups;
-  c.split = gates == 1 || gate_rows >= c.group_rows;
-  c.pieces = c.split ? (gate_rows + c.group_rows - 1) / c.group_rows : 1;
-  c.gates_each = c.split ? 1 : static_cast<int>(std::max<int64_t>(c.group_rows / gate_rows, 1));
-  c.blocks = c.split ? gates * c.pieces : (gates + c.gates_each - 1) / c.gates_each;
+  const int64_t want = c.shape.threads > 512 ? 256 : c.shape.threads > 256 ? 512 : 768, rounds = (rows / gates + c.shape.groups - 1) / c.shape.groups;
+  c.split = gates <= want;
+  if (c.split) {
+    const int64_t most = want / gates, each = (rounds + most - 1) / most;
+    c.pieces = (rounds + each - 1) / each;
+    c.gates_each = 1;
+    c.blocks = gates * c.pieces;
+  } else {
+    c.pieces = 1;
+    c.gates_each = static_cast<int>((gates + want - 1) / want);
+    c.blocks = (gates + c.gates_each - 1) / c.gates_each;
+  }
   return c;
 }
 
@@ -579,22 +640,25 @@ int launch_fwd_of(Context* ctx, const NormArgs& a, const Shape& s, int br, dim3 
   if (s.lanes == 32) return launch_fwd<T, 32, false>(ctx, a, br, grid, block, names[1], bytes);
   return s.waves > 8 ? launch_fwd<T, 64, true>(ctx, a, br, grid, block, names[3], bytes) : launch_fwd<T, 64, false>(ctx, a, br, grid, block, names[2], bytes);
 }
-template <typename T, int L, bool WIDE>
-int launch_bwd(Context* ctx, const NormArgs& a, int br, bool many, dim3 grid, dim3 block, const char* name, double bytes) {
-  if (br == kNoBranch) return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kNoBranch, false>, grid, block, a, name, bytes, 1);
-  if (br == kBranch)
-    return many ? launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kBranch, true>, grid, block, a, name, bytes, 1)
-                : launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kBranch, false>, grid, block, a, name, bytes, 1);
-  return many ? launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kPostNorm, true>, grid, block, a, name, bytes, 1)
-              : launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, kPostNorm, false>, grid, block, a, name, bytes, 1);
+template <typename T, int L, bool WIDE, int BR>
+int launch_bwd(Context* ctx, const NormArgs& a, int mode, dim3 grid, dim3 block, const char* name, double bytes) {
+  if (mode == kFullRms) return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kFullRms>, grid, block, a, name, bytes, 1);
+  if (mode == kFullLayer) return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kFullLayer>, grid, block, a, name, bytes, 1);
+  return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kAnything>, grid, block, a, name, bytes, 1);
+}
+template <typename T, int BR>
+int launch_bwd_of(Context* ctx, const NormArgs& a, const Shape& s, int mode, dim3 grid, const char* const* names, double bytes) {
+  const dim3 block(s.threads);
+  if (s.lanes == 16) return launch_bwd<T, 16, false, BR>(ctx, a, mode, grid, block, names[0], bytes);
+  if (s.lanes == 32) return launch_bwd<T, 32, false, BR>(ctx, a, mode, grid, block, names[1], bytes);
+  return s.waves > 8 ? launch_bwd<T, 64, true, BR>(ctx, a, mode, grid, block, names[3], bytes)
+                     : launch_bwd<T, 64, false, BR>(ctx, a, mode, grid, block, names[2], bytes);
 }
 template <typename T>
-int launch_bwd_of(Context* ctx, const NormArgs& a, const Shape& s, int br, bool many, dim3 grid, const char* const* names, double bytes) {
-  const dim3 block(s.threads);
-  if (s.lanes == 16) return launch_bwd<T, 16, false>(ctx, a, br, many, grid, block, names[0], bytes);
-  if (s.lanes == 32) return launch_bwd<T, 32, false>(ctx, a, br, many, grid, block, names[1], bytes);
-  return s.waves > 8 ? launch_bwd<T, 64, true>(ctx, a, br, many, grid, block, names[3], bytes)
-                     : launch_bwd<T, 64, false>(ctx, a, br, many, grid, block, names[2], bytes);
+int launch_bwd_branch(Context* ctx, const NormArgs& a, const Shape& s, int br, int mode, dim3 grid, const char* const* names, double bytes) {
+  if (br == kNoBranch) return launch_bwd_of<T, kNoBranch>(ctx, a, s, mode, grid, names, bytes);
+  if (br == kBranch) return launch_bwd_of<T, kBranch>(ctx, a, s, mode, grid, names, bytes);
+  return launch_bwd_of<T, kPostNorm>(ctx, a, s, mode, grid, names, bytes);
 }
 const char* const kFwdNames[2][4] = {
     {"residual_norm_fwd_kernel<f32,16>", "residual_norm_fwd_kernel<f32,32>", "residual_norm_fwd_kernel<f32>", "residual_norm_fwd_kernel<f32,wide>"},
@@ -712,7 +776,7 @@ int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
   a.gate = n.gate, a.gate_f32 = n.gate_f32 || dtype == kF32, a.gate_rows = rows / n.gates;
   a.gates = static_cast<int>(n.gates);
   a.rows = rows, a.C = static_cast<int>(C);
-  a.group_rows = cut.group_rows, a.split_gates = cut.split, a.gates_each = cut.gates_each;
+  a.split_gates = cut.split, a.pieces = static_cast<int>(cut.pieces), a.gates_each = cut.gates_each;
   a.waves = s.waves, a.groups = s.groups;
   a.layer = n.layer, a.scale = n.scale, a.eps = n.eps;
   a.sums = static_cast<float*>(workspace);
@@ -721,8 +785,10 @@ int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
   const int br = !branch.ptr ? kNoBranch : n.post_weight ? kPostNorm : kBranch;
   const double bytes = static_cast<double>(rows) * C * eb * ((dy.ptr ? 2.0 : 0) + (dtotal.ptr ? 1 : 0) + (dx.ptr ? 1 : 0) + (branch.ptr ? 2 : 0)) + need;
   const dim3 grid(static_cast<unsigned>(cut.blocks));
-  const int rc = dtype == kBF16 ? launch_bwd_of<bf16>(ctx, a, s, br, many, grid, kBwdNames[1], bytes)
-                                : launch_bwd_of<float>(ctx, a, s, br, many, grid, kBwdNames[0], bytes);
+  const bool full = n.weight && dtotal.ptr && dx.ptr && !many;
+  const int mode = full && n.layer ? kFullLayer : full && a.plane_of[1] < 0 && a.plane_of[3] < 0 ? kFullRms : kAnything;
+  const int rc = dtype == kBF16 ? launch_bwd_branch<bf16>(ctx, a, s, br, mode, grid, kBwdNames[1], bytes)
+                                : launch_bwd_branch<float>(ctx, a, s, br, mode, grid, kBwdNames[0], bytes);
   if (rc || a.planes == 0) return rc;
   NormSumArgs f{};
   f.sums = a.sums;
@@ -732,8 +798,10 @@ int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
   f.C = static_cast<int>(C), f.blocks = static_cast<int>(cut.blocks), f.planes = a.planes;
   for (int i = 0; i < 4; ++i) f.plane_of[i] = a.plane_of[i];
   f.pieces = static_cast<int>(cut.pieces), f.add = accumulate;
+  f.div = FastDiv(static_cast<uint32_t>(cut.pieces));
   const dim3 blocks(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(gates_later ? 2 + n.gates : 2));
-  return launch(ctx, residual_norm_sum_kernel, blocks, dim3(256), f, "residual_norm_sum_kernel", static_cast<double>(need), 1);
+  return cut.blocks > 256 ? launch(ctx, residual_norm_sum_kernel<16>, blocks, dim3(512), f, "residual_norm_sum_kernel<16>", static_cast<double>(need), 1)
+                          : launch(ctx, residual_norm_sum_kernel<8>, blocks, dim3(256), f, "residual_norm_sum_kernel<8>", static_cast<double>(need), 1);
 }
 
 }  // namespace tch
