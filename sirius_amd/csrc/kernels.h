@@ -153,6 +153,20 @@ __device__ inline uint4 load_streaming_u4(const void* base, int64_t i) {
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+// A kernel whose tensors do not fit the last level of cache streams them past it, so that it is not emptied for what will not be read again;
+// smaller ones are left there for the kernel that reads them next.  (A template's flag: of two stores behind a flag at run time the
+// compiler makes one, without the hint.)
+constexpr double kStreamBytes = 256e6;
+template <bool STREAM>
+__device__ __forceinline__ void store_u4(void* base, int64_t i, const uint4& v) {
+  if constexpr (STREAM) {
+    const stream_u4 q = {v.x, v.y, v.z, v.w};
+    __builtin_nontemporal_store(q, static_cast<stream_u4*>(base) + i);
+  } else {
+    static_cast<uint4*>(base)[i] = v;
+  }
+}
+
 // 16-byte fp32 accesses that do not ask the caches to keep the line: optimizer state and master weights are touched
 // once per step and are larger than every cache
 typedef float stream_f4 __attribute__((ext_vector_type(4)));

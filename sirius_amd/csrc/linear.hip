@@ -76,7 +76,7 @@ struct ActBwdKept {
 };
 
 // The chunks of one place: what is read, and the gradients from it, stored and (unrounded) returned in o and u.
-template <typename T, int GATED, int FORMAT>
+template <typename T, int GATED, int FORMAT, bool STREAM>
 struct ActBwdChunks {
   static constexpr int E = Elem<T>::kPerChunk;
   Chunk dy;
@@ -94,14 +94,14 @@ struct ActBwdChunks {
     if (GATED) zu.get(fu);
     combine<T, GATED ? kGatedBwd : kLinBwd, ACT, E>(v, u, fg, fu, o, h);
     T* dz = static_cast<T*>(p.dz) + row * p.lddz;
-    reinterpret_cast<uint4*>(dz)[col] = float_to_chunk<T>(o).u;
+    store_u4<STREAM>(dz, col, float_to_chunk<T>(o).u);
     if (GATED) {
-      reinterpret_cast<uint4*>(dz + p.N)[col] = float_to_chunk<T>(u).u;
-      if (p.h) reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row * p.ldh)[col] = float_to_chunk<T>(h).u;
+      store_u4<STREAM>(dz + p.N, col, float_to_chunk<T>(u).u);
+      if (p.h) store_u4<STREAM>(static_cast<T*>(p.h) + row * p.ldh, col, float_to_chunk<T>(h).u);
     } else if (FORMAT != kDense && p.h) {
 #pragma unroll
       for (int e = 0; e < E; ++e) h[e] = act_value<T, ACT>(fg[e]);
-      reinterpret_cast<uint4*>(static_cast<T*>(p.h) + row * p.ldh)[col] = float_to_chunk<T>(h).u;
+      store_u4<STREAM>(static_cast<T*>(p.h) + row * p.ldh, col, float_to_chunk<T>(h).u);
     }
     if constexpr (sizeof(T) == 2) {
       if (p.low) {
@@ -119,14 +119,14 @@ struct ActBwdChunks {
   }
 };
 
-template <typename T, int GATED, int FORMAT = kDense>
+template <typename T, int GATED, int FORMAT, bool STREAM>
 __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
   constexpr int E = Elem<T>::kPerChunk;
   with_activation(p.act, [&](auto act_c) {
     constexpr int ACT = decltype(act_c)::value;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * kAtOnce);
     for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * kAtOnce) + threadIdx.x; base < p.chunks; base += stride) {
-      ActBwdChunks<T, GATED, FORMAT> c[kAtOnce];
+      ActBwdChunks<T, GATED, FORMAT, STREAM> c[kAtOnce];
       uint32_t row[kAtOnce], col[kAtOnce];
 #pragma unroll
       for (int i = 0; i < kAtOnce; ++i) {
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void act_bwd_kernel(ActBwdArgs p) {
 // The same with the column sums of the unrounded gradients, which are the bias gradient: added up from their rounded parts they would be as far off
 // as the parts (8192 rows: 2.5e-6 of the result; this way 1.1e-7).  A workgroup has a block of rows and 2^lanes_log chunks of columns; a thread walks down the
 // rows of its chunk, the threads of a column meet in LDS in their order, and the row blocks' sums are added up by a second launch.
-template <typename T, int GATED, int FORMAT = kDense>
+template <typename T, int GATED, int FORMAT, bool STREAM>
 __global__ __launch_bounds__(256) void act_bwd_sum_kernel(ActBwdArgs p) {
   constexpr int E = Elem<T>::kPerChunk, PARTS = GATED ? 2 : 1;
   __shared__ float meet[PARTS][256 * E];
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void act_bwd_sum_kernel(ActBwdArgs p) {
     constexpr int ACT = decltype(act_c)::value;
     if (col < p.row_chunks)
       for (int64_t base = row0 + line; base < behind; base += kAtOnce * lines) {
-        ActBwdChunks<T, GATED, FORMAT> c[kAtOnce];
+        ActBwdChunks<T, GATED, FORMAT, STREAM> c[kAtOnce];
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i)
           if (base + i * lines < behind) c[i].request(p, base + i * lines, col);
@@ -301,10 +301,16 @@ int launch_act_bwd_of(Context* ctx, dim3 grid, const ActBwdArgs& a, double bytes
        {{"act_bwd_sum_kernel<bf16>", "act_bwd_sum_kernel<bf16,int8>", "act_bwd_sum_kernel<bf16,e4m3>"},
         {"act_bwd_sum_kernel<bf16,gated>", "act_bwd_sum_kernel<bf16,gated,int8>", "act_bwd_sum_kernel<bf16,gated,e4m3>"}}}};
   const char* name = names[SUMS][sizeof(T) == 2][GATED][FORMAT + 1];
-  if constexpr (SUMS)
-    return launch(ctx, act_bwd_sum_kernel<T, GATED, FORMAT>, grid, dim3(256), a, name, bytes, 1);
-  else
-    return launch(ctx, act_bwd_kernel<T, GATED, FORMAT>, grid, dim3(256), a, name, bytes, 1);
+  auto of = [&](auto stream_c) {
+    constexpr bool STREAM = decltype(stream_c)::value;
+    if constexpr (SUMS)
+      return launch(ctx, act_bwd_sum_kernel<T, GATED, FORMAT, STREAM>, grid, dim3(256), a, name, bytes, 1);
+    else
+      return launch(ctx, act_bwd_kernel<T, GATED, FORMAT, STREAM>, grid, dim3(256), a, name, bytes, 1);
+  };
+  if constexpr (FORMAT != kDense)
+    if (bytes > kStreamBytes) return of(std::true_type{});   // (8192 x 2 x 5632 in bf16 with h: 74 us, 82 without)
+  return of(std::false_type{});
 }
 template <bool SUMS, typename T, int GATED>
 int launch_act_bwd_format(Context* ctx, int format, dim3 grid, const ActBwdArgs& a, double bytes) {

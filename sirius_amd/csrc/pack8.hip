@@ -13,7 +13,6 @@
 namespace tch {
 namespace {
 
-constexpr int kPackAtOnce = 4;   // eights of a thread, on their way together
 
 struct PackArgs {
   const void* x;          // kept: rows ldx apart
@@ -42,10 +41,11 @@ struct EightOf {
 #pragma unroll
     for (int i = 0; i < N; ++i) chunk_to_float<T>(c[i], v + i * (8 / N));
   }
+  template <bool STREAM>
   __device__ __forceinline__ static void store(T* to, const float* v, int live) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (i * (8 / N) < live) reinterpret_cast<uint4*>(to)[i] = float_to_chunk<T>(v + i * (8 / N)).u;
+      if (i * (8 / N) < live) store_u4<STREAM>(to, i, float_to_chunk<T>(v + i * (8 / N)).u);
   }
 };
 
@@ -64,22 +64,22 @@ __device__ __forceinline__ At place(const PackArgs& p, uint64_t q) {
   return a;
 }
 
-// The four lanes of a group are neighbours (a row has whole groups of them), and all lanes of a wavefront go round together.
-template <typename T, int FMT>
+// AT_ONCE eights of a thread are on their way together.  The four lanes of a group are neighbours (a row has whole groups of them), and all lanes of a wavefront go round together.
+template <typename T, int FMT, int AT_ONCE, bool STREAM>
 __global__ __launch_bounds__(256) void pack8_kernel(PackArgs p) {
-  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * kPackAtOnce);
-  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * kPackAtOnce); base < p.total; base += stride) {
-    EightOf<T> x[kPackAtOnce];
-    At at[kPackAtOnce];
+  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * AT_ONCE);
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * AT_ONCE); base < p.total; base += stride) {
+    EightOf<T> x[AT_ONCE];
+    At at[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < kPackAtOnce; ++i) {
+    for (int i = 0; i < AT_ONCE; ++i) {
       at[i] = place(p, base + 256 * i + threadIdx.x);
       x[i].load(static_cast<const T*>(p.x) + at[i].row * p.ldx + at[i].col, at[i].live);
     }
     with_activation(p.act, [&](auto act_c) {
       constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
-      for (int i = 0; i < kPackAtOnce; ++i) {
+      for (int i = 0; i < AT_ONCE; ++i) {
         float v[8];
         uint32_t words[2];
         x[i].get(v);
@@ -89,37 +89,37 @@ __global__ __launch_bounds__(256) void pack8_kernel(PackArgs p) {
         if (p.h) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = act_value<T, ACT>(v[e]);
-          EightOf<T>::store(static_cast<T*>(p.h) + at[i].row * p.ldh + at[i].col, v, at[i].live);
+          EightOf<T>::template store<STREAM>(static_cast<T*>(p.h) + at[i].row * p.ldh + at[i].col, v, at[i].live);
         }
       }
     });
   }
 }
 
-template <typename T, int FMT>
+template <typename T, int FMT, int AT_ONCE, bool STREAM>
 __global__ __launch_bounds__(256) void unpack8_kernel(PackArgs p) {
-  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * kPackAtOnce);
-  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * kPackAtOnce) + threadIdx.x; base < p.total; base += stride) {
-    At at[kPackAtOnce];
-    uint32_t words[kPackAtOnce][2], code[kPackAtOnce];
+  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * AT_ONCE);
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * AT_ONCE) + threadIdx.x; base < p.total; base += stride) {
+    At at[AT_ONCE];
+    uint32_t words[AT_ONCE][2], code[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < kPackAtOnce; ++i) {
+    for (int i = 0; i < AT_ONCE; ++i) {
       at[i] = place(p, base + 256 * i);
       pack8_load<T>(p.data + at[i].row * p.C + at[i].col, words[i], at[i].live, p.C);
       code[i] = at[i].live > 0 ? p.codes[at[i].row * p.groups + at[i].col / kPackGroup] : 0;
     }
 #pragma unroll
-    for (int i = 0; i < kPackAtOnce; ++i) {
+    for (int i = 0; i < AT_ONCE; ++i) {
       float v[8];
       const float unit = pack8_unit(code[i]);
       unpack8_word<FMT>(words[i][0], unit, v);
       unpack8_word<FMT>(words[i][1], unit, v + 4);
-      EightOf<T>::store(static_cast<T*>(p.out) + at[i].row * p.ldx + at[i].col, v, at[i].live);
+      EightOf<T>::template store<STREAM>(static_cast<T*>(p.out) + at[i].row * p.ldx + at[i].col, v, at[i].live);
     }
   }
 }
 
-int bind(const char* what, PackArgs& a, int dtype, void* data, void* codes, int format, int64_t M, int64_t C, dim3* grid) {
+int bind(const char* what, PackArgs& a, int dtype, void* data, void* codes, int format, int64_t M, int64_t C) {
   const std::string name(what);
   TCH_CHECK_ARG(dtype == kBF16 || dtype == kF32, name + ": dtype must be f32(0) or bf16(1)");
   TCH_CHECK_ARG(format >= 0 && format < kPackFormats, name + ": unknown 8-bit format");
@@ -135,9 +135,33 @@ int bind(const char* what, PackArgs& a, int dtype, void* data, void* codes, int 
   TCH_CHECK_ARG(M * eights < (1ll << 31), name + ": tensor exceeds 2^34 elements");
   a.total = static_cast<uint64_t>(M * eights);
   a.eights = FastDiv(static_cast<uint32_t>(eights));
-  *grid = dim3(static_cast<unsigned>(std::min<uint64_t>((a.total + 256 * kPackAtOnce - 1) / (256 * kPackAtOnce), 1 << 20)));
   return 0;
 }
+
+// fn(element type, format, whether to stream past the cache, the kernel's name)
+template <typename T>
+struct Type {
+  typedef T type;
+};
+const char* const kNames[2][2][2] = {{{"pack8_kernel<f32,int8>", "pack8_kernel<f32,e4m3>"}, {"pack8_kernel<bf16,int8>", "pack8_kernel<bf16,e4m3>"}},
+                                     {{"unpack8_kernel<f32,int8>", "unpack8_kernel<f32,e4m3>"}, {"unpack8_kernel<bf16,int8>", "unpack8_kernel<bf16,e4m3>"}}};
+template <typename F>
+int launch_of(int unpack, int dtype, int format, uint64_t total, double bytes, F&& fn) {
+  const char* name = kNames[unpack][dtype == kBF16][format];
+  // Four eights a thread, or one where that leaves the chip fewer than four workgroups a compute unit (1568 x 1000 in fp32 kept and fetched:
+  // AAA us, 9.3 with four).
+  const uint64_t each = total < 4 * 256 * 1024 ? 1 : 4;
+  const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((total + 256 * each - 1) / (256 * each), 1 << 20)));
+  auto sized = [&](auto t, auto format_c) {
+    std::integral_constant<int, 1> one;
+    std::integral_constant<int, 4> four;
+    if (each == 1) return fn(t, format_c, one, std::false_type{}, grid, name);
+    return bytes > kStreamBytes ? fn(t, format_c, four, std::true_type{}, grid, name) : fn(t, format_c, four, std::false_type{}, grid, name);
+  };
+  auto typed = [&](auto t) { return format == kPackInt8 ? sized(t, std::integral_constant<int, kPackInt8>{}) : sized(t, std::integral_constant<int, kPackE4m3>{}); };
+  return dtype == kBF16 ? typed(Type<bf16>{}) : typed(Type<float>{});
+}
+
 bool rows_ok(const void* t, int64_t ld, int64_t C, int eb) {
   return ld >= C && ld % (16 / eb) == 0 && ld <= (1ll << 31) && (reinterpret_cast<uintptr_t>(t) & 15) == 0;
 }
@@ -146,8 +170,7 @@ bool rows_ok(const void* t, int64_t ld, int64_t C, int eb) {
 
 int pack8(Context* ctx, int dtype, const Rows& x, void* data, void* codes, int format, const Rows& h, int act, int64_t M, int64_t C) {
   PackArgs a{};
-  dim3 grid;
-  if (int rc = bind("pack8", a, dtype, data, codes, format, M, C, &grid)) return rc;
+  if (int rc = bind("pack8", a, dtype, data, codes, format, M, C)) return rc;
   TCH_CHECK_ARG(act >= 0 && act < kActCount, "pack8: unknown activation");
   if (M == 0) return 0;
   const int eb = dtype == kBF16 ? 2 : 4;
@@ -161,17 +184,14 @@ int pack8(Context* ctx, int dtype, const Rows& x, void* data, void* codes, int f
   a.h = h.ptr, a.ldh = h.ld;
   a.act = h.ptr ? act : kActNone;
   const double bytes = static_cast<double>(M) * C * (eb * (h.ptr ? 2.0 : 1.0) + 33.0 / 32);
-  if (dtype == kBF16)
-    return format == kPackInt8 ? launch(ctx, pack8_kernel<bf16, kPackInt8>, grid, dim3(256), a, "pack8_kernel<bf16,int8>", bytes, 1)
-                               : launch(ctx, pack8_kernel<bf16, kPackE4m3>, grid, dim3(256), a, "pack8_kernel<bf16,e4m3>", bytes, 1);
-  return format == kPackInt8 ? launch(ctx, pack8_kernel<float, kPackInt8>, grid, dim3(256), a, "pack8_kernel<f32,int8>", bytes, 1)
-                             : launch(ctx, pack8_kernel<float, kPackE4m3>, grid, dim3(256), a, "pack8_kernel<f32,e4m3>", bytes, 1);
+  return launch_of(0, dtype, format, a.total, bytes, [&](auto t, auto format_c, auto each_c, auto stream_c, dim3 grid, const char* name) {
+    return launch(ctx, pack8_kernel<typename decltype(t)::type, decltype(format_c)::value, decltype(each_c)::value, decltype(stream_c)::value>, grid, dim3(256), a, name, bytes, 1);
+  });
 }
 
 int unpack8(Context* ctx, int dtype, const void* data, const void* codes, int format, const Rows& x, int64_t M, int64_t C) {
   PackArgs a{};
-  dim3 grid;
-  if (int rc = bind("unpack8", a, dtype, const_cast<void*>(data), const_cast<void*>(codes), format, M, C, &grid)) return rc;
+  if (int rc = bind("unpack8", a, dtype, const_cast<void*>(data), const_cast<void*>(codes), format, M, C)) return rc;
   if (M == 0) return 0;
   const int eb = dtype == kBF16 ? 2 : 4;
   TCH_CHECK_ARG(x.ptr, "unpack8: null tensor");
@@ -180,11 +200,9 @@ int unpack8(Context* ctx, int dtype, const void* data, const void* codes, int fo
   TCH_CHECK_ARG(apart(out, {data, C, C, M}) && apart(out, {codes, a.groups, a.groups, M}), "unpack8: the output overlaps what is kept");
   a.out = x.ptr, a.ldx = x.ld;
   const double bytes = static_cast<double>(M) * C * (eb + 33.0 / 32);
-  if (dtype == kBF16)
-    return format == kPackInt8 ? launch(ctx, unpack8_kernel<bf16, kPackInt8>, grid, dim3(256), a, "unpack8_kernel<bf16,int8>", bytes, 1)
-                               : launch(ctx, unpack8_kernel<bf16, kPackE4m3>, grid, dim3(256), a, "unpack8_kernel<bf16,e4m3>", bytes, 1);
-  return format == kPackInt8 ? launch(ctx, unpack8_kernel<float, kPackInt8>, grid, dim3(256), a, "unpack8_kernel<f32,int8>", bytes, 1)
-                             : launch(ctx, unpack8_kernel<float, kPackE4m3>, grid, dim3(256), a, "unpack8_kernel<f32,e4m3>", bytes, 1);
+  return launch_of(1, dtype, format, a.total, bytes, [&](auto t, auto format_c, auto each_c, auto stream_c, dim3 grid, const char* name) {
+    return launch(ctx, unpack8_kernel<typename decltype(t)::type, decltype(format_c)::value, decltype(each_c)::value, decltype(stream_c)::value>, grid, dim3(256), a, name, bytes, 1);
+  });
 }
 
 }  // namespace tch

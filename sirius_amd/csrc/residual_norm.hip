@@ -138,7 +138,7 @@ __device__ __forceinline__ float2 row_stats(const float* v, int live, int layer,
 }
 
 // Eight neighbours as they lie in memory; `live`: 8, 4 (fp32) or 0 of them.
-template <typename T>
+template <typename T, bool STREAM = false>
 struct Eight {
   static constexpr int N = sizeof(T) / 2;   // chunks
   Chunk c[N];
@@ -147,7 +147,7 @@ struct Eight {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       c[i] = zero_chunk();
-      if (i * (kEach / N) < live) c[i].u = from[i];
+      if (i * (kEach / N) < live) c[i].u = STREAM ? load_streaming_u4(from, i) : from[i];
     }
   }
   __device__ __forceinline__ void get(float* v) const {
@@ -162,7 +162,7 @@ struct Eight {
     uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(t.at) + row * t.ld + col);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (i * (kEach / N) < live) to[i] = c[i].u;
+      if (i * (kEach / N) < live) store_u4<STREAM>(to, i, c[i].u);
   }
 };
 
@@ -209,7 +209,7 @@ __device__ __forceinline__ Place place(const NormArgs& p) {
 }
 
 // WIDE: rows of more than eight wavefronts
-template <typename T, int L, bool WIDE, int BR>
+template <typename T, int L, bool WIDE, int BR, bool STREAM>
 __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_norm_fwd_kernel(NormArgs p) {
   __shared__ float2 said[2][16];
   const Place at = place<L>(p);
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
   }
   const int64_t step = static_cast<int64_t>(gridDim.x) * p.groups;
   int64_t row = static_cast<int64_t>(blockIdx.x) * p.groups + at.group;
-  Eight<T> x, b;
+  Eight<T, STREAM> x, b;
   auto request = [&](int64_t r) {
     const int live = r < p.rows ? at.live : 0;
     x.load(p.x, r, at.col, live);
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
     if constexpr (BR != kNoBranch) {
 #pragma unroll
       for (int e = 0; e < kEach; ++e) t[e] = fmaf(g[e], n[e], p.scale * t[e]);
-      Eight<T> sum;
+      Eight<T, STREAM> sum;
       sum.set(t);
       sum.store(p.total, row, at.col, live);
       sum.get(t);
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
       stats.z = s.x, stats.w = s.y;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) t[e] = fmaf((t[e] - s.x) * s.y, w[e], c[e]);
-      Eight<T> y;
+      Eight<T, STREAM> y;
       y.set(t);
       y.store(p.y, row, at.col, live);
       if (p.packed) {   // what is kept is y as it is stored
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
 // among it several gates in a workgroup, where what each has to itself is taken here.  (Flags in registers and accumulators that nobody
 // asked for cost 16 x 1024 rows of 8192 in bf16 spills, 330 us.)
 enum BwdMode : int { kAnything = 0, kFullRms = 1, kFullLayer = 2 };
-template <typename T, int L, bool WIDE, int BR, int MODE>
+template <typename T, int L, bool WIDE, int BR, int MODE, bool STREAM>
 __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_norm_bwd_kernel(NormArgs p) {
   constexpr int kLds = L < 64 ? 256 * kEach : WIDE ? 1 : 512 * kEach;   // (a wide row's workgroup has one row at a time, and nothing to add up here)
   const bool has_norm = MODE != kAnything || p.weight, has_dtotal = MODE != kAnything || p.dtotal.at, has_dx = MODE != kAnything || p.dx.at;
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
         for (int e = 0; e < kEach; ++e) k2[e] *= pw[e];
       }
     }
-    Eight<T> dy, d0, t, b;
+    Eight<T, STREAM> dy, d0, t, b;
     float4 stats, next_stats;
     auto request = [&](int64_t row) {
       const int live = row < r1 ? at.live : 0;
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
         for (int e = 0; e < kEach; ++e) d[e] = fmaf(e < 4 ? r_lo : r_hi, fmaf(-h[e], q, k[e]), d[e]);
       }
       if (has_dx) {
-        Eight<T> dx;
+        Eight<T, STREAM> dx;
         if (p.scale != 1.f) {
 #pragma unroll
           for (int e = 0; e < kEach; ++e) h[e] = p.scale * d[e];
@@ -457,7 +457,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
 #pragma unroll
           for (int e = 0; e < kEach; ++e) k[e] = stats.y * fmaf(-bh[e], q, k[e]);
         }
-        Eight<T> db;
+        Eight<T, STREAM> db;
         db.set(k);
         db.store(p.dbranch, row, at.col, live);
       }
@@ -627,32 +627,40 @@ bool aligned(std::initializer_list<const void*> all) {
   return (bits & 15) == 0;
 }
 
-template <typename T, int L, bool WIDE>
+// (Rows shorter than a wavefront's eights are few bytes in all, and what only kAnything does is rare: those are not streamed.)
+template <typename T, int L, bool WIDE, bool STREAM>
 int launch_fwd(Context* ctx, const NormArgs& a, int br, dim3 grid, dim3 block, const char* name, double bytes) {
-  if (br == kNoBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kNoBranch>, grid, block, a, name, bytes, 1);
-  if (br == kBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kBranch>, grid, block, a, name, bytes, 1);
-  return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kPostNorm>, grid, block, a, name, bytes, 1);
+  if (br == kNoBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kNoBranch, STREAM>, grid, block, a, name, bytes, 1);
+  if (br == kBranch) return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kBranch, STREAM>, grid, block, a, name, bytes, 1);
+  return launch(ctx, residual_norm_fwd_kernel<T, L, WIDE, kPostNorm, STREAM>, grid, block, a, name, bytes, 1);
 }
 template <typename T>
 int launch_fwd_of(Context* ctx, const NormArgs& a, const Shape& s, int br, dim3 grid, const char* const* names, double bytes) {
   const dim3 block(s.threads);
-  if (s.lanes == 16) return launch_fwd<T, 16, false>(ctx, a, br, grid, block, names[0], bytes);
-  if (s.lanes == 32) return launch_fwd<T, 32, false>(ctx, a, br, grid, block, names[1], bytes);
-  return s.waves > 8 ? launch_fwd<T, 64, true>(ctx, a, br, grid, block, names[3], bytes) : launch_fwd<T, 64, false>(ctx, a, br, grid, block, names[2], bytes);
+  const bool stream = bytes > kStreamBytes;
+  if (s.lanes == 16) return launch_fwd<T, 16, false, false>(ctx, a, br, grid, block, names[0], bytes);
+  if (s.lanes == 32) return launch_fwd<T, 32, false, false>(ctx, a, br, grid, block, names[1], bytes);
+  if (s.waves > 8)
+    return stream ? launch_fwd<T, 64, true, true>(ctx, a, br, grid, block, names[3], bytes) : launch_fwd<T, 64, true, false>(ctx, a, br, grid, block, names[3], bytes);
+  return stream ? launch_fwd<T, 64, false, true>(ctx, a, br, grid, block, names[2], bytes) : launch_fwd<T, 64, false, false>(ctx, a, br, grid, block, names[2], bytes);
 }
-template <typename T, int L, bool WIDE, int BR>
+template <typename T, int L, bool WIDE, int BR, bool STREAM>
 int launch_bwd(Context* ctx, const NormArgs& a, int mode, dim3 grid, dim3 block, const char* name, double bytes) {
-  if (mode == kFullRms) return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kFullRms>, grid, block, a, name, bytes, 1);
-  if (mode == kFullLayer) return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kFullLayer>, grid, block, a, name, bytes, 1);
-  return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kAnything>, grid, block, a, name, bytes, 1);
+  if (mode == kFullRms) return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kFullRms, STREAM>, grid, block, a, name, bytes, 1);
+  if (mode == kFullLayer) return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kFullLayer, STREAM>, grid, block, a, name, bytes, 1);
+  return launch(ctx, residual_norm_bwd_kernel<T, L, WIDE, BR, kAnything, false>, grid, block, a, name, bytes, 1);
 }
 template <typename T, int BR>
 int launch_bwd_of(Context* ctx, const NormArgs& a, const Shape& s, int mode, dim3 grid, const char* const* names, double bytes) {
   const dim3 block(s.threads);
-  if (s.lanes == 16) return launch_bwd<T, 16, false, BR>(ctx, a, mode, grid, block, names[0], bytes);
-  if (s.lanes == 32) return launch_bwd<T, 32, false, BR>(ctx, a, mode, grid, block, names[1], bytes);
-  return s.waves > 8 ? launch_bwd<T, 64, true, BR>(ctx, a, mode, grid, block, names[3], bytes)
-                     : launch_bwd<T, 64, false, BR>(ctx, a, mode, grid, block, names[2], bytes);
+  const bool stream = bytes > kStreamBytes;
+  if (s.lanes == 16) return launch_bwd<T, 16, false, BR, false>(ctx, a, mode, grid, block, names[0], bytes);
+  if (s.lanes == 32) return launch_bwd<T, 32, false, BR, false>(ctx, a, mode, grid, block, names[1], bytes);
+  if (s.waves > 8)
+    return stream ? launch_bwd<T, 64, true, BR, true>(ctx, a, mode, grid, block, names[3], bytes)
+                  : launch_bwd<T, 64, true, BR, false>(ctx, a, mode, grid, block, names[3], bytes);
+  return stream ? launch_bwd<T, 64, false, BR, true>(ctx, a, mode, grid, block, names[2], bytes)
+                : launch_bwd<T, 64, false, BR, false>(ctx, a, mode, grid, block, names[2], bytes);
 }
 template <typename T>
 int launch_bwd_branch(Context* ctx, const NormArgs& a, const Shape& s, int br, int mode, dim3 grid, const char* const* names, double bytes) {

@@ -50,7 +50,13 @@ template <typename T, int V>
 struct Piece {
   typename Raw<V * sizeof(T)>::type raw;
   __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const decltype(raw)*>(p); }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(raw)*>(p) = raw; }
+  template <bool STREAM>
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(raw, reinterpret_cast<std::remove_const_t<decltype(raw)>*>(p));
+    else
+      *reinterpret_cast<std::remove_const_t<decltype(raw)>*>(p) = raw;
+  }
   __device__ __forceinline__ void get(float* v) const {
     if constexpr (sizeof(T) == 4) {
       __builtin_memcpy(v, &raw, V * 4);
@@ -97,7 +103,7 @@ __device__ inline float2 factors(const RotaryArgs& p, int64_t position, int pair
 
 // A unit is what a thread takes at a time: V pairs from two places of a head (HALVES, and V 1 of either layout), V / 2 pairs from V neighbours, or
 // V elements that are copied.
-template <typename T, int V, bool HALVES>
+template <typename T, int V, bool HALVES, bool STREAM>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
   constexpr bool TWO = HALVES || V == 1;
   __shared__ float2 lds[kMaxPairs];
@@ -148,7 +154,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
           b[i] = b[i] * f.x + x * f.y;
         }
         u.b.set(b);
-        u.b.store(to + b_at);
+        u.b.template store<STREAM>(to + b_at);
       } else {
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
@@ -160,7 +166,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
       }
       u.a.set(a);
     }
-    u.a.store(to);
+    u.a.template store<STREAM>(to);
   };
 
   Unit u[kUnitsAtOnce];
@@ -184,8 +190,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs p) {
 
 template <typename T, int V>
 int launch_rotary(Context* ctx, const RotaryArgs& a, bool halves, dim3 grid, const char* name, double bytes) {
-  return halves ? launch(ctx, rotary_kernel<T, V, true>, grid, dim3(256), a, name, bytes, 1)
-                : launch(ctx, rotary_kernel<T, V, false>, grid, dim3(256), a, name, bytes, 1);
+  if constexpr (V * sizeof(T) == 16)
+    if (bytes > kStreamBytes)   // (131072 x 40 x 128 in bf16: 456 us, 469 without)
+      return halves ? launch(ctx, rotary_kernel<T, V, true, true>, grid, dim3(256), a, name, bytes, 1)
+                    : launch(ctx, rotary_kernel<T, V, false, true>, grid, dim3(256), a, name, bytes, 1);
+  return halves ? launch(ctx, rotary_kernel<T, V, true, false>, grid, dim3(256), a, name, bytes, 1)
+                : launch(ctx, rotary_kernel<T, V, false, false>, grid, dim3(256), a, name, bytes, 1);
 }
 
 }  // namespace
