@@ -46,8 +46,16 @@ class GPT2Engine(EngineBase):
     def __init__(self, vocab=50257, n_pos=1024, n_embd=768, n_layer=12, n_head=12, seq_len=1024, dtype=torch.bfloat16,
                  optimizer="adamw", lr=1e-3, weight_decay=0.01, betas=(0.9, 0.999), eps=1e-8, momentum=0.9,
                  stream=None, allocator=None, overlap_wgrad=True, fused_attention=True, trailing_wgrad=True,
-                 trailing_reduce=None, fused_mlp=False):
+                 trailing_reduce=None, fused_mlp=False, kept="full"):
         self._init_engine(dtype, stream, allocator)
+        # kept: what the backward pass finds of the projections' inputs and the MLP's pre-activations.  "int8" or "e4m3": 8 bits each
+        # (ops.Packed8; the hidden values are computed again from the pre-activations): a layer's activations take 18 C bytes a
+        # token instead of 32 C in bf16, 30 C instead of 64 C in fp32; the loss is the same, weight gradients are those of what is kept.
+        if kept != "full" and kept not in ops.Packed8.FORMATS:
+            raise ValueError(f"kept: full, {' or '.join(ops.Packed8.FORMATS)}")
+        if kept != "full" and fused_mlp:
+            raise ValueError("kept in 8 bits, the MLP's derivative is a pass of its own: not with fused_mlp")
+        self.kept = None if kept == "full" else kept
         # fused_mlp: the activation rides the first MLP projection's launch, its derivative the second one's data gradient: no
         # pass over the 4 C wide tensors in between.  The activation is then taken of the unrounded pre-activation, and the
         # order of additions of small batches is the launch's choice: other roundings than without.
@@ -229,7 +237,9 @@ class GPT2Engine(EngineBase):
         plan.labels = act(R, dtype=torch.int64).zero_()
         plan.loss_rows = act(R, dtype=torch.float32)
         plan.loss = act(1, dtype=torch.float32)
-        ln_mean, ln_rstd = act((2 * L + 1) * R, dtype=torch.float32), act((2 * L + 1) * R, dtype=torch.float32)
+        kept = self.kept
+        n_ln = 1 if kept else 2 * L + 1     # (the layers' own norms leave their statistics in norm_stats then)
+        ln_mean, ln_rstd = act(n_ln * R, dtype=torch.float32), act(n_ln * R, dtype=torch.float32)
         # The column sums of a LayerNorm backward ride the next weight gradient, from a partial buffer of their own.  Six
         # taken in turn: the one a LayerNorm writes was read by a weight gradient two layers ago at the latest, which
         # the main lane has waited for (one layer behind, see below).
@@ -290,6 +300,33 @@ class GPT2Engine(EngineBase):
                 wgrad(as4(x), as4(dy), self._view(self.grads, name + ".weight"), self._view(self.grads, name + ".bias"))
             ops.conv2d_dgrad(ctx, as4(dy), self._wt(name + ".weight"), as4(dx), 1, 0, tile_cfg=ops.LINEAR)
 
+        def keep_room(width):
+            return ops.Packed8(act(R, width, dtype=torch.uint8), act(R, -(-width // ops.Packed8.GROUP), dtype=torch.uint8), kept)
+
+        # What the layers share where they keep 8 bits: the norms' outputs and the MLP's hidden values are on the main lane only,
+        # the inputs that the weight gradients fetch on the second.
+        if kept:
+            norm_stats = act(2 * L, R, 4, dtype=torch.float32)
+            n_t, f_t = act(R, C), act(R, 4 * C)
+            norm_ws = act(ops.residual_norm_bwd_workspace_bytes(n_t), dtype=torch.uint8)
+            fetch_ws = act(max(ops.linear_wgrad_packed_workspace_bytes(ops.Packed8.empty(R, C, kept, device="meta"), torch.empty(R, n, dtype=T_, device="meta"))
+                               for n in (3 * C, 4 * C)), dtype=torch.uint8)
+
+        def norm_fwd(name, idx, x, y, packed):
+            ops.residual_norm_fwd(ctx, x, None, None, y, norm_stats[idx], kind="layer", weight=self._view(self.params, name + ".weight"),
+                                  bias=self._view(self.params, name + ".bias"), packed=packed)
+
+        def norm_bwd(name, idx, dy, x, dx, residual):
+            ops.residual_norm_bwd(ctx, dy, residual, x, None, dx, None, norm_stats[idx], kind="layer", weight=self._view(self.params, name + ".weight"),
+                                  dweight=self._view(self.grads, name + ".weight"), dbias=self._view(self.grads, name + ".bias"), workspace=norm_ws)
+
+        def lin_bwd_kept(name, packed, dy, dx):
+            """lin_bwd from the layer's input in 8 bits"""
+            with side():
+                ops.linear_wgrad_packed(ctx, packed, dy, self._view(self.grads, name + ".weight").view(dy.shape[1], packed.shape[1]),
+                                        dbias=self._view(self.grads, name + ".bias"), workspace=fetch_ws)
+            ops.conv2d_dgrad(ctx, as4(dy), self._wt(name + ".weight"), as4(dx), 1, 0, tile_cfg=ops.LINEAR)
+
         # strides / batch offsets of head h of sample b inside the packed projection and the score tensor
         qkv_row, qkv_b = 3 * C, (T * 3 * C, D)
         s_b, o_b = (H * T * T, T * T), (T * C, D)
@@ -317,9 +354,15 @@ class GPT2Engine(EngineBase):
             saved = []
             for i in range(L):
                 pre = f"transformer.h.{i}."
-                a, qkv = act(R, C), act(R, 3 * C)
-                ln_fwd(pre + "ln_1", 2 * i, h, a)
-                lin_fwd(pre + "attn.c_attn", a, qkv)
+                qkv = act(R, 3 * C)
+                if kept:
+                    a = keep_room(C)
+                    norm_fwd(pre + "ln_1", 2 * i, h, n_t, a)
+                    lin_fwd(pre + "attn.c_attn", n_t, qkv)
+                else:
+                    a = act(R, C)
+                    ln_fwd(pre + "ln_1", 2 * i, h, a)
+                    lin_fwd(pre + "attn.c_attn", a, qkv)
                 flat = qkv.view(-1)
                 o = act(R, C)
                 if fused:
@@ -336,9 +379,16 @@ class GPT2Engine(EngineBase):
                                      causal=2)
                 h1 = act(R, C)
                 lin_fwd(pre + "attn.c_proj", o, h1, add=h)
-                m, f1, f2 = act(R, C), act(R, 4 * C), act(R, 4 * C)
-                ln_fwd(pre + "ln_2", 2 * i + 1, h1, m)
-                if self.fused_mlp:
+                if kept:
+                    m, f1, f2 = keep_room(C), keep_room(4 * C), f_t
+                    norm_fwd(pre + "ln_2", 2 * i + 1, h1, n_t, m)
+                else:
+                    m, f1, f2 = act(R, C), act(R, 4 * C), act(R, 4 * C)
+                    ln_fwd(pre + "ln_2", 2 * i + 1, h1, m)
+                if kept:
+                    lin_fwd(pre + "mlp.c_fc", n_t, f_t)
+                    ops.act_fwd_pack8(ctx, f_t, f_t, f1, "gelu_tanh")
+                elif self.fused_mlp:
                     ops.linear_fwd(ctx, m, self._w(pre + "mlp.c_fc.weight").view(4 * C, C), f2,
                                    bias=self._view(self.params, pre + "mlp.c_fc.bias"), act="gelu_tanh", pre=f1)
                 else:
@@ -350,7 +400,7 @@ class GPT2Engine(EngineBase):
                 h = h2
                 mark("fwd", f"h.{i}")
             hf = act(R, C)
-            ln_fwd("transformer.ln_f", 2 * L, h, hf)
+            ln_fwd("transformer.ln_f", n_ln - 1, h, hf)
             logits = act(R, Vp, dtype=torch.float32)
             ops.conv2d_fwd(ctx, as4(hf), self._w("transformer.wte.weight"), as4(logits), 1, 0, tile_cfg=order)
             dlogits = act(R, Vp).zero_()   # the padding columns stay zero: no kernel writes them
@@ -367,7 +417,8 @@ class GPT2Engine(EngineBase):
             # by a layer: what layer j reads lies in the sets of layers j-1 and j, layer j+1 writes a third set,
             # and before layer j+2 takes the first set again the main lane has waited for layer j's weight gradients.
             n_sets = 3 if self.trailing_wgrad else 1
-            g_sets = [([act(R, C) for _ in range(4 if k == 0 else 3)], act(R, 4 * C), act(R, 3 * C)) for k in range(n_sets)]
+            # (kept in 8 bits, the hidden values that are computed again belong to a set as well)
+            g_sets = [([act(R, C) for _ in range(4 if k == 0 else 3)], act(R, 4 * C), act(R, 3 * C), act(R, 4 * C) if kept else None) for k in range(n_sets)]
             g_c = g_sets[0][0]
             g_f2 = None if self.fused_mlp else act(R, 4 * C)   # main lane only
             dP = act(B * H, T, dtype=torch.float32) if fused else act(B, H, T, T)   # fused: the delta scratch
@@ -375,17 +426,23 @@ class GPT2Engine(EngineBase):
             with side():
                 wgrad(as4(hf), as4(dlogits), self._view(self.grads, "transformer.wte.weight"))
             ops.conv2d_dgrad(ctx, as4(dlogits), self._wt("transformer.wte.weight"), as4(d_hf), 1, 0, tile_cfg=ops.LINEAR)
-            ln_bwd("transformer.ln_f", 2 * L, d_hf, h, g)
+            ln_bwd("transformer.ln_f", n_ln - 1, d_hf, h, g)
             mark("bwd", "ln_f")
             for i in range(L - 1, -1, -1):
                 pre = f"transformer.h.{i}."
                 h_in, a, qkv, P, o, h1, m, f1, f2 = saved[i]
-                own_c, g_f1, g_qkv = g_sets[(L - i) % n_sets]
+                own_c, g_f1, g_qkv, f2_again = g_sets[(L - i) % n_sets]
                 flat, gflat = qkv.view(-1), g_qkv.view(-1)
                 spare = [t for t in own_c if t is not g]
                 d_m, g1, d_o = spare[0], spare[1], spare[2]
                 # MLP
-                if self.fused_mlp:
+                if kept:
+                    ops.conv2d_dgrad(ctx, as4(g), self._wt(pre + "mlp.c_proj.weight"), as4(g_f2), 1, 0, tile_cfg=ops.LINEAR)
+                    ops.act_bwd_packed(ctx, g_f2, f1, g_f1, "gelu_tanh", h=f2_again)
+                    with side():
+                        wgrad(as4(f2_again), as4(g), self._view(self.grads, pre + "mlp.c_proj.weight"),
+                              self._view(self.grads, pre + "mlp.c_proj.bias"))
+                elif self.fused_mlp:
                     with side():
                         wgrad(as4(f2), as4(g), self._view(self.grads, pre + "mlp.c_proj.weight"),
                               self._view(self.grads, pre + "mlp.c_proj.bias"))
@@ -393,8 +450,12 @@ class GPT2Engine(EngineBase):
                 else:
                     lin_bwd(pre + "mlp.c_proj", f2, g, g_f2)
                     ops.gelu_bwd(ctx, g_f2, f1, g_f1, tanh_form=True)
-                lin_bwd(pre + "mlp.c_fc", m, g_f1, d_m)
-                ln_bwd(pre + "ln_2", 2 * i + 1, d_m, h1, g1, residual=g)
+                if kept:
+                    lin_bwd_kept(pre + "mlp.c_fc", m, g_f1, d_m)
+                    norm_bwd(pre + "ln_2", 2 * i + 1, d_m, h1, g1, g)
+                else:
+                    lin_bwd(pre + "mlp.c_fc", m, g_f1, d_m)
+                    ln_bwd(pre + "ln_2", 2 * i + 1, d_m, h1, g1, residual=g)
                 # attention
                 lin_bwd(pre + "attn.c_proj", o, g1, d_o)
                 if fused:
@@ -412,9 +473,13 @@ class GPT2Engine(EngineBase):
                     ops.batched_gemm(ctx, dP, flat, gflat[C:], T, D, T, (1, T), (1, qkv_row), qkv_row, (B, H), s_b, qkv_b,
                                      qkv_b, causal=3)
                 d_a = d_m   # free again
-                lin_bwd(pre + "attn.c_attn", a, g_qkv, d_a)
                 g_next = d_o
-                ln_bwd(pre + "ln_1", 2 * i, d_a, h_in, g_next, residual=g1)
+                if kept:
+                    lin_bwd_kept(pre + "attn.c_attn", a, g_qkv, d_a)
+                    norm_bwd(pre + "ln_1", 2 * i, d_a, h_in, g_next, g1)
+                else:
+                    lin_bwd(pre + "attn.c_attn", a, g_qkv, d_a)
+                    ln_bwd(pre + "ln_1", 2 * i, d_a, h_in, g_next, residual=g1)
                 g = g_next
                 if self.overlap_wgrad:
                     ctx.join(behind=self.trailing_wgrad)
@@ -430,6 +495,7 @@ class GPT2Engine(EngineBase):
         finally:
             ctx.end_record()
         plan.prog, plan.marks, plan.keep, plan.logits = prog, marks, keep, logits
+        plan.kept = [(layer[1], layer[6], layer[7]) for layer in saved] if kept else None   # inputs of c_attn and c_fc, pre-activations
         plan.bytes = sum(t.numel() * t.element_size() for t in keep)
         return plan
 

@@ -82,6 +82,8 @@ def main():
     parser.add_argument('--seq-len', type=int, default=256)
     parser.add_argument('--optimizer', choices=['sgd', 'adamw'], default='sgd')
     parser.add_argument('--fp32', action='store_true')
+    parser.add_argument('--kept', choices=('full', 'int8', 'e4m3'), default='full',
+                        help="what the backward pass finds of the projections' inputs and the MLP's pre-activations: as computed, or 8 bits each")
     parser.add_argument('--fused-mlp', action='store_true', help="activation and its derivative in the MLP projections' launches")
     parser.add_argument('--max-grad-norm', type=float, default=None, help="clip the gradients' global norm ahead of every step")
     parser.add_argument('--peer-script', type=str, default='',
@@ -100,7 +102,7 @@ def main():
         train(args.num_epoch, args.batch_size, global_batch_size=args.global_batch_size,
               dataset_size=args.dataset_size, seq_len=args.seq_len, optimizer=args.optimizer,
               dtype=torch.float32 if args.fp32 else torch.bfloat16, peer=peer, max_grad_norm=args.max_grad_norm,
-              fused_mlp=args.fused_mlp)
+              fused_mlp=args.fused_mlp, kept=args.kept)
     finally:
         if peer is not None:
             peer.stop()
