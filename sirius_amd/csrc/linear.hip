@@ -82,7 +82,8 @@ struct ActBwdChunks {
   Chunk dy;
   std::conditional_t<FORMAT == kDense, ActBwdZ<T, FORMAT>, ActBwdKept<T, FORMAT>> zg, zu;
   __device__ __forceinline__ void request(const ActBwdArgs& p, int64_t row, uint32_t col) {
-    dy.u = load_streaming_u4(static_cast<const T*>(p.dy) + row * p.lddy, col);
+    const T* from = static_cast<const T*>(p.dy) + row * p.lddy;
+    dy.u = FORMAT == kDense || STREAM ? load_streaming_u4(from, col) : reinterpret_cast<const uint4*>(from)[col];
     zg.request(p, row, col, 0);
     if (GATED) zu.request(p, row, col, p.N);
   }

@@ -30,11 +30,12 @@ template <typename T>
 struct EightOf {
   static constexpr int N = sizeof(T) / 2;
   Chunk c[N];
+  template <bool STREAM>
   __device__ __forceinline__ void load(const T* from, int live) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       c[i] = zero_chunk();
-      if (i * (8 / N) < live) c[i].u = load_streaming_u4(from, i);
+      if (i * (8 / N) < live) c[i].u = STREAM ? load_streaming_u4(from, i) : reinterpret_cast<const uint4*>(from)[i];
     }
   }
   __device__ __forceinline__ void get(float* v) const {
@@ -64,58 +65,44 @@ __device__ __forceinline__ At place(const PackArgs& p, uint64_t q) {
   return a;
 }
 
-// AT_ONCE eights of a thread are on their way together.  The four lanes of a group are neighbours (a row has whole groups of them), and all lanes of a wavefront go round together.
-template <typename T, int FMT, int AT_ONCE, bool STREAM>
+// An eight a thread.  (Four on their way together: 8192 x 4096 in bf16 with GELU 33 us instead of 31, fetching 8192 x 1024 7.4 instead of 6.5, and
+// small tensors leave the chip idle.)  The four lanes of a group are neighbours (a row has whole groups of them), and all lanes of a
+// wavefront go round together.
+template <typename T, int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void pack8_kernel(PackArgs p) {
-  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * AT_ONCE);
-  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * AT_ONCE); base < p.total; base += stride) {
-    EightOf<T> x[AT_ONCE];
-    At at[AT_ONCE];
+  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * 256;
+  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * 256; base < p.total; base += stride) {
+    const At at = place(p, base + threadIdx.x);
+    EightOf<T> x;
+    x.template load<STREAM>(static_cast<const T*>(p.x) + at.row * p.ldx + at.col, at.live);
+    float v[8];
+    uint32_t words[2];
+    x.get(v);
+    const uint32_t code = pack8_lane<FMT>(v, at.live, words);
+    pack8_store<T>(p.data + at.row * p.C + at.col, words, at.live, p.C);
+    if (at.live > 0 && threadIdx.x % 4 == 0) p.codes[at.row * p.groups + at.col / kPackGroup] = static_cast<unsigned char>(code);
+    if (p.h)
+      with_activation(p.act, [&](auto act_c) {
+        constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      at[i] = place(p, base + 256 * i + threadIdx.x);
-      x[i].load(static_cast<const T*>(p.x) + at[i].row * p.ldx + at[i].col, at[i].live);
-    }
-    with_activation(p.act, [&](auto act_c) {
-      constexpr int ACT = decltype(act_c)::value;
-#pragma unroll
-      for (int i = 0; i < AT_ONCE; ++i) {
-        float v[8];
-        uint32_t words[2];
-        x[i].get(v);
-        const uint32_t code = pack8_lane<FMT>(v, at[i].live, words);
-        pack8_store<T>(p.data + at[i].row * p.C + at[i].col, words, at[i].live, p.C);
-        if (at[i].live > 0 && threadIdx.x % 4 == 0) p.codes[at[i].row * p.groups + at[i].col / kPackGroup] = static_cast<unsigned char>(code);
-        if (p.h) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = act_value<T, ACT>(v[e]);
-          EightOf<T>::template store<STREAM>(static_cast<T*>(p.h) + at[i].row * p.ldh + at[i].col, v, at[i].live);
-        }
-      }
-    });
+        for (int e = 0; e < 8; ++e) v[e] = act_value<T, ACT>(v[e]);
+        EightOf<T>::template store<STREAM>(static_cast<T*>(p.h) + at.row * p.ldh + at.col, v, at.live);
+      });
   }
 }
 
-template <typename T, int FMT, int AT_ONCE, bool STREAM>
+template <typename T, int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void unpack8_kernel(PackArgs p) {
-  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (256 * AT_ONCE);
-  for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * (256 * AT_ONCE) + threadIdx.x; base < p.total; base += stride) {
-    At at[AT_ONCE];
-    uint32_t words[AT_ONCE][2], code[AT_ONCE];
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      at[i] = place(p, base + 256 * i);
-      pack8_load<T>(p.data + at[i].row * p.C + at[i].col, words[i], at[i].live, p.C);
-      code[i] = at[i].live > 0 ? p.codes[at[i].row * p.groups + at[i].col / kPackGroup] : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      float v[8];
-      const float unit = pack8_unit(code[i]);
-      unpack8_word<FMT>(words[i][0], unit, v);
-      unpack8_word<FMT>(words[i][1], unit, v + 4);
-      EightOf<T>::template store<STREAM>(static_cast<T*>(p.out) + at[i].row * p.ldx + at[i].col, v, at[i].live);
-    }
+  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * 256;
+  for (uint64_t q = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; q < p.total; q += stride) {
+    const At at = place(p, q);
+    uint32_t words[2];
+    pack8_load<T>(p.data + at.row * p.C + at.col, words, at.live, p.C);
+    const float unit = pack8_unit(at.live > 0 ? p.codes[at.row * p.groups + at.col / kPackGroup] : 0);
+    float v[8];
+    unpack8_word<FMT>(words[0], unit, v);
+    unpack8_word<FMT>(words[1], unit, v + 4);
+    EightOf<T>::template store<STREAM>(static_cast<T*>(p.out) + at.row * p.ldx + at.col, v, at.live);
   }
 }
 
@@ -148,17 +135,13 @@ const char* const kNames[2][2][2] = {{{"pack8_kernel<f32,int8>", "pack8_kernel<f
 template <typename F>
 int launch_of(int unpack, int dtype, int format, uint64_t total, double bytes, F&& fn) {
   const char* name = kNames[unpack][dtype == kBF16][format];
-  // Four eights a thread, or one where that leaves the chip fewer than four workgroups a compute unit (1568 x 1000 in fp32 kept and fetched:
-  // AAA us, 9.3 with four).
-  const uint64_t each = total < 4 * 256 * 1024 ? 1 : 4;
-  const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((total + 256 * each - 1) / (256 * each), 1 << 20)));
-  auto sized = [&](auto t, auto format_c) {
-    std::integral_constant<int, 1> one;
-    std::integral_constant<int, 4> four;
-    if (each == 1) return fn(t, format_c, one, std::false_type{}, grid, name);
-    return bytes > kStreamBytes ? fn(t, format_c, four, std::true_type{}, grid, name) : fn(t, format_c, four, std::false_type{}, grid, name);
+  const dim3 grid(static_cast<unsigned>(std::min<uint64_t>((total + 255) / 256, 1 << 20)));
+  auto streamed = [&](auto t, auto format_c) {
+    return bytes > kStreamBytes ? fn(t, format_c, std::true_type{}, grid, name) : fn(t, format_c, std::false_type{}, grid, name);
   };
-  auto typed = [&](auto t) { return format == kPackInt8 ? sized(t, std::integral_constant<int, kPackInt8>{}) : sized(t, std::integral_constant<int, kPackE4m3>{}); };
+  auto typed = [&](auto t) {
+    return format == kPackInt8 ? streamed(t, std::integral_constant<int, kPackInt8>{}) : streamed(t, std::integral_constant<int, kPackE4m3>{});
+  };
   return dtype == kBF16 ? typed(Type<bf16>{}) : typed(Type<float>{});
 }
 
@@ -184,8 +167,8 @@ int pack8(Context* ctx, int dtype, const Rows& x, void* data, void* codes, int f
   a.h = h.ptr, a.ldh = h.ld;
   a.act = h.ptr ? act : kActNone;
   const double bytes = static_cast<double>(M) * C * (eb * (h.ptr ? 2.0 : 1.0) + 33.0 / 32);
-  return launch_of(0, dtype, format, a.total, bytes, [&](auto t, auto format_c, auto each_c, auto stream_c, dim3 grid, const char* name) {
-    return launch(ctx, pack8_kernel<typename decltype(t)::type, decltype(format_c)::value, decltype(each_c)::value, decltype(stream_c)::value>, grid, dim3(256), a, name, bytes, 1);
+  return launch_of(0, dtype, format, a.total, bytes, [&](auto t, auto format_c, auto stream_c, dim3 grid, const char* name) {
+    return launch(ctx, pack8_kernel<typename decltype(t)::type, decltype(format_c)::value, decltype(stream_c)::value>, grid, dim3(256), a, name, bytes, 1);
   });
 }
 
@@ -200,8 +183,8 @@ int unpack8(Context* ctx, int dtype, const void* data, const void* codes, int fo
   TCH_CHECK_ARG(apart(out, {data, C, C, M}) && apart(out, {codes, a.groups, a.groups, M}), "unpack8: the output overlaps what is kept");
   a.out = x.ptr, a.ldx = x.ld;
   const double bytes = static_cast<double>(M) * C * (eb + 33.0 / 32);
-  return launch_of(1, dtype, format, a.total, bytes, [&](auto t, auto format_c, auto each_c, auto stream_c, dim3 grid, const char* name) {
-    return launch(ctx, unpack8_kernel<typename decltype(t)::type, decltype(format_c)::value, decltype(each_c)::value, decltype(stream_c)::value>, grid, dim3(256), a, name, bytes, 1);
+  return launch_of(1, dtype, format, a.total, bytes, [&](auto t, auto format_c, auto stream_c, dim3 grid, const char* name) {
+    return launch(ctx, unpack8_kernel<typename decltype(t)::type, decltype(format_c)::value, decltype(stream_c)::value>, grid, dim3(256), a, name, bytes, 1);
   });
 }
 

@@ -147,6 +147,29 @@ def test_weight_gradients(ctx, dtype, fmt, M, K, N):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("M,K,N", [(31, 8, 8), (33, 24, 520), (95, 1032, 136), (2319, 3976, 8736), (4100, 520, 264), (65, 256, 256)], ids=str)
+def test_weight_gradients_are_those_of_the_fetched_input(ctx, fmt, M, K, N):
+    """Numbers of all sizes in groups of all sizes, rows and columns that end inside a tile or a group of 32: the same products in the
+    same order as from the fetched input in bf16, bit for bit, with and without a low part; nothing is written beside dw."""
+    from sirius_amd import ops
+    x, exact = normal(M, K, dtype=torch.bfloat16), normal(M, N, seed=1)
+    x *= 2.0 ** torch.randint(-30, 30, (M, 1), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).float()
+    x = x.bfloat16()
+    dy = exact.bfloat16()
+    low = (exact - dy.float()).bfloat16()
+    packed, kept = keep(ctx, x, fmt)
+    room = torch.full((N + 2, K), 7.0, device="cuda")
+    want, db, db2 = torch.empty(N, K, device="cuda"), torch.empty(N, device="cuda"), torch.empty(N, device="cuda")
+    ws = torch.empty(ops.linear_wgrad_packed_workspace_bytes(packed, dy), dtype=torch.uint8, device="cuda").fill_(255)
+    dense = torch.empty(ops.linear_bwd_workspace_bytes(kept, N), dtype=torch.uint8, device="cuda")
+    for part in (None, low):
+        ops.linear_wgrad_packed(ctx, packed, dy, room[1:-1], dbias=db, workspace=ws, dy_low=part)
+        ops.linear_wgrad(ctx, kept, dy, want, dbias=db2, workspace=dense, dy_low=part)
+        assert torch.equal(room[1:-1], want) and torch.equal(db, db2)
+        assert (room[0] == 7.0).all() and (room[-1] == 7.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("M,K,N", [(70, 72, 136), (900, 264, 392)], ids=str)
 def test_weight_gradients_of_an_unrounded_gradient(ctx, fmt, M, K, N):
     from sirius_amd import ops
