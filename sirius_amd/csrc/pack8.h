@@ -77,6 +77,20 @@ __device__ __forceinline__ uint32_t pack8_lane(const float* v, int live, uint32_
   return code;
 }
 
+// A lane's four neighbours as one word; all eight lanes of a group are here.
+template <int FMT>
+__device__ __forceinline__ uint32_t pack8_four(const float* v, bool live, uint32_t* word) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (live) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+  top = quad_max(top);
+  top = max(top, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(top), 0x141, 0xf, 0xf, true)));   // the other quad of eight
+  const uint32_t code = pack8_code<FMT>(top);
+  *word = pack8_word<FMT>(v, code);
+  return code;
+}
+
 // A lane's two words to and from memory, as one access where rows of C are whole eights (bf16: always).
 template <typename T>
 __device__ __forceinline__ void pack8_store(unsigned char* to, const uint32_t* words, int live, int C) {

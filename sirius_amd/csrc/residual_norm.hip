@@ -97,27 +97,28 @@ struct Meeting {
   }
 };
 
-// Whether element e of a lane's eight is there: bf16 rows are whole eights, fp32 rows whole fours.
-template <typename T>
-__device__ __forceinline__ bool there(int live, int e) {
-  return live > (sizeof(T) == 2 || e < 4 ? 0 : 4);
-}
+// A lane's eight neighbours of a row in bf16, or in fp32 twice four, a row of lanes apart: an access of the lanes is whole lines either way.
+struct Cols {
+  int at[2];     // of the first and the second four
+  bool on[2];    // whether they are there: bf16 rows are whole eights, fp32 rows whole fours
+  __device__ __forceinline__ Cols in(bool row) const { return {{at[0], at[1]}, {on[0] && row, on[1] && row}}; }
+};
 
 // mean and 1 / deviation of a row
-template <typename T, int L>
-__device__ __forceinline__ float2 row_stats(const float* v, int live, int layer, const NormArgs& p, Meeting& meet, int row_wave) {
+template <int L>
+__device__ __forceinline__ float2 row_stats(const float* v, const Cols& cols, int layer, const NormArgs& p, Meeting& meet, int row_wave) {
   const float inv = 1.f / static_cast<float>(p.C);
   if (!layer) {
     float q = 0.f, none = 0.f;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) q = there<T>(live, e) ? fmaf(v[e], v[e], q) : q;
+    for (int e = 0; e < kEach; ++e) q = cols.on[e / 4] ? fmaf(v[e], v[e], q) : q;
     q = lane_sum<L>(q);
     meet.add(q, none);
     return make_float2(0.f, 1.f / sqrtf(q * inv + p.eps));
   }
   float s = 0.f;
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) s += there<T>(live, e) ? v[e] : 0.f;
+  for (int e = 0; e < kEach; ++e) s += cols.on[e / 4] ? v[e] : 0.f;
   s = lane_sum<L>(s);
   auto elements = [&](int w) { return static_cast<float>(min(p.C - w * 64 * kEach, 64 * kEach)); };   // of a wavefront
   const float n = L < 64 ? static_cast<float>(p.C) : elements(row_wave), mine = s / n;
@@ -125,7 +126,7 @@ __device__ __forceinline__ float2 row_stats(const float* v, int live, int layer,
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const float d = v[e] - mine;
-    q = there<T>(live, e) ? fmaf(d, d, q) : q;
+    q = cols.on[e / 4] ? fmaf(d, d, q) : q;
   }
   q = lane_sum<L>(q);
   if (meet.waves == 1) return make_float2(mine, 1.f / sqrtf(q * inv + p.eps));
@@ -137,17 +138,18 @@ __device__ __forceinline__ float2 row_stats(const float* v, int live, int layer,
   return make_float2(mean, 1.f / sqrtf(q * inv + p.eps));
 }
 
-// Eight neighbours as they lie in memory; `live`: 8, 4 (fp32) or 0 of them.
+// A lane's eight as they lie in memory.
 template <typename T, bool STREAM = false>
 struct Eight {
   static constexpr int N = sizeof(T) / 2;   // chunks
   Chunk c[N];
-  __device__ __forceinline__ void load(const RowsPtr& t, int64_t row, int col, int live) {
-    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(t.at) + row * t.ld + col);
+  __device__ __forceinline__ void load(const RowsPtr& t, int64_t row, const Cols& cols) {
+    const T* from = static_cast<const T*>(t.at) + row * t.ld;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       c[i] = zero_chunk();
-      if (i * (kEach / N) < live) c[i].u = STREAM ? load_streaming_u4(from, i) : from[i];
+      const uint4* chunk = reinterpret_cast<const uint4*>(from + cols.at[i]);
+      if (cols.on[i]) c[i].u = STREAM ? load_streaming_u4(chunk, 0) : *chunk;
     }
   }
   __device__ __forceinline__ void get(float* v) const {
@@ -158,53 +160,77 @@ struct Eight {
 #pragma unroll
     for (int i = 0; i < N; ++i) c[i] = float_to_chunk<T>(v + i * (kEach / N));
   }
-  __device__ __forceinline__ void store(const RowsPtr& t, int64_t row, int col, int live) const {
-    uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(t.at) + row * t.ld + col);
+  __device__ __forceinline__ void store(const RowsPtr& t, int64_t row, const Cols& cols) const {
+    T* to = static_cast<T*>(t.at) + row * t.ld;
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (i * (kEach / N) < live) store_u4<STREAM>(to, i, c[i].u);
+      if (cols.on[i]) store_u4<STREAM>(to + cols.at[i], 0, c[i].u);
   }
 };
 
-__device__ __forceinline__ void load_vector(const float* from, int col, int live, float otherwise, float* v) {
+__device__ __forceinline__ void load_vector(const float* from, const Cols& cols, float otherwise, float* v) {
 #pragma unroll
   for (int i = 0; i < kEach; i += 4) {
     float4 f = make_float4(otherwise, otherwise, otherwise, otherwise);
-    if (from && i < live) f = *reinterpret_cast<const float4*>(from + col + i);
+    if (from && cols.on[i / 4]) f = *reinterpret_cast<const float4*>(from + cols.at[i / 4]);
     v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
   }
 }
 template <typename T>
-__device__ __forceinline__ void load_gate(const NormArgs& p, int64_t gate, int col, int live, float* v) {
+__device__ __forceinline__ void load_gate(const NormArgs& p, int64_t gate, const Cols& cols, float* v) {
   if (!p.gate || p.gate_f32) {
-    load_vector(static_cast<const float*>(p.gate) + (p.gate ? gate * p.C : 0), col, live, 1.f, v);
+    load_vector(static_cast<const float*>(p.gate) + (p.gate ? gate * p.C : 0), cols, 1.f, v);
   } else {
     Eight<T> g;
-    g.load({const_cast<void*>(p.gate), p.C}, gate, col, live);
+    g.load({const_cast<void*>(p.gate), p.C}, gate, cols);
     g.get(v);
   }
 }
 
+// y in 8 bits, as it is stored: the lanes of 32 neighbours are neighbours, four of them in bf16, eight in fp32
+template <typename T, int FORMAT>
+__device__ __forceinline__ void keep(const NormArgs& p, int64_t row, const Cols& cols, const float* v, int lane) {
+  unsigned char* data = p.packed + row * p.C;
+  unsigned char* codes = p.codes + row * ((p.C + kPackGroup - 1) / kPackGroup);
+  if constexpr (sizeof(T) == 2) {
+    uint32_t words[2];
+    const uint32_t code = pack8_lane<FORMAT>(v, cols.on[0] ? 8 : 0, words);
+    if (cols.on[0]) *reinterpret_cast<uint2*>(data + cols.at[0]) = make_uint2(words[0], words[1]);
+    if (cols.on[0] && lane % 4 == 0) codes[cols.at[0] / kPackGroup] = static_cast<unsigned char>(code);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t word;
+      const uint32_t code = pack8_four<FORMAT>(v + 4 * i, cols.on[i], &word);
+      if (cols.on[i]) *reinterpret_cast<uint32_t*>(data + cols.at[i]) = word;
+      if (cols.on[i] && lane % 8 == 0) codes[cols.at[i] / kPackGroup] = static_cast<unsigned char>(code);
+    }
+  }
+}
+
 struct Place {   // of a lane
-  int lane, wave, row_wave, group, col, live;
+  int lane, wave, row_wave, group;
+  Cols cols;
 };
-template <int L>
+template <typename T, int L>
 __device__ __forceinline__ Place place(const NormArgs& p) {
   Place a;
   a.lane = threadIdx.x & 63;
   a.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int sub;
+  a.row_wave = 0;
   if (L < 64) {
-    a.row_wave = 0;
     a.group = threadIdx.x / L;
-    sub = threadIdx.x % L;
   } else {
     a.group = a.wave / p.waves;
     a.row_wave = a.wave - a.group * p.waves;
-    sub = a.row_wave * 64 + a.lane;
   }
-  a.col = sub * kEach;
-  a.live = max(0, min(p.C - a.col, kEach));
+  const int first = a.row_wave * 64 * kEach, sub = a.lane % L;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    a.cols.at[i] = first + (sizeof(T) == 2 ? sub * 8 + i * 4 : (i * L + sub) * 4);
+    a.cols.on[i] = a.cols.at[i] < p.C;
+  }
+  if (sizeof(T) == 2) a.cols.on[1] = a.cols.on[0];
   return a;
 }
 
@@ -212,37 +238,37 @@ __device__ __forceinline__ Place place(const NormArgs& p) {
 template <typename T, int L, bool WIDE, int BR, bool STREAM>
 __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_norm_fwd_kernel(NormArgs p) {
   __shared__ float2 said[2][16];
-  const Place at = place<L>(p);
+  const Place at = place<T, L>(p);
   Meeting meet{said, 0, at.group * p.waves, p.waves, at.lane, at.wave};
   const bool samples = p.gate_rows < p.rows;
   float w[kEach], c[kEach], pw[kEach], pb[kEach], g[kEach];
-  load_vector(p.weight, at.col, at.live, 1.f, w);
-  load_vector(p.bias, at.col, at.live, 0.f, c);
-  if constexpr (BR != kNoBranch) load_gate<T>(p, 0, at.col, at.live, g);
+  load_vector(p.weight, at.cols, 1.f, w);
+  load_vector(p.bias, at.cols, 0.f, c);
+  if constexpr (BR != kNoBranch) load_gate<T>(p, 0, at.cols, g);
   if constexpr (BR == kPostNorm) {
-    load_vector(p.post_weight, at.col, at.live, 1.f, pw);
-    load_vector(p.post_bias, at.col, at.live, 0.f, pb);
+    load_vector(p.post_weight, at.cols, 1.f, pw);
+    load_vector(p.post_bias, at.cols, 0.f, pb);
   }
   const int64_t step = static_cast<int64_t>(gridDim.x) * p.groups;
   int64_t row = static_cast<int64_t>(blockIdx.x) * p.groups + at.group;
   Eight<T, STREAM> x, b;
   auto request = [&](int64_t r) {
-    const int live = r < p.rows ? at.live : 0;
-    x.load(p.x, r, at.col, live);
-    if constexpr (BR != kNoBranch) b.load(p.branch, r, at.col, live);
+    const Cols cols = at.cols.in(r < p.rows);
+    x.load(p.x, r, cols);
+    if constexpr (BR != kNoBranch) b.load(p.branch, r, cols);
   };
   request(row);
   // (every wavefront of the workgroup makes as many rounds: they meet in each)
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * p.groups; first < p.rows; first += step, row += step) {
-    const int live = row < p.rows ? at.live : 0;
+    const Cols cols = at.cols.in(row < p.rows);
     float t[kEach], n[kEach];
     x.get(t);
     if constexpr (BR != kNoBranch) b.get(n);
-    if (BR != kNoBranch && samples && row < p.rows) load_gate<T>(p, row / p.gate_rows, at.col, live, g);
+    if (BR != kNoBranch && samples && row < p.rows) load_gate<T>(p, row / p.gate_rows, cols, g);
     request(row + step);
     float4 stats = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (BR == kPostNorm) {
-      const float2 s = row_stats<T, L>(n, at.live, p.layer, p, meet, at.row_wave);
+      const float2 s = row_stats<L>(n, at.cols, p.layer, p, meet, at.row_wave);
       stats.x = s.x, stats.y = s.y;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) n[e] = fmaf((n[e] - s.x) * s.y, pw[e], pb[e]);
@@ -252,26 +278,23 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
       for (int e = 0; e < kEach; ++e) t[e] = fmaf(g[e], n[e], p.scale * t[e]);
       Eight<T, STREAM> sum;
       sum.set(t);
-      sum.store(p.total, row, at.col, live);
+      sum.store(p.total, row, cols);
       sum.get(t);
     }
     if (p.weight) {
-      const float2 s = row_stats<T, L>(t, at.live, p.layer, p, meet, at.row_wave);
+      const float2 s = row_stats<L>(t, at.cols, p.layer, p, meet, at.row_wave);
       stats.z = s.x, stats.w = s.y;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) t[e] = fmaf((t[e] - s.x) * s.y, w[e], c[e]);
       Eight<T, STREAM> y;
       y.set(t);
-      y.store(p.y, row, at.col, live);
+      y.store(p.y, row, cols);
       if (p.packed) {   // what is kept is y as it is stored
         y.get(t);
-        uint32_t words[2];
-        const uint32_t code = p.format == kPackInt8 ? pack8_lane<kPackInt8>(t, live, words) : pack8_lane<kPackE4m3>(t, live, words);
-        pack8_store<T>(p.packed + row * p.C + at.col, words, live, p.C);
-        if (live > 0 && at.lane % 4 == 0) p.codes[row * ((p.C + kPackGroup - 1) / kPackGroup) + at.col / kPackGroup] = static_cast<unsigned char>(code);
+        p.format == kPackInt8 ? keep<T, kPackInt8>(p, row, cols, t, at.lane) : keep<T, kPackE4m3>(p, row, cols, t, at.lane);
       }
     }
-    if (row < p.rows && at.col == 0) p.stats[row] = stats;
+    if (row < p.rows && at.cols.at[0] == 0) p.stats[row] = stats;
   }
 }
 
@@ -290,11 +313,11 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
   const bool rows_of_dy = MODE == kAnything ? p.plane_of[1] >= 0 : MODE == kFullLayer, rows_of_dt = MODE == kAnything || MODE == kFullLayer;
   __shared__ float2 said[2][16];
   __shared__ float lds[kLds];
-  const Place at = place<L>(p);
+  const Place at = place<T, L>(p);
   Meeting meet{said, 0, at.group * p.waves, p.waves, at.lane, at.wave};
   const float inv = 1.f / static_cast<float>(p.C);
   float w[kEach], k2[kEach];   // k2: what dt is multiplied by in front of the post norm, g . pw; the gate where there is none
-  load_vector(p.weight, at.col, at.live, 0.f, w);
+  load_vector(p.weight, at.cols, 0.f, w);
   float sum[4][kEach], gated[2][kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) sum[0][e] = sum[1][e] = sum[2][e] = sum[3][e] = gated[0][e] = gated[1][e] = 0.f;
@@ -304,8 +327,8 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
     if (WIDE || p.groups == 1) {
 #pragma unroll
       for (int i = 0; i < kEach; i += 4) {
-        if (i >= at.live) break;
-        float4* out = reinterpret_cast<float4*>(to + at.col + i);
+        if (!at.cols.on[i / 4]) break;
+        float4* out = reinterpret_cast<float4*>(to + at.cols.at[i / 4]);
         float4 s = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         if (add) {
           const float4 old = *out;
@@ -318,7 +341,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
     const int span = (L < 64 ? L : p.waves * 64) * kEach;
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) lds[at.group * span + at.col + e] = v[e];
+    for (int e = 0; e < kEach; ++e) lds[at.group * span + at.cols.at[e / 4] + e % 4] = v[e];
     __syncthreads();
     for (int c = threadIdx.x; c < p.C; c += blockDim.x) {
       float s = 0.f;
@@ -343,10 +366,10 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
   for (; gate < behind_gate; ++gate) {
     const int64_t r0 = gate * p.gate_rows + offset, r1 = min((gate + 1) * p.gate_rows, p.rows);
     if constexpr (BR != kNoBranch) {
-      load_gate<T>(p, gate, at.col, at.live, k2);
+      load_gate<T>(p, gate, at.cols, k2);
       if constexpr (BR == kPostNorm) {
         float pw[kEach];
-        load_vector(p.post_weight, at.col, at.live, 0.f, pw);
+        load_vector(p.post_weight, at.cols, 0.f, pw);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) k2[e] *= pw[e];
       }
@@ -354,20 +377,20 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
     Eight<T, STREAM> dy, d0, t, b;
     float4 stats, next_stats;
     auto request = [&](int64_t row) {
-      const int live = row < r1 ? at.live : 0;
+      const Cols cols = at.cols.in(row < r1);
       if (has_norm) {
-        dy.load(p.dy, row, at.col, live);
-        t.load(p.total, row, at.col, live);
+        dy.load(p.dy, row, cols);
+        t.load(p.total, row, cols);
       }
-      if (has_dtotal) d0.load(p.dtotal, row, at.col, live);
-      if constexpr (BR != kNoBranch) b.load(p.branch, row, at.col, live);
+      if (has_dtotal) d0.load(p.dtotal, row, cols);
+      if constexpr (BR != kNoBranch) b.load(p.branch, row, cols);
       next_stats = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < r1) next_stats = p.stats[row];
     };
     request(r0 + at.group);
     for (int64_t first = r0; first < r1; first += step) {
       const int64_t row = first + at.group;
-      const int live = row < r1 ? at.live : 0;
+      const Cols cols = at.cols.in(row < r1);
       stats = next_stats;
       float d[kEach], h[kEach], k[kEach], bh[kEach];
       if (has_dtotal)
@@ -409,7 +432,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
 #pragma unroll
           for (int e = 0; e < kEach; ++e) k[e] -= a;
         }
-        const float r_lo = live > 0 ? stats.w : 0.f, r_hi = there<T>(live, 4) ? stats.w : 0.f;   // (d stays 0 where nothing is)
+        const float r_lo = cols.on[0] ? stats.w : 0.f, r_hi = cols.on[1] ? stats.w : 0.f;   // (d stays 0 where nothing is)
 #pragma unroll
         for (int e = 0; e < kEach; ++e) d[e] = fmaf(e < 4 ? r_lo : r_hi, fmaf(-h[e], q, k[e]), d[e]);
       }
@@ -422,7 +445,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
         } else {
           dx.set(d);
         }
-        dx.store(p.dx, row, at.col, live);
+        dx.store(p.dx, row, cols);
       }
       if constexpr (BR != kNoBranch) {
         if (BR == kPostNorm && layer)
@@ -459,15 +482,15 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
         }
         Eight<T, STREAM> db;
         db.set(k);
-        db.store(p.dbranch, row, at.col, live);
+        db.store(p.dbranch, row, cols);
       }
     }
     if (many) {
       // dg of these rows, and what the post norm's gradients have from them
       float g[kEach], dg[kEach], pw[kEach], pb[kEach];
-      load_gate<T>(p, gate, at.col, at.live, g);
-      load_vector(p.post_weight, at.col, at.live, 1.f, pw);
-      load_vector(p.post_bias, at.col, at.live, 0.f, pb);
+      load_gate<T>(p, gate, at.cols, g);
+      load_vector(p.post_weight, at.cols, 1.f, pw);
+      load_vector(p.post_bias, at.cols, 0.f, pb);
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         dg[e] = fmaf(pw[e], sum[2][e], pb[e] * sum[3][e]);
@@ -717,7 +740,7 @@ int residual_norm_fwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
   a.waves = s.waves, a.groups = s.groups;
   a.layer = n.layer, a.scale = n.scale, a.eps = n.eps;
   const int64_t blocks = (rows + s.groups - 1) / s.groups;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 8192 / (s.threads / 64))));
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 4096 / (s.threads / 64))));
   const int br = !branch.ptr ? kNoBranch : n.post_weight ? kPostNorm : kBranch;
   const double bytes = static_cast<double>(rows) * C * (eb * (1.0 + (branch.ptr ? 2 : 0) + (y.ptr ? 1 : 0)) + (packed ? 33.0 / 32 : 0));
   return dtype == kBF16 ? launch_fwd_of<bf16>(ctx, a, s, br, grid, kFwdNames[1], bytes) : launch_fwd_of<float>(ctx, a, s, br, grid, kFwdNames[0], bytes);
