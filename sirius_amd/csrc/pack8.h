@@ -91,28 +91,4 @@ __device__ __forceinline__ uint32_t pack8_four(const float* v, bool live, uint32
   return code;
 }
 
-// A lane's two words to and from memory, as one access where rows of C are whole eights (bf16: always).
-template <typename T>
-__device__ __forceinline__ void pack8_store(unsigned char* to, const uint32_t* words, int live, int C) {
-  if (sizeof(T) == 2 || C % 8 == 0) {
-    if (live > 0) *reinterpret_cast<uint2*>(to) = make_uint2(words[0], words[1]);
-  } else {
-    if (live > 0) reinterpret_cast<uint32_t*>(to)[0] = words[0];
-    if (live > 4) reinterpret_cast<uint32_t*>(to)[1] = words[1];
-  }
-}
-template <typename T>
-__device__ __forceinline__ void pack8_load(const unsigned char* from, uint32_t* words, int live, int C) {
-  words[0] = words[1] = 0;
-  if (sizeof(T) == 2 || C % 8 == 0) {
-    if (live > 0) {
-      const uint2 v = *reinterpret_cast<const uint2*>(from);
-      words[0] = v.x, words[1] = v.y;
-    }
-  } else {
-    if (live > 0) words[0] = reinterpret_cast<const uint32_t*>(from)[0];
-    if (live > 4) words[1] = reinterpret_cast<const uint32_t*>(from)[1];
-  }
-}
-
 }  // namespace tch

@@ -13,7 +13,6 @@
 namespace tch {
 namespace {
 
-
 struct PackArgs {
   const void* x;          // kept: rows ldx apart
   void* h;                // act(x); may be null
@@ -21,88 +20,79 @@ struct PackArgs {
   unsigned char* data;    // [M][C]
   unsigned char* codes;   // [M][groups of 32]
   int64_t ldx, ldh;
-  uint64_t total;         // rows * eights of a row, whole groups
+  uint64_t total;         // rows * chunks of a row, whole groups
   int C, groups, act;
-  FastDiv eights;
+  FastDiv chunks;
 };
 
+// A lane has a 16-byte chunk: eight numbers in bf16, four in fp32, and the four or eight lanes of a group are neighbours (a row has whole groups of
+// them; all lanes of a wavefront go round together).  One chunk a lane: with four on their way together 8192 x 4096 in bf16 with GELU takes 33
+// us instead of 31, fetching 8192 x 1024 7.4 instead of 6.5, and small tensors leave the chip idle.
 template <typename T>
-struct EightOf {
-  static constexpr int N = sizeof(T) / 2;
-  Chunk c[N];
-  template <bool STREAM>
-  __device__ __forceinline__ void load(const T* from, int live) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      c[i] = zero_chunk();
-      if (i * (8 / N) < live) c[i].u = STREAM ? load_streaming_u4(from, i) : reinterpret_cast<const uint4*>(from)[i];
-    }
-  }
-  __device__ __forceinline__ void get(float* v) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) chunk_to_float<T>(c[i], v + i * (8 / N));
-  }
-  template <bool STREAM>
-  __device__ __forceinline__ static void store(T* to, const float* v, int live) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i * (8 / N) < live) store_u4<STREAM>(to, i, float_to_chunk<T>(v + i * (8 / N)).u);
-  }
-};
-
 struct At {
+  static constexpr int E = Elem<T>::kPerChunk;
   int64_t row;
-  int col, live;
+  int col;
+  bool on;
+  __device__ __forceinline__ At(const PackArgs& p, uint64_t q) : row(0), col(0), on(false) {
+    if (q >= p.total) return;
+    uint32_t r, chunk;
+    p.chunks.divmod(static_cast<uint32_t>(q), r, chunk);
+    row = r;
+    col = static_cast<int>(chunk) * E;
+    on = col < p.C;
+  }
 };
-__device__ __forceinline__ At place(const PackArgs& p, uint64_t q) {
-  At a{0, 0, 0};
-  if (q >= p.total) return a;
-  uint32_t row, eight;
-  p.eights.divmod(static_cast<uint32_t>(q), row, eight);
-  a.row = row;
-  a.col = static_cast<int>(eight) * 8;
-  a.live = max(0, min(p.C - a.col, 8));
-  return a;
-}
 
-// An eight a thread.  (Four on their way together: 8192 x 4096 in bf16 with GELU 33 us instead of 31, fetching 8192 x 1024 7.4 instead of 6.5, and
-// small tensors leave the chip idle.)  The four lanes of a group are neighbours (a row has whole groups of them), and all lanes of a
-// wavefront go round together.
 template <typename T, int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void pack8_kernel(PackArgs p) {
+  constexpr int E = Elem<T>::kPerChunk;
   const uint64_t stride = static_cast<uint64_t>(gridDim.x) * 256;
   for (uint64_t base = static_cast<uint64_t>(blockIdx.x) * 256; base < p.total; base += stride) {
-    const At at = place(p, base + threadIdx.x);
-    EightOf<T> x;
-    x.template load<STREAM>(static_cast<const T*>(p.x) + at.row * p.ldx + at.col, at.live);
-    float v[8];
-    uint32_t words[2];
-    x.get(v);
-    const uint32_t code = pack8_lane<FMT>(v, at.live, words);
-    pack8_store<T>(p.data + at.row * p.C + at.col, words, at.live, p.C);
-    if (at.live > 0 && threadIdx.x % 4 == 0) p.codes[at.row * p.groups + at.col / kPackGroup] = static_cast<unsigned char>(code);
+    const At<T> at(p, base + threadIdx.x);
+    const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + at.row * p.ldx + at.col);
+    Chunk x = zero_chunk();
+    if (at.on) x.u = STREAM ? load_streaming_u4(from, 0) : *from;
+    float v[E];
+    chunk_to_float<T>(x, v);
+    unsigned char* data = p.data + at.row * p.C + at.col;
+    uint32_t words[2], code;
+    if constexpr (E == 8) {
+      code = pack8_lane<FMT>(v, at.on ? 8 : 0, words);
+      if (at.on) *reinterpret_cast<uint2*>(data) = make_uint2(words[0], words[1]);
+    } else {
+      code = pack8_four<FMT>(v, at.on, words);
+      if (at.on) *reinterpret_cast<uint32_t*>(data) = words[0];
+    }
+    if (at.on && threadIdx.x % (kPackGroup / E) == 0) p.codes[at.row * p.groups + at.col / kPackGroup] = static_cast<unsigned char>(code);
     if (p.h)
       with_activation(p.act, [&](auto act_c) {
         constexpr int ACT = decltype(act_c)::value;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = act_value<T, ACT>(v[e]);
-        EightOf<T>::template store<STREAM>(static_cast<T*>(p.h) + at.row * p.ldh + at.col, v, at.live);
+        for (int e = 0; e < E; ++e) v[e] = act_value<T, ACT>(v[e]);
+        if (at.on) store_u4<STREAM>(static_cast<T*>(p.h) + at.row * p.ldh + at.col, 0, float_to_chunk<T>(v).u);
       });
   }
 }
 
 template <typename T, int FMT, bool STREAM>
 __global__ __launch_bounds__(256) void unpack8_kernel(PackArgs p) {
+  constexpr int E = Elem<T>::kPerChunk;
   const uint64_t stride = static_cast<uint64_t>(gridDim.x) * 256;
   for (uint64_t q = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; q < p.total; q += stride) {
-    const At at = place(p, q);
-    uint32_t words[2];
-    pack8_load<T>(p.data + at.row * p.C + at.col, words, at.live, p.C);
-    const float unit = pack8_unit(at.live > 0 ? p.codes[at.row * p.groups + at.col / kPackGroup] : 0);
-    float v[8];
-    unpack8_word<FMT>(words[0], unit, v);
-    unpack8_word<FMT>(words[1], unit, v + 4);
-    EightOf<T>::template store<STREAM>(static_cast<T*>(p.out) + at.row * p.ldx + at.col, v, at.live);
+    const At<T> at(p, q);
+    if (!at.on) continue;
+    const unsigned char* data = p.data + at.row * p.C + at.col;
+    const float unit = pack8_unit(p.codes[at.row * p.groups + at.col / kPackGroup]);
+    float v[E];
+    if constexpr (E == 8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(data);
+      unpack8_word<FMT>(w.x, unit, v);
+      unpack8_word<FMT>(w.y, unit, v + 4);
+    } else {
+      unpack8_word<FMT>(*reinterpret_cast<const uint32_t*>(data), unit, v);
+    }
+    store_u4<STREAM>(static_cast<T*>(p.out) + at.row * p.ldx + at.col, 0, float_to_chunk<T>(v).u);
   }
 }
 
@@ -118,10 +108,10 @@ int bind(const char* what, PackArgs& a, int dtype, void* data, void* codes, int 
   a.data = static_cast<unsigned char*>(data), a.codes = static_cast<unsigned char*>(codes);
   a.C = static_cast<int>(C);
   a.groups = static_cast<int>((C + kPackGroup - 1) / kPackGroup);
-  const int64_t eights = a.groups * 4ll;
-  TCH_CHECK_ARG(M * eights < (1ll << 31), name + ": tensor exceeds 2^34 elements");
-  a.total = static_cast<uint64_t>(M * eights);
-  a.eights = FastDiv(static_cast<uint32_t>(eights));
+  const int64_t chunks = a.groups * (dtype == kBF16 ? 4ll : 8ll);
+  TCH_CHECK_ARG(M * chunks < (1ll << 31), name + ": tensor exceeds 2^31 chunks");
+  a.total = static_cast<uint64_t>(M * chunks);
+  a.chunks = FastDiv(static_cast<uint32_t>(chunks));
   return 0;
 }
 
