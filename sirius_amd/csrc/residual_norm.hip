@@ -620,7 +620,8 @@ Shape shape_of(int64_t rows, int C) {
   return {64, waves, groups, waves * groups * 64};
 }
 
-// The backward's workgroups: as many as the chip holds (three of four wavefronts a compute unit, one of a wide row), with equally many rounds each.
+// The backward's workgroups: sixteen of a wide row's wavefronts a compute unit, eight otherwise, with equally many rounds each.  (Twelve are resident,
+// but every workgroup leaves its sums: 8192 x 4096 in bf16 84 us with 512 of eight, 78 with 256.)
 struct Cut {
   Shape shape;
   int64_t blocks, pieces;   // pieces: workgroups of a gate's rows
@@ -630,7 +631,7 @@ struct Cut {
 Cut cut_rows(int64_t rows, int C, int64_t gates) {
   Cut c{};
   c.shape = shape_of(rows, C);
-  const int64_t want = c.shape.threads > 512 ? 256 : c.shape.threads > 256 ? 512 : 768, rounds = (rows / gates + c.shape.groups - 1) / c.shape.groups;
+  const int64_t want = c.shape.threads > 512 ? 256 : c.shape.threads > 256 ? 256 : 512, rounds = (rows / gates + c.shape.groups - 1) / c.shape.groups;
   c.split = gates <= want;
   if (c.split) {
     const int64_t most = want / gates, each = (rounds + most - 1) / most;
