@@ -193,3 +193,25 @@ def test_a_step_on_other_batches_and_clipping():
     assert eng.release_activations() > 0
     eng.forward_backward(tokens(SMALL, 2, 32).cuda())
     assert math.isfinite(eng.last_loss())
+
+
+from test_colocate_gpu import clean_runtime  # noqa: E402,F401
+
+
+def test_handover_with_8_bits_kept(clean_runtime, monkeypatch, tmp_path):  # noqa: F811
+    """The train script under the colocation protocol with the activations in the shared pool: the peer asks for memory, a micro-batch is
+    killed between its launches and trained again, and every sequence counts once."""
+    from sirius_amd.train import gpt2 as script
+    env = {"COLTRAIN_MODE": "colocate-l1", "COLTRAIN_HOOK_MODE": "xsched-sync", "COLTRAIN_USE_XSCHED": "1", "COLTRAIN_HAS_INFER_SERVER": "1",
+           "COLTRAIN_USE_SHARED_TENSOR": "1", "COLTRAIN_SHARED_TENSOR_POOL_GB": "2", "COLTRAIN_PROFILE_LOG_PATH": str(tmp_path / "train-profile.csv")}
+    for k, v in env.items():
+        monkeypatch.setenv(k, v)
+    peer = script.PeerScript({3: ("l1", 2), 10: ("exit", 8)}, delay_ms=1.0)
+    try:
+        out = script.train(1, 8, dataset_size=8 * 8, seq_len=64, dtype=torch.bfloat16, optimizer="adamw", peer=peer, num_distinct_samples=16,
+                           n_embd=64, n_layer=2, n_head=4, n_pos=64, kept="int8")
+    finally:
+        peer.stop()
+    assert out["trainer"].get_last_epoch_stat().finished_sample == 8 * 8
+    assert [k for _, k, _ in peer.sent] == ["l1", "exit"]
+    assert all(torch.isfinite(v).all() for v in out["model"].state_dict().values())

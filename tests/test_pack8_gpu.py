@@ -154,3 +154,29 @@ def test_no_rows_and_replays(ctx):
         c.run(prog)
         c.synchronize()
         assert torch.equal(back.double(), kept_of(x, "e4m3")[0])
+
+
+def test_offsets_beyond_four_gib(ctx):
+    """Rows of x 2^31 bytes apart, and kept numbers behind 2^31 of their own."""
+    from sirius_amd import ops
+    ld, C = 2 ** 30 + 64, 96
+    x = torch.empty(4 * ld, dtype=torch.bfloat16, device="cuda").view(4, ld)[:, :C]
+    x.copy_(make(4, C, "bf16"))
+    packed = ops.Packed8.empty(4, C)
+    ops.pack8(ctx, x, packed)
+    kept, codes = kept_of(x.contiguous(), "int8")
+    assert torch.equal(packed.scales, codes)
+    x.zero_()
+    ops.unpack8(ctx, packed, x)
+    assert torch.equal(x.double(), kept)
+    del x
+    rows, C = 270_000, 8192
+    x = torch.zeros(rows, C, dtype=torch.bfloat16, device="cuda")
+    x[-5:] = make(5, C, "bf16")
+    packed = ops.Packed8.empty(rows, C, "e4m3")
+    ops.pack8(ctx, x, packed)
+    kept, codes = kept_of(x[-5:], "e4m3")
+    assert torch.equal(packed.scales[-5:], codes) and int(packed.data[:-5].max()) == 0
+    x.fill_(7.0)
+    ops.unpack8(ctx, packed, x)
+    assert torch.equal(x[-5:].double(), kept) and x[:-5].abs().max().item() == 0

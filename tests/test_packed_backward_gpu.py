@@ -240,3 +240,62 @@ def test_recorded_and_replayed(ctx):
         ctx.synchronize()
         for a, b in zip(got, (h, dz, low, dw, db)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_more_than_the_cache_holds(ctx, fmt):
+    """The kernels that stream past the cache: the bits of those that do not, on a part of the rows."""
+    from sirius_amd import ops
+    M, F, few = 8192, 5632, 300
+    pre, dh = normal(M, 2 * F, dtype=torch.bfloat16), normal(M, F, dtype=torch.bfloat16, seed=1)
+    packed, kept = keep(ctx, pre, fmt)
+    part, kept_part = keep(ctx, pre[:few].contiguous(), fmt)
+    assert torch.equal(packed.data[:few], part.data) and torch.equal(packed.scales[:few], part.scales) and torch.equal(kept[:few], kept_part)
+    out, h, low = torch.empty_like(pre), torch.empty_like(dh), torch.empty_like(pre)
+    ops.gated_act_bwd_packed(ctx, dh, packed, out, "silu", h=h, dpre_low=low)
+    out2, h2, low2 = torch.empty_like(pre[:few]), torch.empty_like(dh[:few]), torch.empty_like(pre[:few])
+    ops.gated_act_bwd_packed(ctx, dh[:few], part, out2, "silu", h=h2, dpre_low=low2)
+    assert torch.equal(out[:few], out2) and torch.equal(h[:few], h2) and torch.equal(low[:few], low2)
+    big, dz, z = normal(M, 2 * F, dtype=torch.bfloat16, seed=2), torch.empty_like(pre), torch.empty_like(pre)
+    ops.act_fwd_pack8(ctx, pre, z, packed, "gelu")
+    ops.act_bwd_packed(ctx, big, packed, dz, "gelu")
+    z2, dz2 = torch.empty_like(pre[:few]), torch.empty_like(pre[:few])
+    ops.act_fwd_pack8(ctx, pre[:few], z2, part, "gelu")
+    ops.act_bwd_packed(ctx, big[:few], part, dz2, "gelu")
+    assert torch.equal(z[:few], z2) and torch.equal(dz[:few], dz2)
+
+
+def test_two_streams_at_once(ctx):
+    """Two contexts on streams of their own, each with its own buffers and workspace, submitted in turn."""
+    from sirius_amd import ops
+    M, K, N = 2048, 512, 768
+    sides = []
+    for seed in (1, 2):
+        s = torch.cuda.Stream()
+        x, dy = normal(M, K, dtype=torch.bfloat16, seed=seed), normal(M, N, dtype=torch.bfloat16, seed=seed + 5)
+        packed = ops.Packed8.empty(M, K, "e4m3")
+        stats, y = torch.empty(M, 4, device="cuda"), torch.empty_like(x)
+        w, dwn = torch.rand(K, device="cuda"), torch.empty(K, device="cuda")
+        dw, dx = torch.empty(N, K, device="cuda"), torch.empty_like(x)
+        ws = torch.empty(ops.linear_wgrad_packed_workspace_bytes(packed, dy), dtype=torch.uint8, device="cuda")
+        ws2 = torch.empty(ops.residual_norm_bwd_workspace_bytes(x), dtype=torch.uint8, device="cuda")
+        sides.append((s, x, dy, packed, stats, y, w, dwn, dw, dx, ws, ws2))
+    torch.cuda.synchronize()
+
+    def go(c, side):
+        _, x, dy, packed, stats, y, w, dwn, dw, dx, ws, ws2 = side
+        ops.residual_norm_fwd(c, x, None, None, y, stats, weight=w, packed=packed)
+        ops.linear_wgrad_packed(c, packed, dy, dw, workspace=ws)
+        ops.residual_norm_bwd(c, y, None, x, None, dx, None, stats, weight=w, dweight=dwn, workspace=ws2)
+    contexts = [ops.Context(side[0]) for side in sides]
+    for _ in range(5):
+        for c, side in zip(contexts, sides):
+            go(c, side)
+    for c in contexts:
+        c.synchronize()
+    both = [[t.clone() for t in (side[5], side[7], side[8], side[9])] for side in sides]
+    for side, got in zip(sides, both):
+        go(ctx, side)
+        ctx.synchronize()
+        for a, b in zip(got, (side[5], side[7], side[8], side[9])):
+            assert torch.equal(a, b)

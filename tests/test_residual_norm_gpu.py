@@ -319,3 +319,38 @@ def test_against_differences(ctx, kind):
     size = sum((ref["d" + k][0].abs() * along[k].view_as(ref["d" + k][0]).abs()).sum() for k in names).item()
     # (total is stored in fp32: the gradients are taken half a step beside the formula's place)
     assert abs(slope - mine) <= tol + 100 * h * h * size + 2.0 ** -20 * size, (slope, mine, tol, size)
+
+
+def test_rows_beyond_four_gib(ctx):
+    """Rows 2^31 bytes apart: 64-bit offsets, forward and back."""
+    rows, C, ld = 4, 520, 2 ** 30 + 64
+    s = make(rows, C, "bf16", "layer")
+    want = forward(ctx, s, "layer", 1.0)
+    grads = backward(ctx, s, want["total"], want["stats"], "layer", 1.0)
+    far = {k: torch.empty(rows * ld, dtype=torch.bfloat16, device="cuda").view(rows, ld)[:, :C] for k in ("x", "branch", "dy", "dtotal", "total", "y", "dx", "dbranch")}
+    for k in ("x", "branch", "dy", "dtotal"):
+        far[k].copy_(s[k])
+    t = dict(s, **{k: far[k] for k in ("x", "branch", "dy", "dtotal")})
+    out = forward(ctx, t, "layer", 1.0, total=far["total"], y=far["y"])
+    assert torch.equal(out["total"], want["total"]) and torch.equal(out["y"], want["y"])
+    got = backward(ctx, t, far["total"], out["stats"], "layer", 1.0, dx=far["dx"], dbranch=far["dbranch"])
+    for k in grads:
+        assert torch.equal(got[k], grads[k]), k
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_more_than_the_cache_holds(ctx, dtype):
+    """The kernels that stream past the cache give the same bits as those that do not: a part of the rows alone."""
+    rows, C = (6000, 8192) if dtype == "bf16" else (9000, 4096)
+    for kind in ("rms", "layer"):
+        s = make(rows, C, dtype, kind, gates=1)
+        out = forward(ctx, s, kind, 1.0)
+        got = backward(ctx, s, out["total"], out["stats"], kind, 1.0)
+        part = {k: t[:200].contiguous() if k in ("x", "branch", "dy", "dtotal") and t is not None else t for k, t in s.items()}
+        few = forward(ctx, part, kind, 1.0)
+        back = backward(ctx, part, few["total"], few["stats"], kind, 1.0)
+        for k in ("total", "y", "stats"):
+            assert torch.equal(out[k][:200], few[k]), k
+        for k in ("dx", "dbranch"):
+            assert torch.equal(got[k][:200], back[k]), k
+        check_backward(s, {k: t for k, t in got.items() if k in GRADS}, out["total"], kind, 1.0)

@@ -177,3 +177,17 @@ def test_rows_beyond_four_gib(ctx):
     freqs, y = ops.rotary_freqs(D).cuda(), torch.empty(rows, 2 * D, dtype=torch.bfloat16, device="cuda")
     ops.rotary_fwd(ctx, x, y, freqs, D, start=math.floor(1e6), seq=rows)
     close(y, *oracle(x, freqs, D, "half", torch.arange(rows) + 1_000_000, 1.0), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_more_than_the_cache_holds(ctx, dtype, layout):
+    """The kernel that streams past the cache: the bits of the one that does not, on a part of the rows."""
+    from sirius_amd import ops
+    rows = 14_000 if dtype == "bf16" else 7_000
+    x, freqs = make((rows, 40 * 128), TYPES[dtype]), ops.rotary_freqs(128).cuda()
+    y, few = torch.empty_like(x), torch.empty_like(x[:300])
+    ops.rotary_fwd(ctx, x, y, freqs, 128, layout=layout, start=0, seq=rows)
+    ops.rotary_fwd(ctx, x[:300], few, freqs, 128, layout=layout, start=0, seq=rows)
+    assert torch.equal(y[:300], few)
+    close(y[-50:], *oracle(x[-50:], freqs, 128, layout, torch.arange(rows - 50, rows), 1.0), TYPES[dtype])
