@@ -14,7 +14,7 @@
 // parts are joined about the row's.  What a workgroup adds up over its rows goes to the workspace, where a second launch adds the
 // workgroups up in fp64 in their order: the same bits every run.
 // In bf16 with both norms and a gate 8192 x 4096 forward 49 us (5.5 TB/s), backward 78 (5.2); 16384 x 8192 199 (5.4) and 280 (5.8); in fp32 8192 x 4096
-// 89 (6.0) and 140 (5.8); 8192 x 1024 with a LayerNorm and a gate forward 13.3; one token of 4096 3.5.
+// 89 (6.0) and 140 (5.8); 8192 x 1024 with a LayerNorm and a gate forward 12.5; one token of 4096 3.5.
 //
 // Reference call sites: the blocks that train/gpt2.py:26 and train/swin_b.py:38 build have a LayerNorm in front of each half and a
 // plain residual.
@@ -107,24 +107,33 @@ struct Cols {
   __device__ __forceinline__ Cols in(bool row) const { return {{at[0], at[1]}, {on[0] && row, on[1] && row}}; }
 };
 
+// What the lanes of a row know of its wavefronts' elements: divided once for all rows (LayerNorms 8192 x 4096 53 us for 59).
+struct Counts {
+  float inv, inv_here, there, inv_there;   // 1 / C, 1 / those of this wavefront, those of wavefront lane % 16 of the row and 1 / them
+};
+template <int L>
+__device__ __forceinline__ Counts counts(const NormArgs& p, int row_wave, int lane) {
+  auto elements = [&](int w) { return L < 64 ? p.C : max(min(p.C - w * 64 * kEach, 64 * kEach), 1); };
+  const float there = static_cast<float>(elements(lane & 15));
+  return {1.f / static_cast<float>(p.C), 1.f / static_cast<float>(elements(row_wave)), there, 1.f / there};
+}
+
 // mean and 1 / deviation of a row
 template <int L>
-__device__ __forceinline__ float2 row_stats(const float* v, const Cols& cols, int layer, const NormArgs& p, Meeting& meet, int row_wave) {
-  const float inv = 1.f / static_cast<float>(p.C);
+__device__ __forceinline__ float2 row_stats(const float* v, const Cols& cols, int layer, float eps, const Counts& n, Meeting& meet) {
   if (!layer) {
     float q = 0.f, none = 0.f;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) q = cols.on[e / 4] ? fmaf(v[e], v[e], q) : q;
     q = lane_sum<L>(q);
     meet.add(q, none);
-    return make_float2(0.f, 1.f / sqrtf(q * inv + p.eps));
+    return make_float2(0.f, rsqrtf(q * n.inv + eps));
   }
   float s = 0.f;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) s += cols.on[e / 4] ? v[e] : 0.f;
   s = lane_sum<L>(s);
-  auto elements = [&](int w) { return static_cast<float>(min(p.C - w * 64 * kEach, 64 * kEach)); };   // of a wavefront
-  const float n = L < 64 ? static_cast<float>(p.C) : elements(row_wave), mine = s / n;
+  const float mine = s * n.inv_here;
   float q = 0.f;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
@@ -132,13 +141,11 @@ __device__ __forceinline__ float2 row_stats(const float* v, const Cols& cols, in
     q = cols.on[e / 4] ? fmaf(d, d, q) : q;
   }
   q = lane_sum<L>(q);
-  if (meet.waves == 1) return make_float2(mine, 1.f / sqrtf(q * inv + p.eps));
+  if (meet.waves == 1) return make_float2(mine, rsqrtf(q * n.inv + eps));
   const float2 h = meet.say(s, q);
-  const float mean = lane_sum<16>(h.x) * inv;
-  const int w = meet.lane & 15;
-  const float m = elements(w), d = h.x / m - mean;
-  q = lane_sum<16>(w < meet.waves ? fmaf(m * d, d, h.y) : 0.f);
-  return make_float2(mean, 1.f / sqrtf(q * inv + p.eps));
+  const float mean = lane_sum<16>(h.x) * n.inv, d = h.x * n.inv_there - mean;
+  q = lane_sum<16>((meet.lane & 15) < meet.waves ? fmaf(n.there * d, d, h.y) : 0.f);
+  return make_float2(mean, rsqrtf(q * n.inv + eps));
 }
 
 // A lane's eight as they lie in memory.
@@ -243,6 +250,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
   __shared__ float2 said[2][16];
   const Place at = place<T, L>(p);
   Meeting meet{said, 0, at.group * p.waves, p.waves, at.lane, at.wave};
+  const Counts count = counts<L>(p, at.row_wave, at.lane);
   const bool samples = p.gate_rows < p.rows;
   float w[kEach], c[kEach], pw[kEach], pb[kEach], g[kEach];
   load_vector(p.weight, at.cols, 1.f, w);
@@ -275,7 +283,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
     request(x, b, row + AHEAD * step);
     float4 stats = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (BR == kPostNorm) {
-      const float2 s = row_stats<L>(n, at.cols, p.layer, p, meet, at.row_wave);
+      const float2 s = row_stats<L>(n, at.cols, p.layer, p.eps, count, meet);
       stats.x = s.x, stats.y = s.y;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) n[e] = fmaf((n[e] - s.x) * s.y, pw[e], pb[e]);
@@ -289,7 +297,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
       sum.get(t);
     }
     if (p.weight) {
-      const float2 s = row_stats<L>(t, at.cols, p.layer, p, meet, at.row_wave);
+      const float2 s = row_stats<L>(t, at.cols, p.layer, p.eps, count, meet);
       stats.z = s.x, stats.w = s.y;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) t[e] = fmaf((t[e] - s.x) * s.y, w[e], c[e]);
@@ -321,7 +329,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
 enum BwdMode : int { kAnything = 0, kFullRms = 1, kFullLayer = 2 };
 template <typename T, int L, bool WIDE, int BR, int MODE, bool STREAM>
 __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_norm_bwd_kernel(NormArgs p) {
-  constexpr int kLds = L < 64 ? 256 * kEach : WIDE ? 1 : 512 * kEach;   // (a wide row's workgroup has one row at a time, and nothing to add up here)
+  constexpr int kLds = WIDE ? 1 : 256 * kEach;   // (rows of more than four wavefronts come one at a time: there is nothing to add up here)
   const bool has_norm = MODE != kAnything || p.weight, has_dtotal = MODE != kAnything || p.dtotal.at, has_dx = MODE != kAnything || p.dx.at;
   const bool layer = MODE == kAnything ? p.layer != 0 : MODE == kFullLayer;
   const bool many = MODE == kAnything && !p.split_gates;
