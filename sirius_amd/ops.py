@@ -1220,7 +1220,7 @@ def _rotary(ctx, x, y, freqs, head_dim, layout, positions, start, seq, scale, ba
         assert x.dim() >= 2, "the length of a sequence"
         seq = x.shape[-2]
     check(lib().tch_rotary(ctx.handle, dtype_code(x), xp, ldx, yp, ldy, _p(freqs), _p(positions),
-                           int(positions is not None and positions.dtype == torch.int64), int(start), max(int(seq), 1), rows, width // head_dim,
+                           int(positions is not None and positions.dtype == torch.int64), int(start), int(seq) if rows else 1, rows, width // head_dim,
                            head_dim, 2 * freqs.numel(), int(layout == "interleaved"), float(scale), int(back)), "tch_rotary")
 
 

@@ -53,3 +53,19 @@ def test_frequencies():
         share = min(max((turns - 1.0) / 31.0, 0.0), 1.0)
         assert abs(g[i].item() - f[i].item() * (share + (1 - share) / 4.0)) <= 2.0 ** -50 * f[i].item()
     assert g[0] == f[0] and g[-1] == f[-1] / 4.0
+
+
+@pytest.mark.parametrize("seq", [0, -4])
+def test_a_length_that_is_none_is_not_taken_for_one(seq, monkeypatch):
+    from sirius_amd import ops
+
+    class Here:
+        handle = None
+
+        class stream:
+            device = torch.device("cpu")
+    monkeypatch.setattr(ops, "_matrix", lambda ctx, name, t, *more: (A if name == "x" else B, 128, 4))
+    monkeypatch.setattr(ops, "_p", lambda t: None if t is None else C)
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="length of a sequence"):
+        ops.rotary_fwd(Here, x, x, torch.zeros(32, dtype=torch.float64), 64, seq=seq)
