@@ -1329,7 +1329,7 @@ def linear_wgrad_packed(ctx, packed, dy, dw, dbias=None, accumulate=False, works
     assert workspace is not None and workspace.is_contiguous() and workspace.device == ctx.stream.device, "workspace: contiguous, on the context's device"
     space = workspace.view(-1).view(torch.uint8)
     assert space.numel() >= linear_wgrad_packed_workspace_bytes(packed, dy), "linear_wgrad_packed workspace too small"
-    for name, t in (("dy", dy), ("dw", dw), ("dbias", dbias), ("dy_low", dy_low)):
+    for name, t in (("packed data", packed.data), ("packed scales", packed.scales), ("dy", dy), ("dw", dw), ("dbias", dbias), ("dy_low", dy_low)):
         assert t is None or t.data_ptr() >= space.data_ptr() + space.numel() or t.data_ptr() + t.numel() * t.element_size() <= space.data_ptr(), \
             f"the workspace overlaps {name}"
     x = space[:M * K * dy.element_size()].view(dy.dtype).view(M, K)

@@ -83,3 +83,25 @@ def test_weight_gradient_wrapper():
         ops.linear_wgrad_packed(Here, packed, dy, torch.zeros(32, 64))
     with pytest.raises(AssertionError, match="workspace"):
         ops.linear_wgrad_packed(Here, packed, dy, torch.zeros(32, 64), workspace=torch.zeros(2, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("which", ["data", "scales"])
+def test_a_workspace_over_what_is_kept(which):
+    """The weight gradient's own part of the workspace comes behind the fetched input: it is not over the kept numbers either."""
+    from sirius_amd import ops
+
+    class Here:
+        handle = None
+
+        class stream:
+            device = torch.device("cpu")
+    dy = torch.zeros(16, 32, dtype=torch.bfloat16)
+    need = ops.linear_wgrad_packed_workspace_bytes(ops.Packed8.empty(16, 64, device="cpu"), dy)
+    room = torch.zeros(need + 1024, dtype=torch.uint8)
+    data, scales = torch.zeros(16, 64, dtype=torch.uint8), torch.zeros(16, 2, dtype=torch.uint8)
+    if which == "data":
+        data = room[need - 16:need - 16 + 1024].view(16, 64)
+    else:
+        scales = room[need - 16:need + 16].view(16, 2)
+    with pytest.raises(AssertionError, match=f"overlaps packed {which}"):
+        ops.linear_wgrad_packed(Here, ops.Packed8(data, scales), dy, torch.zeros(32, 64), workspace=room[:need])
