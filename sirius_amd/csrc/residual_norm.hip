@@ -58,7 +58,7 @@ struct NormArgs {
   float* sums;                            // [workgroups][planes][C]
   float* dgate;                           // [gates][C]: written here where a workgroup has all rows of its gates
   int planes, plane_of[4];                // -1: nobody wants it
-  int split_gates, pieces;                // several workgroups have a part of a gate's rows: so many
+  int split_gates, pieces;                // a gate's rows are so many workgroups'
   int gates_each;                         // otherwise: gates of a workgroup
   int gates, add_gates;
 };
@@ -321,16 +321,16 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
   }
 }
 
-// What a call asks for, as far as it is worth a kernel of its own: kFullRms and kFullLayer have the norm behind the sum with dtotal and dx, and
-// a workgroup's rows have one gate, whose sums of dt b^ and dt go out as they are (what the gate makes of them the second launch does,
-// once for all of its rows); kFullRms adds no rows of dy and dt up (there are no biases).  kAnything is told the rest by its arguments:
-// among it several gates in a workgroup, where what each has to itself is taken here.  (Flags at run time and accumulators that nobody
-// asked for make 10 to 110 registers of a wide row's spill.)
+// What a call asks for, as far as it is worth a kernel of its own: kFullRms and kFullLayer have the norm behind the sum, and a workgroup's rows
+// have one gate, whose sums of dt b^ and dt go out as they are (what the gate makes of them the second launch does, once for all of
+// its rows); kFullRms adds no rows of dy and dt up (there are no biases).  kAnything is told the rest by its arguments: among it several
+// gates in a workgroup, where what each has to itself is taken here.  (Branches at run time and accumulators that nobody asked for make 10 to
+// 110 registers of a wide row's spill; what is only loaded or stored on request costs none.)
 enum BwdMode : int { kAnything = 0, kFullRms = 1, kFullLayer = 2 };
 template <typename T, int L, bool WIDE, int BR, int MODE, bool STREAM>
 __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_norm_bwd_kernel(NormArgs p) {
   constexpr int kLds = WIDE ? 1 : 256 * kEach;   // (rows of more than four wavefronts come one at a time: there is nothing to add up here)
-  const bool has_norm = MODE != kAnything || p.weight, has_dtotal = MODE != kAnything || p.dtotal.at, has_dx = MODE != kAnything || p.dx.at;
+  const bool has_norm = MODE != kAnything || p.weight, has_dtotal = p.dtotal.at, has_dx = p.dx.at;
   const bool layer = MODE == kAnything ? p.layer != 0 : MODE == kFullLayer;
   const bool many = MODE == kAnything && !p.split_gates;
   const bool rows_of_dy = MODE == kAnything ? p.plane_of[1] >= 0 : MODE == kFullLayer, rows_of_dt = MODE == kAnything || MODE == kFullLayer;
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
         dy.load(p.dy, row, cols);
         t.load(p.total, row, cols);
       }
-      if (has_dtotal) d0.load(p.dtotal, row, cols);
+      d0.load(p.dtotal, row, cols.in(has_dtotal));
       if constexpr (BR != kNoBranch) b.load(p.branch, row, cols);
       next_stats = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < r1) next_stats = p.stats[row];
@@ -416,11 +416,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
       const Cols cols = at.cols.in(row < r1);
       stats = next_stats;
       float d[kEach], h[kEach], k[kEach], bh[kEach];
-      if (has_dtotal)
-        d0.get(d);
-      else
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) d[e] = 0.f;
+      d0.get(d);
       if (has_norm) {
         dy.get(k);
         t.get(h);
@@ -637,16 +633,16 @@ struct Cut {
   Shape shape;
   int64_t blocks, pieces;   // pieces: workgroups of a gate's rows
   int gates_each;           // gates of a workgroup
-  bool split;               // a gate's rows are several workgroups'; otherwise a workgroup has all rows of its gates
+  bool split;               // a gate's rows are one or more workgroups'; otherwise a workgroup has all rows of several gates
 };
 Cut cut_rows(int64_t rows, int C, int64_t gates) {
   Cut c{};
   c.shape = shape_of(rows, C);
-  const int64_t want = c.shape.threads > 512 ? 256 : c.shape.threads > 256 ? 256 : 512, rounds = (rows / gates + c.shape.groups - 1) / c.shape.groups;
+  const int64_t want = c.shape.threads > 256 ? 256 : 512, rounds = (rows / gates + c.shape.groups - 1) / c.shape.groups;
   const int64_t most = std::max<int64_t>(want / gates, 1), each = (rounds + most - 1) / most;
   c.pieces = (rounds + each - 1) / each;
   c.gates_each = static_cast<int>((gates + want - 1) / want);
-  c.split = gates == 1 || c.pieces > 1;
+  c.split = c.gates_each == 1;
   c.blocks = c.split ? gates * c.pieces : (gates + c.gates_each - 1) / c.gates_each;
   return c;
 }
@@ -835,7 +831,7 @@ int residual_norm_bwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
   const int br = !branch.ptr ? kNoBranch : n.post_weight ? kPostNorm : kBranch;
   const double bytes = static_cast<double>(rows) * C * eb * ((dy.ptr ? 2.0 : 0) + (dtotal.ptr ? 1 : 0) + (dx.ptr ? 1 : 0) + (branch.ptr ? 2 : 0)) + need;
   const dim3 grid(static_cast<unsigned>(cut.blocks));
-  const bool full = n.weight && dtotal.ptr && dx.ptr && !many;
+  const bool full = n.weight && !many;
   const int mode = full && n.layer ? kFullLayer : full && a.plane_of[1] < 0 && a.plane_of[3] < 0 ? kFullRms : kAnything;
   const int rc = dtype == kBF16 ? launch_bwd_branch<bf16>(ctx, a, s, br, mode, grid, kBwdNames[1], bytes)
                                 : launch_bwd_branch<float>(ctx, a, s, br, mode, grid, kBwdNames[0], bytes);
