@@ -58,7 +58,7 @@ struct NormArgs {
   float* sums;                            // [workgroups][planes][C]
   float* dgate;                           // [gates][C]: written here where a workgroup has all rows of its gates
   int planes, plane_of[4];                // -1: nobody wants it
-  int split_gates, pieces;                // a gate's rows are so many workgroups'
+  int split_gates, pieces;                // several workgroups have a part of a gate's rows: so many
   int gates_each;                         // otherwise: gates of a workgroup
   int gates, add_gates;
 };
@@ -633,7 +633,7 @@ struct Cut {
   Shape shape;
   int64_t blocks, pieces;   // pieces: workgroups of a gate's rows
   int gates_each;           // gates of a workgroup
-  bool split;               // a gate's rows are one or more workgroups'; otherwise a workgroup has all rows of several gates
+  bool split;               // a gate's rows are several workgroups'; otherwise a workgroup has all rows of its gates
 };
 Cut cut_rows(int64_t rows, int C, int64_t gates) {
   Cut c{};
@@ -642,7 +642,7 @@ Cut cut_rows(int64_t rows, int C, int64_t gates) {
   const int64_t most = std::max<int64_t>(want / gates, 1), each = (rounds + most - 1) / most;
   c.pieces = (rounds + each - 1) / each;
   c.gates_each = static_cast<int>((gates + want - 1) / want);
-  c.split = c.gates_each == 1;
+  c.split = gates == 1 || c.pieces > 1;   // (256 gates of 8192 x 4096 from their sums in a second launch 110 us, with all their rows in a workgroup 91)
   c.blocks = c.split ? gates * c.pieces : (gates + c.gates_each - 1) / c.gates_each;
   return c;
 }
