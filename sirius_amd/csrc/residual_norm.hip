@@ -340,10 +340,31 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
   Meeting meet{said, 0, at.group * p.waves, p.waves, at.lane, at.wave};
   const float inv = 1.f / static_cast<float>(p.C);
   float w[kEach], k2[kEach];   // k2: what dt is multiplied by in front of the post norm, g . pw; the gate where there is none
+  // Where a wide row's lanes would spill they have what they need once a row or once a gate in places of their own there (256 gates of 16384 x
+  // 8192 with LayerNorms in bf16 382 -> 331 us, 4096 x 8192 in fp32 161 -> 158; bf16 with one gate 281 -> 289 us, so not there).
+  constexpr bool OWN = WIDE && (MODE == kAnything || sizeof(T) == 4);
+  __shared__ float4 own[!OWN ? 1 : MODE == kAnything ? 8 : 4][OWN ? 1024 : 1];
+  auto hold = [&](int i, const float* v) {
+    if constexpr (OWN) {
+      own[2 * i][threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+      own[2 * i + 1][threadIdx.x] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  };
+  auto fetch = [&](int i, float* v) {
+    if constexpr (OWN) {
+      const float4 lo = own[2 * i][threadIdx.x], hi = own[2 * i + 1][threadIdx.x];
+      v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+    }
+  };
   load_vector(p.weight, at.cols, 0.f, w);
+  hold(0, w);
   float sum[4][kEach], gated[2][kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) sum[0][e] = sum[1][e] = sum[2][e] = sum[3][e] = gated[0][e] = gated[1][e] = 0.f;
+  if constexpr (MODE == kAnything) {
+    hold(2, gated[0]);
+    hold(3, gated[1]);
+  }
 
   // The lanes' eight sums over the row groups of the workgroup, to `to` [C].
   auto add_up = [&](const float* v, float* to, bool add) {
@@ -396,6 +417,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
 #pragma unroll
         for (int e = 0; e < kEach; ++e) k2[e] *= pw[e];
       }
+      hold(1, k2);
     }
     Eight<T, STREAM> dy, d0, t, b;
     float4 stats, next_stats;
@@ -425,6 +447,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
       request(row + step);
       if (has_norm) {
         float a = 0.f, q = 0.f;
+        fetch(0, w);
         if (layer)
 #pragma unroll
           for (int e = 0; e < kEach; ++e) h[e] -= stats.z;
@@ -467,6 +490,7 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
         dx.store(p.dx, row, cols);
       }
       if constexpr (BR != kNoBranch) {
+        fetch(1, k2);
         if (BR == kPostNorm && layer)
 #pragma unroll
           for (int e = 0; e < kEach; ++e) bh[e] -= stats.x;
@@ -510,6 +534,10 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
       load_gate<T>(p, gate, at.cols, g);
       load_vector(p.post_weight, at.cols, 1.f, pw);
       load_vector(p.post_bias, at.cols, 0.f, pb);
+      if constexpr (MODE == kAnything) {
+        fetch(2, gated[0]);
+        fetch(3, gated[1]);
+      }
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         dg[e] = fmaf(pw[e], sum[2][e], pb[e] * sum[3][e]);
@@ -517,10 +545,18 @@ __global__ __launch_bounds__(L < 64 ? 256 : WIDE ? 1024 : 512) void residual_nor
         gated[1][e] = fmaf(g[e], sum[3][e], gated[1][e]);
         sum[2][e] = sum[3][e] = 0.f;
       }
+      if constexpr (MODE == kAnything) {
+        hold(2, gated[0]);
+        hold(3, gated[1]);
+      }
       if (p.dgate) add_up(dg, p.dgate + static_cast<int64_t>(gate) * p.C, p.add_gates);
     }
   }
   if (many) {
+    if constexpr (MODE == kAnything) {
+      fetch(2, gated[0]);
+      fetch(3, gated[1]);
+    }
 #pragma unroll
     for (int e = 0; e < kEach; ++e) sum[2][e] = gated[0][e], sum[3][e] = gated[1][e];
   }
@@ -755,7 +791,8 @@ int residual_norm_fwd(Context* ctx, int dtype, const ResidualNorm& n, const Rows
   a.waves = s.waves, a.groups = s.groups;
   a.layer = n.layer, a.scale = n.scale, a.eps = n.eps;
   const int64_t blocks = (rows + s.groups - 1) / s.groups;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 4096 / (s.threads / 64))));
+  // (sixteen wavefronts a compute unit at most and equally many workgroups on each: 16384 x 7168 in bf16 172 us, 259 with 292 workgroups)
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 256 * (1024 / s.threads))));
   const int br = !branch.ptr ? kNoBranch : n.post_weight ? kPostNorm : kBranch;
   const double bytes = static_cast<double>(rows) * C * (eb * (1.0 + (branch.ptr ? 2 : 0) + (y.ptr ? 1 : 0)) + (packed ? 33.0 / 32 : 0));
   return dtype == kBF16 ? launch_fwd_of<bf16>(ctx, a, s, br, grid, kFwdNames[1], bytes) : launch_fwd_of<float>(ctx, a, s, br, grid, kFwdNames[0], bytes);
