@@ -13,7 +13,7 @@
 // worked on.  Means, deviations and sums are fp32 in registers; a wavefront's part of a deviation is taken about its own mean, and the
 // parts are joined about the row's.  What a workgroup adds up over its rows goes to the workspace, where a second launch adds the
 // workgroups up in fp64 in their order: the same bits every run.
-// In bf16 with both norms and a gate 8192 x 4096 forward 49 us (5.5 TB/s), backward 78 (5.2); 16384 x 8192 199 (5.4) and 280 (5.8); in fp32 8192 x 4096
+// In bf16 with RMS norms and a gate 8192 x 4096 forward 47 us (5.7 TB/s), backward 77 (5.2); 16384 x 8192 189 (5.7) and 280 (5.8); in fp32 8192 x 4096
 // 89 (6.0) and 140 (5.8); 8192 x 1024 with a LayerNorm and a gate forward 12.5; one token of 4096 3.5.
 //
 // Reference call sites: the blocks that train/gpt2.py:26 and train/swin_b.py:38 build have a LayerNorm in front of each half and a

@@ -354,3 +354,49 @@ def test_more_than_the_cache_holds(ctx, dtype):
         for k in ("dx", "dbranch"):
             assert torch.equal(got[k][:200], back[k]), k
         check_backward(s, {k: t for k, t in got.items() if k in GRADS}, out["total"], kind, 1.0)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("rows,C,gates", [(600, 4608, 300), (772, 8192, 193), (258, 6152, 258), (40, 8184, 5)], ids=str)
+@pytest.mark.parametrize("post", [True, False])
+def test_gates_of_long_rows(ctx, dtype, kind, rows, C, gates, post):
+    """Rows of more than eight wavefronts: a workgroup has one gate, several, or a part of one's rows."""
+    s = make(rows, C, dtype, kind, gates=gates, post=post)
+    out = forward(ctx, s, kind, 1.25)
+    check_forward(s, out, kind, 1.25)
+    check_backward(s, backward(ctx, s, out["total"], out["stats"], kind, 1.25), out["total"], kind, 1.25)
+    check_backward(s, backward(ctx, s, out["total"], out["stats"], kind, 1.25, accumulate=True), out["total"], kind, 1.25, accumulate=True)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("parts", [dict(post=False, gates=0), dict(gates=0), dict(pre=False), dict(pre=False, post=False), dict(branch=False), dict(biases=False)], ids=str)
+@pytest.mark.parametrize("rows,C", [(300, 4104), (7, 5128), (513, 6144), (260, 7168)], ids=str)
+def test_parts_of_long_rows(ctx, dtype, kind, parts, rows, C):
+    s = make(rows, C, dtype, kind, **parts)
+    scale = 0.5 if s["branch"] is not None else 1.0
+    out = forward(ctx, s, kind, scale)
+    check_forward(s, out, kind, scale)
+    total = out["total"] if s["branch"] is not None else s["x"]
+    check_backward(s, backward(ctx, s, total, out["stats"], kind, scale), total, kind, scale)
+    if s["weight"] is not None:
+        s["dtotal"] = None
+        check_backward(s, backward(ctx, s, total, out["stats"], kind, scale), total, kind, scale)
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("rows,C", [(37, 200), (70, 1000), (300, 8192)], ids=str)
+def test_nobody_wants_the_gradient_of_x(ctx, kind, rows, C):
+    """dx None (the first block): everything else as with it, to the last bit."""
+    from sirius_amd import ops
+    s = make(rows, C, "bf16", kind)
+    out = forward(ctx, s, kind, 1.0)
+    want = backward(ctx, s, out["total"], out["stats"], kind, 1.0)
+    got = {k: None if v is None else torch.empty_like(v) for k, v in want.items()}
+    ws = torch.empty(ops.residual_norm_bwd_workspace_bytes(s["x"], s["gate"]), dtype=torch.uint8, device="cuda")
+    ops.residual_norm_bwd(ctx, s["dy"], s["dtotal"], out["total"], s["branch"], None, got["dbranch"], out["stats"], kind=kind, weight=s["weight"],
+                          post_weight=s["post_weight"], post_bias=s["post_bias"], gate=s["gate"], scale=1.0, workspace=ws, **{k: got[k] for k in GRADS})
+    torch.cuda.synchronize()
+    for k, v in want.items():
+        assert k == "dx" or v is None or torch.equal(got[k], v), k
