@@ -161,7 +161,7 @@ inline bool apart(const Span& a, const Span& b, bool in_place = false) {
   if (pa + (a.rows - 1) * a.ld + a.width <= pb || pb + (b.rows - 1) * b.ld + b.width <= pa) return true;
   const bool same_ld = a.ld == b.ld || (a.rows == 1 && b.rows == 1);
   if (pa == pb && same_ld && a.width == b.width) return in_place;
-  if (a.ld != b.ld) return false;
+  if (a.ld != b.ld || a.ld == 0) return false;   // (a single row's distance to the next may be 0)
   const int64_t ld = a.ld, shift = ((static_cast<int64_t>(pb) - static_cast<int64_t>(pa)) % ld + ld) % ld;   // columns of one matrix?
   return shift >= a.width && shift + b.width <= ld;
 }

@@ -69,3 +69,11 @@ def test_a_length_that_is_none_is_not_taken_for_one(seq, monkeypatch):
     x = torch.zeros(4, 128, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="length of a sequence"):
         ops.rotary_fwd(Here, x, x, torch.zeros(32, dtype=torch.float64), 64, seq=seq)
+
+
+@pytest.mark.parametrize("ld", [0, 8, 128])
+@pytest.mark.parametrize("dtype,shift", [(BF16, 16), (BF16, -16), (F32, 64), (F32, 256)], ids=str)
+def test_one_row_over_another(ld, dtype, shift):
+    """A single row needs no distance to the next one, 0 among them: two of them that overlap are refused all the same."""
+    rc, message = call(dtype=dtype, ldx=ld, ldy=ld, y=ctypes.c_void_p(0x100000 + shift), rows=1, seq=1)
+    assert rc == -22 and "overlaps" in message
