@@ -1385,7 +1385,8 @@ def residual_norm_bwd(ctx, dy, dtotal, total, branch, dx, dbranch, stats, kind="
     dbranch like x and branch, dweight, dbias, dpost_weight, dpost_bias [C] and dgate (like gate) fp32, each on request and (+)= with
     accumulate; the same bits every run.  total: the forward's x where there is no branch.  dx and dbranch may be dy, dtotal, total or
     branch.  workspace: residual_norm_bwd_workspace_bytes."""
-    shaped = next(t for t in (total, dy, dtotal) if t is not None)
+    shaped = next((t for t in (total, dy, dtotal) if t is not None), None)
+    assert shaped is not None, "no gradient, and no sum that it could be of"
     C = shaped.shape[-1]
     M = _matrix(ctx, "total", shaped, C)[2]
     t = {name: _matrix(ctx, name, v, C, M, shaped.dtype)[:2]

@@ -110,3 +110,10 @@ def test_the_oracles_gradients_against_differences(kind, post, gates, pre):
         slope = (loss(**{name: value + h * along}) - loss(**{name: value - h * along})) / (2 * h)
         mine = (grads["d" + name][0].view_as(value) * along).sum()
         assert abs(slope - mine) <= 1e-7 * (1 + abs(slope)), name
+
+
+def test_no_gradient_at_all():
+    """Refused as such: a StopIteration would quietly end the generator that the call is made in."""
+    from sirius_amd import ops
+    with pytest.raises(AssertionError, match="no gradient"):
+        ops.residual_norm_bwd(None, None, None, None, None, None, None, None)
