@@ -400,3 +400,47 @@ def test_nobody_wants_the_gradient_of_x(ctx, kind, rows, C):
     torch.cuda.synchronize()
     for k, v in want.items():
         assert k == "dx" or v is None or torch.equal(got[k], v), k
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("gates", [1, 4])
+def test_every_row_of_more_than_the_cache_holds(ctx, dtype, kind, gates):
+    """A workgroup of a streaming launch goes round many times: what it stores in each, and in the last one, which not all of them have, is
+    to the last bit what launches over a sixth of the rows store, which do not stream.  (With a gate a sample too.)"""
+    rows, C = (6008, 8192) if dtype == "bf16" else (9004, 4096)
+    s = make(rows, C, dtype, kind, gates=gates)
+    out = forward(ctx, s, kind, 1.25)
+    got = backward(ctx, s, out["total"], out["stats"], kind, 1.25)
+    each = rows // 4
+    for gate in range(4):
+        for r0, r1 in ((gate * each, gate * each + each // 2 + 1), (gate * each + each // 2 + 1, (gate + 1) * each)):
+            part = {k: t[r0:r1].contiguous() if k in ("x", "branch", "dy", "dtotal") else t for k, t in s.items()}
+            part["gate"] = s["gate"][gate % gates:gate % gates + 1].contiguous()
+            few = forward(ctx, part, kind, 1.25)
+            back = backward(ctx, part, few["total"], few["stats"], kind, 1.25)
+            for k in ("total", "y", "stats"):
+                assert torch.equal(out[k][r0:r1], few[k]), (k, r0)
+            for k in ("dx", "dbranch"):
+                assert torch.equal(got[k][r0:r1], back[k]), (k, r0)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("rows,C", [(40000, 128), (20001, 256), (9001, 512), (3001, 2304), (1030, 8192)], ids=str)
+def test_in_place_over_many_rounds(ctx, dtype, kind, rows, C):
+    """The next rows are on their way when a row's results go over what it was read from: all of them, in every place that may be shared."""
+    s = make(rows, C, dtype, kind)
+    want = forward(ctx, s, kind, 1.25)
+    grads = backward(ctx, s, want["total"], want["stats"], kind, 1.25)
+    for total, y in (("x", "branch"), ("branch", "x")):
+        t = dict(s, x=s["x"].clone(), branch=s["branch"].clone())
+        out = forward(ctx, t, kind, 1.25, total=t[total], y=t[y])
+        for k in ("total", "y", "stats"):
+            assert torch.equal(out[k], want[k]), (k, total, y)
+    for dx, dbranch in (("dtotal", "dy"), ("dy", "dtotal"), ("total", "branch"), ("branch", "total")):
+        t = dict(s, **{k: s[k].clone() for k in ("dy", "dtotal", "branch")})
+        t["total"] = want["total"].clone()
+        got = backward(ctx, t, t["total"], want["stats"], kind, 1.25, dx=t[dx], dbranch=t[dbranch])
+        for k in grads:
+            assert torch.equal(got[k], grads[k]), (k, dx, dbranch)
