@@ -299,3 +299,43 @@ def test_two_streams_at_once(ctx):
         ctx.synchronize()
         for a, b in zip(got, (side[5], side[7], side[8], side[9])):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_every_row_and_the_sums_of_more_than_the_cache_holds(ctx, dtype, fmt, gated):
+    """Kept, fetched and taken derivatives of with column sums, streaming past the cache: every row as launches over an eighth of the rows
+    have it, which do not stream, and the sums as the dense call adds them up."""
+    from sirius_amd import ops
+    dt, M, N = TYPES[dtype], 8200 if dtype == "bf16" else 4616, 5640
+    wide = N * (2 if gated else 1)
+    M = M if gated else 2 * M
+    pre, dy = normal(M, wide, dtype=dt, std=2.0), normal(M, N, dtype=dt, seed=1)
+    h, dz, again = torch.empty_like(pre), torch.empty_like(pre), torch.empty_like(dy)
+    packed, back = ops.Packed8.empty(M, wide, fmt), torch.empty_like(pre)
+    low = torch.empty_like(pre) if dtype == "bf16" else None
+    db = torch.empty(wide, device="cuda")
+    ws = torch.empty(max(ops.act_bwd_workspace_bytes(dy, gated=gated), 4), dtype=torch.uint8, device="cuda").fill_(255)
+
+    def bwd(*args, low=None, **more):
+        (ops.gated_act_bwd_packed if gated else ops.act_bwd_packed)(*args, **{"dpre_low" if gated else "dz_low": low}, **more)
+    ops.act_fwd_pack8(ctx, pre, h, packed, "gelu")
+    ops.unpack8(ctx, packed, back)
+    bwd(ctx, dy, packed, dz, "silu", h=again, low=low, dbias=db, workspace=ws)
+    each = M // 8
+    for r0 in range(0, M, each):
+        rows = slice(r0, r0 + each)
+        part = ops.Packed8.empty(each, wide, fmt)
+        h2, back2, dz2, again2 = torch.empty_like(h[rows]), torch.empty_like(h[rows]), torch.empty_like(h[rows]), torch.empty_like(dy[rows])
+        low2 = None if low is None else torch.empty_like(dz2)
+        ops.act_fwd_pack8(ctx, pre[rows], h2, part, "gelu")
+        ops.unpack8(ctx, part, back2)
+        bwd(ctx, dy[rows], part, dz2, "silu", h=again2, low=low2)
+        for a, b in ((h, h2), (packed.data, part.data), (packed.scales, part.scales), (back, back2), (dz, dz2), (again, again2)):
+            assert torch.equal(a[rows], b), r0
+        assert low is None or torch.equal(low[rows], low2), r0
+    dz2, db2 = torch.empty_like(dz), torch.empty_like(db)
+    (ops.gated_act_bwd if gated else ops.act_bwd)(ctx, dy, back, dz2, "silu", dbias=db2, workspace=ws)
+    assert torch.equal(dz, dz2)
+    sums_close(db, db2, dz)
