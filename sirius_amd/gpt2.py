@@ -48,9 +48,11 @@ class GPT2Engine(EngineBase):
                  stream=None, allocator=None, overlap_wgrad=True, fused_attention=True, trailing_wgrad=True,
                  trailing_reduce=None, fused_mlp=False, kept="full"):
         self._init_engine(dtype, stream, allocator)
-        # kept: what the backward pass finds of the projections' inputs and the MLP's pre-activations.  "int8" or "e4m3": 8 bits each
-        # (ops.Packed8; the hidden values are computed again from the pre-activations): a layer's activations take 18 C bytes a
-        # token instead of 32 C in bf16, 30 C instead of 64 C in fp32; the loss is the same, weight gradients are those of what is kept.
+        # kept: what the backward pass finds of the inputs of the projections behind the LayerNorms (c_attn, c_fc) and of the MLP's
+        # pre-activations.  "int8" or "e4m3": 8 bits each (ops.Packed8; the hidden values are computed again from the pre-activations;
+        # attn.c_proj's input stays as it is): a layer's activations take 18 C bytes a token instead of 32 C in bf16, 30 C instead of
+        # 64 C in fp32.  The forward pass computes the same, by other kernels for the norms and GELU: the loss differs by roundings.
+        # Weight gradients are those of what is kept, and GELU's derivative is taken of it: so every gradient in front of an MLP differs.
         if kept != "full" and kept not in ops.Packed8.FORMATS:
             raise ValueError(f"kept: full, {' or '.join(ops.Packed8.FORMATS)}")
         if kept != "full" and fused_mlp:

@@ -83,7 +83,7 @@ def main():
     parser.add_argument('--optimizer', choices=['sgd', 'adamw'], default='sgd')
     parser.add_argument('--fp32', action='store_true')
     parser.add_argument('--kept', choices=('full', 'int8', 'e4m3'), default='full',
-                        help="what the backward pass finds of the projections' inputs and the MLP's pre-activations: as computed, or 8 bits each")
+                        help="what the backward pass finds of the inputs of attn.c_attn and mlp.c_fc and of the MLP's pre-activations: as computed, or 8 bits each")
     parser.add_argument('--fused-mlp', action='store_true', help="activation and its derivative in the MLP projections' launches")
     parser.add_argument('--max-grad-norm', type=float, default=None, help="clip the gradients' global norm ahead of every step")
     parser.add_argument('--peer-script', type=str, default='',
