@@ -1194,7 +1194,8 @@ def rotary_fwd(ctx, x, y, freqs, head_dim, layout="half", positions=None, start=
     call), for flash_attn_fwd: the first 2 * freqs.numel() elements of a head are pairs (i, i + half) ("half") or (2 i, 2 i + 1)
     ("interleaved"); pair i of a row at position p is turned by p * freqs[i] and multiplied by scale, the rest of the head is copied.
     freqs: rotary_freqs on the GPU.  positions: int32 or int64, one a row, as deep in a cache as they like; None: row r stands at
-    start + r % seq (seq: the second to last size of x, so pass [batch, tokens, heads, head_dim] with its last two sizes as one).  x and y are rows of any type and alignment, y may be x."""
+    start + r % seq (seq: the second to last size of x, so pass [batch, tokens, heads, head_dim] with its last two sizes as one).
+    x and y are rows of any type and alignment, y may be x."""
     _rotary(ctx, x, y, freqs, head_dim, layout, positions, start, seq, scale, False)
 
 
